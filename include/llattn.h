@@ -388,6 +388,48 @@ int llattn_gdn_grad_out(const void* q, const void* k, const float* dq, const flo
                         const float* dg, void* gq, void* gk, void* gbeta, void* glambda, float* gg, long rows, int rep, int K, int K_in, int L,
                         float scale, float lambda_mul, void* stream);
 
+/* ---- operators of the layers that stand between the log-linear ones in a hybrid stack.  (No counterparts in the reference.)
+ *
+ * Gated linear recurrence of independent channels: o_t = h_t = exp(g_t) h_{t-1} + x_t.  x, o, dx (B,T,D) bf16 or fp32; g, dg (B,T,D) fp32 (g_is_f32)
+ * or, with bf16 x, bf16; g is a log decay, <= 0 (-inf starts a channel anew; above 0 the products over 128 tokens have to stay finite).  States are
+ * (B,D) fp32: h0 may be NULL (zeros), h_last and the gradients dh_last, dh0 may be NULL.  `states` (llattn_recurrence_states_bytes) receives the states
+ * that the backward starts from; NULL in a forward without one.  Any T >= 1 and D >= 1. */
+size_t llattn_recurrence_states_bytes(int B, int T, int D);
+int llattn_recurrence_fwd(const void* x, int x_is_f32, const void* g, int g_is_f32, const float* h0, void* o, float* h_last, float* states,
+                          int B, int T, int D, void* stream);
+int llattn_recurrence_bwd(const void* x, int x_is_f32, const void* g, int g_is_f32, const float* states, const void* d_o, const float* dh_last,
+                          void* dx, void* dg, float* dh0, int B, int T, int D, void* stream);
+/* One token: h (B,D) is advanced in place, o (B,D). */
+int llattn_recurrence_step(float* h, const void* x, int x_is_f32, const void* g, int g_is_f32, void* o, int B, int D, void* stream);
+
+/* Softmax attention over a sliding window with sinks: query t sees the tokens s <= t with t - s < window or s < sinks.  q, o, do, dq (B,T,H,K),
+ * k, v, dk, dv (B,T,G,K) bf16, K in {64,128}; head h uses k / v head h / (H/G).  window >= 1, sinks >= 0, scale > 0.  lse (llattn_window_lse_bytes)
+ * receives the softmax statistics that the backward reads; NULL in a forward without one.  The workspace (256 bytes for the forward,
+ * llattn_window_workspace_bytes for the backward) begins with a status word, see above.  Values that a query does not see have to be finite. */
+size_t llattn_window_lse_bytes(int B, int T, int H);
+size_t llattn_window_workspace_bytes(int B, int T, int H);
+int llattn_window_fwd(const void* q, const void* k, const void* v, void* o, float* lse, void* workspace, size_t workspace_bytes, int B, int T, int H, int G,
+                      int K, int window, int sinks, float scale, void* stream);
+int llattn_window_bwd(const void* q, const void* k, const void* v, const void* o, const float* lse, const void* d_o, void* dq, void* dk, void* dv,
+                      void* workspace, size_t workspace_bytes, int B, int T, int H, int G, int K, int window, int sinks, float scale, void* stream);
+/* The cache of a decoding sequence: sinks + window slots of (G,K), k_cache and v_cache (B,sinks + window,G,K) bf16.  Token t is in slot t if t < sinks, else in
+ * slot sinks + (t - sinks) % window.  counts (B,G): tokens seen so far, the same number for every head of a sequence.
+ *   fill: the cache after the first lengths[b] of T tokens (NULL: all of them; clamped to [0,T]); slots without a token are cleared.
+ *   step: appends one token's k, v (B,G,K), counts it, and attends: q, o (B,H,K).  Slots that hold no token are not read. */
+int llattn_window_fill(const void* k, const void* v, const long long* lengths, void* k_cache, void* v_cache, long long* counts, int B, int T, int G, int K,
+                       int window, int sinks, void* stream);
+int llattn_window_step(const void* q, const void* k, const void* v, void* k_cache, void* v_cache, long long* counts, void* o, int B, int H, int G, int K,
+                       int window, int sinks, float scale, void* stream);
+
+/* Layer norm of rows of N values: y = (x - mean) rstd w + b.  x, y, dy, dx (rows,N) bf16 or fp32; w, b, dw, db (N) fp32 (w_is_f32) or, with bf16 x, bf16;
+ * w and b may be NULL (ones, zeros).  mean and rstd (rows) fp32 are what the backward reads; NULL in a forward without one.  dw and db may be NULL; with one
+ * of them the backward needs a workspace (llattn_layer_norm_bwd_workspace_bytes).  The sums over rows are in an order that the sizes alone decide. */
+size_t llattn_layer_norm_bwd_workspace_bytes(long rows, int N);
+int llattn_layer_norm_fwd(const void* x, int x_is_f32, const void* w, const void* b, int w_is_f32, void* y, float* mean, float* rstd, float eps, long rows,
+                          int N, void* stream);
+int llattn_layer_norm_bwd(const void* x, int x_is_f32, const void* w, int w_is_f32, const float* mean, const float* rstd, const void* dy, void* dx, void* dw,
+                          void* db, void* workspace, size_t workspace_bytes, long rows, int N, void* stream);
+
 /* Diagnostic: one 128 x N x kred bf16 tensor-core product (tcgen05.mma, accumulator in tensor
  * memory) per operand-layout combination used by the kernels: mode 0: D = A B^T with A [128][kred],
  * B [N][kred]; mode 1: D = A B with B [kred][N]; mode 2: D = A^T B with A [kred][128], B [kred][N].

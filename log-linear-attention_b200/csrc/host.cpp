@@ -14,6 +14,7 @@
 #include <torch/extension.h>
 
 #include <ATen/cuda/EmptyTensor.h>
+#include <cmath>
 #include "../../include/llattn.h"
 
 namespace {
@@ -30,7 +31,10 @@ using torch::autograd::variable_list;
     F(llattn_mixer_prep_bwd) F(llattn_mixer_norm_fwd) F(llattn_mixer_norm_bwd) F(llattn_gdn_prompt_prep)                             \
     F(llattn_gdn_fwd_workspace_bytes) F(llattn_gdn_fwd_keep_workspace_bytes) F(llattn_gdn_fwd) F(llattn_gdn_fwd_keep)                \
     F(llattn_gdn_prompt) F(llattn_gdn_prompt_scratch_bytes) F(llattn_gdn_bwd_workspace_bytes) F(llattn_gdn_bwd)                      \
-    F(llattn_gdn_bwd_kept_workspace_bytes) F(llattn_gdn_bwd_kept_bf16dv) F(llattn_gdn_bwd_kept_normed) F(llattn_gdn_grad_out) F(llattn_workspace_status) F(llattn_clear)
+    F(llattn_gdn_bwd_kept_workspace_bytes) F(llattn_gdn_bwd_kept_bf16dv) F(llattn_gdn_bwd_kept_normed) F(llattn_gdn_grad_out) F(llattn_workspace_status) F(llattn_clear) \
+    F(llattn_recurrence_states_bytes) F(llattn_recurrence_fwd) F(llattn_recurrence_bwd) F(llattn_recurrence_step)                    \
+    F(llattn_window_lse_bytes) F(llattn_window_workspace_bytes) F(llattn_window_fwd) F(llattn_window_bwd) F(llattn_window_fill)      \
+    F(llattn_window_step) F(llattn_layer_norm_bwd_workspace_bytes) F(llattn_layer_norm_fwd) F(llattn_layer_norm_bwd)
 
 struct Library {
 #define LLATTN_MEMBER(name) decltype(&::name) name = nullptr;
@@ -793,6 +797,316 @@ py::object gdn_step(const Tensor& states, const py::list& counts, const Tensor& 
     return py::cast(o);
 }
 
+// ------------------------------------------------------------------------------------------ gated linear recurrence
+// x and g of one of the type pairs that the kernels take: g in fp32, or in x's type
+inline bool row_types(const Tensor& x, const Tensor& g) { return (bf16(x) && (bf16(g) || is(g, at::kFloat))) || (is(x, at::kFloat) && is(g, at::kFloat)); }
+bool recurrence_operands(const Tensor& x, const Tensor& g, const Tensor& h0) {
+    return row_types(x, g) && x.dim() == 3 && g.sizes() == x.sizes() && x.numel() > 0 && native_set({x, g, h0}) &&
+           (!h0.defined() || (is(h0, at::kFloat) && h0.sizes() == at::IntArrayRef({x.size(0), x.size(2)})));
+}
+struct Scanned {
+    Tensor o, last, states;
+};
+Scanned recurrence_fwd(const Tensor& x, const Tensor& g, const Tensor& h0, bool want_last, bool keep, void* stream) {
+    const int B = x.size(0), T = x.size(1), D = x.size(2);
+    Scanned r;
+    r.o = contiguous_like(x);
+    if (want_last) r.last = empty({B, D}, at::kFloat, x);
+    if (keep) r.states = empty({(int64_t)(lib.llattn_recurrence_states_bytes(B, T, D) / sizeof(float))}, at::kFloat, x);
+    check(lib.llattn_recurrence_fwd(x.data_ptr(), f32(x), g.data_ptr(), f32(g), fptr(h0), r.o.data_ptr(), fptr(r.last), fptr(r.states), B, T, D, stream),
+          "llattn_recurrence_fwd");
+    return r;
+}
+struct ScannedGrads {
+    Tensor dx, dg, dh0;
+};
+ScannedGrads recurrence_bwd(const Tensor& x, const Tensor& g, const Tensor& states, const Tensor& d_o, const Tensor& dlast, bool want_dh0, void* stream) {
+    const int B = x.size(0), T = x.size(1), D = x.size(2);
+    ScannedGrads r;
+    r.dx = contiguous_like(x);
+    r.dg = contiguous_like(g);
+    if (want_dh0) r.dh0 = empty({B, D}, at::kFloat, x);
+    check(lib.llattn_recurrence_bwd(x.data_ptr(), f32(x), g.data_ptr(), f32(g), fptr(states), d_o.data_ptr(), fptr(dlast), r.dx.data_ptr(), r.dg.data_ptr(),
+                                    fptr(r.dh0), B, T, D, stream),
+          "llattn_recurrence_bwd");
+    return r;
+}
+struct Recurrence : torch::autograd::Function<Recurrence> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& g, const Maybe& h0, bool want_last) {
+        On on(x);
+        const Tensor x_ = contiguous(x), g_ = contiguous(g);
+        const Scanned r = recurrence_fwd(x_, g_, contiguous(of(h0)), want_last, ctx != nullptr, on.stream);
+        if (ctx) {
+            ctx->save_for_backward({x_, g_, r.states});
+            ctx->saved_data["h0"] = h0.has_value();
+            ctx->set_materialize_grads(false);
+        }
+        if (!want_last) return {r.o};
+        return {r.o, r.last};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list d) {
+        const auto s = saved(ctx);
+        const Tensor &x = s[0], &g = s[1];
+        On on(x);
+        const Tensor d_o = d[0].defined() ? contiguous(d[0].to(x.scalar_type())) : at::zeros_like(x);
+        const Tensor dlast = d.size() > 1 && d[1].defined() ? contiguous(d[1].to(at::kFloat)) : Tensor();
+        const ScannedGrads r = recurrence_bwd(x, g, s[2], d_o, dlast, ctx->saved_data["h0"].toBool(), on.stream);
+        return {r.dx, r.dg, r.dh0, Tensor()};
+    }
+};
+// (o, last state or None), or None
+py::object gated_recurrence(const Tensor& x, const Tensor& g, const Maybe& h0, bool want_last) {
+    if (!recurrence_operands(x, g, of(h0))) return py::none();
+    variable_list r;
+    {
+        py::gil_scoped_release nogil;
+        r = wants_grad({x, g, of(h0)}) ? Recurrence::apply(x, g, h0, want_last) : Recurrence::forward(nullptr, x, g, h0, want_last);
+    }
+    return want_last ? py::make_tuple(r[0], r[1]) : py::make_tuple(r[0], py::none());
+}
+// the two passes on their own, for the dispatcher's operators
+py::object recurrence_forward(const Tensor& x, const Tensor& g, const Maybe& h0_) {
+    const Tensor h0 = of(h0_);
+    if (!recurrence_operands(x, g, h0)) return py::none();
+    On on(x);
+    const Scanned r = recurrence_fwd(contiguous(x), contiguous(g), contiguous(h0), true, true, on.stream);
+    return py::make_tuple(r.o, r.last, r.states);
+}
+py::object recurrence_backward(const Tensor& x, const Tensor& g, const Tensor& states, const Tensor& d_o, const Maybe& dlast_) {
+    const Tensor dlast = of(dlast_);
+    if (!recurrence_operands(x, g, dlast) || d_o.sizes() != x.sizes() || !same_device({x, d_o, states}) || !is(states, at::kFloat) || !states.is_contiguous() ||
+        states.numel() * sizeof(float) != lib.llattn_recurrence_states_bytes(x.size(0), x.size(1), x.size(2)))
+        return py::none();
+    On on(x);
+    const ScannedGrads r = recurrence_bwd(contiguous(x), contiguous(g), contiguous(states), contiguous(d_o.to(x.scalar_type())), contiguous(dlast), true, on.stream);
+    return py::make_tuple(r.dx, r.dg, r.dh0);
+}
+// o (B,D); the state is advanced in place
+py::object gated_recurrence_step(const Tensor& h, const Tensor& x, const Tensor& g) {
+    if (!row_types(x, g) || x.dim() != 2 || g.sizes() != x.sizes() || x.numel() == 0 || !is(h, at::kFloat) || h.sizes() != x.sizes() || !h.is_contiguous() ||
+        !aligned(h) || !native_set({h, x, g}) || wants_grad({h, x, g}))
+        return py::none();
+    On on(x);
+    const Tensor x_ = contiguous(x), g_ = contiguous(g), o = contiguous_like(x_);
+    check(lib.llattn_recurrence_step(fptr(h), x_.data_ptr(), f32(x_), g_.data_ptr(), f32(g_), o.data_ptr(), x.size(0), x.size(1), on.stream),
+          "llattn_recurrence_step");
+    return py::cast(o);
+}
+
+// ------------------------------------------------------------------------------------------ attention over a sliding window with sinks
+constexpr int64_t WINDOW_MAX = int64_t(1) << 29, WINDOW_T_MAX = int64_t(1) << 24;
+bool window_operands(const Tensor& q, const Tensor& k, const Tensor& v, int64_t window, int64_t sinks, double scale) {
+    if (!bf16(q) || !bf16(k) || !bf16(v) || q.dim() != 4 || k.dim() != 4 || v.sizes() != k.sizes() || q.numel() == 0 || k.numel() == 0 || !native_set({q, k, v}))
+        return false;
+    const int64_t B = q.size(0), T = q.size(1), H = q.size(2), K = q.size(3), G = k.size(2);
+    return k.size(0) == B && k.size(1) == T && k.size(3) == K && (K == 64 || K == 128) && H % G == 0 && T <= WINDOW_T_MAX && window >= 1 && sinks >= 0 &&
+           window <= WINDOW_MAX && sinks <= WINDOW_MAX && (float)scale > 0.f && std::isfinite((float)scale);
+}
+struct Windowed {
+    Tensor o, lse;
+};
+Windowed window_fwd(const Tensor& q, const Tensor& k, const Tensor& v, int64_t window, int64_t sinks, double scale, bool keep, bool status, void* stream) {
+    const int B = q.size(0), T = q.size(1), H = q.size(2), G = k.size(2), K = q.size(3);
+    Windowed r;
+    r.o = contiguous_like(q);
+    if (keep) r.lse = empty({(int64_t)(lib.llattn_window_lse_bytes(B, T, H) / sizeof(float))}, at::kFloat, q);
+    const Tensor ws = empty({256}, at::kByte, q);
+    check(lib.llattn_window_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), r.o.data_ptr(), fptr(r.lse), ws.data_ptr(), 256, B, T, H, G, K, (int)window, (int)sinks,
+                                (float)scale, stream),
+          "llattn_window_fwd");
+    if (status) check_status(ws, stream, "llattn_window_fwd");
+    return r;
+}
+struct WindowGrads {
+    Tensor dq, dk, dv;
+};
+WindowGrads window_bwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o, const Tensor& lse, const Tensor& d_o, int64_t window, int64_t sinks,
+                       double scale, bool status, void* stream) {
+    const int B = q.size(0), T = q.size(1), H = q.size(2), G = k.size(2), K = q.size(3);
+    const WindowGrads r = {contiguous_like(q), contiguous_like(k), contiguous_like(v)};
+    const Tensor ws = empty({(int64_t)lib.llattn_window_workspace_bytes(B, T, H)}, at::kByte, q);
+    check(lib.llattn_window_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), fptr(lse), d_o.data_ptr(), r.dq.data_ptr(), r.dk.data_ptr(),
+                                r.dv.data_ptr(), ws.data_ptr(), ws.numel(), B, T, H, G, K, (int)window, (int)sinks, (float)scale, stream),
+          "llattn_window_bwd");
+    if (status) check_status(ws, stream, "llattn_window_bwd");
+    return r;
+}
+struct WindowAttention : torch::autograd::Function<WindowAttention> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, int64_t window, int64_t sinks, double scale, bool status) {
+        On on(q);
+        const Tensor q_ = contiguous(q), k_ = contiguous(k), v_ = contiguous(v);
+        const Windowed r = window_fwd(q_, k_, v_, window, sinks, scale, ctx != nullptr, status, on.stream);
+        if (ctx) {
+            ctx->save_for_backward({q_, k_, v_, r.o, r.lse});
+            ctx->saved_data["window"] = window;
+            ctx->saved_data["sinks"] = sinks;
+            ctx->saved_data["scale"] = scale;
+            ctx->saved_data["status"] = status;
+        }
+        return r.o;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list d) {
+        const auto s = saved(ctx);
+        On on(s[0]);
+        const WindowGrads r = window_bwd(s[0], s[1], s[2], s[3], s[4], contiguous(d[0].to(at::kBFloat16)), ctx->saved_data["window"].toInt(),
+                                         ctx->saved_data["sinks"].toInt(), ctx->saved_data["scale"].toDouble(), ctx->saved_data["status"].toBool(), on.stream);
+        return {r.dq, r.dk, r.dv, Tensor(), Tensor(), Tensor(), Tensor()};
+    }
+};
+py::object sliding_window_attention(const Tensor& q, const Tensor& k, const Tensor& v, int64_t window, int64_t sinks, double scale, bool status) {
+    if (!window_operands(q, k, v, window, sinks, scale)) return py::none();
+    py::gil_scoped_release nogil;
+    Tensor o = wants_grad({q, k, v}) ? WindowAttention::apply(q, k, v, window, sinks, scale, status)
+                                     : WindowAttention::forward(nullptr, q, k, v, window, sinks, scale, status);
+    py::gil_scoped_acquire gil;
+    return py::cast(o);
+}
+// the two passes on their own, for the dispatcher's operators
+py::object window_forward(const Tensor& q, const Tensor& k, const Tensor& v, int64_t window, int64_t sinks, double scale, bool status) {
+    if (!window_operands(q, k, v, window, sinks, scale)) return py::none();
+    On on(q);
+    const Windowed r = window_fwd(contiguous(q), contiguous(k), contiguous(v), window, sinks, scale, true, status, on.stream);
+    return py::make_tuple(r.o, r.lse);
+}
+py::object window_backward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o, const Tensor& lse, const Tensor& d_o, int64_t window, int64_t sinks,
+                           double scale, bool status) {
+    if (!window_operands(q, k, v, window, sinks, scale) || !bf16(o) || o.sizes() != q.sizes() || d_o.sizes() != q.sizes() || !is(lse, at::kFloat) ||
+        !lse.is_contiguous() || !same_device({q, o, lse, d_o}) ||
+        lse.numel() * sizeof(float) != lib.llattn_window_lse_bytes(q.size(0), q.size(1), q.size(2)))
+        return py::none();
+    On on(q);
+    const WindowGrads r = window_bwd(contiguous(q), contiguous(k), contiguous(v), contiguous(o), contiguous(lse), contiguous(d_o.to(at::kBFloat16)), window, sinks,
+                                     scale, status, on.stream);
+    return py::make_tuple(r.dq, r.dk, r.dv);
+}
+// (o, k_cache, v_cache, counts) of a prompt, lengths (B,) int64 or absent; or None
+py::object sliding_window_prefill(const Tensor& q, const Tensor& k, const Tensor& v, int64_t window, int64_t sinks, double scale, const Maybe& lengths, bool status) {
+    const Tensor n = of(lengths);
+    if (!window_operands(q, k, v, window, sinks, scale) || k.size(0) > 65535 ||
+        (n.defined() && (!is(n, at::kLong) || n.sizes() != at::IntArrayRef({k.size(0)}) || !same_device({q, n}))))
+        return py::none();
+    Tensor o, kc, vc, counts;
+    {
+        py::gil_scoped_release nogil;
+        at::NoGradGuard no_grad;
+        On on(q);
+        const int B = k.size(0), T = k.size(1), G = k.size(2), K = k.size(3);
+        const Tensor k_ = contiguous(k), v_ = contiguous(v), n_ = contiguous(n);
+        o = window_fwd(contiguous(q), k_, v_, window, sinks, scale, false, status, on.stream).o;
+        kc = empty({B, sinks + window, G, K}, at::kBFloat16, k);
+        vc = empty({B, sinks + window, G, K}, at::kBFloat16, k);
+        counts = empty({B, G}, at::kLong, k);
+        check(lib.llattn_window_fill(k_.data_ptr(), v_.data_ptr(), n_.defined() ? reinterpret_cast<const long long*>(n_.data_ptr()) : nullptr, kc.data_ptr(),
+                                     vc.data_ptr(), reinterpret_cast<long long*>(counts.data_ptr()), B, T, G, K, (int)window, (int)sinks, on.stream),
+              "llattn_window_fill");
+    }
+    return py::make_tuple(o, kc, vc, counts);
+}
+// o (B,H,K); the caches and counts are advanced in place
+py::object sliding_window_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& kc, const Tensor& vc, const Tensor& counts, int64_t window,
+                               int64_t sinks, double scale) {
+    if (!bf16(q) || !bf16(k) || !bf16(v) || !bf16(kc) || !bf16(vc) || !is(counts, at::kLong) || q.dim() != 3 || k.dim() != 3 || v.sizes() != k.sizes() ||
+        q.numel() == 0 || k.numel() == 0 || !native_set({q, k, v, kc, vc, counts}) || wants_grad({q, k, v, kc, vc}))
+        return py::none();
+    const int64_t B = q.size(0), H = q.size(1), K = q.size(2), G = k.size(1);
+    if (k.size(0) != B || k.size(2) != K || (K != 64 && K != 128) || H % G != 0 || window < 1 || sinks < 0 || window > WINDOW_MAX || sinks > WINDOW_MAX ||
+        !((float)scale > 0.f) || !std::isfinite((float)scale) || kc.sizes() != at::IntArrayRef({B, sinks + window, G, K}) || vc.sizes() != kc.sizes() ||
+        counts.sizes() != at::IntArrayRef({B, G}) || !kc.is_contiguous() || !vc.is_contiguous() || !counts.is_contiguous() || !aligned(kc) || !aligned(vc) ||
+        !aligned(counts))
+        return py::none();
+    On on(q);
+    const Tensor q_ = contiguous(q), k_ = contiguous(k), v_ = contiguous(v), o = contiguous_like(q_);
+    check(lib.llattn_window_step(q_.data_ptr(), k_.data_ptr(), v_.data_ptr(), kc.data_ptr(), vc.data_ptr(), reinterpret_cast<long long*>(counts.data_ptr()),
+                                 o.data_ptr(), B, H, G, K, (int)window, (int)sinks, (float)scale, on.stream),
+          "llattn_window_step");
+    return py::cast(o);
+}
+
+// ------------------------------------------------------------------------------------------ layer norm
+bool norm_operands(const Tensor& x, const Tensor& w, const Tensor& b) {
+    if (!(bf16(x) || is(x, at::kFloat)) || x.dim() < 1 || x.numel() == 0 || x.numel() / x.size(-1) > 0x7fffffffl || x.size(-1) > 0x7fffffffl || !native_set({x, w, b}))
+        return false;
+    for (const Tensor* p : {&w, &b})
+        if (p->defined() && (!row_types(x, *p) || p->sizes() != at::IntArrayRef({x.size(-1)}))) return false;
+    return !w.defined() || !b.defined() || w.scalar_type() == b.scalar_type();
+}
+inline bool params_f32(const Tensor& x, const Tensor& w, const Tensor& b) { return w.defined() ? f32(w) : b.defined() ? f32(b) : f32(x); }
+struct Normed {
+    Tensor y, stats;          // mean and rstd of the rows
+};
+Normed norm_fwd(const Tensor& x, const Tensor& w, const Tensor& b, double eps, bool keep, void* stream) {
+    const int64_t N = x.size(-1), rows = x.numel() / N, pad = (rows + 3) / 4 * 4;
+    Normed r;
+    r.y = contiguous_like(x);
+    if (keep) r.stats = empty({2, pad}, at::kFloat, x);
+    float* m = fptr(r.stats);
+    check(lib.llattn_layer_norm_fwd(x.data_ptr(), f32(x), ptr(w), ptr(b), params_f32(x, w, b), r.y.data_ptr(), m, keep ? m + pad : nullptr, (float)eps, rows, (int)N,
+                                    stream),
+          "llattn_layer_norm_fwd");
+    return r;
+}
+struct NormGrads {
+    Tensor dx, dw, db;
+};
+NormGrads norm_bwd(const Tensor& x, const Tensor& w, const Tensor& stats, const Tensor& dy, at::ScalarType param, bool want_dw, bool want_db, void* stream) {
+    const int64_t N = x.size(-1), rows = x.numel() / N;
+    NormGrads r;
+    r.dx = contiguous_like(x);
+    if (want_dw) r.dw = empty({N}, param, x);
+    if (want_db) r.db = empty({N}, param, x);
+    Tensor ws;
+    if (want_dw || want_db) ws = empty({(int64_t)lib.llattn_layer_norm_bwd_workspace_bytes(rows, (int)N)}, at::kByte, x);
+    check(lib.llattn_layer_norm_bwd(x.data_ptr(), f32(x), ptr(w), param == at::kFloat, fptr(stats), fptr(stats) + stats.size(1), dy.data_ptr(), r.dx.data_ptr(),
+                                    ptr(r.dw), ptr(r.db), ptr(ws), ws.defined() ? ws.numel() : 0, rows, (int)N, stream),
+          "llattn_layer_norm_bwd");
+    return r;
+}
+struct LayerNorm : torch::autograd::Function<LayerNorm> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Maybe& w, const Maybe& b, double eps) {
+        On on(x);
+        const Tensor x_ = contiguous(x), w_ = contiguous(of(w)), b_ = contiguous(of(b));
+        const Normed r = norm_fwd(x_, w_, b_, eps, ctx != nullptr, on.stream);
+        if (ctx) {
+            ctx->save_for_backward({x_, w_, r.stats});
+            ctx->saved_data["param"] = (int64_t)(params_f32(x, w_, b_) ? at::kFloat : at::kBFloat16);
+            ctx->saved_data["dw"] = w_.defined() && w->requires_grad();
+            ctx->saved_data["db"] = b_.defined() && b->requires_grad();
+        }
+        return r.y;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list d) {
+        const auto s = saved(ctx);
+        On on(s[0]);
+        const NormGrads r = norm_bwd(s[0], s[1], s[2], contiguous(d[0].to(s[0].scalar_type())), (at::ScalarType)ctx->saved_data["param"].toInt(),
+                                     ctx->saved_data["dw"].toBool(), ctx->saved_data["db"].toBool(), on.stream);
+        return {r.dx, r.dw, r.db, Tensor()};
+    }
+};
+py::object layer_norm(const Tensor& x, const Maybe& w, const Maybe& b, double eps) {
+    if (!norm_operands(x, of(w), of(b))) return py::none();
+    py::gil_scoped_release nogil;
+    Tensor y = wants_grad({x, of(w), of(b)}) ? LayerNorm::apply(x, w, b, eps) : LayerNorm::forward(nullptr, x, w, b, eps);
+    py::gil_scoped_acquire gil;
+    return py::cast(y);
+}
+// the two passes on their own, for the dispatcher's operators
+py::object layer_norm_forward(const Tensor& x, const Maybe& w, const Maybe& b, double eps) {
+    if (!norm_operands(x, of(w), of(b))) return py::none();
+    On on(x);
+    const Normed r = norm_fwd(contiguous(x), contiguous(of(w)), contiguous(of(b)), eps, true, on.stream);
+    return py::make_tuple(r.y, r.stats);
+}
+py::object layer_norm_backward(const Tensor& x, const Tensor& w, const Tensor& stats, const Tensor& dy) {
+    if (!norm_operands(x, w, Tensor())) return py::none();
+    const int64_t rows = x.numel() / x.size(-1);
+    if (dy.sizes() != x.sizes() || !is(stats, at::kFloat) || !stats.is_contiguous() || !aligned(stats) || stats.sizes() != at::IntArrayRef({2, (rows + 3) / 4 * 4}) ||
+        !same_device({x, stats, dy}))
+        return py::none();
+    On on(x);
+    const NormGrads r = norm_bwd(contiguous(x), contiguous(w), stats, contiguous(dy.to(x.scalar_type())), w.scalar_type(), true, true, on.stream);
+    return py::make_tuple(r.dx, r.dw, r.db);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -806,4 +1120,16 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("hattention_gdn", &hattention_gdn);
     m.def("gdn_prompt", &gdn_prompt);
     m.def("gdn_step", &gdn_step);
+    m.def("gated_recurrence", &gated_recurrence);
+    m.def("recurrence_forward", &recurrence_forward);
+    m.def("recurrence_backward", &recurrence_backward);
+    m.def("gated_recurrence_step", &gated_recurrence_step);
+    m.def("sliding_window_attention", &sliding_window_attention);
+    m.def("window_forward", &window_forward);
+    m.def("window_backward", &window_backward);
+    m.def("sliding_window_prefill", &sliding_window_prefill);
+    m.def("sliding_window_step", &sliding_window_step);
+    m.def("layer_norm", &layer_norm);
+    m.def("layer_norm_forward", &layer_norm_forward);
+    m.def("layer_norm_backward", &layer_norm_backward);
 }

@@ -1,0 +1,338 @@
+// Attention over a sliding window with sinks: query t sees the tokens s <= t with t - s < window or s < sinks,
+//     o_t = sum_s P_ts v_s,   P_ts = exp(scale q_t . k_s - lse_t),   lse_t = log sum_s exp(scale q_t . k_s)
+// and the gradients, with delta_t = do_t . o_t,
+//     dV_s = sum_t P_ts do_t,   dS_ts = P_ts (do_t . v_s - delta_t),   dQ_t = scale sum_s dS_ts k_s,   dK_s = scale sum_t dS_ts q_t.
+// H query heads share G heads of k and v: dK and dV are sums over the H / G heads too.
+//
+// A warp takes one query row (or, for dK and dV, one token of k and v) and walks what it sees: softmax with a running maximum, everything in fp32.
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include "../../include/llattn.h"
+#include "launch_count.h"
+
+namespace llattn {
+namespace win {
+
+typedef __nv_bfloat16 bf16;
+
+struct Params {
+    const bf16 *q, *k, *v, *o, *d_o;
+    bf16 *out, *dq, *dk, *dv;
+    float *lse, *delta;       // (B,H,TP), TP the length up to whole tiles
+    int B, T, TP, H, G, window, sinks;
+    float scale;
+};
+
+template <int K>
+struct Lanes {
+    static constexpr int N = K / 32;
+    float v[N];
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = 0.f;
+    }
+    __device__ __forceinline__ void load(const bf16* row, int lane) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = __bfloat162float(row[lane + 32 * i]);
+    }
+    __device__ __forceinline__ void store(bf16* row, int lane, float f) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) row[lane + 32 * i] = __float2bfloat16(v[i] * f);
+    }
+    __device__ __forceinline__ void add(float f, const Lanes& x) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = fmaf(f, x.v[i], v[i]);
+    }
+};
+template <int K>
+__device__ __forceinline__ float dot(const Lanes<K>& a, const Lanes<K>& b) {
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < Lanes<K>::N; ++i) s = fmaf(a.v[i], b.v[i], s);
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+    return s;
+}
+
+template <int K>
+__global__ void __launch_bounds__(256) window_fwd_kernel(const __grid_constant__ Params p) {
+    chain_wait();
+    const int lane = threadIdx.x & 31;
+    const long row = (long)blockIdx.x * 8 + (threadIdx.x >> 5);            // (b, t, h)
+    if (row >= (long)p.B * p.T * p.H) return;
+    const int h = (int)(row % p.H), t = (int)(row / p.H % p.T), b = (int)(row / p.H / p.T);
+    const long ld = (long)p.G * K;
+    const bf16 *k = p.k + (long)b * p.T * ld + h / (p.H / p.G) * K, *v = p.v + (long)b * p.T * ld + h / (p.H / p.G) * K;
+    Lanes<K> q, acc, x;
+    q.load(p.q + row * K, lane);
+    acc.zero();
+    float m = -INFINITY, sum = 0.f;
+    const int lo = max(0, t - p.window + 1), first = min(p.sinks, lo);
+    for (int i = 0; i < first + t - lo + 1; ++i) {
+        const long s = i < first ? i : lo + i - first;
+        x.load(k + s * ld, lane);
+        const float y = dot<K>(q, x) * p.scale, n = fmaxf(m, y), f = __expf(m - n), e = __expf(y - n);
+        x.load(v + s * ld, lane);
+#pragma unroll
+        for (int j = 0; j < Lanes<K>::N; ++j) acc.v[j] *= f;
+        acc.add(e, x);
+        sum = sum * f + e;
+        m = n;
+    }
+    acc.store(p.out + row * K, lane, 1.f / sum);
+    if (p.lse && lane == 0) p.lse[((long)b * p.H + h) * p.TP + t] = m + logf(sum);
+}
+
+template <int K>
+__global__ void __launch_bounds__(256) window_dq_kernel(const __grid_constant__ Params p) {
+    chain_wait();
+    const int lane = threadIdx.x & 31;
+    const long row = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (row >= (long)p.B * p.T * p.H) return;
+    const int h = (int)(row % p.H), t = (int)(row / p.H % p.T), b = (int)(row / p.H / p.T);
+    const long ld = (long)p.G * K;
+    const bf16 *k = p.k + (long)b * p.T * ld + h / (p.H / p.G) * K, *v = p.v + (long)b * p.T * ld + h / (p.H / p.G) * K;
+    Lanes<K> q, d, acc, x, y;
+    q.load(p.q + row * K, lane);
+    d.load(p.d_o + row * K, lane);
+    x.load(p.o + row * K, lane);
+    acc.zero();
+    const float delta = dot<K>(d, x), lse = p.lse[((long)b * p.H + h) * p.TP + t];
+    if (lane == 0) p.delta[((long)b * p.H + h) * p.TP + t] = delta;
+    const int lo = max(0, t - p.window + 1), first = min(p.sinks, lo);
+    for (int i = 0; i < first + t - lo + 1; ++i) {
+        const long s = i < first ? i : lo + i - first;
+        x.load(k + s * ld, lane);
+        y.load(v + s * ld, lane);
+        acc.add(__expf(dot<K>(q, x) * p.scale - lse) * (dot<K>(d, y) - delta), x);
+    }
+    acc.store(p.dq + row * K, lane, p.scale);
+}
+
+template <int K>
+__global__ void __launch_bounds__(256) window_dkv_kernel(const __grid_constant__ Params p) {
+    chain_wait();
+    const int lane = threadIdx.x & 31;
+    const long row = (long)blockIdx.x * 8 + (threadIdx.x >> 5);            // (b, s, group)
+    if (row >= (long)p.B * p.T * p.G) return;
+    const int grp = (int)(row % p.G), s = (int)(row / p.G % p.T), b = (int)(row / p.G / p.T), R = p.H / p.G;
+    Lanes<K> k, v, dk, dv, x, y;
+    k.load(p.k + row * K, lane);
+    v.load(p.v + row * K, lane);
+    dk.zero();
+    dv.zero();
+    const int end = s < p.sinks ? p.T : (int)min((long)p.T, (long)s + p.window);
+    for (int h = grp * R; h < grp * R + R; ++h)
+        for (int t = s; t < end; ++t) {
+            const long at = (((long)b * p.T + t) * p.H + h) * K, st = ((long)b * p.H + h) * p.TP + t;
+            x.load(p.q + at, lane);
+            y.load(p.d_o + at, lane);
+            const float e = __expf(dot<K>(k, x) * p.scale - p.lse[st]);
+            dv.add(e, y);
+            dk.add(e * (dot<K>(v, y) - p.delta[st]), x);
+        }
+    dk.store(p.dk + row * K, lane, p.scale);
+    dv.store(p.dv + row * K, lane, 1.f);
+}
+
+// Slot c of a sequence of n tokens holds token c if c < sinks, else the last token that is c modulo the window, counted from the end of the sinks; zeros where there is none.
+template <int K>
+__global__ void __launch_bounds__(256) window_fill_kernel(const bf16* k, const bf16* v, const long long* lengths, bf16* kc, bf16* vc, long long* counts, int T,
+                                                          int G, int window, int sinks) {
+    chain_wait();
+    const int slots = sinks + window, b = blockIdx.y;
+    const long words = (long)G * K / 8;                                    // of 16 bytes, a token
+    long long n = lengths ? lengths[b] : T;
+    n = n < 0 ? 0 : n > T ? T : n;
+    const long i = (long)blockIdx.x * 256 + threadIdx.x;
+    if (i < G) counts[(long)b * G + i] = n;
+    if (i >= slots * words) return;
+    const int c = (int)(i / words);
+    const long w = i % words;
+    uint4 kw = make_uint4(0, 0, 0, 0), vw = kw;
+    if (c < n) {
+        const long t = c < sinks ? c : c + (n - 1 - c) / window * window, at = ((long)b * T + t) * words + w;
+        kw = reinterpret_cast<const uint4*>(k)[at];
+        vw = reinterpret_cast<const uint4*>(v)[at];
+    }
+    reinterpret_cast<uint4*>(kc)[(long)b * slots * words + i] = kw;
+    reinterpret_cast<uint4*>(vc)[(long)b * slots * words + i] = vw;
+}
+
+template <int K>
+__global__ void __launch_bounds__(256) window_step_kernel(const bf16* q, const bf16* k, const bf16* v, bf16* kc, bf16* vc, long long* counts, bf16* o, int H,
+                                                          int G, int window, int sinks, float scale) {
+    chain_wait();
+    __shared__ float part[8][K + 2];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, grp = blockIdx.x % G, b = blockIdx.x / G, R = H / G;
+    const long long seen = counts[blockIdx.x] > 0 ? counts[blockIdx.x] : 0;
+    const int slots = sinks + window, slot = (int)(seen < sinks ? seen : sinks + (seen - sinks) % window), held = (int)min((long long)slots, seen + 1);
+    const long ld = (long)G * K;
+    bf16 *kb = kc + (long)b * slots * ld + grp * K, *vb = vc + (long)b * slots * ld + grp * K;
+    if (threadIdx.x < K) {
+        kb[slot * ld + threadIdx.x] = k[(long)blockIdx.x * K + threadIdx.x];
+        vb[slot * ld + threadIdx.x] = v[(long)blockIdx.x * K + threadIdx.x];
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) counts[blockIdx.x] = seen + 1;
+    for (int h = grp * R; h < grp * R + R; ++h) {
+        Lanes<K> x, y, acc;
+        x.load(q + ((long)b * H + h) * K, lane);
+        acc.zero();
+        float m = -INFINITY, sum = 0.f;
+        for (int c = warp; c < held; c += 8) {
+            y.load(kb + c * ld, lane);
+            const float z = dot<K>(x, y) * scale, n = fmaxf(m, z), f = __expf(m - n), e = __expf(z - n);
+            y.load(vb + c * ld, lane);
+#pragma unroll
+            for (int j = 0; j < Lanes<K>::N; ++j) acc.v[j] *= f;
+            acc.add(e, y);
+            sum = sum * f + e;
+            m = n;
+        }
+#pragma unroll
+        for (int j = 0; j < Lanes<K>::N; ++j) part[warp][lane + 32 * j] = acc.v[j];
+        if (lane == 0) {
+            part[warp][K] = m;
+            part[warp][K + 1] = sum;
+        }
+        __syncthreads();
+        if (threadIdx.x < K) {
+            float top = -INFINITY, total = 0.f, r = 0.f;
+            for (int w = 0; w < 8; ++w) top = fmaxf(top, part[w][K]);
+            for (int w = 0; w < 8; ++w) {
+                const float f = __expf(part[w][K] - top);
+                total = fmaf(f, part[w][K + 1], total);
+                r = fmaf(f, part[w][threadIdx.x], r);
+            }
+            o[((long)b * H + h) * K + threadIdx.x] = __float2bfloat16(r / total);
+        }
+        __syncthreads();
+    }
+}
+
+int check(long B, long T, long H, long G, int K, long window, long sinks, float scale) {
+    if (B < 1 || T < 1 || G < 1 || H < 1 || (K != 64 && K != 128) || window < 1 || sinks < 0 || !(scale > 0.f) || !(scale < INFINITY)) return LLATTN_ERR_UNSUPPORTED_SHAPE;
+    if (H % G != 0) return LLATTN_ERR_BAD_GROUPS;
+    if (T > (1 << 24) || window + sinks > (1 << 30) || B * H > (1l << 31) / 128 || B * T * H / 8 >= 0x7fffffffl) return LLATTN_ERR_UNSUPPORTED_SHAPE;
+    return 0;
+}
+int padded(int T) { return (T + 127) / 128 * 128; }
+
+}  // namespace win
+}  // namespace llattn
+
+using namespace llattn;
+
+extern "C" {
+
+size_t llattn_window_lse_bytes(int B, int T, int H) {
+    if (win::check(B, T, H, 1, 64, 1, 0, 1.f) != 0) return 0;
+    return (size_t)B * H * win::padded(T) * sizeof(float);
+}
+size_t llattn_window_workspace_bytes(int B, int T, int H) {
+    const size_t n = llattn_window_lse_bytes(B, T, H);
+    return n == 0 ? 0 : 256 + n;
+}
+
+int llattn_window_fwd(const void* q, const void* k, const void* v, void* o, float* lse, void* workspace, size_t workspace_bytes, int B, int T, int H, int G, int K,
+                      int window, int sinks, float scale, void* stream) {
+    const int rc = win::check(B, T, H, G, K, window, sinks, scale);
+    if (rc != 0) return rc;
+    if (!q || !k || !v || !o) return LLATTN_ERR_NULL;
+    if (misaligned(16, {q, k, v, o, lse})) return LLATTN_ERR_ALIGNMENT;
+    if (!workspace || misaligned(256, {workspace}) || workspace_bytes < 256) return LLATTN_ERR_WORKSPACE;
+    win::Params p = {};
+    p.q = (const win::bf16*)q;
+    p.k = (const win::bf16*)k;
+    p.v = (const win::bf16*)v;
+    p.out = (win::bf16*)o;
+    p.lse = lse;
+    p.B = B;
+    p.T = T;
+    p.TP = win::padded(T);
+    p.H = H;
+    p.G = G;
+    p.window = window;
+    p.sinks = sinks;
+    p.scale = scale;
+    cudaStream_t st = (cudaStream_t)stream;
+    cudaError_t e = cudaMemsetAsync(workspace, 0, 4, st);
+    if (e != cudaSuccess) return (int)e;
+    const unsigned grid = (unsigned)(((long)B * T * H + 7) / 8);
+    e = K == 64 ? launch_chained(win::window_fwd_kernel<64>, grid, 256, 0, st, p) : launch_chained(win::window_fwd_kernel<128>, grid, 256, 0, st, p);
+    if (e == cudaSuccess) LLATTN_LAUNCHED();
+    return (int)e;
+}
+
+int llattn_window_bwd(const void* q, const void* k, const void* v, const void* o, const float* lse, const void* d_o, void* dq, void* dk, void* dv, void* workspace,
+                      size_t workspace_bytes, int B, int T, int H, int G, int K, int window, int sinks, float scale, void* stream) {
+    const int rc = win::check(B, T, H, G, K, window, sinks, scale);
+    if (rc != 0) return rc;
+    if (!q || !k || !v || !o || !lse || !d_o || !dq || !dk || !dv) return LLATTN_ERR_NULL;
+    if (misaligned(16, {q, k, v, o, lse, d_o, dq, dk, dv})) return LLATTN_ERR_ALIGNMENT;
+    if (!workspace || misaligned(256, {workspace}) || workspace_bytes < llattn_window_workspace_bytes(B, T, H)) return LLATTN_ERR_WORKSPACE;
+    win::Params p = {};
+    p.q = (const win::bf16*)q;
+    p.k = (const win::bf16*)k;
+    p.v = (const win::bf16*)v;
+    p.o = (const win::bf16*)o;
+    p.d_o = (const win::bf16*)d_o;
+    p.dq = (win::bf16*)dq;
+    p.dk = (win::bf16*)dk;
+    p.dv = (win::bf16*)dv;
+    p.lse = const_cast<float*>(lse);
+    p.delta = reinterpret_cast<float*>(static_cast<char*>(workspace) + 256);
+    p.B = B;
+    p.T = T;
+    p.TP = win::padded(T);
+    p.H = H;
+    p.G = G;
+    p.window = window;
+    p.sinks = sinks;
+    p.scale = scale;
+    cudaStream_t st = (cudaStream_t)stream;
+    cudaError_t e = cudaMemsetAsync(workspace, 0, 4, st);
+    if (e != cudaSuccess) return (int)e;
+    const unsigned rows = (unsigned)(((long)B * T * H + 7) / 8), tokens = (unsigned)(((long)B * T * G + 7) / 8);
+    e = K == 64 ? launch_chained(win::window_dq_kernel<64>, rows, 256, 0, st, p) : launch_chained(win::window_dq_kernel<128>, rows, 256, 0, st, p);
+    if (e != cudaSuccess) return (int)e;
+    LLATTN_LAUNCHED();
+    e = K == 64 ? launch_chained(win::window_dkv_kernel<64>, tokens, 256, 0, st, p) : launch_chained(win::window_dkv_kernel<128>, tokens, 256, 0, st, p);
+    if (e == cudaSuccess) LLATTN_LAUNCHED();
+    return (int)e;
+}
+
+int llattn_window_fill(const void* k, const void* v, const long long* lengths, void* k_cache, void* v_cache, long long* counts, int B, int T, int G, int K,
+                       int window, int sinks, void* stream) {
+    const int rc = win::check(B, T, G, G, K, window, sinks, 1.f);
+    if (rc != 0) return rc;
+    if (!k || !v || !k_cache || !v_cache || !counts) return LLATTN_ERR_NULL;
+    if (misaligned(16, {k, v, lengths, k_cache, v_cache, counts})) return LLATTN_ERR_ALIGNMENT;
+    const long n = (long)(window + sinks) * G * K / 8, blocks = ((n > G ? n : G) + 255) / 256;
+    if (B > 65535 || blocks > 0x7fffffffl) return LLATTN_ERR_UNSUPPORTED_SHAPE;
+    cudaStream_t st = (cudaStream_t)stream;
+    const dim3 grid((unsigned)blocks, B);
+    const auto *kk = (const win::bf16*)k, *vv = (const win::bf16*)v;
+    const auto kern = K == 64 ? win::window_fill_kernel<64> : win::window_fill_kernel<128>;
+    const cudaError_t e = launch_chained(kern, grid, 256, 0, st, kk, vv, lengths, (win::bf16*)k_cache, (win::bf16*)v_cache, counts, T, G, window, sinks);
+    if (e == cudaSuccess) LLATTN_LAUNCHED();
+    return (int)e;
+}
+
+int llattn_window_step(const void* q, const void* k, const void* v, void* k_cache, void* v_cache, long long* counts, void* o, int B, int H, int G, int K, int window,
+                       int sinks, float scale, void* stream) {
+    const int rc = win::check(B, 1, H, G, K, window, sinks, scale);
+    if (rc != 0) return rc;
+    if (!q || !k || !v || !k_cache || !v_cache || !counts || !o) return LLATTN_ERR_NULL;
+    if (misaligned(16, {q, k, v, k_cache, v_cache, counts, o})) return LLATTN_ERR_ALIGNMENT;
+    cudaStream_t st = (cudaStream_t)stream;
+    const auto kern = K == 64 ? win::window_step_kernel<64> : win::window_step_kernel<128>;
+    const cudaError_t e = launch_chained(kern, (unsigned)(B * G), 256, 0, st, (const win::bf16*)q, (const win::bf16*)k, (const win::bf16*)v, (win::bf16*)k_cache,
+                                         (win::bf16*)v_cache, counts, (win::bf16*)o, H, G, window, sinks, scale);
+    if (e == cudaSuccess) LLATTN_LAUNCHED();
+    return (int)e;
+}
+
+}  // extern "C"

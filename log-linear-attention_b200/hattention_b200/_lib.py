@@ -97,6 +97,24 @@ def lib():
     L.llattn_gdn_bwd_kept.argtypes = [_P] * 15 + [_P, ctypes.c_size_t, _P, ctypes.c_size_t] + [ctypes.c_int] * 6 + [_P]
     L.llattn_gdn_bwd_kept_bf16dv.restype = ctypes.c_int
     L.llattn_gdn_bwd_kept_bf16dv.argtypes = L.llattn_gdn_bwd_kept.argtypes
+    _Z, _L = ctypes.c_size_t, ctypes.c_long
+    for name, res, args in [
+        ("llattn_recurrence_states_bytes", _Z, [_I] * 3),
+        ("llattn_recurrence_fwd", _I, [_P, _I, _P, _I] + [_P] * 4 + [_I] * 3 + [_P]),
+        ("llattn_recurrence_bwd", _I, [_P, _I, _P, _I] + [_P] * 6 + [_I] * 3 + [_P]),
+        ("llattn_recurrence_step", _I, [_P, _P, _I, _P, _I, _P, _I, _I, _P]),
+        ("llattn_window_lse_bytes", _Z, [_I] * 3),
+        ("llattn_window_workspace_bytes", _Z, [_I] * 3),
+        ("llattn_window_fwd", _I, [_P] * 6 + [_Z] + [_I] * 7 + [_F, _P]),
+        ("llattn_window_bwd", _I, [_P] * 10 + [_Z] + [_I] * 7 + [_F, _P]),
+        ("llattn_window_fill", _I, [_P] * 6 + [_I] * 6 + [_P]),
+        ("llattn_window_step", _I, [_P] * 7 + [_I] * 6 + [_F, _P]),
+        ("llattn_layer_norm_bwd_workspace_bytes", _Z, [_L, _I]),
+        ("llattn_layer_norm_fwd", _I, [_P, _I, _P, _P, _I, _P, _P, _P, _F, _L, _I, _P]),
+        ("llattn_layer_norm_bwd", _I, [_P, _I, _P, _I] + [_P] * 7 + [_Z, _L, _I, _P]),
+    ]:
+        fn = getattr(L, name)
+        fn.restype, fn.argtypes = res, args
     L.llattn_selftest_umma_cycles.restype = ctypes.c_int
     L.llattn_selftest_umma_cycles.argtypes = [ctypes.c_int] * 5 + [_P, _P, _P]
     L.llattn_testing_use_tensor_core_path.restype = None        # test-only symbol (csrc/llattn_testing.h)

@@ -10,11 +10,18 @@ the interface that mirrors the reference (`hattention/chunkwise.py`, `hattention
     llattn::gdn_bwd(q, k, v, beta, g_cum, l, Aw, Au, do)     -> (dq, dk, dv, dbeta, dg, dl)
     llattn::l2norm_scale_fwd(x, scale)                       -> y
     llattn::l2norm_scale_bwd(x, dy, scale)                   -> dx
+    llattn::recurrence_fwd(x, g, h0)                         -> (o, h_last, states)
+    llattn::recurrence_bwd(x, g, states, do, dh_last)        -> (dx, dg, dh0)
+    llattn::window_fwd(q, k, v, window, sinks, scale)        -> (o, lse)
+    llattn::window_bwd(q, k, v, o, lse, do, window, sinks, scale) -> (dq, dk, dv)
+    llattn::layer_norm_fwd(x, weight, bias, eps)             -> (y, stats)
+    llattn::layer_norm_bwd(x, weight, stats, dy)             -> (dx, dweight, dbias)
 
 `workspace` of mamba2_fwd is the call's scratch (uint8); handing it to mamba2_bwd lets the backward read the
-segment-level states instead of recomputing them (pass an empty tensor to recompute).
+segment-level states instead of recomputing them (pass an empty tensor to recompute).  `states`, `lse` and `stats` are what the forward
+passes of the hybrid-stack operators keep for their backward passes.
 """
-from typing import Tuple
+from typing import Optional, Tuple
 
 import torch
 
@@ -102,3 +109,75 @@ def l2norm_scale_bwd(x: _T, dy: _T, scale: float) -> _T:
 @l2norm_scale_bwd.register_fake
 def _(x, dy, scale):
     return torch.empty_like(x, dtype=torch.bfloat16)
+
+
+def _taken(r, what: str):
+    if r is None:
+        raise ValueError(f"{what}: operands that the kernels do not take")
+    return r
+
+
+@torch.library.custom_op("llattn::recurrence_fwd", mutates_args=())
+def recurrence_fwd(x: _T, g: _T, h0: Optional[_T]) -> Tuple[_T, _T, _T]:
+    return _taken(_lib.host().recurrence_forward(x, g, h0), "recurrence_fwd")
+
+
+@recurrence_fwd.register_fake
+def _(x, g, h0):
+    B, T, D = x.shape
+    n = _lib.lib().llattn_recurrence_states_bytes(B, T, D) // 4
+    f = torch.float32
+    return x.new_empty(x.shape), x.new_empty((B, D), dtype=f), x.new_empty((int(n),), dtype=f)
+
+
+@torch.library.custom_op("llattn::recurrence_bwd", mutates_args=())
+def recurrence_bwd(x: _T, g: _T, states: _T, do: _T, dh_last: Optional[_T]) -> Tuple[_T, _T, _T]:
+    return _taken(_lib.host().recurrence_backward(x, g, states, do, dh_last), "recurrence_bwd")
+
+
+@recurrence_bwd.register_fake
+def _(x, g, states, do, dh_last):
+    return x.new_empty(x.shape), g.new_empty(g.shape), x.new_empty((x.shape[0], x.shape[2]), dtype=torch.float32)
+
+
+@torch.library.custom_op("llattn::window_fwd", mutates_args=())
+def window_fwd(q: _T, k: _T, v: _T, window: int, sinks: int, scale: float) -> Tuple[_T, _T]:
+    return _taken(_lib.host().window_forward(q, k, v, window, sinks, scale, _lib.CHECK_STATUS), "window_fwd")
+
+
+@window_fwd.register_fake
+def _(q, k, v, window, sinks, scale):
+    B, T, H, _ = q.shape
+    n = _lib.lib().llattn_window_lse_bytes(B, T, H) // 4
+    return q.new_empty(q.shape), q.new_empty((int(n),), dtype=torch.float32)
+
+
+@torch.library.custom_op("llattn::window_bwd", mutates_args=())
+def window_bwd(q: _T, k: _T, v: _T, o: _T, lse: _T, do: _T, window: int, sinks: int, scale: float) -> Tuple[_T, _T, _T]:
+    return _taken(_lib.host().window_backward(q, k, v, o, lse, do, window, sinks, scale, _lib.CHECK_STATUS), "window_bwd")
+
+
+@window_bwd.register_fake
+def _(q, k, v, o, lse, do, window, sinks, scale):
+    return q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+
+
+@torch.library.custom_op("llattn::layer_norm_fwd", mutates_args=())
+def layer_norm_fwd(x: _T, weight: _T, bias: Optional[_T], eps: float) -> Tuple[_T, _T]:
+    return _taken(_lib.host().layer_norm_forward(x, weight, bias, eps), "layer_norm_fwd")
+
+
+@layer_norm_fwd.register_fake
+def _(x, weight, bias, eps):
+    rows = x.numel() // x.shape[-1]
+    return x.new_empty(x.shape), x.new_empty((2, (rows + 3) // 4 * 4), dtype=torch.float32)
+
+
+@torch.library.custom_op("llattn::layer_norm_bwd", mutates_args=())
+def layer_norm_bwd(x: _T, weight: _T, stats: _T, dy: _T) -> Tuple[_T, _T, _T]:
+    return _taken(_lib.host().layer_norm_backward(x, weight, stats, dy), "layer_norm_bwd")
+
+
+@layer_norm_bwd.register_fake
+def _(x, weight, stats, dy):
+    return x.new_empty(x.shape), weight.new_empty(weight.shape), weight.new_empty(weight.shape)
