@@ -5,24 +5,11 @@
 // H query heads share G heads of k and v: dK and dV are sums over the H / G heads too.
 //
 // A warp takes one query row (or, for dK and dV, one token of k and v) and walks what it sees: softmax with a running maximum, everything in fp32.
-#include <cuda_bf16.h>
-#include <cuda_runtime.h>
-
 #include "../../include/llattn.h"
-#include "launch_count.h"
+#include "window.cuh"
 
 namespace llattn {
 namespace win {
-
-typedef __nv_bfloat16 bf16;
-
-struct Params {
-    const bf16 *q, *k, *v, *o, *d_o;
-    bf16 *out, *dq, *dk, *dv;
-    float *lse, *delta;       // (B,H,TP), TP the length up to whole tiles
-    int B, T, TP, H, G, window, sinks;
-    float scale;
-};
 
 template <int K>
 struct Lanes {
@@ -56,35 +43,6 @@ __device__ __forceinline__ float dot(const Lanes<K>& a, const Lanes<K>& b) {
 }
 
 template <int K>
-__global__ void __launch_bounds__(256) window_fwd_kernel(const __grid_constant__ Params p) {
-    chain_wait();
-    const int lane = threadIdx.x & 31;
-    const long row = (long)blockIdx.x * 8 + (threadIdx.x >> 5);            // (b, t, h)
-    if (row >= (long)p.B * p.T * p.H) return;
-    const int h = (int)(row % p.H), t = (int)(row / p.H % p.T), b = (int)(row / p.H / p.T);
-    const long ld = (long)p.G * K;
-    const bf16 *k = p.k + (long)b * p.T * ld + h / (p.H / p.G) * K, *v = p.v + (long)b * p.T * ld + h / (p.H / p.G) * K;
-    Lanes<K> q, acc, x;
-    q.load(p.q + row * K, lane);
-    acc.zero();
-    float m = -INFINITY, sum = 0.f;
-    const int lo = max(0, t - p.window + 1), first = min(p.sinks, lo);
-    for (int i = 0; i < first + t - lo + 1; ++i) {
-        const long s = i < first ? i : lo + i - first;
-        x.load(k + s * ld, lane);
-        const float y = dot<K>(q, x) * p.scale, n = fmaxf(m, y), f = __expf(m - n), e = __expf(y - n);
-        x.load(v + s * ld, lane);
-#pragma unroll
-        for (int j = 0; j < Lanes<K>::N; ++j) acc.v[j] *= f;
-        acc.add(e, x);
-        sum = sum * f + e;
-        m = n;
-    }
-    acc.store(p.out + row * K, lane, 1.f / sum);
-    if (p.lse && lane == 0) p.lse[((long)b * p.H + h) * p.TP + t] = m + logf(sum);
-}
-
-template <int K>
 __global__ void __launch_bounds__(256) window_dq_kernel(const __grid_constant__ Params p) {
     chain_wait();
     const int lane = threadIdx.x & 31;
@@ -105,7 +63,7 @@ __global__ void __launch_bounds__(256) window_dq_kernel(const __grid_constant__ 
         const long s = i < first ? i : lo + i - first;
         x.load(k + s * ld, lane);
         y.load(v + s * ld, lane);
-        acc.add(__expf(dot<K>(q, x) * p.scale - lse) * (dot<K>(d, y) - delta), x);
+        acc.add(exp2_fast(dot<K>(q, x) * p.scale * LOG2E - lse) * (dot<K>(d, y) - delta), x);
     }
     acc.store(p.dq + row * K, lane, p.scale);
 }
@@ -128,7 +86,7 @@ __global__ void __launch_bounds__(256) window_dkv_kernel(const __grid_constant__
             const long at = (((long)b * p.T + t) * p.H + h) * K, st = ((long)b * p.H + h) * p.TP + t;
             x.load(p.q + at, lane);
             y.load(p.d_o + at, lane);
-            const float e = __expf(dot<K>(k, x) * p.scale - p.lse[st]);
+            const float e = exp2_fast(dot<K>(k, x) * p.scale * LOG2E - p.lse[st]);
             dv.add(e, y);
             dk.add(e * (dot<K>(v, y) - p.delta[st]), x);
         }
@@ -215,10 +173,25 @@ __global__ void __launch_bounds__(256) window_step_kernel(const bf16* q, const b
 int check(long B, long T, long H, long G, int K, long window, long sinks, float scale) {
     if (B < 1 || T < 1 || G < 1 || H < 1 || (K != 64 && K != 128) || window < 1 || sinks < 0 || !(scale > 0.f) || !(scale < INFINITY)) return LLATTN_ERR_UNSUPPORTED_SHAPE;
     if (H % G != 0) return LLATTN_ERR_BAD_GROUPS;
-    if (T > (1 << 24) || window + sinks > (1 << 30) || B * H > (1l << 31) / 128 || B * T * H / 8 >= 0x7fffffffl) return LLATTN_ERR_UNSUPPORTED_SHAPE;
+    if (T > (1 << 24) || window > (1 << 29) || sinks > (1 << 29) || B > 65535 || H > 65535 || B * T * H / 8 >= 0x7fffffffl) return LLATTN_ERR_UNSUPPORTED_SHAPE;
     return 0;
 }
-int padded(int T) { return (T + 127) / 128 * 128; }
+int padded(int T) { return (T + TILE - 1) / TILE * TILE; }
+void shape(Params& p, void* workspace, int B, int T, int H, int G, int window, int sinks, float scale) {
+    p.err = static_cast<int*>(workspace);
+    p.B = B;
+    p.T = T;
+    p.TP = padded(T);
+    p.H = H;
+    p.G = G;
+    p.window = window;
+    p.sinks = sinks;
+    p.scale = scale;
+}
+bool maps(Params& p, const void* q, const void* k, const void* v, int K) {
+    return tma::make_seq_map(&p.tq, q, p.B, p.T, p.H, K, TILE, 2) == 0 && tma::make_seq_map(&p.tk, k, p.B, p.T, p.G, K, TILE, 2) == 0 &&
+           tma::make_seq_map(&p.tv, v, p.B, p.T, p.G, K, TILE, 2) == 0;
+}
 
 }  // namespace win
 }  // namespace llattn
@@ -241,29 +214,17 @@ int llattn_window_fwd(const void* q, const void* k, const void* v, void* o, floa
     const int rc = win::check(B, T, H, G, K, window, sinks, scale);
     if (rc != 0) return rc;
     if (!q || !k || !v || !o) return LLATTN_ERR_NULL;
-    if (misaligned(16, {q, k, v, o, lse})) return LLATTN_ERR_ALIGNMENT;
+    if (misaligned(16, {q, k, v, lse}) || misaligned(32, {o})) return LLATTN_ERR_ALIGNMENT;
     if (!workspace || misaligned(256, {workspace}) || workspace_bytes < 256) return LLATTN_ERR_WORKSPACE;
     win::Params p = {};
-    p.q = (const win::bf16*)q;
-    p.k = (const win::bf16*)k;
-    p.v = (const win::bf16*)v;
     p.out = (win::bf16*)o;
     p.lse = lse;
-    p.B = B;
-    p.T = T;
-    p.TP = win::padded(T);
-    p.H = H;
-    p.G = G;
-    p.window = window;
-    p.sinks = sinks;
-    p.scale = scale;
+    win::shape(p, workspace, B, T, H, G, window, sinks, scale);
+    if (!win::maps(p, q, k, v, K)) return LLATTN_ERR_TENSOR_MAP;
     cudaStream_t st = (cudaStream_t)stream;
-    cudaError_t e = cudaMemsetAsync(workspace, 0, 4, st);
+    const cudaError_t e = cudaMemsetAsync(workspace, 0, 4, st);
     if (e != cudaSuccess) return (int)e;
-    const unsigned grid = (unsigned)(((long)B * T * H + 7) / 8);
-    e = K == 64 ? launch_chained(win::window_fwd_kernel<64>, grid, 256, 0, st, p) : launch_chained(win::window_fwd_kernel<128>, grid, 256, 0, st, p);
-    if (e == cudaSuccess) LLATTN_LAUNCHED();
-    return (int)e;
+    return (int)win::forward_tc(p, K, st);
 }
 
 int llattn_window_bwd(const void* q, const void* k, const void* v, const void* o, const float* lse, const void* d_o, void* dq, void* dk, void* dv, void* workspace,
@@ -284,14 +245,7 @@ int llattn_window_bwd(const void* q, const void* k, const void* v, const void* o
     p.dv = (win::bf16*)dv;
     p.lse = const_cast<float*>(lse);
     p.delta = reinterpret_cast<float*>(static_cast<char*>(workspace) + 256);
-    p.B = B;
-    p.T = T;
-    p.TP = win::padded(T);
-    p.H = H;
-    p.G = G;
-    p.window = window;
-    p.sinks = sinks;
-    p.scale = scale;
+    win::shape(p, workspace, B, T, H, G, window, sinks, scale);
     cudaStream_t st = (cudaStream_t)stream;
     cudaError_t e = cudaMemsetAsync(workspace, 0, 4, st);
     if (e != cudaSuccess) return (int)e;

@@ -1,0 +1,99 @@
+// What the kernels of the sliding-window attention share: parameters, which tokens a query sees, tiles.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include "launch_count.h"
+#include "tma.cuh"
+#include "umma.cuh"
+
+namespace llattn {
+namespace win {
+
+typedef __nv_bfloat16 bf16;
+constexpr int TILE = 128;             // tokens of a tile of queries, and of keys
+constexpr float LOG2E = 1.4426950408889634f;
+
+struct Params {
+    CUtensorMap tq, tk, tv, tdo;      // (B,T,heads,K), boxes of 128 tokens x 64 columns of one head
+    const bf16 *q, *k, *v, *o, *d_o;
+    bf16 *out, *dq, *dk, *dv;
+    float *lse, *delta;               // (B,H,TP), TP the length up to whole tiles; lse = log2 of the sum, infinity behind the sequence
+    int* err;                         // status word of the workspace
+    int B, T, TP, H, G, window, sinks;
+    float scale;
+};
+
+// The tiles of keys that the queries [q0, q0 + 128) see are the first `sink` ones and [lo, hi].
+struct Span {
+    int lo, hi, sink;
+    __host__ __device__ Span(int q0, int T, int window, int sinks) {
+        const int first = q0 - window + 1;                 // (window <= 2^29)
+        lo = first > 0 ? first / TILE : 0;
+        hi = q0 < T ? q0 / TILE : -1;
+        const int n = (min_(sinks, T) + TILE - 1) / TILE;
+        sink = n < lo ? n : lo;
+    }
+    static __host__ __device__ int min_(int a, int b) { return a < b ? a : b; }
+    __host__ __device__ bool has(int j) const { return j <= hi && (j >= lo || j < sink); }
+};
+// whether every query of the tile from q0 on sees every key of the tile from s0 on
+__device__ __forceinline__ bool all_seen(int q0, int s0, int window, int sinks) {
+    return s0 + TILE - 1 <= q0 && (q0 + TILE - 1 - s0 < window || s0 + TILE - 1 < sinks);
+}
+__device__ __forceinline__ bool sees(int t, int s, int window, int sinks) { return s <= t && (t - s < window || s < sinks); }
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+// 64 consecutive fp32 columns of this thread's lane, both loads in flight before the wait
+__device__ __forceinline__ void tmem_ld64(uint32_t taddr, float (&v)[64]) {
+    uint32_t r[64];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        asm volatile(
+            "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+            "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+            : "=r"(r[32 * i + 0]), "=r"(r[32 * i + 1]), "=r"(r[32 * i + 2]), "=r"(r[32 * i + 3]), "=r"(r[32 * i + 4]), "=r"(r[32 * i + 5]), "=r"(r[32 * i + 6]),
+              "=r"(r[32 * i + 7]), "=r"(r[32 * i + 8]), "=r"(r[32 * i + 9]), "=r"(r[32 * i + 10]), "=r"(r[32 * i + 11]), "=r"(r[32 * i + 12]), "=r"(r[32 * i + 13]),
+              "=r"(r[32 * i + 14]), "=r"(r[32 * i + 15]), "=r"(r[32 * i + 16]), "=r"(r[32 * i + 17]), "=r"(r[32 * i + 18]), "=r"(r[32 * i + 19]), "=r"(r[32 * i + 20]),
+              "=r"(r[32 * i + 21]), "=r"(r[32 * i + 22]), "=r"(r[32 * i + 23]), "=r"(r[32 * i + 24]), "=r"(r[32 * i + 25]), "=r"(r[32 * i + 26]), "=r"(r[32 * i + 27]),
+              "=r"(r[32 * i + 28]), "=r"(r[32 * i + 29]), "=r"(r[32 * i + 30]), "=r"(r[32 * i + 31])
+            : "r"(taddr + 32 * i)
+            : "memory");
+    asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+    // every destination register passes through here, so that no use of it can be scheduled above the wait
+#pragma unroll
+    for (int i = 0; i < 64; i += 16)
+        asm volatile(""
+                     : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7]), "+r"(r[i + 8]),
+                       "+r"(r[i + 9]), "+r"(r[i + 10]), "+r"(r[i + 11]), "+r"(r[i + 12]), "+r"(r[i + 13]), "+r"(r[i + 14]), "+r"(r[i + 15]));
+#pragma unroll
+    for (int i = 0; i < 64; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(umma::smem_addr(bar)) : "memory");
+}
+// one 32-byte global store: a full sector of a lane's own row
+__device__ __forceinline__ void store_32B(void* dst, const uint32_t (&w)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n"
+                 ::"l"(dst), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+}
+// one tile of a map into a shared-memory operand tile of K / 64 panels
+template <int K>
+__device__ __forceinline__ void load_tile(unsigned char* dst, const CUtensorMap* map, int head, int tok0, int batch, uint64_t* bar) {
+#pragma unroll
+    for (int p = 0; p < K / 64; ++p) tma::load_seq_panel(dst + p * TILE * umma::ROW_BYTES, map, p * 64, head, tok0, batch, bar);
+}
+
+cudaError_t forward_tc(const Params& p, int K, cudaStream_t st);
+
+}  // namespace win
+}  // namespace llattn

@@ -1,0 +1,263 @@
+// Sliding-window attention forward on the 5th-generation tensor cores.
+//
+// A CTA takes two tiles of 128 queries of a head, A and B, and walks the tiles of keys that either sees.  For each of them and each tile of queries
+//     S = Q K^T            128 x 128 x K     into tensor memory
+//     P = exp2(c S - m)    a warpgroup, a thread a row: running maximum m and sum, P as bf16 in the place of S
+//     O += P V             128 x K x 128     P from tensor memory
+// with the products of one tile of queries under the softmax of the other.  The maximum that the exponents refer to moves only when a row's has grown by more than
+// 2^8: O, in tensor memory, is rescaled then alone, and P never exceeds 2^8.
+//     warps 0..3, 4..7   softmax, rescaling and output of A, of B
+//     warp 8             issues the products
+//     warp 9             brings Q, then K and V tiles through a ring
+// A wait that gives up sets the CTA's abort flag, after which every other wait ends at once, and the workspace's status word.
+#include "window.cuh"
+
+namespace llattn {
+namespace win {
+
+namespace fwd {
+constexpr int NST = 4, NTHREADS = 384, MMA_WARP = 8, TMA_WARP = 9;
+constexpr int TM_S = 0, TM_O = 256;            // S of A and B, 128 columns each; O of A and B, 128 columns apart
+constexpr float GROWTH = 8.f;
+
+template <int K>
+struct Smem {
+    static constexpr uint32_t TILE_BYTES = TILE * K * 2;
+    static constexpr uint32_t q_off = 0, st_off = 2 * TILE_BYTES, bar_off = st_off + NST * TILE_BYTES, total = bar_off + 256 + 1024;
+};
+// 128 x (168 - 72) registers go to the 256 threads of the softmax
+__device__ __forceinline__ void regs_issue() { asm volatile("setmaxnreg.dec.sync.aligned.u32 72;\n"); }
+__device__ __forceinline__ void regs_rows() { asm volatile("setmaxnreg.inc.sync.aligned.u32 216;\n"); }
+
+// The tiles of keys that A or B sees, in order: the sinks', then the rest.
+struct Walk {
+    Span a, b;
+    int j, end;
+    __device__ Walk(const Params& p, int q0) : a(q0, p.T, p.window, p.sinks), b(q0 + TILE, p.T, p.window, p.sinks) {
+        j = 0;
+        end = a.hi > b.hi ? a.hi : b.hi;
+        settle();
+    }
+    __device__ void settle() {
+        while (j <= end && !a.has(j) && !b.has(j)) j = j < a.lo ? a.lo : b.lo;      // (a tile that neither sees is in front of A's or B's band)
+    }
+    __device__ bool more() const { return j <= end; }
+    __device__ void next() {
+        ++j;
+        settle();
+    }
+    __device__ bool in(int x) const { return x == 0 ? a.has(j) : b.has(j); }
+};
+}  // namespace fwd
+
+template <int K>
+__global__ void __launch_bounds__(fwd::NTHREADS, 1) window_fwd_tc_kernel(const __grid_constant__ Params p) {
+    chain_wait();
+    using namespace fwd;
+    using SM = Smem<K>;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* smem = umma::align_1024(smem_raw);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + SM::bar_off);
+    uint64_t *full = bars, *empty = bars + NST, *barQ = bars + 2 * NST, *barS = barQ + 1, *barP = barS + 2, *barO = barP + 2;
+    constexpr int NBARS = 2 * NST + 7;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + SM::bar_off + NBARS * 8);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int q0 = blockIdx.x * 2 * TILE, h = blockIdx.y, b = blockIdx.z, grp = h / (p.H / p.G);
+    if (tid == 0) {
+        for (int i = 0; i < NST; ++i) {
+            umma::mbar_init(full + i, 1);
+            umma::mbar_init(empty + i, 1);
+        }
+        umma::mbar_init(barQ, 1);
+        for (int x = 0; x < 2; ++x) {
+            umma::mbar_init(barS + x, 1);
+            umma::mbar_init(barP + x, 4);
+            umma::mbar_init(barO + x, 1);
+        }
+        umma::fence_mbar_init();
+        *abort_flag = 0;
+    }
+    if (warp == MMA_WARP) umma::tmem_alloc(tmem_slot, 512);
+    umma::fence_before_sync();
+    __syncthreads();
+    umma::fence_after_sync();
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp >= 8) {
+        regs_issue();
+        if (warp == TMA_WARP && lane == 0) {
+            const bool two = q0 + TILE < p.T;
+            tma::expect_tx(barQ, (two ? 2 : 1) * SM::TILE_BYTES);
+            load_tile<K>(smem + SM::q_off, &p.tq, h, q0, b, barQ);
+            if (two) load_tile<K>(smem + SM::q_off + SM::TILE_BYTES, &p.tq, h, q0 + TILE, b, barQ);
+            int n = 0;
+            bool ok = true;
+            for (Walk w(p, q0); w.more() && ok; w.next())
+                for (int kv = 0; kv < 2 && ok; ++kv, ++n) {
+                    const int st = n % NST;
+                    if (n >= NST) ok = umma::mbar_wait(empty + st, (n / NST - 1) & 1, abort_flag);
+                    if (!ok) break;
+                    tma::expect_tx(full + st, SM::TILE_BYTES);
+                    load_tile<K>(smem + SM::st_off + st * SM::TILE_BYTES, kv ? &p.tv : &p.tk, grp, w.j * TILE, b, full + st);
+                }
+            // nobody may be left to wait for the last copies after a wait that gave up: they end before the CTA does
+            if (*abort_flag) {
+                umma::mbar_wait(barQ, 0);
+                for (int i = n > NST ? n - NST : 0; i < n; ++i) umma::mbar_wait(full + i % NST, (i / NST) & 1);
+            }
+        } else if (warp == MMA_WARP) {
+            const uint32_t lead = umma::elect_one(), sQ = umma::smem_addr(smem + SM::q_off), sS = umma::smem_addr(smem + SM::st_off);
+            constexpr uint32_t idS = umma::idesc_bf16(128, 128, false, false), idO = umma::idesc_bf16(128, K, false, true);
+            bool ok = umma::mbar_wait_warp(barQ, 0, abort_flag);
+            int done[2] = {0, 0};                       // products P V of A, B issued
+            Walk w(p, q0);
+            // step i: the products P V with tile i - 1, and S with tile i
+            bool before[2] = {false, false};
+            for (int i = 0; ok; ++i) {
+                const bool more = w.more();
+                if (!more && !before[0] && !before[1]) break;
+                bool haveK = false, haveV = false;
+                const int nk = 2 * i, nv = 2 * i - 1;   // positions of K of this step and V of the one before in the ring's sequence
+                bool now[2];
+                for (int x = 0; x < 2; ++x) {
+                    now[x] = more && w.in(x);
+                    if (before[x] && ok) {
+                        if (!haveV) ok = umma::mbar_wait_warp(full + nv % NST, (nv / NST) & 1, abort_flag);
+                        haveV = true;
+                        ok = ok && umma::mbar_wait_warp(barP + x, done[x] & 1, abort_flag);
+                        if (!ok) break;
+                        umma::fence_after_sync();
+                        umma::gemm_tm_lead<TILE, TILE>(lead, tmem + TM_O + 128 * x, tmem + TM_S + 128 * x, sS + (nv % NST) * SM::TILE_BYTES, idO, done[x] > 0);
+                        umma::commit_lead(lead, barO + x);
+                        ++done[x];
+                    }
+                    if (now[x] && ok) {
+                        if (!haveK) ok = umma::mbar_wait_warp(full + nk % NST, (nk / NST) & 1, abort_flag);
+                        haveK = true;
+                        if (!ok) break;
+                        umma::gemm_kk_lead<TILE, TILE, K>(lead, tmem + TM_S + 128 * x, sQ + x * SM::TILE_BYTES, sS + (nk % NST) * SM::TILE_BYTES, idS, false);
+                        umma::commit_lead(lead, barS + x);
+                    }
+                }
+                if (!ok) break;
+                if (i > 0) umma::commit_lead(lead, empty + nv % NST);
+                if (more) umma::commit_lead(lead, empty + nk % NST);
+                before[0] = now[0];
+                before[1] = now[1];
+                if (more) w.next();
+            }
+        }
+    } else {
+        regs_rows();
+        const int x = warp >> 2, row = (warp & 3) * 32 + lane, t0 = q0 + x * TILE, t = t0 + row;
+        const uint32_t tS = umma::tmem_addr(tmem, warp, TM_S + 128 * x), tO = umma::tmem_addr(tmem, warp, TM_O + 128 * x);
+        const float c = p.scale * LOG2E;
+        float m = -INFINITY, sum = 0.f;
+        int n = 0;
+        bool ok = true;
+        for (Walk w(p, q0); w.more(); w.next()) {
+            if (!w.in(x)) continue;
+            ok = umma::mbar_wait_warp(barS + x, n & 1, abort_flag);
+            if (!ok) break;
+            umma::fence_after_sync();
+            float s[2][64];
+            tmem_ld64(tS, s[0]);
+            tmem_ld64(tS + 64, s[1]);
+            const int s0 = w.j * TILE;
+            if (!all_seen(t0, s0, p.window, p.sinks)) {
+#pragma unroll
+                for (int i = 0; i < 128; ++i)
+                    if (!sees(t, s0 + i, p.window, p.sinks)) s[i >> 6][i & 63] = -INFINITY;
+            }
+            float top[4] = {s[0][0], s[0][1], s[0][2], s[0][3]};
+#pragma unroll
+            for (int i = 4; i < 128; ++i) top[i & 3] = fmaxf(top[i & 3], s[i >> 6][i & 63]);
+            const float now = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
+            const bool grown = now > m + GROWTH || (m == -INFINITY && now > m);
+            if (n == 0) {
+                m = now;
+            } else if (__any_sync(0xffffffffu, grown)) {
+                ok = umma::mbar_wait_warp(barO + x, (n - 1) & 1, abort_flag);
+                if (!ok) break;
+                umma::fence_after_sync();
+                const float f = grown ? exp2_fast(m - now) : 1.f;
+                if (grown) m = now;
+                sum *= f;
+#pragma unroll
+                for (int i = 0; i < K; i += 16) {
+                    float o[16];
+                    umma::tmem_ld16(tO + i, o);
+#pragma unroll
+                    for (int u = 0; u < 16; ++u) o[u] *= f;
+                    umma::tmem_st16(tO + i, o);
+                }
+            }
+            const float ref = m == -INFINITY ? 0.f : m;        // a row that has seen nothing yet
+            float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < 128; i += 32) {
+                uint32_t w16[16];
+#pragma unroll
+                for (int u = 0; u < 32; u += 2) {
+                    const float e0 = exp2_fast(fmaf(s[(i + u) >> 6][(i + u) & 63], c, -ref)), e1 = exp2_fast(fmaf(s[(i + u) >> 6][(i + u + 1) & 63], c, -ref));
+                    part[u & 2] += e0;
+                    part[(u & 2) + 1] += e1;
+                    w16[u >> 1] = pack_bf16(e0, e1);
+                }
+                umma::tmem_st16u(tS + i / 2, w16);
+            }
+            sum += (part[0] + part[1]) + (part[2] + part[3]);
+            umma::tmem_wait_st();
+            umma::fence_before_sync();
+            __syncwarp();
+            if (lane == 0) arrive(barP + x);
+            ++n;
+        }
+        if (ok && n > 0) ok = umma::mbar_wait_warp(barO + x, (n - 1) & 1, abort_flag);
+        if (ok && n > 0) {
+            umma::fence_after_sync();
+            const float f = 1.f / sum;
+            bf16* out = p.out + (((long)b * p.T + t) * p.H + h) * K;
+#pragma unroll
+            for (int i = 0; i < K; i += 16) {
+                float o[16];
+                umma::tmem_ld16(tO + i, o);
+                uint32_t w8[8];
+#pragma unroll
+                for (int u = 0; u < 8; ++u) w8[u] = pack_bf16(o[2 * u] * f, o[2 * u + 1] * f);
+                if (t < p.T) store_32B(out + i, w8);
+            }
+            if (p.lse) p.lse[((long)b * p.H + h) * p.TP + t] = t < p.T ? m + log2f(sum) : INFINITY;
+        }
+        umma::fence_before_sync();
+    }
+    __syncthreads();
+    umma::fence_after_sync();
+    if (warp == MMA_WARP) {
+        // products that nobody waited for, after a wait that gave up, end before their memory is handed back
+        if (*abort_flag) {
+            const uint32_t lead = umma::elect_one();
+            umma::commit_lead(lead, barQ);
+            umma::mbar_wait(barQ, 1);
+            if (lane == 0) atomicExch(p.err, 1);
+        }
+        umma::tmem_dealloc(tmem, 512);
+    }
+}
+
+template <int K>
+static cudaError_t launch(const Params& p, cudaStream_t st) {
+    const auto kern = window_fwd_tc_kernel<K>;
+    cudaError_t e = allow_smem(kern, fwd::Smem<K>::total);
+    if (e != cudaSuccess) return e;
+    const dim3 grid((unsigned)((p.T + 2 * TILE - 1) / (2 * TILE)), p.H, p.B);
+    e = launch_chained(kern, grid, fwd::NTHREADS, fwd::Smem<K>::total, st, p);
+    if (e == cudaSuccess) LLATTN_LAUNCHED();
+    return e;
+}
+cudaError_t forward_tc(const Params& p, int K, cudaStream_t st) { return K == 64 ? launch<64>(p, st) : launch<128>(p, st); }
+
+}  // namespace win
+}  // namespace llattn
