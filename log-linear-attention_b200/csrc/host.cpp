@@ -52,10 +52,11 @@ void bind(const std::string& path) {
 #undef LLATTN_BIND
 }
 
+// (numbers as text of their own: streams write them through locale facets, which this module may have a second copy of, unset outside the main thread)
 void check(int rc, const char* what) {
     if (rc == 0) return;
-    TORCH_CHECK_VALUE(rc > 0, what, ": unsupported arguments (code ", rc, ")");
-    TORCH_CHECK(false, what, ": CUDA error ", rc);
+    TORCH_CHECK_VALUE(rc > 0, std::string(what) + ": unsupported arguments (code " + std::to_string(rc) + ")");
+    TORCH_CHECK(false, std::string(what) + ": CUDA error " + std::to_string(rc));
 }
 
 // ------------------------------------------------------------------------------------------ small helpers
