@@ -405,7 +405,7 @@ int llattn_recurrence_step(float* h, const void* x, int x_is_f32, const void* g,
 /* Softmax attention over a sliding window with sinks: query t sees the tokens s <= t with t - s < window or s < sinks.  q, o, do, dq (B,T,H,K),
  * k, v, dk, dv (B,T,G,K) bf16, K in {64,128}; head h uses k / v head h / (H/G).  window >= 1, sinks >= 0, scale > 0.  lse (llattn_window_lse_bytes)
  * receives the softmax statistics that the backward reads; NULL in a forward without one.  The workspace (256 bytes for the forward,
- * llattn_window_workspace_bytes for the backward) begins with a status word, see above.  Values that a query does not see have to be finite. */
+ * llattn_window_workspace_bytes for the backward) begins with a status word, see above.  o, dq, dk and dv start at 32-byte boundaries.  Values that a query does not see have to be finite. */
 size_t llattn_window_lse_bytes(int B, int T, int H);
 size_t llattn_window_workspace_bytes(int B, int T, int H);
 int llattn_window_fwd(const void* q, const void* k, const void* v, void* o, float* lse, void* workspace, size_t workspace_bytes, int B, int T, int H, int G,

@@ -4,7 +4,7 @@
 //     dV_s = sum_t P_ts do_t,   dS_ts = P_ts (do_t . v_s - delta_t),   dQ_t = scale sum_s dS_ts k_s,   dK_s = scale sum_t dS_ts q_t.
 // H query heads share G heads of k and v: dK and dV are sums over the H / G heads too.
 //
-// A warp takes one query row (or, for dK and dV, one token of k and v) and walks what it sees: softmax with a running maximum, everything in fp32.
+// Here: the C entries, the cache of a decoding sequence, the step.  Forward: window_fwd_tc.cu, backward: window_bwd_tc.cu.
 #include "../../include/llattn.h"
 #include "window.cuh"
 
@@ -40,58 +40,6 @@ __device__ __forceinline__ float dot(const Lanes<K>& a, const Lanes<K>& b) {
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
     return s;
-}
-
-template <int K>
-__global__ void __launch_bounds__(256) window_dq_kernel(const __grid_constant__ Params p) {
-    chain_wait();
-    const int lane = threadIdx.x & 31;
-    const long row = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (row >= (long)p.B * p.T * p.H) return;
-    const int h = (int)(row % p.H), t = (int)(row / p.H % p.T), b = (int)(row / p.H / p.T);
-    const long ld = (long)p.G * K;
-    const bf16 *k = p.k + (long)b * p.T * ld + h / (p.H / p.G) * K, *v = p.v + (long)b * p.T * ld + h / (p.H / p.G) * K;
-    Lanes<K> q, d, acc, x, y;
-    q.load(p.q + row * K, lane);
-    d.load(p.d_o + row * K, lane);
-    x.load(p.o + row * K, lane);
-    acc.zero();
-    const float delta = dot<K>(d, x), lse = p.lse[((long)b * p.H + h) * p.TP + t];
-    if (lane == 0) p.delta[((long)b * p.H + h) * p.TP + t] = delta;
-    const int lo = max(0, t - p.window + 1), first = min(p.sinks, lo);
-    for (int i = 0; i < first + t - lo + 1; ++i) {
-        const long s = i < first ? i : lo + i - first;
-        x.load(k + s * ld, lane);
-        y.load(v + s * ld, lane);
-        acc.add(exp2_fast(dot<K>(q, x) * p.scale * LOG2E - lse) * (dot<K>(d, y) - delta), x);
-    }
-    acc.store(p.dq + row * K, lane, p.scale);
-}
-
-template <int K>
-__global__ void __launch_bounds__(256) window_dkv_kernel(const __grid_constant__ Params p) {
-    chain_wait();
-    const int lane = threadIdx.x & 31;
-    const long row = (long)blockIdx.x * 8 + (threadIdx.x >> 5);            // (b, s, group)
-    if (row >= (long)p.B * p.T * p.G) return;
-    const int grp = (int)(row % p.G), s = (int)(row / p.G % p.T), b = (int)(row / p.G / p.T), R = p.H / p.G;
-    Lanes<K> k, v, dk, dv, x, y;
-    k.load(p.k + row * K, lane);
-    v.load(p.v + row * K, lane);
-    dk.zero();
-    dv.zero();
-    const int end = s < p.sinks ? p.T : (int)min((long)p.T, (long)s + p.window);
-    for (int h = grp * R; h < grp * R + R; ++h)
-        for (int t = s; t < end; ++t) {
-            const long at = (((long)b * p.T + t) * p.H + h) * K, st = ((long)b * p.H + h) * p.TP + t;
-            x.load(p.q + at, lane);
-            y.load(p.d_o + at, lane);
-            const float e = exp2_fast(dot<K>(k, x) * p.scale * LOG2E - p.lse[st]);
-            dv.add(e, y);
-            dk.add(e * (dot<K>(v, y) - p.delta[st]), x);
-        }
-    dk.store(p.dk + row * K, lane, p.scale);
-    dv.store(p.dv + row * K, lane, 1.f);
 }
 
 // Slot c of a sequence of n tokens holds token c if c < sinks, else the last token that is c modulo the window, counted from the end of the sinks; zeros where there is none.
@@ -173,7 +121,7 @@ __global__ void __launch_bounds__(256) window_step_kernel(const bf16* q, const b
 int check(long B, long T, long H, long G, int K, long window, long sinks, float scale) {
     if (B < 1 || T < 1 || G < 1 || H < 1 || (K != 64 && K != 128) || window < 1 || sinks < 0 || !(scale > 0.f) || !(scale < INFINITY)) return LLATTN_ERR_UNSUPPORTED_SHAPE;
     if (H % G != 0) return LLATTN_ERR_BAD_GROUPS;
-    if (T > (1 << 24) || window > (1 << 29) || sinks > (1 << 29) || B > 65535 || H > 65535 || B * T * H / 8 >= 0x7fffffffl) return LLATTN_ERR_UNSUPPORTED_SHAPE;
+    if (T > (1 << 24) || window > (1 << 29) || sinks > (1 << 29) || B > 65535 || H > 65535) return LLATTN_ERR_UNSUPPORTED_SHAPE;
     return 0;
 }
 int padded(int T) { return (T + TILE - 1) / TILE * TILE; }
@@ -220,10 +168,10 @@ int llattn_window_fwd(const void* q, const void* k, const void* v, void* o, floa
     p.out = (win::bf16*)o;
     p.lse = lse;
     win::shape(p, workspace, B, T, H, G, window, sinks, scale);
-    if (!win::maps(p, q, k, v, K)) return LLATTN_ERR_TENSOR_MAP;
     cudaStream_t st = (cudaStream_t)stream;
-    const cudaError_t e = cudaMemsetAsync(workspace, 0, 4, st);
+    const cudaError_t e = cudaMemsetAsync(workspace, 0, 4, st);        // (before the maps: the first runtime call of a thread gives it the context that they need)
     if (e != cudaSuccess) return (int)e;
+    if (!win::maps(p, q, k, v, K)) return LLATTN_ERR_TENSOR_MAP;
     return (int)win::forward_tc(p, K, st);
 }
 
@@ -232,12 +180,9 @@ int llattn_window_bwd(const void* q, const void* k, const void* v, const void* o
     const int rc = win::check(B, T, H, G, K, window, sinks, scale);
     if (rc != 0) return rc;
     if (!q || !k || !v || !o || !lse || !d_o || !dq || !dk || !dv) return LLATTN_ERR_NULL;
-    if (misaligned(16, {q, k, v, o, lse, d_o, dq, dk, dv})) return LLATTN_ERR_ALIGNMENT;
+    if (misaligned(16, {q, k, v, o, lse, d_o}) || misaligned(32, {dq, dk, dv})) return LLATTN_ERR_ALIGNMENT;
     if (!workspace || misaligned(256, {workspace}) || workspace_bytes < llattn_window_workspace_bytes(B, T, H)) return LLATTN_ERR_WORKSPACE;
     win::Params p = {};
-    p.q = (const win::bf16*)q;
-    p.k = (const win::bf16*)k;
-    p.v = (const win::bf16*)v;
     p.o = (const win::bf16*)o;
     p.d_o = (const win::bf16*)d_o;
     p.dq = (win::bf16*)dq;
@@ -247,15 +192,10 @@ int llattn_window_bwd(const void* q, const void* k, const void* v, const void* o
     p.delta = reinterpret_cast<float*>(static_cast<char*>(workspace) + 256);
     win::shape(p, workspace, B, T, H, G, window, sinks, scale);
     cudaStream_t st = (cudaStream_t)stream;
-    cudaError_t e = cudaMemsetAsync(workspace, 0, 4, st);
+    const cudaError_t e = cudaMemsetAsync(workspace, 0, 4, st);
     if (e != cudaSuccess) return (int)e;
-    const unsigned rows = (unsigned)(((long)B * T * H + 7) / 8), tokens = (unsigned)(((long)B * T * G + 7) / 8);
-    e = K == 64 ? launch_chained(win::window_dq_kernel<64>, rows, 256, 0, st, p) : launch_chained(win::window_dq_kernel<128>, rows, 256, 0, st, p);
-    if (e != cudaSuccess) return (int)e;
-    LLATTN_LAUNCHED();
-    e = K == 64 ? launch_chained(win::window_dkv_kernel<64>, tokens, 256, 0, st, p) : launch_chained(win::window_dkv_kernel<128>, tokens, 256, 0, st, p);
-    if (e == cudaSuccess) LLATTN_LAUNCHED();
-    return (int)e;
+    if (!win::maps(p, q, k, v, K) || tma::make_seq_map(&p.tdo, d_o, B, T, H, K, win::TILE, 2) != 0) return LLATTN_ERR_TENSOR_MAP;
+    return (int)win::backward_tc(p, K, st);
 }
 
 int llattn_window_fill(const void* k, const void* v, const long long* lengths, void* k_cache, void* v_cache, long long* counts, int B, int T, int G, int K,

@@ -94,6 +94,7 @@ __device__ __forceinline__ void load_tile(unsigned char* dst, const CUtensorMap*
 }
 
 cudaError_t forward_tc(const Params& p, int K, cudaStream_t st);
+cudaError_t backward_tc(const Params& p, int K, cudaStream_t st);
 
 }  // namespace win
 }  // namespace llattn

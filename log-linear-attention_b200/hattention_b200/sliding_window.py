@@ -50,7 +50,7 @@ def _scale(scale: Optional[float], K: int) -> float:
 def sliding_window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int, sinks: int = 0,
                              scale: Optional[float] = None) -> torch.Tensor:
     """o (B,T,H,K) = softmax attention of q (B,T,H,K) over k, v (B,T,G,K), H a multiple of G, each query over the last `window` tokens,
-    itself among them, and the first `sinks`; with gradients.  bf16, K = 64 or 128, any T up to 2^24; scale K^-0.5 unless it is given.
+    itself among them, and the first `sinks`; with gradients.  bf16, K = 64 or 128, any T up to 2^24, B and H up to 65535; scale K^-0.5 unless it is given.
     A window of T or more is plain causal attention.
 
     Values of tokens that a query does not see reach it as 0 times themselves where they share a tile with ones that it sees: a batch

@@ -270,6 +270,28 @@ def test_refusals_on_the_gpu():
         sliding_window_step(s._replace(k=s.k.transpose(0, 1).contiguous().transpose(0, 1)), q[:, 0], k[:, 0], v[:, 0])
 
 
+def test_calls_and_errors_of_a_thread():
+    """A fresh thread makes the same calls, and gets an exception for one that the C entry refuses."""
+    import threading
+    from hattention_b200 import sliding_window_attention
+    q, k, v, _ = make(1, 150, 2, 1, 64)
+    many = torch.zeros(65536, 1, 1, 64, device="cuda", dtype=torch.bfloat16)
+    got = []
+
+    def call():
+        got.append(sliding_window_attention(q, k, v, 50, 1))
+        for _ in range(2):
+            with pytest.raises(ValueError):
+                sliding_window_attention(many, many, many, 1)
+        got.append("refused")
+    thread = threading.Thread(target=call)
+    thread.start()
+    thread.join()
+    assert len(got) == 2 and torch.equal(got[0], sliding_window_attention(q, k, v, 50, 1))
+    with pytest.raises(ValueError):
+        sliding_window_attention(many, many, many, 1)
+
+
 def test_empty_operands():
     from hattention_b200 import sliding_window_attention, sliding_window_prefill
     q = torch.zeros(2, 0, 4, 64, device="cuda", dtype=torch.bfloat16, requires_grad=True)
