@@ -4,43 +4,12 @@
 //     dV_s = sum_t P_ts do_t,   dS_ts = P_ts (do_t . v_s - delta_t),   dQ_t = scale sum_s dS_ts k_s,   dK_s = scale sum_t dS_ts q_t.
 // H query heads share G heads of k and v: dK and dV are sums over the H / G heads too.
 //
-// Here: the C entries, the cache of a decoding sequence, the step.  Forward: window_fwd_tc.cu, backward: window_bwd_tc.cu.
+// Here: the C entries and the cache of a decoding sequence.  Forward: window_fwd_tc.cu, backward: window_bwd_tc.cu, steps: window_step.cu.
 #include "../../include/llattn.h"
 #include "window.cuh"
 
 namespace llattn {
 namespace win {
-
-template <int K>
-struct Lanes {
-    static constexpr int N = K / 32;
-    float v[N];
-    __device__ __forceinline__ void zero() {
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = 0.f;
-    }
-    __device__ __forceinline__ void load(const bf16* row, int lane) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = __bfloat162float(row[lane + 32 * i]);
-    }
-    __device__ __forceinline__ void store(bf16* row, int lane, float f) const {
-#pragma unroll
-        for (int i = 0; i < N; ++i) row[lane + 32 * i] = __float2bfloat16(v[i] * f);
-    }
-    __device__ __forceinline__ void add(float f, const Lanes& x) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = fmaf(f, x.v[i], v[i]);
-    }
-};
-template <int K>
-__device__ __forceinline__ float dot(const Lanes<K>& a, const Lanes<K>& b) {
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < Lanes<K>::N; ++i) s = fmaf(a.v[i], b.v[i], s);
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-    return s;
-}
 
 // Slot c of a sequence of n tokens holds token c if c < sinks, else the last token that is c modulo the window, counted from the end of the sinks; zeros where there is none.
 template <int K>
@@ -64,58 +33,6 @@ __global__ void __launch_bounds__(256) window_fill_kernel(const bf16* k, const b
     }
     reinterpret_cast<uint4*>(kc)[(long)b * slots * words + i] = kw;
     reinterpret_cast<uint4*>(vc)[(long)b * slots * words + i] = vw;
-}
-
-template <int K>
-__global__ void __launch_bounds__(256) window_step_kernel(const bf16* q, const bf16* k, const bf16* v, bf16* kc, bf16* vc, long long* counts, bf16* o, int H,
-                                                          int G, int window, int sinks, float scale) {
-    chain_wait();
-    __shared__ float part[8][K + 2];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, grp = blockIdx.x % G, b = blockIdx.x / G, R = H / G;
-    const long long seen = counts[blockIdx.x] > 0 ? counts[blockIdx.x] : 0;
-    const int slots = sinks + window, slot = (int)(seen < sinks ? seen : sinks + (seen - sinks) % window), held = (int)min((long long)slots, seen + 1);
-    const long ld = (long)G * K;
-    bf16 *kb = kc + (long)b * slots * ld + grp * K, *vb = vc + (long)b * slots * ld + grp * K;
-    if (threadIdx.x < K) {
-        kb[slot * ld + threadIdx.x] = k[(long)blockIdx.x * K + threadIdx.x];
-        vb[slot * ld + threadIdx.x] = v[(long)blockIdx.x * K + threadIdx.x];
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) counts[blockIdx.x] = seen + 1;
-    for (int h = grp * R; h < grp * R + R; ++h) {
-        Lanes<K> x, y, acc;
-        x.load(q + ((long)b * H + h) * K, lane);
-        acc.zero();
-        float m = -INFINITY, sum = 0.f;
-        for (int c = warp; c < held; c += 8) {
-            y.load(kb + c * ld, lane);
-            const float z = dot<K>(x, y) * scale, n = fmaxf(m, z), f = __expf(m - n), e = __expf(z - n);
-            y.load(vb + c * ld, lane);
-#pragma unroll
-            for (int j = 0; j < Lanes<K>::N; ++j) acc.v[j] *= f;
-            acc.add(e, y);
-            sum = sum * f + e;
-            m = n;
-        }
-#pragma unroll
-        for (int j = 0; j < Lanes<K>::N; ++j) part[warp][lane + 32 * j] = acc.v[j];
-        if (lane == 0) {
-            part[warp][K] = m;
-            part[warp][K + 1] = sum;
-        }
-        __syncthreads();
-        if (threadIdx.x < K) {
-            float top = -INFINITY, total = 0.f, r = 0.f;
-            for (int w = 0; w < 8; ++w) top = fmaxf(top, part[w][K]);
-            for (int w = 0; w < 8; ++w) {
-                const float f = __expf(part[w][K] - top);
-                total = fmaf(f, part[w][K + 1], total);
-                r = fmaf(f, part[w][threadIdx.x], r);
-            }
-            o[((long)b * H + h) * K + threadIdx.x] = __float2bfloat16(r / total);
-        }
-        __syncthreads();
-    }
 }
 
 int check(long B, long T, long H, long G, int K, long window, long sinks, float scale) {
@@ -222,11 +139,8 @@ int llattn_window_step(const void* q, const void* k, const void* v, void* k_cach
     if (!q || !k || !v || !k_cache || !v_cache || !counts || !o) return LLATTN_ERR_NULL;
     if (misaligned(16, {q, k, v, k_cache, v_cache, counts, o})) return LLATTN_ERR_ALIGNMENT;
     cudaStream_t st = (cudaStream_t)stream;
-    const auto kern = K == 64 ? win::window_step_kernel<64> : win::window_step_kernel<128>;
-    const cudaError_t e = launch_chained(kern, (unsigned)(B * G), 256, 0, st, (const win::bf16*)q, (const win::bf16*)k, (const win::bf16*)v, (win::bf16*)k_cache,
-                                         (win::bf16*)v_cache, counts, (win::bf16*)o, H, G, window, sinks, scale);
-    if (e == cudaSuccess) LLATTN_LAUNCHED();
-    return (int)e;
+    return (int)win::decode_step((const win::bf16*)q, (const win::bf16*)k, (const win::bf16*)v, (win::bf16*)k_cache, (win::bf16*)v_cache, counts, (win::bf16*)o, B, H, G, K,
+                                 window, sinks, scale, st);
 }
 
 }  // extern "C"

@@ -95,6 +95,8 @@ __device__ __forceinline__ void load_tile(unsigned char* dst, const CUtensorMap*
 
 cudaError_t forward_tc(const Params& p, int K, cudaStream_t st);
 cudaError_t backward_tc(const Params& p, int K, cudaStream_t st);
+cudaError_t decode_step(const bf16* q, const bf16* k, const bf16* v, bf16* kc, bf16* vc, long long* counts, bf16* o, int B, int H, int G, int K, int window,
+                        int sinks, float scale, cudaStream_t st);
 
 }  // namespace win
 }  // namespace llattn
