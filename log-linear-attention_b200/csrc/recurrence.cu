@@ -5,7 +5,9 @@
 //
 // A run of tokens acts on a state as h -> A h + H, with A the product of its decays and H its own final state, and on e in the same form
 // from its other end; runs compose.  A warp takes RUN tokens of 32 VEC neighbouring channels, a CTA the runs of a tile of TILE tokens, and walks the
-// tiles of its strip of channels: one pass over the data, all sums in fp32, in an order that the sizes alone decide.
+// tiles of its strip of channels: one pass over the data, all sums in fp32, in an order that the sizes alone decide.  Where there are fewer strips than the
+// chip has room for, a cluster of CTAs takes neighbouring tiles of a strip at once and exchanges the tiles' (A, H) through shared memory, a barrier for all of them.
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -16,7 +18,8 @@ namespace llattn {
 namespace rec {
 
 typedef __nv_bfloat16 bf16;
-constexpr int WARPS = 8, RUN = 16, TILE = WARPS * RUN;
+namespace cg = cooperative_groups;
+constexpr int WARPS = 8, RUN = 16, TILE = WARPS * RUN, MAX_RANKS = 16;
 
 struct Params {
     const void *x, *g, *d_o;
@@ -74,26 +77,52 @@ __device__ __forceinline__ void load_run(const E* p, long ld, int left, bool the
     }
 }
 
+// A tile's (A, H) to every CTA of the cluster: warp w writes those of ranks w and w + 8.
+template <int VEC>
+__device__ __forceinline__ void publish(cg::cluster_group& cluster, float2 (*slot)[VEC], int ranks, int warp, int lane, const float (&A)[VEC], const float (&H)[VEC]) {
+    for (int x = warp; x < ranks; x += WARPS) {
+        float2* to = cluster.map_shared_rank(&slot[lane][0], x);
+#pragma unroll
+        for (int u = 0; u < VEC; ++u) to[u] = make_float2(A[u], H[u]);
+    }
+}
+// Takes `carry` over the cluster's tiles, in the order of the ranks; `mine` is what reaches this CTA's.
+template <int VEC>
+__device__ __forceinline__ void over_ranks(const float2 (*all)[32][VEC], int ranks, int rank, int lane, float (&carry)[VEC], float (&mine)[VEC]) {
+    for (int x = 0; x < ranks; ++x)
+#pragma unroll
+        for (int u = 0; u < VEC; ++u) {
+            const float2 r = all[x][lane][u];
+            if (x == rank) mine[u] = carry[u];
+            carry[u] = fmaf(r.x, carry[u], r.y);
+        }
+}
+
 template <typename X, typename G, int VEC>
 __global__ void __launch_bounds__(32 * WARPS, 2) recurrence_fwd_kernel(const __grid_constant__ Params p) {
     chain_wait();
-    __shared__ float2 agg[2][WARPS][32][VEC];             // (A, H) of the warps' runs, for every other tile
+    __shared__ float2 agg[2][WARPS][32][VEC];             // (A, H) of the warps' runs, for every other round
+    __shared__ float2 all[2][MAX_RANKS][32][VEC];         // of the cluster's tiles
+    cg::cluster_group cluster = cg::this_cluster();
+    const int ranks = cluster.num_blocks(), rank = cluster.block_rank(), unit = blockIdx.x / ranks;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int b = blockIdx.x / p.strips, c = (blockIdx.x % p.strips * 32 + lane) * VEC;
+    const int b = unit / p.strips, c = (unit % p.strips * 32 + lane) * VEC;
     const bool there = c < p.D;
     const long ld = p.D, base = (long)b * p.T * ld + c;
     const X* x = static_cast<const X*>(p.x) + base;
     const G* g = static_cast<const G*>(p.g) + base;
     X* o = static_cast<X*>(p.o) + base;
+    if (ranks > 1) cluster.sync();                        // every CTA is there to be written to
     float carry[VEC];
 #pragma unroll
     for (int u = 0; u < VEC; ++u) carry[u] = p.h0 && there ? p.h0[(long)b * p.D + c + u] : 0.f;
-    for (int tile = 0; tile < p.NT; ++tile) {
-        const int t0 = tile * TILE + warp * RUN, left = p.T - t0;
+    int par = 0;
+    for (int first = 0; first < p.NT; first += ranks, par ^= 1) {
+        const int tile = first + rank, t0 = tile * TILE + warp * RUN, left = p.T - t0;      // (a tile behind the last changes nothing)
         float v[RUN][VEC], a[RUN][VEC];
         load_run<X, VEC>(x + (long)t0 * ld, ld, left, there, 0.f, v);
         load_run<G, VEC>(g + (long)t0 * ld, ld, left, there, 0.f, a);
-        float A[VEC], H[VEC], h[VEC];
+        float A[VEC], H[VEC], h[VEC], mine[VEC];
 #pragma unroll
         for (int u = 0; u < VEC; ++u) {
             A[u] = 1.f;
@@ -108,17 +137,45 @@ __global__ void __launch_bounds__(32 * WARPS, 2) recurrence_fwd_kernel(const __g
                 H[u] = fmaf(a[i][u], H[u], v[i][u]);
             }
 #pragma unroll
-        for (int u = 0; u < VEC; ++u) agg[tile & 1][warp][lane][u] = make_float2(A[u], H[u]);
+        for (int u = 0; u < VEC; ++u) agg[par][warp][lane][u] = make_float2(A[u], H[u]);
         __syncthreads();
-        if (p.starts && warp == 0 && there) Row<float, VEC>::store(p.starts + ((long)b * p.NT + tile) * p.D + c, carry);
+        if (ranks == 1) {
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w)
+            for (int u = 0; u < VEC; ++u) mine[u] = carry[u];
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w)
+#pragma unroll
+                for (int u = 0; u < VEC; ++u) {
+                    const float2 r = agg[par][w][lane][u];
+                    if (w == warp) h[u] = carry[u];
+                    carry[u] = fmaf(r.x, carry[u], r.y);
+                }
+        } else {
+            float Ab[VEC], Hb[VEC];                       // of the runs before this warp's; then of the tile
 #pragma unroll
             for (int u = 0; u < VEC; ++u) {
-                const float2 r = agg[tile & 1][w][lane][u];
-                if (w == warp) h[u] = carry[u];
-                carry[u] = fmaf(r.x, carry[u], r.y);
+                A[u] = 1.f;
+                H[u] = 0.f;
             }
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w)
+#pragma unroll
+                for (int u = 0; u < VEC; ++u) {
+                    const float2 r = agg[par][w][lane][u];
+                    if (w == warp) {
+                        Ab[u] = A[u];
+                        Hb[u] = H[u];
+                    }
+                    A[u] *= r.x;
+                    H[u] = fmaf(r.x, H[u], r.y);
+                }
+            publish<VEC>(cluster, all[par][rank], ranks, warp, lane, A, H);
+            cluster.sync();
+            over_ranks<VEC>(all[par], ranks, rank, lane, carry, mine);
+#pragma unroll
+            for (int u = 0; u < VEC; ++u) h[u] = fmaf(Ab[u], mine[u], Hb[u]);
+        }
+        if (p.starts && warp == 0 && there && tile < p.NT) Row<float, VEC>::store(p.starts + ((long)b * p.NT + tile) * p.D + c, mine);
         if (there) {
 #pragma unroll
             for (int i = 0; i < RUN; ++i) {
@@ -130,15 +187,19 @@ __global__ void __launch_bounds__(32 * WARPS, 2) recurrence_fwd_kernel(const __g
             }
         }
     }
-    if (p.h_last && warp == 0 && there) Row<float, VEC>::store(p.h_last + (long)b * p.D + c, carry);
+    if (p.h_last && rank == 0 && warp == 0 && there) Row<float, VEC>::store(p.h_last + (long)b * p.D + c, carry);
 }
 
+// The same from the other end: e takes the place of the state, the cluster's tiles are counted from the last one.
 template <typename X, typename G, int VEC>
 __global__ void __launch_bounds__(32 * WARPS, 2) recurrence_bwd_kernel(const __grid_constant__ Params p) {
     chain_wait();
     __shared__ float agg[2][3][WARPS][32][VEC];           // A, H and E of the warps' runs
+    __shared__ float2 all[2][MAX_RANKS][32][VEC];
+    cg::cluster_group cluster = cg::this_cluster();
+    const int ranks = cluster.num_blocks(), rank = cluster.block_rank(), unit = blockIdx.x / ranks;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int b = blockIdx.x / p.strips, c = (blockIdx.x % p.strips * 32 + lane) * VEC;
+    const int b = unit / p.strips, c = (unit % p.strips * 32 + lane) * VEC;
     const bool there = c < p.D;
     const long ld = p.D, base = (long)b * p.T * ld + c;
     const X* x = static_cast<const X*>(p.x) + base;
@@ -146,21 +207,23 @@ __global__ void __launch_bounds__(32 * WARPS, 2) recurrence_bwd_kernel(const __g
     const X* d_o = static_cast<const X*>(p.d_o) + base;
     X* dx = static_cast<X*>(p.dx) + base;
     G* dg = static_cast<G*>(p.dg) + base;
+    if (ranks > 1) cluster.sync();
     float carry[VEC];
 #pragma unroll
     for (int u = 0; u < VEC; ++u) carry[u] = p.h0 && there ? p.h0[(long)b * p.D + c + u] : 0.f;
-    for (int tile = p.NT - 1; tile >= 0; --tile) {
-        const int t0 = tile * TILE + warp * RUN, left = p.T - t0, par = tile & 1;
+    int par = 0;
+    for (int first = p.NT - 1; first >= 0; first -= ranks, par ^= 1) {
+        const int tile = first - rank, t0 = tile * TILE + warp * RUN, left = tile < 0 ? 0 : p.T - t0;
         float v[RUN][VEC], a[RUN][VEC], d[RUN][VEC];
         load_run<X, VEC>(x + (long)t0 * ld, ld, left, there, 0.f, v);
         load_run<G, VEC>(g + (long)t0 * ld, ld, left, there, 0.f, a);
         load_run<X, VEC>(d_o + (long)t0 * ld, ld, left, there, 0.f, d);
-        float A[VEC], H[VEC], E[VEC], h[VEC], e[VEC];
+        float A[VEC], H[VEC], E[VEC], h[VEC], e[VEC], mine[VEC];
 #pragma unroll
         for (int u = 0; u < VEC; ++u) {
             A[u] = 1.f;
             H[u] = E[u] = 0.f;
-            h[u] = there ? p.starts[((long)b * p.NT + tile) * p.D + c + u] : 0.f;
+            h[u] = there && tile >= 0 ? p.starts[((long)b * p.NT + tile) * p.D + c + u] : 0.f;
         }
 #pragma unroll
         for (int i = 0; i < RUN; ++i)
@@ -182,15 +245,40 @@ __global__ void __launch_bounds__(32 * WARPS, 2) recurrence_bwd_kernel(const __g
         }
         __syncthreads();
 #pragma unroll
-        for (int u = 0; u < VEC; ++u) {
+        for (int u = 0; u < VEC; ++u)
 #pragma unroll
             for (int w = 0; w < WARPS; ++w)
                 if (w < warp) h[u] = fmaf(agg[par][0][w][lane][u], h[u], agg[par][1][w][lane][u]);
+        if (ranks == 1) {
 #pragma unroll
-            for (int w = WARPS - 1; w >= 0; --w) {
-                if (w == warp) e[u] = carry[u];
-                carry[u] = fmaf(agg[par][0][w][lane][u], carry[u], agg[par][2][w][lane][u]);
+            for (int u = 0; u < VEC; ++u)
+#pragma unroll
+                for (int w = WARPS - 1; w >= 0; --w) {
+                    if (w == warp) e[u] = carry[u];
+                    carry[u] = fmaf(agg[par][0][w][lane][u], carry[u], agg[par][2][w][lane][u]);
+                }
+        } else {
+            float Ab[VEC], Eb[VEC];                       // of the runs behind this warp's; then of the tile
+#pragma unroll
+            for (int u = 0; u < VEC; ++u) {
+                A[u] = 1.f;
+                E[u] = 0.f;
+#pragma unroll
+                for (int w = WARPS - 1; w >= 0; --w) {
+                    const float aw = agg[par][0][w][lane][u];
+                    if (w == warp) {
+                        Ab[u] = A[u];
+                        Eb[u] = E[u];
+                    }
+                    A[u] *= aw;
+                    E[u] = fmaf(aw, E[u], agg[par][2][w][lane][u]);
+                }
             }
+            publish<VEC>(cluster, all[par][rank], ranks, warp, lane, A, E);
+            cluster.sync();
+            over_ranks<VEC>(all[par], ranks, rank, lane, carry, mine);
+#pragma unroll
+            for (int u = 0; u < VEC; ++u) e[u] = fmaf(Ab[u], mine[u], Eb[u]);
         }
         // the states before the run's tokens, in the place of x
 #pragma unroll
@@ -218,7 +306,7 @@ __global__ void __launch_bounds__(32 * WARPS, 2) recurrence_bwd_kernel(const __g
             }
         }
     }
-    if (p.h_last && warp == 0 && there) Row<float, VEC>::store(p.h_last + (long)b * p.D + c, carry);
+    if (p.h_last && rank == 0 && warp == 0 && there) Row<float, VEC>::store(p.h_last + (long)b * p.D + c, carry);
 }
 
 template <typename X, typename G>
@@ -234,18 +322,42 @@ __global__ void __launch_bounds__(256) recurrence_step_kernel(float* h, const X*
     Row<X, 1>::store(o + i, v);
 }
 
+// Clusters of as many CTAs as fill the chip twice over, and no more than there are tiles.
+inline int ranks_of(long units, int NT) {
+    int n = 1;
+    while (n < MAX_RANKS && 2 * n <= NT && units * n < 2 * 148) n *= 2;
+    return n;
+}
+template <typename KernT>
+cudaError_t launch(KernT kern, const Params& p, long units, cudaStream_t st) {
+    const int n = ranks_of(units, p.NT);
+    if (n > 8) {
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e != cudaSuccess) return e;
+    }
+    cudaLaunchAttribute attr[2] = {};
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = n;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(units * n));
+    cfg.blockDim = dim3(32 * WARPS);
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
+    if (e == cudaSuccess) LLATTN_LAUNCHED();
+    return e;
+}
 template <typename X, typename G>
 cudaError_t scan(bool backward, Params p, int B, cudaStream_t st) {
     const bool pairs = p.D % 2 == 0;
     p.strips = (p.D + (pairs ? 64 : 32) - 1) / (pairs ? 64 : 32);
-    const unsigned grid = (unsigned)(B * p.strips);
-    cudaError_t e;
-    if (backward)
-        e = pairs ? launch_chained(recurrence_bwd_kernel<X, G, 2>, grid, 32 * WARPS, 0, st, p) : launch_chained(recurrence_bwd_kernel<X, G, 1>, grid, 32 * WARPS, 0, st, p);
-    else
-        e = pairs ? launch_chained(recurrence_fwd_kernel<X, G, 2>, grid, 32 * WARPS, 0, st, p) : launch_chained(recurrence_fwd_kernel<X, G, 1>, grid, 32 * WARPS, 0, st, p);
-    if (e == cudaSuccess) LLATTN_LAUNCHED();
-    return e;
+    const long units = (long)B * p.strips;
+    if (backward) return pairs ? launch(recurrence_bwd_kernel<X, G, 2>, p, units, st) : launch(recurrence_bwd_kernel<X, G, 1>, p, units, st);
+    return pairs ? launch(recurrence_fwd_kernel<X, G, 2>, p, units, st) : launch(recurrence_fwd_kernel<X, G, 1>, p, units, st);
 }
 int scan_of(bool backward, int x_f32, int g_f32, const Params& p, int B, void* stream) {
     cudaStream_t st = (cudaStream_t)stream;
