@@ -4,9 +4,12 @@
 //     dh_t = do_t + e_{t+1},   dx_t = dh_t,   dg_t = e_t h_{t-1},   dh_0 = e_1.
 //
 // A run of tokens acts on a state as h -> A h + H, with A the product of its decays and H its own final state, and on e in the same form
-// from its other end; runs compose.  A warp takes RUN tokens of 32 VEC neighbouring channels, a CTA the runs of a tile of TILE tokens, and walks the
-// tiles of its strip of channels: one pass over the data, all sums in fp32, in an order that the sizes alone decide.  Where there are fewer strips than the
-// chip has room for, a cluster of CTAs takes neighbouring tiles of a strip at once and exchanges the tiles' (A, H) through shared memory, a barrier for all of them.
+// from its other end; runs compose.  A warp takes RUN tokens of 32 VEC neighbouring channels, a CTA the runs of a tile of TILE tokens, a cluster of CTAs
+// neighbouring tiles of a strip of channels, and the cluster walks the strip: one pass over the data, all sums in fp32, in an order that the sizes alone decide.
+//
+// It is bound by memory as long as little else is issued.  Tiles come to shared memory by asynchronous copies a round ahead, each warp its own rows, and are
+// read, and their decays formed, once.  A cluster's barrier costs its CTAs about a microsecond a round, hence runs as long as registers and shared memory
+// leave room for with two CTAs an SM, and clusters no larger than fill the chip.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -19,16 +22,26 @@ namespace rec {
 
 typedef __nv_bfloat16 bf16;
 namespace cg = cooperative_groups;
-constexpr int WARPS = 8, RUN = 16, TILE = WARPS * RUN, MAX_RANKS = 16;
+constexpr int WARPS = 8, SLOTS = 2, MAX_RANKS = 16;
+constexpr int FWD_RUN = 16, BWD_RUN = 8;         // (three tensors: 16 tokens leave room for one CTA an SM)
+constexpr int STATES = 64;                       // tokens from one state that the forward keeps to the next
 
 struct Params {
     const void *x, *g, *d_o;
     const float* h0;          // (B,D) or null: zeros.  Backward: the gradient of the last state, or null
     void *o, *dx, *dg;
     float* h_last;            // (B,D) or null.  Backward: the gradient of the initial state, or null
-    float* starts;            // (B,NT,D) or null: the state before every tile
-    int T, D, NT, strips;     // strips of channels a sequence
+    float* starts;            // (B, ceil(T / STATES), D) or null: the state before every STATES-th token
+    int T, D, strips;         // strips of channels a sequence
 };
+
+// exp(g): a multiplication and ex2.approx, 2^-22 of the value at most and 4e-8 (rms) where decays are (g in (-1,0)); expf has 3.5e-8 there for four times the
+// instructions, which the tiles that come from memory at full rate leave no room for
+__device__ __forceinline__ float decay(float g) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(g * 1.4426950408889634f));
+    return y;
+}
 
 template <typename E, int VEC>
 struct Row;
@@ -63,95 +76,163 @@ struct Row<float, 2> {
     static __device__ __forceinline__ void store(float* p, const float (&v)[2]) { *reinterpret_cast<float2*>(p) = make_float2(v[0], v[1]); }
 };
 
-// RUN tokens from t0 on; tokens at or behind `left` and absent channels read as `fill`
-template <typename E, int VEC>
-__device__ __forceinline__ void load_run(const E* p, long ld, int left, bool there, float fill, float (&v)[RUN][VEC]) {
+// A warp's RUN rows of 32 VEC values of a tensor in shared memory, brought there by asynchronous copies of CP bytes (0: by loads and stores); what lies behind
+// the sequence or the channels is filled with zeros, which change nothing (a decay of 1, nothing added).
+template <int RUN, typename E, int VEC, int CP>
+struct Stage {
+    static constexpr int ROW = 32 * VEC * sizeof(E), BYTES = RUN * ROW;
+    // `src`: row 0, channel 0 of the strip (read where `left` > 0 alone); `cols` channels and `left` tokens are there
+    static __device__ __forceinline__ void issue(unsigned char* dst, const E* src, long ld, int left, int cols, int lane) {
+        if constexpr (CP == 0) {
+            static_assert(VEC == 1, "a value a lane");
+            E v[RUN];
 #pragma unroll
-    for (int i = 0; i < RUN; ++i) {
-        if (there && i < left) {
-            Row<E, VEC>::load(p + i * ld, v[i]);
+            for (int i = 0; i < RUN; ++i) v[i] = i < left && lane < cols ? src[i * ld + lane] : E(0.f);
+#pragma unroll
+            for (int i = 0; i < RUN; ++i) reinterpret_cast<E*>(dst + i * ROW)[lane] = v[i];
         } else {
+            constexpr int PER = CP / (int)sizeof(E), A_ROW = ROW / CP, N = RUN * A_ROW / 32;              // values a copy, copies a row, copies a lane
+            static_assert(32 % A_ROW == 0, "a copy of the warp takes whole rows");
+            const int row = lane / A_ROW, at = lane % A_ROW * PER;
+            const uint32_t to = (uint32_t)__cvta_generic_to_shared(dst + lane * CP);
+            const E* from = src + row * ld + at;
+            if (left >= RUN && cols == 32 * VEC) {                                                        // most tiles: nothing to test
 #pragma unroll
-            for (int u = 0; u < VEC; ++u) v[i][u] = fill;
+                for (int i = 0; i < N; ++i, from += 32 / A_ROW * ld) copy(to + i * 32 * CP, from, CP);
+            } else {
+#pragma unroll
+                for (int i = 0; i < N; ++i, from += 32 / A_ROW * ld) {
+                    const bool in = row + i * (32 / A_ROW) < left && at < cols;                           // (cols is a multiple of PER)
+                    copy(to + i * 32 * CP, in ? from : src, in ? CP : 0);
+                }
+            }
         }
     }
-}
-
-// A tile's (A, H) to every CTA of the cluster: warp w writes those of ranks w and w + 8.
-template <int VEC>
-__device__ __forceinline__ void publish(cg::cluster_group& cluster, float2 (*slot)[VEC], int ranks, int warp, int lane, const float (&A)[VEC], const float (&H)[VEC]) {
-    for (int x = warp; x < ranks; x += WARPS) {
-        float2* to = cluster.map_shared_rank(&slot[lane][0], x);
-#pragma unroll
-        for (int u = 0; u < VEC; ++u) to[u] = make_float2(A[u], H[u]);
+    // `bytes` of CP bytes (a constant where nothing was tested); the rest are zeros
+    static __device__ __forceinline__ void copy(uint32_t to, const E* from, int bytes) {
+        if constexpr (CP == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+        else if constexpr (CP > 0) asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;\n" ::"r"(to), "l"(from), "n"(CP), "r"(bytes) : "memory");
     }
-}
-// Takes `carry` over the cluster's tiles, in the order of the ranks; `mine` is what reaches this CTA's.
-template <int VEC>
-__device__ __forceinline__ void over_ranks(const float2 (*all)[32][VEC], int ranks, int rank, int lane, float (&carry)[VEC], float (&mine)[VEC]) {
-    for (int x = 0; x < ranks; ++x)
+    static __device__ __forceinline__ void read(const unsigned char* at, int lane, float (&v)[RUN][VEC]) {
 #pragma unroll
-        for (int u = 0; u < VEC; ++u) {
-            const float2 r = all[x][lane][u];
-            if (x == rank) mine[u] = carry[u];
-            carry[u] = fmaf(r.x, carry[u], r.y);
-        }
+        for (int i = 0; i < RUN; ++i) Row<E, VEC>::load(reinterpret_cast<const E*>(at + i * ROW) + lane * VEC, v[i]);
+    }
+};
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_but() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory"); }
+template <int RUN, int VEC>
+__device__ __forceinline__ void decays(float (&a)[RUN][VEC]) {
+#pragma unroll
+    for (int i = 0; i < RUN; ++i)
+#pragma unroll
+        for (int u = 0; u < VEC; ++u) a[i][u] = decay(a[i][u]);
 }
 
-template <typename X, typename G, int VEC>
+// Where a CTA is, and what forward and backward do alike.
+template <int VEC, int TILE>
+struct Place {
+    cg::cluster_group cluster;
+    int ranks, rank, lane, warp, b, c0, c, cols, NT, rounds;
+    bool there;
+    float2 (*all)[32][VEC];       // [2][ranks]: the cluster's tiles' (A, H) of every other round
+    __device__ Place(const Params& p, unsigned char* behind_slots) : cluster(cg::this_cluster()) {
+        ranks = cluster.num_blocks();
+        rank = cluster.block_rank();
+        lane = threadIdx.x & 31;
+        warp = threadIdx.x >> 5;
+        const int unit = blockIdx.x / ranks;
+        b = unit / p.strips;
+        c0 = unit % p.strips * 32 * VEC;
+        c = c0 + lane * VEC;
+        cols = min(32 * VEC, p.D - c0);
+        there = c < p.D;
+        NT = (p.T + TILE - 1) / TILE;
+        rounds = (NT + ranks - 1) / ranks;
+        all = reinterpret_cast<float2(*)[32][VEC]>(behind_slots);
+    }
+    // a round's (A, H) of this CTA's tile to every CTA of the cluster: warp w writes those of ranks w and w + 8
+    __device__ __forceinline__ void publish(int round, const float (&A)[VEC], const float (&H)[VEC]) {
+        for (int x = warp; x < ranks; x += WARPS) {
+            float2* to = cluster.map_shared_rank(&all[(round & 1) * ranks + rank][lane][0], x);
+#pragma unroll
+            for (int u = 0; u < VEC; ++u) to[u] = make_float2(A[u], H[u]);
+        }
+        asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
+    }
+    // takes `carry` over the round's tiles, in the order of the ranks; `mine` is what reaches this CTA's
+    __device__ __forceinline__ void collect(int round, float (&carry)[VEC], float (&mine)[VEC]) {
+        asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+        for (int x = 0; x < ranks; ++x)
+#pragma unroll
+            for (int u = 0; u < VEC; ++u) {
+                const float2 r = all[(round & 1) * ranks + x][lane][u];
+                if (x == rank) mine[u] = carry[u];
+                carry[u] = fmaf(r.x, carry[u], r.y);
+            }
+    }
+};
+
+template <typename X, typename G, int VEC, int CPX, int CPG>
 __global__ void __launch_bounds__(32 * WARPS, 2) recurrence_fwd_kernel(const __grid_constant__ Params p) {
     chain_wait();
-    __shared__ float2 agg[2][WARPS][32][VEC];             // (A, H) of the warps' runs, for every other round
-    __shared__ float2 all[2][MAX_RANKS][32][VEC];         // of the cluster's tiles
-    cg::cluster_group cluster = cg::this_cluster();
-    const int ranks = cluster.num_blocks(), rank = cluster.block_rank(), unit = blockIdx.x / ranks;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int b = unit / p.strips, c = (unit % p.strips * 32 + lane) * VEC;
-    const bool there = c < p.D;
-    const long ld = p.D, base = (long)b * p.T * ld + c;
-    const X* x = static_cast<const X*>(p.x) + base;
-    const G* g = static_cast<const G*>(p.g) + base;
-    X* o = static_cast<X*>(p.o) + base;
-    if (ranks > 1) cluster.sync();                        // every CTA is there to be written to
+    constexpr int RUN = FWD_RUN, TILE = WARPS * RUN;
+    static_assert(STATES % RUN == 0, "states are kept at the starts of runs");
+    using SX = Stage<RUN, X, VEC, CPX>;
+    using SG = Stage<RUN, G, VEC, CPG>;
+    constexpr int BYTES = SX::BYTES + SG::BYTES;
+    extern __shared__ __align__(16) unsigned char staged[];           // [SLOTS][WARPS][BYTES], then Place::all
+    __shared__ float2 agg[2][WARPS][32][VEC];                         // (A, H) of the warps' runs, for every other round
+    Place<VEC, TILE> at(p, staged + SLOTS * WARPS * BYTES);
+    const int lane = at.lane, warp = at.warp;
+    const long ld = p.D, base = (long)at.b * p.T * ld + at.c0;
+    const auto slot = [&](int round) { return staged + (round % SLOTS * WARPS + warp) * BYTES; };
+    const auto bring = [&](int round) {
+        if (round < at.rounds) {
+            const int t0 = (round * at.ranks + at.rank) * TILE + warp * RUN, left = p.T - t0;
+            const long from = base + (left > 0 ? t0 * ld : 0);
+            SX::issue(slot(round), static_cast<const X*>(p.x) + from, ld, left, at.cols, lane);
+            SG::issue(slot(round) + SX::BYTES, static_cast<const G*>(p.g) + from, ld, left, at.cols, lane);
+        }
+        copies_commit();
+    };
+    bring(0);
+    if (at.ranks > 1) at.cluster.sync();                              // every CTA is there to be written to
     float carry[VEC];
 #pragma unroll
-    for (int u = 0; u < VEC; ++u) carry[u] = p.h0 && there ? p.h0[(long)b * p.D + c + u] : 0.f;
-    int par = 0;
-    for (int first = 0; first < p.NT; first += ranks, par ^= 1) {
-        const int tile = first + rank, t0 = tile * TILE + warp * RUN, left = p.T - t0;      // (a tile behind the last changes nothing)
-        float v[RUN][VEC], a[RUN][VEC];
-        load_run<X, VEC>(x + (long)t0 * ld, ld, left, there, 0.f, v);
-        load_run<G, VEC>(g + (long)t0 * ld, ld, left, there, 0.f, a);
-        float A[VEC], H[VEC], h[VEC], mine[VEC];
+    for (int u = 0; u < VEC; ++u) carry[u] = p.h0 && at.there ? p.h0[(long)at.b * p.D + at.c + u] : 0.f;
+    for (int round = 0; round < at.rounds; ++round) {
+        const int t0 = (round * at.ranks + at.rank) * TILE + warp * RUN, left = p.T - t0;      // (a tile behind the last changes nothing)
+        bring(round + 1);                                             // (into the slot of the round before, which all lanes have read)
+        copies_but<1>();
+        __syncwarp();
+        float v[RUN][VEC], a[RUN][VEC], A[VEC], H[VEC], h[VEC];
+        SX::read(slot(round), lane, v);
+        SG::read(slot(round) + SX::BYTES, lane, a);
+        decays<RUN, VEC>(a);
 #pragma unroll
         for (int u = 0; u < VEC; ++u) {
             A[u] = 1.f;
             H[u] = 0.f;
-        }
 #pragma unroll
-        for (int i = 0; i < RUN; ++i)
-#pragma unroll
-            for (int u = 0; u < VEC; ++u) {
-                a[i][u] = expf(a[i][u]);
+            for (int i = 0; i < RUN; ++i) {
                 A[u] *= a[i][u];
                 H[u] = fmaf(a[i][u], H[u], v[i][u]);
             }
-#pragma unroll
-        for (int u = 0; u < VEC; ++u) agg[par][warp][lane][u] = make_float2(A[u], H[u]);
+            agg[round & 1][warp][lane][u] = make_float2(A[u], H[u]);
+        }
         __syncthreads();
-        if (ranks == 1) {
-#pragma unroll
-            for (int u = 0; u < VEC; ++u) mine[u] = carry[u];
+        if (at.ranks == 1) {
 #pragma unroll
             for (int w = 0; w < WARPS; ++w)
 #pragma unroll
                 for (int u = 0; u < VEC; ++u) {
-                    const float2 r = agg[par][w][lane][u];
+                    const float2 r = agg[round & 1][w][lane][u];
                     if (w == warp) h[u] = carry[u];
                     carry[u] = fmaf(r.x, carry[u], r.y);
                 }
         } else {
-            float Ab[VEC], Hb[VEC];                       // of the runs before this warp's; then of the tile
+            float Ab[VEC], Hb[VEC], mine[VEC];                        // of the runs before this warp's; A, H: of the tile
 #pragma unroll
             for (int u = 0; u < VEC; ++u) {
                 A[u] = 1.f;
@@ -161,7 +242,7 @@ __global__ void __launch_bounds__(32 * WARPS, 2) recurrence_fwd_kernel(const __g
             for (int w = 0; w < WARPS; ++w)
 #pragma unroll
                 for (int u = 0; u < VEC; ++u) {
-                    const float2 r = agg[par][w][lane][u];
+                    const float2 r = agg[round & 1][w][lane][u];
                     if (w == warp) {
                         Ab[u] = A[u];
                         Hb[u] = H[u];
@@ -169,79 +250,85 @@ __global__ void __launch_bounds__(32 * WARPS, 2) recurrence_fwd_kernel(const __g
                     A[u] *= r.x;
                     H[u] = fmaf(r.x, H[u], r.y);
                 }
-            publish<VEC>(cluster, all[par][rank], ranks, warp, lane, A, H);
-            cluster.sync();
-            over_ranks<VEC>(all[par], ranks, rank, lane, carry, mine);
+            at.publish(round, A, H);
+            at.collect(round, carry, mine);
 #pragma unroll
             for (int u = 0; u < VEC; ++u) h[u] = fmaf(Ab[u], mine[u], Hb[u]);
         }
-        if (p.starts && warp == 0 && there && tile < p.NT) Row<float, VEC>::store(p.starts + ((long)b * p.NT + tile) * p.D + c, mine);
-        if (there) {
+        if (p.starts && t0 % STATES == 0 && at.there && left > 0)
+            Row<float, VEC>::store(p.starts + ((long)at.b * ((p.T + STATES - 1) / STATES) + t0 / STATES) * p.D + at.c, h);
+        if (at.there) {
+            X* o = static_cast<X*>(p.o) + base + t0 * ld + lane * VEC;
 #pragma unroll
-            for (int i = 0; i < RUN; ++i) {
+            for (int i = 0; i < RUN; ++i, o += ld) {
                 if (i < left) {
 #pragma unroll
                     for (int u = 0; u < VEC; ++u) h[u] = fmaf(a[i][u], h[u], v[i][u]);
-                    Row<X, VEC>::store(o + (long)(t0 + i) * ld, h);
+                    Row<X, VEC>::store(o, h);
                 }
             }
         }
+        __syncwarp();
     }
-    if (p.h_last && rank == 0 && warp == 0 && there) Row<float, VEC>::store(p.h_last + (long)b * p.D + c, carry);
+    if (p.h_last && at.rank == 0 && warp == 0 && at.there) Row<float, VEC>::store(p.h_last + (long)at.b * p.D + at.c, carry);
 }
 
-// The same from the other end: e takes the place of the state, the cluster's tiles are counted from the last one.
-template <typename X, typename G, int VEC>
+// The same from the other end: e takes the place of the state, the cluster's tiles are counted from the last one.  The states before a tile's tokens are
+// made again from the one that the forward kept.
+template <typename X, typename G, int VEC, int CPX, int CPG>
 __global__ void __launch_bounds__(32 * WARPS, 2) recurrence_bwd_kernel(const __grid_constant__ Params p) {
     chain_wait();
-    __shared__ float agg[2][3][WARPS][32][VEC];           // A, H and E of the warps' runs
-    __shared__ float2 all[2][MAX_RANKS][32][VEC];
-    cg::cluster_group cluster = cg::this_cluster();
-    const int ranks = cluster.num_blocks(), rank = cluster.block_rank(), unit = blockIdx.x / ranks;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int b = unit / p.strips, c = (unit % p.strips * 32 + lane) * VEC;
-    const bool there = c < p.D;
-    const long ld = p.D, base = (long)b * p.T * ld + c;
-    const X* x = static_cast<const X*>(p.x) + base;
-    const G* g = static_cast<const G*>(p.g) + base;
-    const X* d_o = static_cast<const X*>(p.d_o) + base;
-    X* dx = static_cast<X*>(p.dx) + base;
-    G* dg = static_cast<G*>(p.dg) + base;
-    if (ranks > 1) cluster.sync();
+    constexpr int RUN = BWD_RUN, TILE = WARPS * RUN;
+    static_assert(TILE % STATES == 0, "a tile starts where a state is kept");
+    using SX = Stage<RUN, X, VEC, CPX>;
+    using SG = Stage<RUN, G, VEC, CPG>;
+    constexpr int BYTES = 2 * SX::BYTES + SG::BYTES;
+    extern __shared__ __align__(16) unsigned char staged[];
+    __shared__ float agg[2][3][WARPS][32][VEC];                       // A, H and E of the warps' runs
+    Place<VEC, TILE> at(p, staged + SLOTS * WARPS * BYTES);
+    const int lane = at.lane, warp = at.warp, NS = (p.T + STATES - 1) / STATES;
+    const long ld = p.D, base = (long)at.b * p.T * ld + at.c0;
+    const auto tile_of = [&](int round) { return at.NT - 1 - round * at.ranks - at.rank; };        // (below 0: nothing there)
+    const auto slot = [&](int round) { return staged + (round % SLOTS * WARPS + warp) * BYTES; };
+    const auto bring = [&](int round) {
+        if (round < at.rounds) {
+            const int tile = tile_of(round), t0 = tile * TILE + warp * RUN, left = tile < 0 ? 0 : p.T - t0;
+            const long from = base + (left > 0 ? t0 * ld : 0);
+            SX::issue(slot(round), static_cast<const X*>(p.x) + from, ld, left, at.cols, lane);
+            SX::issue(slot(round) + SX::BYTES, static_cast<const X*>(p.d_o) + from, ld, left, at.cols, lane);
+            SG::issue(slot(round) + 2 * SX::BYTES, static_cast<const G*>(p.g) + from, ld, left, at.cols, lane);
+        }
+        copies_commit();
+    };
+    bring(0);
+    if (at.ranks > 1) at.cluster.sync();
     float carry[VEC];
 #pragma unroll
-    for (int u = 0; u < VEC; ++u) carry[u] = p.h0 && there ? p.h0[(long)b * p.D + c + u] : 0.f;
-    int par = 0;
-    for (int first = p.NT - 1; first >= 0; first -= ranks, par ^= 1) {
-        const int tile = first - rank, t0 = tile * TILE + warp * RUN, left = tile < 0 ? 0 : p.T - t0;
-        float v[RUN][VEC], a[RUN][VEC], d[RUN][VEC];
-        load_run<X, VEC>(x + (long)t0 * ld, ld, left, there, 0.f, v);
-        load_run<G, VEC>(g + (long)t0 * ld, ld, left, there, 0.f, a);
-        load_run<X, VEC>(d_o + (long)t0 * ld, ld, left, there, 0.f, d);
-        float A[VEC], H[VEC], E[VEC], h[VEC], e[VEC], mine[VEC];
+    for (int u = 0; u < VEC; ++u) carry[u] = p.h0 && at.there ? p.h0[(long)at.b * p.D + at.c + u] : 0.f;
+    for (int round = 0; round < at.rounds; ++round) {
+        const int tile = tile_of(round), t0 = tile * TILE + warp * RUN, left = tile < 0 ? 0 : p.T - t0, par = round & 1;
+        bring(round + 1);
+        float v[RUN][VEC], a[RUN][VEC], d[RUN][VEC], h[VEC], e[VEC];
+#pragma unroll
+        for (int u = 0; u < VEC; ++u) h[u] = at.there && tile >= 0 ? p.starts[((long)at.b * NS + tile * (TILE / STATES)) * p.D + at.c + u] : 0.f;
+        copies_but<1>();
+        __syncwarp();
+        SX::read(slot(round), lane, v);
+        SX::read(slot(round) + SX::BYTES, lane, d);
+        SG::read(slot(round) + 2 * SX::BYTES, lane, a);
+        decays<RUN, VEC>(a);
 #pragma unroll
         for (int u = 0; u < VEC; ++u) {
-            A[u] = 1.f;
-            H[u] = E[u] = 0.f;
-            h[u] = there && tile >= 0 ? p.starts[((long)b * p.NT + tile) * p.D + c + u] : 0.f;
-        }
+            float A = 1.f, H = 0.f, E = 0.f;
 #pragma unroll
-        for (int i = 0; i < RUN; ++i)
-#pragma unroll
-            for (int u = 0; u < VEC; ++u) {
-                a[i][u] = expf(a[i][u]);
-                A[u] *= a[i][u];
-                H[u] = fmaf(a[i][u], H[u], v[i][u]);
+            for (int i = 0; i < RUN; ++i) {
+                A *= a[i][u];
+                H = fmaf(a[i][u], H, v[i][u]);
+                E = a[RUN - 1 - i][u] * (d[RUN - 1 - i][u] + E);
             }
-#pragma unroll
-        for (int i = RUN - 1; i >= 0; --i)
-#pragma unroll
-            for (int u = 0; u < VEC; ++u) E[u] = a[i][u] * (d[i][u] + E[u]);
-#pragma unroll
-        for (int u = 0; u < VEC; ++u) {
-            agg[par][0][warp][lane][u] = A[u];
-            agg[par][1][warp][lane][u] = H[u];
-            agg[par][2][warp][lane][u] = E[u];
+            agg[par][0][warp][lane][u] = A;
+            agg[par][1][warp][lane][u] = H;
+            agg[par][2][warp][lane][u] = E;
         }
         __syncthreads();
 #pragma unroll
@@ -249,7 +336,7 @@ __global__ void __launch_bounds__(32 * WARPS, 2) recurrence_bwd_kernel(const __g
 #pragma unroll
             for (int w = 0; w < WARPS; ++w)
                 if (w < warp) h[u] = fmaf(agg[par][0][w][lane][u], h[u], agg[par][1][w][lane][u]);
-        if (ranks == 1) {
+        if (at.ranks == 1) {
 #pragma unroll
             for (int u = 0; u < VEC; ++u)
 #pragma unroll
@@ -258,7 +345,7 @@ __global__ void __launch_bounds__(32 * WARPS, 2) recurrence_bwd_kernel(const __g
                     carry[u] = fmaf(agg[par][0][w][lane][u], carry[u], agg[par][2][w][lane][u]);
                 }
         } else {
-            float Ab[VEC], Eb[VEC];                       // of the runs behind this warp's; then of the tile
+            float A[VEC], E[VEC], Ab[VEC], Eb[VEC], mine[VEC];        // of the tile; of the runs behind this warp's
 #pragma unroll
             for (int u = 0; u < VEC; ++u) {
                 A[u] = 1.f;
@@ -274,22 +361,24 @@ __global__ void __launch_bounds__(32 * WARPS, 2) recurrence_bwd_kernel(const __g
                     E[u] = fmaf(aw, E[u], agg[par][2][w][lane][u]);
                 }
             }
-            publish<VEC>(cluster, all[par][rank], ranks, warp, lane, A, E);
-            cluster.sync();
-            over_ranks<VEC>(all[par], ranks, rank, lane, carry, mine);
+            at.publish(round, A, E);
+            at.collect(round, carry, mine);
 #pragma unroll
             for (int u = 0; u < VEC; ++u) e[u] = fmaf(Ab[u], mine[u], Eb[u]);
         }
         // the states before the run's tokens, in the place of x
 #pragma unroll
-        for (int i = 0; i < RUN; ++i)
+        for (int u = 0; u < VEC; ++u)
 #pragma unroll
-            for (int u = 0; u < VEC; ++u) {
+            for (int i = 0; i < RUN; ++i) {
                 const float next = fmaf(a[i][u], h[u], v[i][u]);
                 v[i][u] = h[u];
                 h[u] = next;
             }
-        if (there) {
+        if (at.there && left > 0) {
+            const long to = base + t0 * ld + lane * VEC;
+            X* dx = static_cast<X*>(p.dx) + to;
+            G* dg = static_cast<G*>(p.dg) + to;
 #pragma unroll
             for (int i = RUN - 1; i >= 0; --i) {
                 if (i < left) {
@@ -300,13 +389,14 @@ __global__ void __launch_bounds__(32 * WARPS, 2) recurrence_bwd_kernel(const __g
                         e[u] = a[i][u] * dh[u];
                         dgi[u] = e[u] * v[i][u];
                     }
-                    Row<X, VEC>::store(dx + (long)(t0 + i) * ld, dh);
-                    Row<G, VEC>::store(dg + (long)(t0 + i) * ld, dgi);
+                    Row<X, VEC>::store(dx + i * ld, dh);
+                    Row<G, VEC>::store(dg + i * ld, dgi);
                 }
             }
         }
+        __syncwarp();
     }
-    if (p.h_last && rank == 0 && warp == 0 && there) Row<float, VEC>::store(p.h_last + (long)b * p.D + c, carry);
+    if (p.h_last && at.rank == 0 && warp == 0 && at.there) Row<float, VEC>::store(p.h_last + (long)at.b * p.D + at.c, carry);
 }
 
 template <typename X, typename G>
@@ -317,47 +407,75 @@ __global__ void __launch_bounds__(256) recurrence_step_kernel(float* h, const X*
     float v[1], a[1];
     Row<X, 1>::load(x + i, v);
     Row<G, 1>::load(g + i, a);
-    v[0] = fmaf(expf(a[0]), h[i], v[0]);
+    v[0] = fmaf(decay(a[0]), h[i], v[0]);
     h[i] = v[0];
     Row<X, 1>::store(o + i, v);
 }
 
-// Clusters of as many CTAs as fill the chip twice over, and no more than there are tiles.
-inline int ranks_of(long units, int NT) {
-    int n = 1;
-    while (n < MAX_RANKS && 2 * n <= NT && units * n < 2 * 148) n *= 2;
-    return n;
-}
+// Clusters of as many CTAs as there are tiles, and as run at once for all strips: a second wave costs what the first one does.
 template <typename KernT>
-cudaError_t launch(KernT kern, const Params& p, long units, cudaStream_t st) {
-    const int n = ranks_of(units, p.NT);
-    if (n > 8) {
-        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+cudaError_t launch(KernT kern, const Params& p, long units, int NT, size_t smem, size_t tile, cudaStream_t st) {
+    struct Room {
+        int dev;
+        const void* kern;
+        int clusters[MAX_RANKS + 1];          // of n CTAs that the device runs at once (0: not asked yet)
+    };
+    static thread_local Room room = {-1, nullptr, {}};        // (a template's own: one a kernel)
+    int dev;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (room.dev != dev || room.kern != reinterpret_cast<const void*>(kern)) {
+        e = allow_smem(kern, smem + 2 * MAX_RANKS * tile);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e != cudaSuccess) return e;
+        room = Room{dev, reinterpret_cast<const void*>(kern), {}};
     }
     cudaLaunchAttribute attr[2] = {};
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = n;
-    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(units * n));
     cfg.blockDim = dim3(32 * WARPS);
     cfg.stream = st;
     cfg.attrs = attr;
+    int n = NT < MAX_RANKS ? NT : MAX_RANKS;
+    for (;; --n) {
+        attr[0].val.clusterDim.x = n;
+        cfg.gridDim = dim3((unsigned)(units * n));
+        cfg.dynamicSmemBytes = smem + 2 * n * tile;
+        if (n == 1) break;
+        if (units * n > 148 * 8) continue;    // (more than could be there)
+        if (room.clusters[n] == 0) {
+            cfg.numAttrs = 1;
+            e = cudaOccupancyMaxActiveClusters(&room.clusters[n], kern, &cfg);
+            if (e != cudaSuccess) return e;
+            if (room.clusters[n] == 0) room.clusters[n] = -1;
+        }
+        if (room.clusters[n] >= units) break;
+    }
     cfg.numAttrs = 2;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
+    e = cudaLaunchKernelEx(&cfg, kern, p);
     if (e == cudaSuccess) LLATTN_LAUNCHED();
     return e;
 }
-template <typename X, typename G>
-cudaError_t scan(bool backward, Params p, int B, cudaStream_t st) {
-    const bool pairs = p.D % 2 == 0;
-    p.strips = (p.D + (pairs ? 64 : 32) - 1) / (pairs ? 64 : 32);
+// VEC channels a lane; copies of CPX and CPG bytes (0: straight loads)
+template <typename X, typename G, int VEC, int CPX, int CPG>
+cudaError_t scan_as(bool backward, Params p, int B, cudaStream_t st) {
+    p.strips = (p.D + 32 * VEC - 1) / (32 * VEC);
+    const int tile = WARPS * (backward ? BWD_RUN : FWD_RUN), NT = (p.T + tile - 1) / tile;
+    const size_t smem = (size_t)SLOTS * tile * 32 * VEC * ((backward ? 2 : 1) * sizeof(X) + sizeof(G));
     const long units = (long)B * p.strips;
-    if (backward) return pairs ? launch(recurrence_bwd_kernel<X, G, 2>, p, units, st) : launch(recurrence_bwd_kernel<X, G, 1>, p, units, st);
-    return pairs ? launch(recurrence_fwd_kernel<X, G, 2>, p, units, st) : launch(recurrence_fwd_kernel<X, G, 1>, p, units, st);
+    if (backward) return launch(recurrence_bwd_kernel<X, G, VEC, CPX, CPG>, p, units, NT, smem, 32 * VEC * sizeof(float2), st);
+    return launch(recurrence_fwd_kernel<X, G, VEC, CPX, CPG>, p, units, NT, smem, 32 * VEC * sizeof(float2), st);
+}
+// Copies as wide as rows of D values start: 16 bytes where D fills whole words of them, else the pair or the value of a lane.
+template <typename X, typename G>
+cudaError_t scan(bool backward, const Params& p, int B, cudaStream_t st) {
+    if (p.D % (16 / (int)sizeof(X)) == 0) return scan_as<X, G, 2, 16, 16>(backward, p, B, st);
+    if (p.D % 2 == 0) return scan_as<X, G, 2, 2 * sizeof(X), 2 * sizeof(G)>(backward, p, B, st);
+    if (sizeof(X) == 4) return scan_as<X, G, 1, 4, 4>(backward, p, B, st);
+    return scan_as<X, G, 1, 0, 0>(backward, p, B, st);
 }
 int scan_of(bool backward, int x_f32, int g_f32, const Params& p, int B, void* stream) {
     cudaStream_t st = (cudaStream_t)stream;
@@ -382,7 +500,7 @@ extern "C" {
 
 size_t llattn_recurrence_states_bytes(int B, int T, int D) {
     if (rec::check(0, 0, B, T, D) != 0) return 0;
-    return (size_t)B * ((T + rec::TILE - 1) / rec::TILE) * D * sizeof(float);
+    return (size_t)B * ((T + rec::STATES - 1) / rec::STATES) * D * sizeof(float);
 }
 
 int llattn_recurrence_fwd(const void* x, int x_is_f32, const void* g, int g_is_f32, const float* h0, void* o, float* h_last, float* states,
@@ -400,7 +518,6 @@ int llattn_recurrence_fwd(const void* x, int x_is_f32, const void* g, int g_is_f
     p.starts = states;
     p.T = T;
     p.D = D;
-    p.NT = (T + rec::TILE - 1) / rec::TILE;
     return rec::scan_of(false, x_is_f32, g_is_f32, p, B, stream);
 }
 
@@ -421,7 +538,6 @@ int llattn_recurrence_bwd(const void* x, int x_is_f32, const void* g, int g_is_f
     p.starts = const_cast<float*>(states);
     p.T = T;
     p.D = D;
-    p.NT = (T + rec::TILE - 1) / rec::TILE;
     return rec::scan_of(true, x_is_f32, g_is_f32, p, B, stream);
 }
 
