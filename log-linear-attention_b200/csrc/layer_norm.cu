@@ -3,6 +3,12 @@
 //     dx = rstd (z - mean(z) - xhat mean(z xhat)),   z = w dy,  xhat = (x - mean) rstd
 //     dw = sum over rows of dy xhat,   db = sum over rows of dy
 // w absent is ones, b absent zeros.  All sums in fp32; the variance from the differences to the mean.
+//
+// Bound by memory as long as few instructions are issued a value.  CTAs stay on the chip and take rows in turn, LANES lanes a row, which comes two or three rows ahead of
+// its sums by asynchronous copies to shared memory, each lane its own 16-byte words (single values where rows do not start at their boundaries).  A lane sees the same
+// columns of every row: w and b stay in its registers (re-read from L1 for every row they cost bf16 rows more than the rows themselves, 61 us for 32768 x 2048), and dw
+// and db are sums in registers, then over the CTA's rows in shared memory, then over the CTAs in a second kernel, always in the same order.  Arithmetic is
+// on pairs (f32x2).  Rows longer than a CTA's registers hold are read again for each sum, and the column sums are a pass of their own.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -29,43 +35,439 @@ __device__ __forceinline__ float get(const bf16* p) { return __bfloat162float(*p
 __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 __device__ __forceinline__ void put(bf16* p, float v) { *p = __float2bfloat16(v); }
 
-// sums of a and b over the CTA's 256 threads
-__device__ __forceinline__ float2 cta_sum(float a, float b, float2* sh) {
+// ---- one value, or two in one 64-bit register
+struct F2 {
+    unsigned long long v;
+};
+__device__ __forceinline__ F2 pair(float lo, float hi) {
+    F2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ float2 both(F2 a) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
+    return r;
+}
+__device__ __forceinline__ F2 add(F2 a, F2 b) {
+    F2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ F2 mul(F2 a, F2 b) {
+    F2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+    F2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
+__device__ __forceinline__ float add(float a, float b) { return a + b; }
+__device__ __forceinline__ float mul(float a, float b) { return a * b; }
+__device__ __forceinline__ float fma2(float a, float b, float c) { return fmaf(a, b, c); }
+__device__ __forceinline__ float total(F2 a) {
+    const float2 f = both(a);
+    return f.x + f.y;
+}
+__device__ __forceinline__ float total(float a) { return a; }
+template <typename T>
+__device__ __forceinline__ T splat(float a);
+template <>
+__device__ __forceinline__ float splat<float>(float a) { return a; }
+template <>
+__device__ __forceinline__ F2 splat<F2>(float a) { return pair(a, a); }
+
+// VEC neighbouring values of a row as N numbers; VEC is 1 or a multiple of a 16-byte word
+template <int VEC>
+struct Lane {
+    typedef F2 T;
+    static constexpr int N = VEC / 2;
+    static __device__ __forceinline__ void load(const float* p, T (&v)[N]) {
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) {
-        a += __shfl_xor_sync(0xffffffffu, a, d);
-        b += __shfl_xor_sync(0xffffffffu, b, d);
+        for (int i = 0; i < N; i += 2) {
+            const float4 f = *reinterpret_cast<const float4*>(p + 2 * i);
+            v[i] = pair(f.x, f.y);
+            v[i + 1] = pair(f.z, f.w);
+        }
     }
-    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = make_float2(a, b);
-    __syncthreads();
-    float2 s = make_float2(0.f, 0.f);
+    static __device__ __forceinline__ void load(const bf16* p, T (&v)[N]) {
 #pragma unroll
-    for (int w = 0; w < 8; ++w) {
-        s.x += sh[w].x;
-        s.y += sh[w].y;
+        for (int i = 0; i < N; i += 4) {
+            const uint4 q = *reinterpret_cast<const uint4*>(p + 2 * i);
+            const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[i + k] = pair(__uint_as_float(w[k] << 16), __uint_as_float(w[k] & 0xffff0000u));
+        }
     }
-    __syncthreads();
-    return s;
+    static __device__ __forceinline__ void store(float* p, const T (&v)[N]) {
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            const float2 a = both(v[i]), b = both(v[i + 1]);
+            *reinterpret_cast<float4*>(p + 2 * i) = make_float4(a.x, a.y, b.x, b.y);
+        }
+    }
+    static __device__ __forceinline__ void store(bf16* p, const T (&v)[N]) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            uint32_t w[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float2 f = both(v[i + k]);
+                asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[k]) : "f"(f.y), "f"(f.x));
+            }
+            *reinterpret_cast<uint4*>(p + 2 * i) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
+};
+template <>
+struct Lane<1> {
+    typedef float T;
+    static constexpr int N = 1;
+    template <typename E>
+    static __device__ __forceinline__ void load(const E* p, T (&v)[1]) { v[0] = get(p); }
+    template <typename E>
+    static __device__ __forceinline__ void store(E* p, const T (&v)[1]) { put(p, v[0]); }
+};
+
+// Sum over the LANES lanes of a row: a warp's or fewer by exchange, more through shared memory (all threads of the CTA take part).
+template <int LANES, int THREADS, int V>
+__device__ __forceinline__ void row_sum(float (&s)[V], float (*sh)[THREADS / 32]) {
+#pragma unroll
+    for (int d = (LANES < 32 ? LANES : 32) / 2; d > 0; d >>= 1)
+#pragma unroll
+        for (int i = 0; i < V; ++i) s[i] += __shfl_xor_sync(0xffffffffu, s[i], d);
+    if constexpr (LANES > 32) {
+        constexpr int W = LANES / 32;
+        const int warp = threadIdx.x >> 5, first = warp / W * W;
+        if ((threadIdx.x & 31) == 0)
+#pragma unroll
+            for (int i = 0; i < V; ++i) sh[i][warp] = s[i];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            s[i] = 0.f;
+#pragma unroll
+            for (int w = 0; w < W; ++w) s[i] += sh[i][first + w];
+        }
+    }
 }
 
-template <typename X, typename W>
-__global__ void __launch_bounds__(256) layer_norm_fwd_kernel(const __grid_constant__ Params p) {
+// The rows to come, in shared memory.  Words of 16 bytes, or of one fp32 value: [STAGES][ROWS][ITER][TENSORS][THREADS], each lane's own.  bf16 rows that do not start
+// at 16-byte boundaries: [STAGES][ROWS][TENSORS][GROUPS] rows as they are in memory, from the 4-byte boundary at or before their start on (there are no copies
+// of two bytes), so that a lane's values come with another lane's copies.
+template <typename X, int VEC, int ITER, int ROWS, int LANES, int THREADS, int TENSORS>
+struct Ring {
+    static constexpr bool SHARED = VEC * sizeof(X) == 2;
+    static constexpr int GROUPS = THREADS / LANES, CAP = LANES * ITER * VEC + (SHARED ? 8 : 0);         // values of a row
+    static constexpr int BYTES = VEC * ITER * (int)sizeof(X), STAGES = BYTES * TENSORS * ROWS > 64 ? 3 : 4;
+    static constexpr size_t SIZE = (size_t)STAGES * ROWS * TENSORS * GROUPS * CAP * sizeof(X);
+    static __device__ __forceinline__ X* word(X* ring, int stage, int j, int i, int t) {
+        return ring + ((((stage * ROWS + j) * ITER + i) * TENSORS + t) * THREADS + (int)threadIdx.x) * VEC;
+    }
+    static __device__ __forceinline__ X* whole(X* ring, int stage, int j, int t) {
+        return ring + (((stage * ROWS + j) * TENSORS + t) * GROUPS + (int)threadIdx.x / LANES) * CAP;
+    }
+    static __device__ __forceinline__ void bring(X* ring, int stage, int j, int t, const X* x, long row, long rows, int N, int lane) {
+        if constexpr (SHARED) {
+            const int odd = (int)(row * N & 1), words = (N + odd + 1) / 2;
+            const X* from = x + row * N - odd;
+            const uint32_t to = (uint32_t)__cvta_generic_to_shared(whole(ring, stage, j, t));
+            const bool last = row + 1 == rows && (N + odd) % 2 != 0;                 // the tensor ends in the middle of the last word
+#pragma unroll
+            for (int i = 0; i < ITER / 2 + 1; ++i) {
+                const int k = i * LANES + lane;
+                if (k < words)
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(to + 4 * k), "l"(from + 2 * k), "r"(last && k + 1 == words ? 2 : 4) : "memory");
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < ITER; ++i) {
+                const int c = (i * LANES + lane) * VEC;
+                const uint32_t to = (uint32_t)__cvta_generic_to_shared(word(ring, stage, j, i, t));
+                if (c < N) {
+                    if constexpr (VEC * sizeof(X) == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(to), "l"(x + row * N + c) : "memory");
+                    else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"(to), "l"(x + row * N + c) : "memory");
+                }
+            }
+        }
+    }
+    template <typename T, int N_>
+    static __device__ __forceinline__ void read(X* ring, int stage, int j, int i, int t, long row, int N, int lane, T (&v)[N_]) {
+        if constexpr (SHARED) Lane<VEC>::load(whole(ring, stage, j, t) + (int)(row * N & 1) + i * LANES + lane, v);
+        else Lane<VEC>::load(word(ring, stage, j, i, t), v);
+    }
+};
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_but() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory"); }
+
+// CTA i of the grid takes the rows from i GROUPS on, GROUPS = THREADS / LANES of them at once, then those a grid further on.
+template <typename X, typename W, int VEC, int ITER, int LANES, int THREADS>
+__global__ void __launch_bounds__(THREADS, 2) layer_norm_fwd_kernel(const __grid_constant__ Params p) {
     chain_wait();
-    __shared__ float2 sh[8];
+    constexpr int GROUPS = THREADS / LANES;
+    using R = Ring<X, VEC, ITER, 1, LANES, THREADS, 1>;
+    using L = Lane<VEC>;
+    typedef typename L::T T;
+    __shared__ float sh[2][1][THREADS / 32];
+    extern __shared__ __align__(16) unsigned char ring_raw[];
+    X* ring = reinterpret_cast<X*>(ring_raw);
+    const int N = p.N, lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
+    const float inv = 1.f / (float)N;
+    const X* x = static_cast<const X*>(p.x);
+    const W *w = static_cast<const W*>(p.w), *b = static_cast<const W*>(p.b);
+    const long stride = (long)gridDim.x * GROUPS, first = (long)blockIdx.x * GROUPS + group;
+    const auto fetch = [&](long row, int stage) {
+        if (row < p.rows) R::bring(ring, stage, 0, 0, x, row, p.rows, N, lane);
+        copies_commit();
+    };
+#pragma unroll
+    for (int k = 0; k < R::STAGES - 1; ++k) fetch(first + k * stride, k);
+    T wv[ITER][L::N], bv[ITER][L::N];
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) {
+        const int c = (i * LANES + lane) * VEC;
+#pragma unroll
+        for (int u = 0; u < L::N; ++u) {
+            wv[i][u] = splat<T>(1.f);
+            bv[i][u] = splat<T>(0.f);
+        }
+        if (w && c < N) L::load(w + c, wv[i]);
+        if (b && c < N) L::load(b + c, bv[i]);
+    }
+    int stage = 0;
+    for (long row = first; row - group < p.rows; row += stride, stage = stage + 1 == R::STAGES ? 0 : stage + 1) {
+        copies_but<R::STAGES - 2>();
+        if constexpr (R::SHARED) __syncthreads();
+        T v[ITER][L::N], t = splat<T>(0.f);
+#pragma unroll
+        for (int i = 0; i < ITER; ++i) {
+            if (row < p.rows && (i * LANES + lane) * VEC < N) {
+                R::read(ring, stage, 0, i, 0, row, N, lane, v[i]);
+            } else {
+#pragma unroll
+                for (int u = 0; u < L::N; ++u) v[i][u] = splat<T>(0.f);
+            }
+#pragma unroll
+            for (int u = 0; u < L::N; ++u) t = add(t, v[i][u]);
+        }
+        fetch(row + (R::STAGES - 1) * stride, stage == 0 ? R::STAGES - 1 : stage - 1);       // (where the row before this one was)
+        float s[1] = {total(t)}, ss[1];
+        row_sum<LANES, THREADS>(s, sh[0]);
+        const float mean = s[0] * inv;
+        t = splat<T>(0.f);
+#pragma unroll
+        for (int i = 0; i < ITER; ++i)
+            if ((i * LANES + lane) * VEC < N)
+#pragma unroll
+                for (int u = 0; u < L::N; ++u) {
+                    v[i][u] = add(v[i][u], splat<T>(-mean));
+                    t = fma2(v[i][u], v[i][u], t);
+                }
+        ss[0] = total(t);
+        row_sum<LANES, THREADS>(ss, sh[1]);
+        const float rstd = rsqrtf(ss[0] * inv + p.eps);
+        if (row < p.rows) {
+            X* y = static_cast<X*>(p.y) + row * N;
+#pragma unroll
+            for (int i = 0; i < ITER; ++i) {
+                const int c = (i * LANES + lane) * VEC;
+                if (c < N) {
+#pragma unroll
+                    for (int u = 0; u < L::N; ++u) v[i][u] = fma2(mul(v[i][u], splat<T>(rstd)), wv[i][u], bv[i][u]);
+                    L::store(y + c, v[i]);
+                }
+            }
+            if (lane == 0 && p.mean) {
+                p.mean[row] = mean;
+                p.rstd[row] = rstd;
+            }
+        }
+    }
+}
+
+// The same with ROWS rows a lane at once, which share the latency of the sums over the lanes (most of what a round of one row consists of).
+template <typename X, typename W, int VEC, int ITER, int ROWS, int LANES, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1) layer_norm_bwd_kernel(const __grid_constant__ Params p) {
+    chain_wait();
+    constexpr int GROUPS = THREADS / LANES;
+    using R = Ring<X, VEC, ITER, ROWS, LANES, THREADS, 2>;
+    using L = Lane<VEC>;
+    typedef typename L::T T;
+    __shared__ float sh[2][2 * ROWS][THREADS / 32];
+    extern __shared__ __align__(16) unsigned char ring_raw[];
+    X* ring = reinterpret_cast<X*>(ring_raw);
+    float* cols = reinterpret_cast<float*>(ring_raw);     // [2][N], after the last row
+    const int N = p.N, lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
+    const float inv = 1.f / (float)N;
+    const X *x = static_cast<const X*>(p.x), *dy = static_cast<const X*>(p.dy);
+    X* dx = static_cast<X*>(p.dx);
+    const W* w = static_cast<const W*>(p.w);
+    const long stride = (long)gridDim.x * GROUPS * ROWS, first = (long)blockIdx.x * GROUPS * ROWS;
+    const auto fetch = [&](long base, int stage) {
+#pragma unroll
+        for (int j = 0; j < ROWS; ++j) {
+            const long row = base + j * GROUPS + group;
+            if (row < p.rows) {
+                R::bring(ring, stage, j, 0, x, row, p.rows, N, lane);
+                R::bring(ring, stage, j, 1, dy, row, p.rows, N, lane);
+            }
+        }
+        copies_commit();
+    };
+#pragma unroll
+    for (int k = 0; k < R::STAGES - 1; ++k) fetch(first + k * stride, k);
+    T dw[ITER][L::N], db[ITER][L::N], wv[ITER][L::N];
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) {
+        const int c = (i * LANES + lane) * VEC;
+#pragma unroll
+        for (int u = 0; u < L::N; ++u) {
+            dw[i][u] = db[i][u] = splat<T>(0.f);
+            wv[i][u] = splat<T>(1.f);
+        }
+        if (w && c < N) L::load(w + c, wv[i]);
+    }
+    float mean[ROWS], rstd[ROWS];
+    const auto stats = [&](long base) {
+#pragma unroll
+        for (int j = 0; j < ROWS; ++j) {
+            const long row = base + j * GROUPS + group;
+            mean[j] = row < p.rows ? p.mean[row] : 0.f;
+            rstd[j] = row < p.rows ? p.rstd[row] : 0.f;
+        }
+    };
+    stats(first);
+    int stage = 0, par = 0;
+    for (long base = first; base < p.rows; base += stride, par ^= 1, stage = stage + 1 == R::STAGES ? 0 : stage + 1) {
+        copies_but<R::STAGES - 2>();
+        if constexpr (R::SHARED) __syncthreads();
+        T xh[ROWS][ITER][L::N], d[ROWS][ITER][L::N];
+#pragma unroll
+        for (int j = 0; j < ROWS; ++j)
+#pragma unroll
+            for (int i = 0; i < ITER; ++i) {
+                const long row = base + j * GROUPS + group;
+                if (row < p.rows && (i * LANES + lane) * VEC < N) {
+                    R::read(ring, stage, j, i, 0, row, N, lane, xh[j][i]);
+                    R::read(ring, stage, j, i, 1, row, N, lane, d[j][i]);
+                } else {
+#pragma unroll
+                    for (int u = 0; u < L::N; ++u) xh[j][i][u] = d[j][i][u] = splat<T>(0.f);      // (d of zero adds nothing)
+                }
+            }
+        fetch(base + (R::STAGES - 1) * stride, stage == 0 ? R::STAGES - 1 : stage - 1);
+        float s[2 * ROWS], r[ROWS];
+#pragma unroll
+        for (int j = 0; j < ROWS; ++j) {
+            const T neg = splat<T>(-mean[j]), r2 = splat<T>(rstd[j]);
+            T s0 = splat<T>(0.f), s1 = s0;
+            r[j] = rstd[j];
+#pragma unroll
+            for (int i = 0; i < ITER; ++i)
+#pragma unroll
+                for (int u = 0; u < L::N; ++u) {
+                    xh[j][i][u] = mul(add(xh[j][i][u], neg), r2);
+                    dw[i][u] = fma2(d[j][i][u], xh[j][i][u], dw[i][u]);
+                    db[i][u] = add(db[i][u], d[j][i][u]);
+                    d[j][i][u] = mul(d[j][i][u], wv[i][u]);
+                    s0 = add(s0, d[j][i][u]);
+                    s1 = fma2(d[j][i][u], xh[j][i][u], s1);
+                }
+            s[2 * j] = total(s0);
+            s[2 * j + 1] = total(s1);
+        }
+        stats(base + stride);
+        row_sum<LANES, THREADS>(s, sh[par]);
+        // rstd (z - mean(z) - xhat mean(z xhat))
+#pragma unroll
+        for (int j = 0; j < ROWS; ++j) {
+            const long row = base + j * GROUPS + group;
+            const T m1 = splat<T>(-s[2 * j] * inv), m2 = splat<T>(-s[2 * j + 1] * inv), rr = splat<T>(r[j]);
+            if (row < p.rows) {
+#pragma unroll
+                for (int i = 0; i < ITER; ++i) {
+                    const int c = (i * LANES + lane) * VEC;
+                    if (c < N) {
+#pragma unroll
+                        for (int u = 0; u < L::N; ++u) d[j][i][u] = mul(fma2(xh[j][i][u], m2, add(d[j][i][u], m1)), rr);
+                        L::store(dx + row * N + c, d[j][i]);
+                    }
+                }
+            }
+        }
+    }
+    if (!p.part) return;
+    copies_but<0>();
+    __syncthreads();
+    float* part = p.part + (long)blockIdx.x * 2 * N;
+    if constexpr (GROUPS == 1) {
+#pragma unroll
+        for (int i = 0; i < ITER; ++i) {
+            const int c = (i * LANES + lane) * VEC;
+            if (c < N) {
+                L::store(part + c, dw[i]);
+                L::store(part + N + c, db[i]);
+            }
+        }
+    } else {
+        // the groups in turn
+        for (int g = 0; g < GROUPS; ++g) {
+            __syncthreads();
+            if (group == g) {
+#pragma unroll
+                for (int i = 0; i < ITER; ++i) {
+                    const int c = (i * LANES + lane) * VEC;
+                    if (c < N) {
+                        if (g) {
+                            T a[L::N], e[L::N];
+                            L::load(cols + c, a);
+                            L::load(cols + N + c, e);
+#pragma unroll
+                            for (int u = 0; u < L::N; ++u) {
+                                dw[i][u] = add(a[u], dw[i][u]);
+                                db[i][u] = add(e[u], db[i][u]);
+                            }
+                        }
+                        L::store(cols + c, dw[i]);
+                        L::store(cols + N + c, db[i]);
+                    }
+                }
+            }
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < 2 * N; i += THREADS) part[i] = cols[i];
+    }
+}
+
+// ---- rows of any length: 256 threads a row, read again for each sum
+template <int V>
+__device__ __forceinline__ void wide_sum(float (&s)[V], float (*sh)[8]) {
+    row_sum<256, 256>(s, sh);
+    __syncthreads();
+}
+template <typename X, typename W>
+__global__ void __launch_bounds__(256) layer_norm_wide_fwd_kernel(const __grid_constant__ Params p) {
+    chain_wait();
+    __shared__ float sh[1][8];
     const int N = p.N;
     const float inv = 1.f / (float)N;
     const long row = blockIdx.x;
     const X* x = static_cast<const X*>(p.x) + row * N;
     X* y = static_cast<X*>(p.y) + row * N;
     const W *w = static_cast<const W*>(p.w), *b = static_cast<const W*>(p.b);
-    float s = 0.f, ss = 0.f;
-    for (int i = threadIdx.x; i < N; i += 256) s += get(x + i);
-    const float mean = cta_sum(s, 0.f, sh).x * inv;
+    float s[1] = {0.f}, ss[1] = {0.f};
+    for (int i = threadIdx.x; i < N; i += 256) s[0] += get(x + i);
+    wide_sum(s, sh);
+    const float mean = s[0] * inv;
     for (int i = threadIdx.x; i < N; i += 256) {
         const float d = get(x + i) - mean;
-        ss = fmaf(d, d, ss);
+        ss[0] = fmaf(d, d, ss[0]);
     }
-    const float rstd = rsqrtf(cta_sum(ss, 0.f, sh).x * inv + p.eps);
+    wide_sum(ss, sh);
+    const float rstd = rsqrtf(ss[0] * inv + p.eps);
     for (int i = threadIdx.x; i < N; i += 256) {
         float v = (get(x + i) - mean) * rstd;
         if (w) v *= get(w + i);
@@ -77,11 +479,10 @@ __global__ void __launch_bounds__(256) layer_norm_fwd_kernel(const __grid_consta
         p.rstd[row] = rstd;
     }
 }
-
 template <typename X, typename W>
-__global__ void __launch_bounds__(256) layer_norm_dx_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(256) layer_norm_wide_dx_kernel(const __grid_constant__ Params p) {
     chain_wait();
-    __shared__ float2 sh[8];
+    __shared__ float sh[2][8];
     const int N = p.N;
     const float inv = 1.f / (float)N;
     const long row = blockIdx.x;
@@ -89,22 +490,21 @@ __global__ void __launch_bounds__(256) layer_norm_dx_kernel(const __grid_constan
     X* dx = static_cast<X*>(p.dx) + row * N;
     const W* w = static_cast<const W*>(p.w);
     const float mean = p.mean[row], rstd = p.rstd[row];
-    float s = 0.f, sx = 0.f;
+    float s[2] = {0.f, 0.f};
     for (int i = threadIdx.x; i < N; i += 256) {
         const float z = w ? get(dy + i) * get(w + i) : get(dy + i);
-        s += z;
-        sx = fmaf(z, (get(x + i) - mean) * rstd, sx);
+        s[0] += z;
+        s[1] = fmaf(z, (get(x + i) - mean) * rstd, s[1]);
     }
-    const float2 m = cta_sum(s, sx, sh);
+    wide_sum(s, sh);
     for (int i = threadIdx.x; i < N; i += 256) {
         const float z = w ? get(dy + i) * get(w + i) : get(dy + i), xhat = (get(x + i) - mean) * rstd;
-        put(dx + i, rstd * (z - m.x * inv - xhat * (m.y * inv)));
+        put(dx + i, rstd * (z - s[0] * inv - xhat * (s[1] * inv)));
     }
 }
-
 // partial sums over every parts-th row, a thread a column
 template <typename X>
-__global__ void __launch_bounds__(256) layer_norm_columns_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(256) layer_norm_wide_columns_kernel(const __grid_constant__ Params p) {
     chain_wait();
     const int c = blockIdx.x * 256 + threadIdx.x;
     if (c >= p.N) return;
@@ -119,40 +519,101 @@ __global__ void __launch_bounds__(256) layer_norm_columns_kernel(const __grid_co
     p.part[((long)blockIdx.y * 2 + 1) * p.N + c] = db;
 }
 
+// dw and db of 32 columns a CTA: 32 warps take the parts in turn, four in flight each, then the warps' sums
 template <typename W>
-__global__ void __launch_bounds__(256) layer_norm_gather_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(1024) layer_norm_gather_kernel(const __grid_constant__ Params p) {
     chain_wait();
-    const int c = blockIdx.x * 256 + threadIdx.x;
-    if (c >= p.N) return;
-    float dw = 0.f, db = 0.f;
-    for (int i = 0; i < p.parts; ++i) {
-        dw += p.part[(long)i * 2 * p.N + c];
-        db += p.part[((long)i * 2 + 1) * p.N + c];
+    __shared__ float sh[32][33];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const long c = (long)blockIdx.x * 32 + lane;          // of the 2 N of a part
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    if (c < 2l * p.N)
+        for (int i = warp; i < p.parts; i += 128)
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (i + 32 * u < p.parts) s[u] += p.part[(long)(i + 32 * u) * 2 * p.N + c];
+    sh[warp][lane] = (s[0] + s[1]) + (s[2] + s[3]);
+    __syncthreads();
+    // a warp a column, a lane a warp's sum
+    float t = sh[lane][warp];
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) t += __shfl_xor_sync(0xffffffffu, t, d);
+    const long at = (long)blockIdx.x * 32 + warp;
+    if (lane == 0 && at < 2l * p.N) {
+        if (at < p.N) {
+            if (p.dw) put(static_cast<W*>(p.dw) + at, t);
+        } else if (p.db) {
+            put(static_cast<W*>(p.db) + at - p.N, t);
+        }
     }
-    if (p.dw) put(static_cast<W*>(p.dw) + c, dw);
-    if (p.db) put(static_cast<W*>(p.db) + c, db);
 }
 
-int parts_of(long rows) { return (int)(rows < 64 ? rows : 64); }
-
-template <typename X, typename W>
-cudaError_t forward(const Params& p, cudaStream_t st) {
-    const cudaError_t e = launch_chained(layer_norm_fwd_kernel<X, W>, (unsigned)p.rows, 256, 0, st, p);
+// ---- which kernel: a row in the registers of LANES lanes, ITER words of VEC values each
+template <typename KernT>
+cudaError_t run(KernT kern, dim3 grid, int threads, size_t smem, const Params& p, cudaStream_t st) {
+    if (smem > 0) {
+        const cudaError_t e = allow_smem(kern, smem);
+        if (e != cudaSuccess) return e;
+    }
+    const cudaError_t e = launch_chained(kern, grid, threads, smem, st, p);
     if (e == cudaSuccess) LLATTN_LAUNCHED();
     return e;
 }
+// 512 threads, as many lanes a row as give each 8 values of it (16 in rows above 4096).  Two CTAs an SM in the forward, one in the backward, and no more than there are rows
+// for; several rows a lane at once as soon as every CTA has more than one.
+constexpr int THREADS = 512, MAX_N = THREADS * 16, SMS = 148;
+int lanes_of(int N) {
+    int lanes = 32;
+    while (lanes * 8 < N && lanes < THREADS) lanes *= 2;
+    return lanes;
+}
+int ctas_of(long rows, int N, int per_sm) {
+    const long g = THREADS / lanes_of(N), n = (rows + g - 1) / g;
+    return (int)(n < per_sm * SMS ? n : per_sm * SMS);
+}
+int parts_of(long rows, int N) { return N > MAX_N ? (int)(rows < 64 ? rows : 64) : ctas_of(rows, N, 1); }
+// Rows of x at once that a lane of the backward takes: two where it has 16 bytes of each (32768 x 2048 bf16, us: one 111, two 92, four 102).  The forward is better off
+// with a second CTA on the SM (one row a lane 59, two 70, four 104; one CTA with two or four 64).
+template <typename X, typename W, int VEC, int ITER, int LANES>
+cudaError_t pass(bool back, const Params& p, cudaStream_t st) {
+    if (!back) return run(layer_norm_fwd_kernel<X, W, VEC, ITER, LANES, THREADS>, ctas_of(p.rows, p.N, 2), THREADS, Ring<X, VEC, ITER, 1, LANES, THREADS, 1>::SIZE, p, st);
+    constexpr int ROWS = VEC * ITER * sizeof(X) > 16 ? 1 : 2;
+    if (ROWS == 1 || p.rows <= (long)p.parts * (THREADS / LANES))
+        return run(layer_norm_bwd_kernel<X, W, VEC, ITER, 1, LANES, THREADS>, p.parts, THREADS, Ring<X, VEC, ITER, 1, LANES, THREADS, 2>::SIZE, p, st);
+    return run(layer_norm_bwd_kernel<X, W, VEC, ITER, ROWS, LANES, THREADS>, p.parts, THREADS, Ring<X, VEC, ITER, ROWS, LANES, THREADS, 2>::SIZE, p, st);
+}
+template <typename X, typename W, int VEC>
+cudaError_t pass_vec(bool back, const Params& p, cudaStream_t st) {
+    switch (lanes_of(p.N)) {
+        case 32: return pass<X, W, VEC, 8 / VEC, 32>(back, p, st);
+        case 64: return pass<X, W, VEC, 8 / VEC, 64>(back, p, st);
+        case 128: return pass<X, W, VEC, 8 / VEC, 128>(back, p, st);
+        case 256: return pass<X, W, VEC, 8 / VEC, 256>(back, p, st);
+        default: return p.N <= 8 * THREADS ? pass<X, W, VEC, 8 / VEC, THREADS>(back, p, st) : pass<X, W, VEC, 16 / VEC, THREADS>(back, p, st);
+    }
+}
 template <typename X, typename W>
-cudaError_t backward(const Params& p, cudaStream_t st) {
-    cudaError_t e = launch_chained(layer_norm_dx_kernel<X, W>, (unsigned)p.rows, 256, 0, st, p);
-    if (e != cudaSuccess) return e;
-    LLATTN_LAUNCHED();
-    if (!p.dw && !p.db) return e;
-    const unsigned blocks = (p.N + 255) / 256;
-    e = launch_chained(layer_norm_columns_kernel<X>, dim3(blocks, p.parts), 256, 0, st, p);
-    if (e != cudaSuccess) return e;
-    LLATTN_LAUNCHED();
-    e = launch_chained(layer_norm_gather_kernel<W>, blocks, 256, 0, st, p);
-    if (e == cudaSuccess) LLATTN_LAUNCHED();
+cudaError_t rows_in_registers(bool back, const Params& p, cudaStream_t st) {
+    constexpr int VEC = 16 / (int)sizeof(X);
+    return p.N % VEC == 0 ? pass_vec<X, W, VEC>(back, p, st) : pass_vec<X, W, 1>(back, p, st);
+}
+template <typename X, typename W>
+cudaError_t forward(const Params& p, cudaStream_t st) {
+    if (p.N > MAX_N) return run(layer_norm_wide_fwd_kernel<X, W>, (unsigned)p.rows, 256, 0, p, st);
+    return rows_in_registers<X, W>(false, p, st);
+}
+template <typename X, typename W>
+cudaError_t backward(Params p, cudaStream_t st) {
+    const bool sums = p.dw || p.db;
+    if (!sums) p.part = nullptr;
+    cudaError_t e;
+    if (p.N > MAX_N) {
+        e = run(layer_norm_wide_dx_kernel<X, W>, (unsigned)p.rows, 256, 0, p, st);
+        if (e == cudaSuccess && sums) e = run(layer_norm_wide_columns_kernel<X>, dim3((p.N + 255) / 256, p.parts), 256, 0, p, st);
+    } else {
+        e = rows_in_registers<X, W>(true, p, st);
+    }
+    if (e == cudaSuccess && sums) e = run(layer_norm_gather_kernel<W>, (unsigned)((2l * p.N + 31) / 32), 1024, 0, p, st);
     return e;
 }
 int check(int x_f32, int w_f32, long rows, int N) {
@@ -169,7 +630,7 @@ extern "C" {
 
 size_t llattn_layer_norm_bwd_workspace_bytes(long rows, int N) {
     if (norm::check(0, 0, rows, N) != 0) return 0;
-    return (size_t)norm::parts_of(rows) * 2 * N * sizeof(float);
+    return (size_t)norm::parts_of(rows, N) * 2 * N * sizeof(float);
 }
 
 int llattn_layer_norm_fwd(const void* x, int x_is_f32, const void* w, const void* b, int w_is_f32, void* y, float* mean, float* rstd, float eps, long rows,
@@ -212,7 +673,7 @@ int llattn_layer_norm_bwd(const void* x, int x_is_f32, const void* w, int w_is_f
     p.part = static_cast<float*>(workspace);
     p.rows = rows;
     p.N = N;
-    p.parts = norm::parts_of(rows);
+    p.parts = norm::parts_of(rows, N);
     cudaStream_t st = (cudaStream_t)stream;
     if (x_is_f32) return (int)norm::backward<float, float>(p, st);
     return (int)(w_is_f32 ? norm::backward<norm::bf16, float>(p, st) : norm::backward<norm::bf16, norm::bf16>(p, st));
