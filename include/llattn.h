@@ -407,7 +407,7 @@ int llattn_recurrence_step(float* h, const void* x, int x_is_f32, const void* g,
  * receives the softmax statistics that the backward reads; NULL in a forward without one.  The workspace (256 bytes for the forward,
  * llattn_window_workspace_bytes for the backward) begins with a status word, see above.  o, dq, dk and dv start at 32-byte boundaries.  Values that a query does not see have to be finite. */
 size_t llattn_window_lse_bytes(int B, int T, int H);
-size_t llattn_window_workspace_bytes(int B, int T, int H);
+size_t llattn_window_workspace_bytes(int B, int T, int H, int G, int K, int window, int sinks);
 int llattn_window_fwd(const void* q, const void* k, const void* v, void* o, float* lse, void* workspace, size_t workspace_bytes, int B, int T, int H, int G,
                       int K, int window, int sinks, float scale, void* stream);
 int llattn_window_bwd(const void* q, const void* k, const void* v, const void* o, const float* lse, const void* d_o, void* dq, void* dk, void* dv,

@@ -925,7 +925,7 @@ WindowGrads window_bwd(const Tensor& q, const Tensor& k, const Tensor& v, const 
                        double scale, bool status, void* stream) {
     const int B = q.size(0), T = q.size(1), H = q.size(2), G = k.size(2), K = q.size(3);
     const WindowGrads r = {contiguous_like(q), contiguous_like(k), contiguous_like(v)};
-    const Tensor ws = empty({(int64_t)lib.llattn_window_workspace_bytes(B, T, H)}, at::kByte, q);
+    const Tensor ws = empty({(int64_t)lib.llattn_window_workspace_bytes(B, T, H, G, K, (int)window, (int)sinks)}, at::kByte, q);
     check(lib.llattn_window_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), fptr(lse), d_o.data_ptr(), r.dq.data_ptr(), r.dk.data_ptr(),
                                 r.dv.data_ptr(), ws.data_ptr(), ws.numel(), B, T, H, G, K, (int)window, (int)sinks, (float)scale, stream),
           "llattn_window_bwd");

@@ -69,9 +69,10 @@ size_t llattn_window_lse_bytes(int B, int T, int H) {
     if (win::check(B, T, H, 1, 64, 1, 0, 1.f) != 0) return 0;
     return (size_t)B * H * win::padded(T) * sizeof(float);
 }
-size_t llattn_window_workspace_bytes(int B, int T, int H) {
-    const size_t n = llattn_window_lse_bytes(B, T, H);
-    return n == 0 ? 0 : 256 + n;
+size_t llattn_window_workspace_bytes(int B, int T, int H, int G, int K, int window, int sinks) {
+    if (win::check(B, T, H, G, K, window, sinks, 1.f) != 0) return 0;
+    const win::Shares sh(B, T, H, G, window, sinks);
+    return 256 + llattn_window_lse_bytes(B, T, H) + (sh.near_floats(B, G, K) + sh.far_floats(B, G, K, sinks)) * sizeof(float);
 }
 
 int llattn_window_fwd(const void* q, const void* k, const void* v, void* o, float* lse, void* workspace, size_t workspace_bytes, int B, int T, int H, int G, int K,
@@ -98,7 +99,7 @@ int llattn_window_bwd(const void* q, const void* k, const void* v, const void* o
     if (rc != 0) return rc;
     if (!q || !k || !v || !o || !lse || !d_o || !dq || !dk || !dv) return LLATTN_ERR_NULL;
     if (misaligned(16, {q, k, v, o, lse, d_o}) || misaligned(32, {dq, dk, dv})) return LLATTN_ERR_ALIGNMENT;
-    if (!workspace || misaligned(256, {workspace}) || workspace_bytes < llattn_window_workspace_bytes(B, T, H)) return LLATTN_ERR_WORKSPACE;
+    if (!workspace || misaligned(256, {workspace}) || workspace_bytes < llattn_window_workspace_bytes(B, T, H, G, K, window, sinks)) return LLATTN_ERR_WORKSPACE;
     win::Params p = {};
     p.o = (const win::bf16*)o;
     p.d_o = (const win::bf16*)d_o;
@@ -107,6 +108,8 @@ int llattn_window_bwd(const void* q, const void* k, const void* v, const void* o
     p.dv = (win::bf16*)dv;
     p.lse = const_cast<float*>(lse);
     p.delta = reinterpret_cast<float*>(static_cast<char*>(workspace) + 256);
+    p.near_part = p.delta + (long)B * H * win::padded(T);
+    p.far_part = p.near_part + win::Shares(B, T, H, G, window, sinks).near_floats(B, G, K);
     win::shape(p, workspace, B, T, H, G, window, sinks, scale);
     cudaStream_t st = (cudaStream_t)stream;
     const cudaError_t e = cudaMemsetAsync(workspace, 0, 4, st);

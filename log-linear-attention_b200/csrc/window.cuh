@@ -22,6 +22,39 @@ struct Params {
     int* err;                         // status word of the workspace
     int B, T, TP, H, G, window, sinks;
     float scale;
+    // backward of k and v, see Shares: fp32 parts of dK and dV
+    float *near_part, *far_part;
+};
+
+// How the sums of dK and dV are shared out.  A tile of 128 tokens is seen by the queries of its own tile and of the `near - 1` behind it; its CTA takes their heads, or
+// one of `splits` shares of them where there are too few tiles to fill the chip.  The first `far_tiles` tiles, of sinks, are seen by all later queries too: those come in
+// `chunks` shares of `chunk` tiles, about as long as the others (one CTA for all of them would run on alone: T = 16384, window 2048, 4 sinks, 8 groups 2.7 ms
+// in the place of 1.9 for the whole backward).  What is shared is left as fp32 parts, and added up in a fixed order.
+struct Shares {
+    int tiles, near, splits, far_tiles, chunks, chunk;
+    Shares(int B, int T, int H, int G, int window, int sinks) {
+        const long units = (long)B * G;
+        const int R = H / G;
+        tiles = (T + TILE - 1) / TILE;
+        near = (TILE - 1 + window - 1) / TILE + 1;
+        splits = (int)(148 / (units * tiles) < R ? 148 / (units * tiles) : R);
+        if (splits < 1) splits = 1;
+        const int sink_tiles = ((sinks < T ? sinks : T) + TILE - 1) / TILE;
+        far_tiles = sink_tiles < tiles - near ? sink_tiles : tiles - near > 0 ? tiles - near : 0;
+        chunks = chunk = 0;
+        if (far_tiles > 0) {
+            const int length = tiles - near;
+            long n = 2 * 148 / (units * far_tiles);
+            if (n > 32) n = 32;
+            if (n > (length + near - 1) / near) n = (length + near - 1) / near;
+            chunk = (int)((length + (n < 1 ? 1 : n) - 1) / (n < 1 ? 1 : n));
+            chunks = (length + chunk - 1) / chunk;
+        }
+    }
+    __host__ __device__ int near_tiles() const { return splits > 1 ? tiles : far_tiles; }          // tiles with parts of their own queries
+    __host__ __device__ int far_rows(int sinks) const { return sinks < TILE ? sinks : TILE; }      // rows of a far part
+    size_t near_floats(int B, int G, int K) const { return (size_t)B * G * splits * near_tiles() * TILE * 2 * K; }
+    size_t far_floats(int B, int G, int K, int sinks) const { return (size_t)B * G * far_tiles * chunks * far_rows(sinks) * 2 * K; }
 };
 
 // The tiles of keys that the queries [q0, q0 + 128) see are the first `sink` ones and [lo, hi].

@@ -59,6 +59,18 @@ __device__ __forceinline__ void put_row(uint32_t taddr, bf16* out, float f, bool
         if (there) store_32B(out + i, w);
     }
 }
+// the same unrounded
+template <int K>
+__device__ __forceinline__ void put_part(uint32_t taddr, float* out, bool there) {
+#pragma unroll
+    for (int i = 0; i < K / 2; i += 16) {
+        float o[16];
+        umma::tmem_ld16(taddr + i, o);
+        if (there)
+#pragma unroll
+            for (int u = 0; u < 16; u += 4) *reinterpret_cast<float4*>(out + i + u) = make_float4(o[u], o[u + 1], o[u + 2], o[u + 3]);
+    }
+}
 __device__ __forceinline__ void load_stat(float* dst, const float* src, uint64_t* bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n"
                  ::"r"(umma::smem_addr(dst)), "l"(src), "r"(TILE * 4), "r"(umma::smem_addr(bar)) : "memory");
@@ -228,7 +240,7 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dq_tc_kernel(const __
 }
 
 template <int K>
-__global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dkv_tc_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dkv_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Shares sh) {
     chain_wait();
     using namespace bwd;
     using SM = Smem<K>;
@@ -242,10 +254,14 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dkv_tc_kernel(const _
     float* sStat = reinterpret_cast<float*>(smem + SM::stat_off);
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int j = blockIdx.x, s0 = j * TILE, grp = blockIdx.y, b = blockIdx.z, R = p.H / p.G;
-    // tiles of queries from the token's own to the last that sees one of the tile's tokens
-    const int last = (p.T - 1) / TILE, reach = (s0 + TILE - 1 + p.window - 1) / TILE, hi = s0 < p.sinks || reach > last ? last : reach;
-    const int per = hi - j + 1, steps = R * per;
+    const int grp = blockIdx.y, b = blockIdx.z, R = p.H / p.G, last = sh.tiles - 1;
+    // far shares first, then the near ones; tile j of k and v, tiles [lo, hi] of queries, heads h0 on
+    const bool far = (int)blockIdx.x < sh.far_tiles * sh.chunks;
+    const int x = far ? blockIdx.x : blockIdx.x - sh.far_tiles * sh.chunks, j = far ? x / sh.chunks : x / sh.splits, share = far ? x % sh.chunks : x % sh.splits;
+    const int lo = far ? j + sh.near + share * sh.chunk : j, end = far ? lo + sh.chunk - 1 : j + sh.near - 1, hi = end < last ? end : last;
+    const int each = far ? R : (R + sh.splits - 1) / sh.splits, h0 = grp * R + (far ? 0 : share * each), heads = min(each, grp * R + R - h0);
+    if (lo > last || heads <= 0) return;                    // (a share that the last tiles do not reach; fewer heads than shares)
+    const int s0 = j * TILE, per = hi - lo + 1, steps = heads * per;
     if (tid == 0) {
         for (int i = 0; i < NST; ++i) {
             umma::mbar_init(full + i, 1);
@@ -273,7 +289,7 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dkv_tc_kernel(const _
             load_tile<K>(smem + SM::a_off, &p.tk, grp, s0, b, barKV);
             load_tile<K>(smem + SM::a_off + SM::TILE_BYTES, &p.tv, grp, s0, b, barKV);
             bool ok = true;
-            int n = 0, h = grp * R, i = j;
+            int n = 0, h = h0, i = lo;
             for (; n < 2 * steps; ++n) {
                 const int st = n % NST;
                 if (n >= NST) ok = umma::mbar_wait(empty + st, (n / NST - 1) & 1, abort_flag);
@@ -282,7 +298,7 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dkv_tc_kernel(const _
                 load_tile<K>(smem + SM::st_off + st * SM::TILE_BYTES, n & 1 ? &p.tdo : &p.tq, h, i * TILE, b, full + st);
                 load_stat(sStat + st * TILE, (n & 1 ? p.delta : p.lse) + ((long)b * p.H + h) * p.TP + i * TILE, full + st);
                 if ((n & 1) && ++i > hi) {
-                    i = j;
+                    i = lo;
                     ++h;
                 }
             }
@@ -335,10 +351,10 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dkv_tc_kernel(const _
         const uint32_t tS = umma::tmem_addr(tmem, warp, TM_S + 64 * half), tDP = umma::tmem_addr(tmem, warp, TM_DP + 64 * half);
         const float c = p.scale * LOG2E;
         bool ok = true;
-        int i = j;
+        int i = lo;
         for (int n = 0; n < steps; ++n) {
             const int t0 = i * TILE;
-            if (++i > hi) i = j;
+            if (++i > hi) i = lo;
             const float *lse = sStat + 2 * n % NST * TILE + half * 64, *delta = sStat + (2 * n + 1) % NST * TILE + half * 64;
             ok = umma::mbar_wait_warp(full + 2 * n % NST, (2 * n / NST) & 1, abort_flag) && umma::mbar_wait_warp(barS, n & 1, abort_flag);
             if (!ok) break;
@@ -378,9 +394,21 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dkv_tc_kernel(const _
         if (ok) ok = umma::mbar_wait_warp(barDone, 0, abort_flag);
         if (ok) {
             umma::fence_after_sync();
-            const long at = (((long)b * p.T + s) * p.G + grp) * K + half * (K / 2);
-            put_row<K>(umma::tmem_addr(tmem, warp, TM_DV + half * (K / 2)), p.dv + at, 1.f, s < p.T);
-            put_row<K>(umma::tmem_addr(tmem, warp, TM_DK + half * (K / 2)), p.dk + at, p.scale, s < p.T);
+            const long at = (((long)b * p.T + s) * p.G + grp) * K + half * (K / 2), unit = (long)b * p.G + grp;
+            const uint32_t tDV = umma::tmem_addr(tmem, warp, TM_DV + half * (K / 2)), tDK = umma::tmem_addr(tmem, warp, TM_DK + half * (K / 2));
+            const bool sink = j < sh.far_tiles && s < p.sinks;                     // a token with parts from far
+            if (far || sh.splits > 1 || j < sh.far_tiles) {
+                const int row = s - s0;
+                float* part = far ? p.far_part + (((unit * sh.far_tiles + j) * sh.chunks + share) * sh.far_rows(p.sinks) + row) * 2 * K
+                                  : p.near_part + (((unit * sh.splits + share) * sh.near_tiles() + j) * TILE + row) * 2 * K;
+                const bool there = s < p.T && (sink || (!far && sh.splits > 1));
+                put_part<K>(tDK, part + half * (K / 2), there);
+                put_part<K>(tDV, part + K + half * (K / 2), there);
+            }
+            if (!far && sh.splits == 1) {
+                put_row<K>(tDV, p.dv + at, 1.f, s < p.T && !sink);
+                put_row<K>(tDK, p.dk + at, p.scale, s < p.T && !sink);
+            }
         }
         umma::fence_before_sync();
     }
@@ -396,18 +424,57 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dkv_tc_kernel(const _
     }
 }
 
+// Adds up the parts: a warp a token and group.  The tokens with parts are all of them, or the sinks among the first tiles.
+template <int K>
+__global__ void __launch_bounds__(256) window_join_kernel(const __grid_constant__ Params p, const __grid_constant__ Shares sh, int tokens) {
+    chain_wait();
+    const int lane = threadIdx.x & 31, R = p.H / p.G;
+    const long row = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (row >= (long)p.B * p.G * tokens) return;
+    const int s = (int)(row % tokens), j = s / TILE;
+    const long unit = row / tokens, b = unit / p.G, grp = unit % p.G;
+    constexpr int N = K / 64;                             // pairs of columns a lane, of dk and of dv
+    float2 sum[2 * N];
+#pragma unroll
+    for (int i = 0; i < 2 * N; ++i) sum[i] = make_float2(0.f, 0.f);
+    const auto add = [&](const float* part) {
+#pragma unroll
+        for (int i = 0; i < 2 * N; ++i) {
+            const float2 v = reinterpret_cast<const float2*>(part)[lane + 32 * i];
+            sum[i].x += v.x;
+            sum[i].y += v.y;
+        }
+    };
+    const int each = (R + sh.splits - 1) / sh.splits;
+    for (int x = 0; x * each < R; ++x) add(p.near_part + (((unit * sh.splits + x) * sh.near_tiles() + j) * TILE + s % TILE) * 2 * K);
+    if (j < sh.far_tiles && s < p.sinks)
+        for (int x = 0; j + sh.near + x * sh.chunk < sh.tiles; ++x) add(p.far_part + (((unit * sh.far_tiles + j) * sh.chunks + x) * sh.far_rows(p.sinks) + s % TILE) * 2 * K);
+    const long at = ((b * p.T + s) * p.G + grp) * K;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        reinterpret_cast<uint32_t*>(p.dk + at)[lane + 32 * i] = pack_bf16(sum[i].x * p.scale, sum[i].y * p.scale);
+        reinterpret_cast<uint32_t*>(p.dv + at)[lane + 32 * i] = pack_bf16(sum[N + i].x, sum[N + i].y);
+    }
+}
+
 template <int K>
 static cudaError_t launch(const Params& p, cudaStream_t st) {
     const size_t smem = bwd::Smem<K>::total;
-    const auto dq = window_dq_tc_kernel<K>, dkv = window_dkv_tc_kernel<K>;
+    const Shares sh(p.B, p.T, p.H, p.G, p.window, p.sinks);
+    const auto dq = window_dq_tc_kernel<K>;
+    const auto dkv = window_dkv_tc_kernel<K>;
     cudaError_t e = allow_smem(dq, smem);
     if (e == cudaSuccess) e = allow_smem(dkv, smem);
     if (e != cudaSuccess) return e;
-    const unsigned tiles = (unsigned)((p.T + TILE - 1) / TILE);
-    e = launch_chained(dq, dim3(tiles, p.H, p.B), bwd::NTHREADS, smem, st, p);
+    e = launch_chained(dq, dim3(sh.tiles, p.H, p.B), bwd::NTHREADS, smem, st, p);
     if (e != cudaSuccess) return e;
     LLATTN_LAUNCHED();
-    e = launch_chained(dkv, dim3(tiles, p.G, p.B), bwd::NTHREADS, smem, st, p);
+    e = launch_chained(dkv, dim3(sh.far_tiles * sh.chunks + sh.tiles * sh.splits, p.G, p.B), bwd::NTHREADS, smem, st, p, sh);
+    if (e != cudaSuccess) return e;
+    LLATTN_LAUNCHED();
+    const int some = sh.far_tiles * TILE < p.sinks ? sh.far_tiles * TILE : p.sinks, tokens = sh.splits > 1 ? p.T : some;
+    if (tokens == 0 || (sh.splits == 1 && sh.far_tiles == 0)) return e;
+    e = launch_chained(window_join_kernel<K>, (unsigned)(((long)p.B * p.G * tokens + 7) / 8), 256, 0, st, p, sh, tokens);
     if (e == cudaSuccess) LLATTN_LAUNCHED();
     return e;
 }

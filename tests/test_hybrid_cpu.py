@@ -98,7 +98,7 @@ def test_c_entries_reject_bad_arguments(pkg):
         assert wfwd(**bad) == -1, bad
     assert wfwd(H=3) == -4 and wfwd(q=null) == -6 and wfwd(q=odd) == -9
     assert wfwd(ws=null) == -5 and wfwd(n=255) == -5 and wfwd(ws=P(4096 + 16)) == -5
-    need = lib.llattn_window_workspace_bytes(1, 8, 4)
+    need = lib.llattn_window_workspace_bytes(1, 8, 4, 2, 64, 4, 0)
     assert need >= 256 + 4 * 8 * 4 and lib.llattn_window_lse_bytes(1, 8, 4) >= 4 * 8 * 4
     wbwd = lambda lse, n: lib.llattn_window_bwd(*[ok] * 4, lse, *[ok] * 5, n, 1, 8, 4, 2, 64, 4, 0, 1.0, null)
     assert wbwd(null, need) == -6 and wbwd(odd, need) == -9 and wbwd(ok, need - 1) == -5
