@@ -95,8 +95,8 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dq_tc_kernel(const __
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int q0 = blockIdx.x * TILE, h = blockIdx.y, b = blockIdx.z, grp = h / (p.H / p.G);
     const Span span(q0, p.T, p.window, p.sinks);
-    const int steps = span.sink + span.hi - span.lo + 1;
-    const auto tile = [&](int n) { return n < span.sink ? n : span.lo + n - span.sink; };
+    const int steps = span.count();
+    const auto tile = [&](int n) { return span.tile(n); };
     if (tid == 0) {
         for (int i = 0; i < NST; ++i) {
             umma::mbar_init(full + i, 1);

@@ -10,6 +10,8 @@
 //     warp 8             issues the products
 //     warp 9             brings Q, then K and V tiles through a ring
 // A wait that gives up sets the CTA's abort flag, after which every other wait ends at once, and the workspace's status word.
+#include <type_traits>
+
 #include "window.cuh"
 
 namespace llattn {
@@ -29,24 +31,20 @@ struct Smem {
 __device__ __forceinline__ void regs_issue() { asm volatile("setmaxnreg.dec.sync.aligned.u32 72;\n"); }
 __device__ __forceinline__ void regs_rows() { asm volatile("setmaxnreg.inc.sync.aligned.u32 216;\n"); }
 
-// The tiles of keys that A or B sees, in order: the sinks', then the rest.
-struct Walk {
+#ifndef WIN_POLY
+#define WIN_POLY 4
+#endif
+// Of the pairs of exponentials of a tile every POLY-th goes to the FMA pipes.
+constexpr int POLY = WIN_POLY;
+
+// The tiles of keys that A or B sees: A's list up to the end of the longer one.  (B's band starts no earlier, and where more of the sinks' tiles are in front of it than in
+// front of A's, those are tiles of A's band.)
+struct Both {
     Span a, b;
-    int j, end;
-    __device__ Walk(const Params& p, int q0) : a(q0, p.T, p.window, p.sinks), b(q0 + TILE, p.T, p.window, p.sinks) {
-        j = 0;
-        end = a.hi > b.hi ? a.hi : b.hi;
-        settle();
-    }
-    __device__ void settle() {
-        while (j <= end && !a.has(j) && !b.has(j)) j = j < a.lo ? a.lo : b.lo;      // (a tile that neither sees is in front of A's or B's band)
-    }
-    __device__ bool more() const { return j <= end; }
-    __device__ void next() {
-        ++j;
-        settle();
-    }
-    __device__ bool in(int x) const { return x == 0 ? a.has(j) : b.has(j); }
+    int count;
+    __device__ Both(const Params& p, int q0) : a(q0, p.T, p.window, p.sinks), b(q0 + TILE, p.T, p.window, p.sinks) { count = a.count() + (b.hi > a.hi ? b.hi - a.hi : 0); }
+    __device__ int tile(int n) const { return a.tile(n); }
+    __device__ bool in(int x, int j) const { return x == 0 ? a.has(j) : b.has(j); }
 };
 }  // namespace fwd
 
@@ -58,8 +56,8 @@ __global__ void __launch_bounds__(fwd::NTHREADS, 1) window_fwd_tc_kernel(const _
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = umma::align_1024(smem_raw);
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + SM::bar_off);
-    uint64_t *full = bars, *empty = bars + NST, *barQ = bars + 2 * NST, *barS = barQ + 1, *barP = barS + 2, *barO = barP + 2;
-    constexpr int NBARS = 2 * NST + 7;
+    uint64_t *full = bars, *empty = bars + NST, *barQ = bars + 2 * NST, *barS = barQ + 1, *barP = barS + 2, *barO = barP + 4;
+    constexpr int NBARS = 2 * NST + 9;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + SM::bar_off + NBARS * 8);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -73,7 +71,8 @@ __global__ void __launch_bounds__(fwd::NTHREADS, 1) window_fwd_tc_kernel(const _
         umma::mbar_init(barQ, 1);
         for (int x = 0; x < 2; ++x) {
             umma::mbar_init(barS + x, 1);
-            umma::mbar_init(barP + x, 4);
+            umma::mbar_init(barP + 2 * x, 4);
+            umma::mbar_init(barP + 2 * x + 1, 4);
             umma::mbar_init(barO + x, 1);
         }
         umma::fence_mbar_init();
@@ -92,16 +91,14 @@ __global__ void __launch_bounds__(fwd::NTHREADS, 1) window_fwd_tc_kernel(const _
             tma::expect_tx(barQ, (two ? 2 : 1) * SM::TILE_BYTES);
             load_tile<K>(smem + SM::q_off, &p.tq, h, q0, b, barQ);
             if (two) load_tile<K>(smem + SM::q_off + SM::TILE_BYTES, &p.tq, h, q0 + TILE, b, barQ);
+            const Both w(p, q0);
             int n = 0;
-            bool ok = true;
-            for (Walk w(p, q0); w.more() && ok; w.next())
-                for (int kv = 0; kv < 2 && ok; ++kv, ++n) {
-                    const int st = n % NST;
-                    if (n >= NST) ok = umma::mbar_wait(empty + st, (n / NST - 1) & 1, abort_flag);
-                    if (!ok) break;
-                    tma::expect_tx(full + st, SM::TILE_BYTES);
-                    load_tile<K>(smem + SM::st_off + st * SM::TILE_BYTES, kv ? &p.tv : &p.tk, grp, w.j * TILE, b, full + st);
-                }
+            for (; n < 2 * w.count; ++n) {
+                const int st = n % NST;
+                if (n >= NST && !umma::mbar_wait(empty + st, (n / NST - 1) & 1, abort_flag)) break;
+                tma::expect_tx(full + st, SM::TILE_BYTES);
+                load_tile<K>(smem + SM::st_off + st * SM::TILE_BYTES, n & 1 ? &p.tv : &p.tk, grp, w.tile(n >> 1) * TILE, b, full + st);
+            }
             // nobody may be left to wait for the last copies after a wait that gave up: they end before the CTA does
             if (*abort_flag) {
                 umma::mbar_wait(barQ, 0);
@@ -112,28 +109,30 @@ __global__ void __launch_bounds__(fwd::NTHREADS, 1) window_fwd_tc_kernel(const _
             constexpr uint32_t idS = umma::idesc_bf16(128, 128, false, false), idO = umma::idesc_bf16(128, K, false, true);
             bool ok = umma::mbar_wait_warp(barQ, 0, abort_flag);
             int done[2] = {0, 0};                       // products P V of A, B issued
-            Walk w(p, q0);
+            const Both w(p, q0);
             // step i: the products P V with tile i - 1, and S with tile i
             bool before[2] = {false, false};
-            for (int i = 0; ok; ++i) {
-                const bool more = w.more();
-                if (!more && !before[0] && !before[1]) break;
+            for (int i = 0; i <= w.count && ok; ++i) {
                 bool haveK = false, haveV = false;
                 const int nk = 2 * i, nv = 2 * i - 1;   // positions of K of this step and V of the one before in the ring's sequence
-                bool now[2];
-                for (int x = 0; x < 2; ++x) {
-                    now[x] = more && w.in(x);
-                    if (before[x] && ok) {
+                for (int x = 0; x < 2 && ok; ++x) {
+                    if (before[x]) {
                         if (!haveV) ok = umma::mbar_wait_warp(full + nv % NST, (nv / NST) & 1, abort_flag);
                         haveV = true;
-                        ok = ok && umma::mbar_wait_warp(barP + x, done[x] & 1, abort_flag);
+                        // P comes in two halves, the first product under the exponentials of the second
+                        for (int half = 0; half < 2; ++half) {
+                            ok = ok && umma::mbar_wait_warp(barP + 2 * x + half, done[x] & 1, abort_flag);
+                            if (!ok) break;
+                            umma::fence_after_sync();
+                            umma::gemm_tm_lead<TILE, 64>(lead, tmem + TM_O + 128 * x, tmem + TM_S + 128 * x + 32 * half,
+                                                         sS + (nv % NST) * SM::TILE_BYTES + half * 64 * umma::ROW_BYTES, idO, done[x] > 0 || half > 0);
+                        }
                         if (!ok) break;
-                        umma::fence_after_sync();
-                        umma::gemm_tm_lead<TILE, TILE>(lead, tmem + TM_O + 128 * x, tmem + TM_S + 128 * x, sS + (nv % NST) * SM::TILE_BYTES, idO, done[x] > 0);
                         umma::commit_lead(lead, barO + x);
                         ++done[x];
                     }
-                    if (now[x] && ok) {
+                    before[x] = i < w.count && w.in(x, w.tile(i));
+                    if (before[x]) {
                         if (!haveK) ok = umma::mbar_wait_warp(full + nk % NST, (nk / NST) & 1, abort_flag);
                         haveK = true;
                         if (!ok) break;
@@ -143,10 +142,7 @@ __global__ void __launch_bounds__(fwd::NTHREADS, 1) window_fwd_tc_kernel(const _
                 }
                 if (!ok) break;
                 if (i > 0) umma::commit_lead(lead, empty + nv % NST);
-                if (more) umma::commit_lead(lead, empty + nk % NST);
-                before[0] = now[0];
-                before[1] = now[1];
-                if (more) w.next();
+                if (i < w.count) umma::commit_lead(lead, empty + nk % NST);
             }
         }
     } else {
@@ -154,66 +150,92 @@ __global__ void __launch_bounds__(fwd::NTHREADS, 1) window_fwd_tc_kernel(const _
         const int x = warp >> 2, row = (warp & 3) * 32 + lane, t0 = q0 + x * TILE, t = t0 + row;
         const uint32_t tS = umma::tmem_addr(tmem, warp, TM_S + 128 * x), tO = umma::tmem_addr(tmem, warp, TM_O + 128 * x);
         const float c = p.scale * LOG2E;
+        const f32x2 c2 = pack2(c, c);
+        const Span span(t0, p.T, p.window, p.sinks);
+        const int n = span.count();
         float m = -INFINITY, sum = 0.f;
-        int n = 0;
         bool ok = true;
-        for (Walk w(p, q0); w.more(); w.next()) {
-            if (!w.in(x)) continue;
-            ok = umma::mbar_wait_warp(barS + x, n & 1, abort_flag);
+        for (int i = 0; i < n; ++i) {
+            const int s0 = span.tile(i) * TILE;
+            const bool whole = all_seen(t0, s0, p.window, p.sinks);
+            ok = umma::mbar_wait_warp(barS + x, i & 1, abort_flag);
             if (!ok) break;
             umma::fence_after_sync();
             float s[2][64];
             tmem_ld64(tS, s[0]);
             tmem_ld64(tS + 64, s[1]);
-            const int s0 = w.j * TILE;
-            if (!all_seen(t0, s0, p.window, p.sinks)) {
+            if (!whole) {
 #pragma unroll
-                for (int i = 0; i < 128; ++i)
-                    if (!sees(t, s0 + i, p.window, p.sinks)) s[i >> 6][i & 63] = -INFINITY;
+                for (int k = 0; k < 4; ++k) {
+                    const uint32_t bits = seen_bits(t, s0 + 32 * k, p.window, p.sinks);
+#pragma unroll
+                    for (int u = 0; u < 32; ++u)
+                        if (!(bits & (1u << u))) s[k >> 1][(k & 1) * 32 + u] = -INFINITY;
+                }
             }
             float top[4] = {s[0][0], s[0][1], s[0][2], s[0][3]};
 #pragma unroll
-            for (int i = 4; i < 128; ++i) top[i & 3] = fmaxf(top[i & 3], s[i >> 6][i & 63]);
+            for (int k = 4; k < 128; k += 8)
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const int e = k + u, f = k + 4 + u < 128 ? k + 4 + u : e;
+                    top[u] = fmaxf(fmaxf(top[u], s[e >> 6][e & 63]), s[f >> 6][f & 63]);
+                }
             const float now = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
             const bool grown = now > m + GROWTH || (m == -INFINITY && now > m);
-            if (n == 0) {
+            if (i == 0) {
                 m = now;
             } else if (__any_sync(0xffffffffu, grown)) {
-                ok = umma::mbar_wait_warp(barO + x, (n - 1) & 1, abort_flag);
+                ok = umma::mbar_wait_warp(barO + x, (i - 1) & 1, abort_flag);
                 if (!ok) break;
                 umma::fence_after_sync();
                 const float f = grown ? exp2_fast(m - now) : 1.f;
                 if (grown) m = now;
                 sum *= f;
 #pragma unroll
-                for (int i = 0; i < K; i += 16) {
+                for (int k = 0; k < K; k += 16) {
                     float o[16];
-                    umma::tmem_ld16(tO + i, o);
+                    umma::tmem_ld16(tO + k, o);
 #pragma unroll
                     for (int u = 0; u < 16; ++u) o[u] *= f;
-                    umma::tmem_st16(tO + i, o);
+                    umma::tmem_st16(tO + k, o);
                 }
             }
             const float ref = m == -INFINITY ? 0.f : m;        // a row that has seen nothing yet
-            float part[4] = {0.f, 0.f, 0.f, 0.f};
+            const f32x2 shift = pack2(-ref, -ref);
+            f32x2 part[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
 #pragma unroll
-            for (int i = 0; i < 128; i += 32) {
-                uint32_t w16[16];
+            for (int half = 0; half < 2; ++half) {
+                const auto exponentials = [&](auto mixed) {
 #pragma unroll
-                for (int u = 0; u < 32; u += 2) {
-                    const float e0 = exp2_fast(fmaf(s[(i + u) >> 6][(i + u) & 63], c, -ref)), e1 = exp2_fast(fmaf(s[(i + u) >> 6][(i + u + 1) & 63], c, -ref));
-                    part[u & 2] += e0;
-                    part[(u & 2) + 1] += e1;
-                    w16[u >> 1] = pack_bf16(e0, e1);
-                }
-                umma::tmem_st16u(tS + i / 2, w16);
+                    for (int k = 0; k < 64; k += 32) {
+                        uint32_t w[16];
+#pragma unroll
+                        for (int u = 0; u < 16; ++u) {
+                            const f32x2 y = fma2(pack2(s[half][k + 2 * u], s[half][k + 2 * u + 1]), c2, shift);
+                            float2 e;
+                            if (decltype(mixed)::value && u % POLY == POLY - 1) {
+                                e = exp2_poly(y);
+                            } else {
+                                const float2 v = unpack2(y);
+                                e = make_float2(exp2_fast(v.x), exp2_fast(v.y));
+                            }
+                            part[u & 1] = add2(part[u & 1], pack2(e.x, e.y));
+                            w[u] = pack_bf16(e.x, e.y);
+                        }
+                        umma::tmem_st16u(tS + 32 * half + k / 2, w);
+                    }
+                };
+                // (hidden keys are exact zeros: the special-function unit's)
+                if (whole) exponentials(std::true_type{});
+                else exponentials(std::false_type{});
+                umma::tmem_wait_st();
+                umma::fence_before_sync();
+                __syncwarp();
+                if (lane == 0) arrive(barP + 2 * x + half);
             }
-            sum += (part[0] + part[1]) + (part[2] + part[3]);
-            umma::tmem_wait_st();
-            umma::fence_before_sync();
-            __syncwarp();
-            if (lane == 0) arrive(barP + x);
-            ++n;
+            const float2 a = unpack2(add2(part[0], part[1]));
+            sum += a.x + a.y;
         }
         if (ok && n > 0) ok = umma::mbar_wait_warp(barO + x, (n - 1) & 1, abort_flag);
         if (ok && n > 0) {
