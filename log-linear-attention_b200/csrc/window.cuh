@@ -77,12 +77,13 @@ struct Span {
 __device__ __forceinline__ bool all_seen(int q0, int s0, int window, int sinks) {
     return s0 + TILE - 1 <= q0 && (q0 + TILE - 1 - s0 < window || s0 + TILE - 1 < sinks);
 }
-__device__ __forceinline__ bool sees(int t, int s, int window, int sinks) { return s <= t && (t - s < window || s < sinks); }
-
-// Which of 32 keys from s0 on query t sees, a bit each.
+// Which of 32 keys from s0 on query t sees, and which of 32 queries from t0 on see key s: a bit each.
+__device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
 __device__ __forceinline__ uint32_t seen_bits(int t, int s0, int window, int sinks) {
-    const auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; };
     return below(t - s0 + 1) & (~below(t - window + 1 - s0) | below(sinks - s0));
+}
+__device__ __forceinline__ uint32_t seeing_bits(int t0, int s, int window, int sinks) {
+    return ~below(s - t0) & (s < sinks ? 0xffffffffu : below(s + window - t0));
 }
 
 // ---- two fp32 values in a 64-bit register

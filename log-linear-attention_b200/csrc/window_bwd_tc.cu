@@ -15,18 +15,65 @@ namespace win {
 
 namespace bwd {
 constexpr int NTHREADS = 384, MMA_WARP = 8, TMA_WARP = 9;
+// Two rings of tiles: those that two products of a step need, far apart (NA of them), and those of one (NB).  With K = 128 five tiles fit beside the two that stay, three
+// and two: the next but one of either kind is on its way while a step runs.  (One ring of four for both kinds: the dQ kernel waited for its keys, 527 us at T = 8192,
+// 32 heads, window 2048.)
 template <int K>
 struct Smem {
-    static constexpr int NST = K == 64 ? 8 : 4;
+    static constexpr int NA = K == 64 ? 4 : 3, NB = K == 64 ? 4 : 2;
     static constexpr uint32_t TILE_BYTES = TILE * K * 2;
-    static constexpr uint32_t a_off = 0, st_off = 2 * TILE_BYTES;                    // the two tiles that stay, the ring
-    static constexpr uint32_t stat_off = st_off + NST * TILE_BYTES;                  // float [NST / 2][2][128]: lse, delta of a step's queries
-    static constexpr uint32_t bar_off = stat_off + NST / 2 * 1024, total = bar_off + 256 + 1024;
+    static constexpr uint32_t stay_off = 0, a_off = 2 * TILE_BYTES, b_off = a_off + NA * TILE_BYTES;
+    static constexpr uint32_t stat_off = b_off + NB * TILE_BYTES;                    // float [NA + NB][128]: lse beside A tiles of queries, delta beside B tiles
+    static constexpr uint32_t bar_off = stat_off + (NA + NB) * TILE * 4, total = bar_off + 256;
+    static_assert(total <= 227 * 1024, "one CTA");
+};
+// The steps of a ring of N tiles: slot and phase of step n.
+template <int N>
+struct Ring {
+    uint64_t *full, *empty;
+    __device__ __forceinline__ uint64_t* filled(int n) const { return full + n % N; }
+    __device__ __forceinline__ uint64_t* freed(int n) const { return empty + n % N; }
+    static __device__ __forceinline__ uint32_t phase(int n) { return (n / N) & 1; }
+    // the slot of step n is free
+    __device__ __forceinline__ bool wait_free(int n, volatile int* abort) const { return n < N || umma::mbar_wait(freed(n), phase(n) ^ 1, abort); }
+    __device__ __forceinline__ void init() const {
+        for (int i = 0; i < N; ++i) {
+            umma::mbar_init(full + i, 1);
+            umma::mbar_init(empty + i, 1);
+        }
+    }
+    // after a wait that gave up: the copies in flight end before the CTA does
+    __device__ __forceinline__ void drain(int issued) const {
+        for (int i = issued > N ? issued - N : 0; i < issued; ++i) umma::mbar_wait(filled(i), phase(i));
+    }
 };
 // 128 x (168 - 72) registers go to the 256 threads of the exponentials
 __device__ __forceinline__ void regs_issue() { asm volatile("setmaxnreg.dec.sync.aligned.u32 72;\n"); }
 __device__ __forceinline__ void regs_rows() { asm volatile("setmaxnreg.inc.sync.aligned.u32 216;\n"); }
 
+// exp2(c s - shift) of 64 scores, a quarter of them on the FMA pipes where no key is hidden (whose value has to be an exact zero); shift(u) gives the pair of values for keys u, u + 1
+template <typename ShiftT>
+__device__ __forceinline__ void exponentials(float (&e)[64], float c, bool whole, ShiftT shift) {
+    const f32x2 c2 = pack2(c, c);
+    if (whole) {
+#pragma unroll
+        for (int u = 0; u < 64; u += 2) {
+            const f32x2 y = fma2(pack2(e[u], e[u + 1]), c2, shift(u));
+            float2 v = unpack2(y);
+            if (u % 8 == 6) v = exp2_poly(y);
+            else v = make_float2(exp2_fast(v.x), exp2_fast(v.y));
+            e[u] = v.x;
+            e[u + 1] = v.y;
+        }
+    } else {
+#pragma unroll
+        for (int u = 0; u < 64; u += 2) {
+            const float2 v = unpack2(fma2(pack2(e[u], e[u + 1]), c2, shift(u)));
+            e[u] = exp2_fast(v.x);
+            e[u + 1] = exp2_fast(v.y);
+        }
+    }
+}
 // 64 values of a row as bf16 into the first half of the columns they came from
 __device__ __forceinline__ void put_half(uint32_t taddr, const float (&v)[64]) {
 #pragma unroll
@@ -82,14 +129,15 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dq_tc_kernel(const __
     chain_wait();
     using namespace bwd;
     using SM = Smem<K>;
-    constexpr int NST = SM::NST, TM_S = 0, TM_DP = 256, TM_DQ = 384;         // S twice
-    extern __shared__ unsigned char smem_raw[];
-    unsigned char* smem = umma::align_1024(smem_raw);
+    constexpr int NA = SM::NA, NB = SM::NB, TM_S = 0, TM_DP = 256, TM_DQ = 384;         // S twice
+    extern __shared__ __align__(1024) unsigned char smem[];
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + SM::bar_off);
-    uint64_t *full = bars, *empty = bars + NST, *barQ = bars + 2 * NST, *barS = barQ + 1, *barDP = barS + 2, *barE = barDP + 1, *barDone = barE + 1;
+    const Ring<NA> ringK = {bars, bars + NA};
+    const Ring<NB> ringV = {bars + 2 * NA, bars + 2 * NA + NB};
+    uint64_t *barQ = bars + 2 * (NA + NB), *barS = barQ + 1, *barDP = barS + 2, *barE = barDP + 1, *barDone = barE + 1;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(barDone + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    static_assert((2 * NST + 6) * 8 + 8 <= 256, "barriers");
+    static_assert((2 * (NA + NB) + 6) * 8 + 8 <= 256, "barriers");
     float* sDelta = reinterpret_cast<float*>(smem + SM::stat_off);           // [2][128]: the halves of the rows' sums
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -98,10 +146,8 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dq_tc_kernel(const __
     const int steps = span.count();
     const auto tile = [&](int n) { return span.tile(n); };
     if (tid == 0) {
-        for (int i = 0; i < NST; ++i) {
-            umma::mbar_init(full + i, 1);
-            umma::mbar_init(empty + i, 1);
-        }
+        ringK.init();
+        ringV.init();
         umma::mbar_init(barQ, 1);
         umma::mbar_init(barS, 1);
         umma::mbar_init(barS + 1, 1);
@@ -121,42 +167,41 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dq_tc_kernel(const __
         regs_issue();
         if (warp == TMA_WARP && lane == 0) {
             tma::expect_tx(barQ, 2 * SM::TILE_BYTES);
-            load_tile<K>(smem + SM::a_off, &p.tq, h, q0, b, barQ);
-            load_tile<K>(smem + SM::a_off + SM::TILE_BYTES, &p.tdo, h, q0, b, barQ);
-            bool ok = true;
-            int n = 0;
-            for (; n < 2 * steps; ++n) {
-                const int st = n % NST;
-                if (n >= NST) ok = umma::mbar_wait(empty + st, (n / NST - 1) & 1, abort_flag);
-                if (!ok) break;
-                tma::expect_tx(full + st, SM::TILE_BYTES);
-                load_tile<K>(smem + SM::st_off + st * SM::TILE_BYTES, n & 1 ? &p.tv : &p.tk, grp, tile(n >> 1) * TILE, b, full + st);
+            load_tile<K>(smem + SM::stay_off, &p.tq, h, q0, b, barQ);
+            load_tile<K>(smem + SM::stay_off + SM::TILE_BYTES, &p.tdo, h, q0, b, barQ);
+            int nk = 0, nv = 0;
+            while (nv < steps) {
+                if (!ringK.wait_free(nk, abort_flag)) break;
+                tma::expect_tx(ringK.filled(nk), SM::TILE_BYTES);
+                load_tile<K>(smem + SM::a_off + nk % NA * SM::TILE_BYTES, &p.tk, grp, tile(nk) * TILE, b, ringK.filled(nk));
+                ++nk;
+                if (!ringV.wait_free(nv, abort_flag)) break;
+                tma::expect_tx(ringV.filled(nv), SM::TILE_BYTES);
+                load_tile<K>(smem + SM::b_off + nv % NB * SM::TILE_BYTES, &p.tv, grp, tile(nv) * TILE, b, ringV.filled(nv));
+                ++nv;
             }
-            // after a wait that gave up: the copies in flight end before the CTA does
             if (*abort_flag) {
                 umma::mbar_wait(barQ, 0);
-                for (int i = n > NST ? n - NST : 0; i < n; ++i) umma::mbar_wait(full + i % NST, (i / NST) & 1);
+                ringK.drain(nk);
+                ringV.drain(nv);
             }
         } else if (warp == MMA_WARP) {
-            const uint32_t lead = umma::elect_one(), sQ = umma::smem_addr(smem + SM::a_off), sDO = sQ + SM::TILE_BYTES, sT = umma::smem_addr(smem + SM::st_off);
+            const uint32_t lead = umma::elect_one(), sQ = umma::smem_addr(smem + SM::stay_off), sDO = sQ + SM::TILE_BYTES;
+            const uint32_t sK = umma::smem_addr(smem + SM::a_off), sV = umma::smem_addr(smem + SM::b_off);
             constexpr uint32_t idS = umma::idesc_bf16(128, 128, false, false), idQ = umma::idesc_bf16(128, K, false, true);
             bool ok = umma::mbar_wait_warp(barQ, 0, abort_flag);
-            const auto wait_tile = [&](int n) {                  // position n of the ring's sequence; its address
-                ok = ok && umma::mbar_wait_warp(full + n % NST, (n / NST) & 1, abort_flag);
-                return sT + (n % NST) * SM::TILE_BYTES;
-            };
             const auto scores = [&](int n) {
-                const uint32_t at = wait_tile(2 * n);
+                ok = ok && umma::mbar_wait_warp(ringK.filled(n), ringK.phase(n), abort_flag);
                 if (!ok) return;
-                umma::gemm_kk_lead<TILE, TILE, K>(lead, tmem + TM_S + 128 * (n & 1), sQ, at, idS, false);
+                umma::gemm_kk_lead<TILE, TILE, K>(lead, tmem + TM_S + 128 * (n & 1), sQ, sK + n % NA * SM::TILE_BYTES, idS, false);
                 umma::commit_lead(lead, barS + (n & 1));
             };
             const auto products = [&](int n) {
-                const uint32_t at = wait_tile(2 * n + 1);
+                ok = ok && umma::mbar_wait_warp(ringV.filled(n), ringV.phase(n), abort_flag);
                 if (!ok) return;
-                umma::gemm_kk_lead<TILE, TILE, K>(lead, tmem + TM_DP, sDO, at, idS, false);
+                umma::gemm_kk_lead<TILE, TILE, K>(lead, tmem + TM_DP, sDO, sV + n % NB * SM::TILE_BYTES, idS, false);
                 umma::commit_lead(lead, barDP);
-                umma::commit_lead(lead, empty + (2 * n + 1) % NST);
+                umma::commit_lead(lead, ringV.freed(n));
             };
             scores(0);
             products(0);
@@ -166,8 +211,8 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dq_tc_kernel(const __
                 umma::fence_after_sync();
                 if (n + 1 < steps) products(n + 1);
                 if (!ok) break;
-                gemm_halves<K>(lead, tmem + TM_DQ, tmem + TM_S + 128 * (n & 1), sT + (2 * n % NST) * SM::TILE_BYTES, idQ, n > 0);
-                umma::commit_lead(lead, empty + 2 * n % NST);
+                gemm_halves<K>(lead, tmem + TM_DQ, tmem + TM_S + 128 * (n & 1), sK + n % NA * SM::TILE_BYTES, idQ, n > 0);
+                umma::commit_lead(lead, ringK.freed(n));
             }
             if (ok) umma::commit_lead(lead, barDone);
         }
@@ -203,19 +248,27 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dq_tc_kernel(const __
             umma::fence_after_sync();
             float e[64], d[64];
             tmem_ld64(tS + 128 * (n & 1), e);
+            const bool whole = all_seen(q0, s0, p.window, p.sinks);
+            exponentials(e, c, whole, [&](int) { return pack2(-lse, -lse); });
+            if (!whole) {
 #pragma unroll
-            for (int i = 0; i < 64; ++i) e[i] = exp2_fast(fmaf(e[i], c, -lse));
-            if (!all_seen(q0, s0, p.window, p.sinks)) {
+                for (int i = 0; i < 64; i += 32) {
+                    const uint32_t bits = seen_bits(t, s0 + half * 64 + i, p.window, p.sinks);
 #pragma unroll
-                for (int i = 0; i < 64; ++i)
-                    if (!sees(t, s0 + half * 64 + i, p.window, p.sinks)) e[i] = 0.f;
+                    for (int u = 0; u < 32; ++u)
+                        if (!(bits & (1u << u))) e[i + u] = 0.f;
+                }
             }
             ok = umma::mbar_wait_warp(barDP, n & 1, abort_flag);
             if (!ok) break;
             umma::fence_after_sync();
             tmem_ld64(tDP, d);
 #pragma unroll
-            for (int i = 0; i < 64; ++i) e[i] *= d[i] - delta;
+            for (int i = 0; i < 64; i += 2) {
+                const float2 v = unpack2(mul2(pack2(e[i], e[i + 1]), add2(pack2(d[i], d[i + 1]), pack2(-delta, -delta))));
+                e[i] = v.x;
+                e[i + 1] = v.y;
+            }
             put_half(tS + 128 * (n & 1), e);
             if (lane == 0) arrive(barE);
         }
@@ -244,11 +297,12 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dkv_tc_kernel(const _
     chain_wait();
     using namespace bwd;
     using SM = Smem<K>;
-    constexpr int NST = SM::NST, TM_S = 0, TM_DP = 128, TM_DV = 256, TM_DK = 384;
-    extern __shared__ unsigned char smem_raw[];
-    unsigned char* smem = umma::align_1024(smem_raw);
+    constexpr int NA = SM::NA, NB = SM::NB, TM_S = 0, TM_DP = 128, TM_DV = 256, TM_DK = 384;
+    extern __shared__ __align__(1024) unsigned char smem[];
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + SM::bar_off);
-    uint64_t *full = bars, *empty = bars + NST, *barKV = bars + 2 * NST, *barS = barKV + 1, *barDP = barS + 1, *barP = barDP + 1, *barDS = barP + 1, *barDone = barDS + 1;
+    const Ring<NA> ringQ = {bars, bars + NA};
+    const Ring<NB> ringDO = {bars + 2 * NA, bars + 2 * NA + NB};
+    uint64_t *barKV = bars + 2 * (NA + NB), *barS = barKV + 1, *barDP = barS + 1, *barP = barDP + 1, *barDS = barP + 1, *barDone = barDS + 1;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(barDone + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     float* sStat = reinterpret_cast<float*>(smem + SM::stat_off);
@@ -263,10 +317,8 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dkv_tc_kernel(const _
     if (lo > last || heads <= 0) return;                    // (a share that the last tiles do not reach; fewer heads than shares)
     const int s0 = j * TILE, per = hi - lo + 1, steps = heads * per;
     if (tid == 0) {
-        for (int i = 0; i < NST; ++i) {
-            umma::mbar_init(full + i, 1);
-            umma::mbar_init(empty + i, 1);
-        }
+        ringQ.init();
+        ringDO.init();
         umma::mbar_init(barKV, 1);
         umma::mbar_init(barS, 1);
         umma::mbar_init(barDP, 1);
@@ -286,44 +338,46 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dkv_tc_kernel(const _
         regs_issue();
         if (warp == TMA_WARP && lane == 0) {
             tma::expect_tx(barKV, 2 * SM::TILE_BYTES);
-            load_tile<K>(smem + SM::a_off, &p.tk, grp, s0, b, barKV);
-            load_tile<K>(smem + SM::a_off + SM::TILE_BYTES, &p.tv, grp, s0, b, barKV);
-            bool ok = true;
-            int n = 0, h = h0, i = lo;
-            for (; n < 2 * steps; ++n) {
-                const int st = n % NST;
-                if (n >= NST) ok = umma::mbar_wait(empty + st, (n / NST - 1) & 1, abort_flag);
-                if (!ok) break;
-                tma::expect_tx(full + st, SM::TILE_BYTES + TILE * 4);
-                load_tile<K>(smem + SM::st_off + st * SM::TILE_BYTES, n & 1 ? &p.tdo : &p.tq, h, i * TILE, b, full + st);
-                load_stat(sStat + st * TILE, (n & 1 ? p.delta : p.lse) + ((long)b * p.H + h) * p.TP + i * TILE, full + st);
-                if ((n & 1) && ++i > hi) {
+            load_tile<K>(smem + SM::stay_off, &p.tk, grp, s0, b, barKV);
+            load_tile<K>(smem + SM::stay_off + SM::TILE_BYTES, &p.tv, grp, s0, b, barKV);
+            int nq = 0, nd = 0, h = h0, i = lo;
+            while (nd < steps) {
+                const long stat = ((long)b * p.H + h) * p.TP + i * TILE;
+                if (!ringQ.wait_free(nq, abort_flag)) break;
+                tma::expect_tx(ringQ.filled(nq), SM::TILE_BYTES + TILE * 4);
+                load_tile<K>(smem + SM::a_off + nq % NA * SM::TILE_BYTES, &p.tq, h, i * TILE, b, ringQ.filled(nq));
+                load_stat(sStat + nq % NA * TILE, p.lse + stat, ringQ.filled(nq));
+                ++nq;
+                if (!ringDO.wait_free(nd, abort_flag)) break;
+                tma::expect_tx(ringDO.filled(nd), SM::TILE_BYTES + TILE * 4);
+                load_tile<K>(smem + SM::b_off + nd % NB * SM::TILE_BYTES, &p.tdo, h, i * TILE, b, ringDO.filled(nd));
+                load_stat(sStat + (NA + nd % NB) * TILE, p.delta + stat, ringDO.filled(nd));
+                ++nd;
+                if (++i > hi) {
                     i = lo;
                     ++h;
                 }
             }
             if (*abort_flag) {
                 umma::mbar_wait(barKV, 0);
-                for (int m = n > NST ? n - NST : 0; m < n; ++m) umma::mbar_wait(full + m % NST, (m / NST) & 1);
+                ringQ.drain(nq);
+                ringDO.drain(nd);
             }
         } else if (warp == MMA_WARP) {
-            const uint32_t lead = umma::elect_one(), sK = umma::smem_addr(smem + SM::a_off), sV = sK + SM::TILE_BYTES, sT = umma::smem_addr(smem + SM::st_off);
+            const uint32_t lead = umma::elect_one(), sK = umma::smem_addr(smem + SM::stay_off), sV = sK + SM::TILE_BYTES;
+            const uint32_t sQ = umma::smem_addr(smem + SM::a_off), sDO = umma::smem_addr(smem + SM::b_off);
             constexpr uint32_t idS = umma::idesc_bf16(128, 128, false, false), idG = umma::idesc_bf16(128, K, false, true);
             bool ok = umma::mbar_wait_warp(barKV, 0, abort_flag);
-            const auto wait_tile = [&](int n) {
-                ok = ok && umma::mbar_wait_warp(full + n % NST, (n / NST) & 1, abort_flag);
-                return sT + (n % NST) * SM::TILE_BYTES;
-            };
             const auto scores = [&](int n) {
-                const uint32_t at = wait_tile(2 * n);
+                ok = ok && umma::mbar_wait_warp(ringQ.filled(n), ringQ.phase(n), abort_flag);
                 if (!ok) return;
-                umma::gemm_kk_lead<TILE, TILE, K>(lead, tmem + TM_S, sK, at, idS, false);
+                umma::gemm_kk_lead<TILE, TILE, K>(lead, tmem + TM_S, sK, sQ + n % NA * SM::TILE_BYTES, idS, false);
                 umma::commit_lead(lead, barS);
             };
             const auto products = [&](int n) {
-                const uint32_t at = wait_tile(2 * n + 1);
+                ok = ok && umma::mbar_wait_warp(ringDO.filled(n), ringDO.phase(n), abort_flag);
                 if (!ok) return;
-                umma::gemm_kk_lead<TILE, TILE, K>(lead, tmem + TM_DP, sV, at, idS, false);
+                umma::gemm_kk_lead<TILE, TILE, K>(lead, tmem + TM_DP, sV, sDO + n % NB * SM::TILE_BYTES, idS, false);
                 umma::commit_lead(lead, barDP);
             };
             scores(0);
@@ -332,15 +386,15 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dkv_tc_kernel(const _
                 ok = umma::mbar_wait_warp(barP, n & 1, abort_flag);
                 if (!ok) break;
                 umma::fence_after_sync();
-                gemm_halves<K>(lead, tmem + TM_DV, tmem + TM_S, sT + (2 * n + 1) % NST * SM::TILE_BYTES, idG, n > 0);
+                gemm_halves<K>(lead, tmem + TM_DV, tmem + TM_S, sDO + n % NB * SM::TILE_BYTES, idG, n > 0);
                 if (n + 1 < steps) scores(n + 1);
                 ok = ok && umma::mbar_wait_warp(barDS, n & 1, abort_flag);
                 if (!ok) break;
                 umma::fence_after_sync();
-                gemm_halves<K>(lead, tmem + TM_DK, tmem + TM_DP, sT + 2 * n % NST * SM::TILE_BYTES, idG, n > 0);
+                gemm_halves<K>(lead, tmem + TM_DK, tmem + TM_DP, sQ + n % NA * SM::TILE_BYTES, idG, n > 0);
                 // (delta, beside dO, is read until dS is there)
-                umma::commit_lead(lead, empty + (2 * n + 1) % NST);
-                umma::commit_lead(lead, empty + 2 * n % NST);
+                umma::commit_lead(lead, ringDO.freed(n));
+                umma::commit_lead(lead, ringQ.freed(n));
                 if (n + 1 < steps) products(n + 1);
             }
             if (ok) umma::commit_lead(lead, barDone);
@@ -355,38 +409,39 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dkv_tc_kernel(const _
         for (int n = 0; n < steps; ++n) {
             const int t0 = i * TILE;
             if (++i > hi) i = lo;
-            const float *lse = sStat + 2 * n % NST * TILE + half * 64, *delta = sStat + (2 * n + 1) % NST * TILE + half * 64;
-            ok = umma::mbar_wait_warp(full + 2 * n % NST, (2 * n / NST) & 1, abort_flag) && umma::mbar_wait_warp(barS, n & 1, abort_flag);
+            const float *lse = sStat + n % NA * TILE + half * 64, *delta = sStat + (NA + n % NB) * TILE + half * 64;
+            ok = umma::mbar_wait_warp(ringQ.filled(n), ringQ.phase(n), abort_flag) && umma::mbar_wait_warp(barS, n & 1, abort_flag);
             if (!ok) break;
             umma::fence_after_sync();
             float e[64], d[64];
             tmem_ld64(tS, e);
+            const bool whole = all_seen(t0, s0, p.window, p.sinks);
+            exponentials(e, c, whole, [&](int u) {
+                const float2 m = *reinterpret_cast<const float2*>(lse + u);
+                return pack2(-m.x, -m.y);
+            });
+            if (!whole) {
+                // token s is seen by the queries from s on, as far as the window goes; a sink by all of them
 #pragma unroll
-            for (int u = 0; u < 64; u += 4) {
-                const float4 m = *reinterpret_cast<const float4*>(lse + u);
-                e[u] = exp2_fast(fmaf(e[u], c, -m.x));
-                e[u + 1] = exp2_fast(fmaf(e[u + 1], c, -m.y));
-                e[u + 2] = exp2_fast(fmaf(e[u + 2], c, -m.z));
-                e[u + 3] = exp2_fast(fmaf(e[u + 3], c, -m.w));
-            }
-            if (!all_seen(t0, s0, p.window, p.sinks)) {
+                for (int k = 0; k < 64; k += 32) {
+                    const uint32_t bits = seeing_bits(t0 + half * 64 + k, s, p.window, p.sinks);
 #pragma unroll
-                for (int u = 0; u < 64; ++u)
-                    if (!sees(t0 + half * 64 + u, s, p.window, p.sinks)) e[u] = 0.f;
+                    for (int u = 0; u < 32; ++u)
+                        if (!(bits & (1u << u))) e[k + u] = 0.f;
+                }
             }
             put_half(tS, e);
             if (lane == 0) arrive(barP);
-            ok = umma::mbar_wait_warp(full + (2 * n + 1) % NST, ((2 * n + 1) / NST) & 1, abort_flag) && umma::mbar_wait_warp(barDP, n & 1, abort_flag);
+            ok = umma::mbar_wait_warp(ringDO.filled(n), ringDO.phase(n), abort_flag) && umma::mbar_wait_warp(barDP, n & 1, abort_flag);
             if (!ok) break;
             umma::fence_after_sync();
             tmem_ld64(tDP, d);
 #pragma unroll
-            for (int u = 0; u < 64; u += 4) {
-                const float4 m = *reinterpret_cast<const float4*>(delta + u);
-                e[u] *= d[u] - m.x;
-                e[u + 1] *= d[u + 1] - m.y;
-                e[u + 2] *= d[u + 2] - m.z;
-                e[u + 3] *= d[u + 3] - m.w;
+            for (int u = 0; u < 64; u += 2) {
+                const float2 m = *reinterpret_cast<const float2*>(delta + u);
+                const float2 v = unpack2(mul2(pack2(e[u], e[u + 1]), add2(pack2(d[u], d[u + 1]), pack2(-m.x, -m.y))));
+                e[u] = v.x;
+                e[u + 1] = v.y;
             }
             put_half(tDP, e);
             if (lane == 0) arrive(barDS);
