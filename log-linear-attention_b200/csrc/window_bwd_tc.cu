@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dq_tc_kernel(const __
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(barDone + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     static_assert((2 * (NA + NB) + 6) * 8 + 8 <= 256, "barriers");
-    float* sDelta = reinterpret_cast<float*>(smem + SM::stat_off);           // [2][128]: the halves of the rows' sums
+    float* sDelta = reinterpret_cast<float*>(smem + SM::stat_off);           // [128]
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int q0 = blockIdx.x * TILE, h = blockIdx.y, b = blockIdx.z, grp = h / (p.H / p.G);
@@ -223,22 +223,31 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dq_tc_kernel(const __
         const long at = (((long)b * p.T + t) * p.H + h) * K + half * (K / 2), stat = ((long)b * p.H + h) * p.TP + t;
         const uint32_t tS = umma::tmem_addr(tmem, warp, TM_S + 64 * half), tDP = umma::tmem_addr(tmem, warp, TM_DP + 64 * half);
         const float c = p.scale * LOG2E, lse = p.lse[stat];
-        float delta = 0.f;
-        if (there) {
+        // delta of the tile's rows: a warp takes 16 of them, K / 8 lanes a row (a thread a row: 10 k cycles, for loads that touch a line a lane)
+        constexpr int LANES = K / 8, ROWS = 32 / LANES;
+        uint4 xo[16 / ROWS], xd[16 / ROWS];
 #pragma unroll
-            for (int i = 0; i < K / 2; i += 8) {
-                const uint4 x = *reinterpret_cast<const uint4*>(p.o + at + i), y = *reinterpret_cast<const uint4*>(p.d_o + at + i);
-                const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    delta = fmaf(__uint_as_float(xs[u] << 16), __uint_as_float(ys[u] << 16), delta);
-                    delta = fmaf(__uint_as_float(xs[u] & 0xffff0000u), __uint_as_float(ys[u] & 0xffff0000u), delta);
-                }
-            }
+        for (int i = 0; i < 16 / ROWS; ++i) {
+            const int r = q0 + warp * 16 + i * ROWS + lane / LANES;
+            const long from = (((long)b * p.T + r) * p.H + h) * K + lane % LANES * 8;
+            xo[i] = r < p.T ? *reinterpret_cast<const uint4*>(p.o + from) : make_uint4(0, 0, 0, 0);
+            xd[i] = r < p.T ? *reinterpret_cast<const uint4*>(p.d_o + from) : make_uint4(0, 0, 0, 0);
         }
-        sDelta[half * TILE + row] = delta;
+#pragma unroll
+        for (int i = 0; i < 16 / ROWS; ++i) {
+            const uint32_t xs[4] = {xo[i].x, xo[i].y, xo[i].z, xo[i].w}, ys[4] = {xd[i].x, xd[i].y, xd[i].z, xd[i].w};
+            float d = 0.f;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                d = fmaf(__uint_as_float(xs[u] << 16), __uint_as_float(ys[u] << 16), d);
+                d = fmaf(__uint_as_float(xs[u] & 0xffff0000u), __uint_as_float(ys[u] & 0xffff0000u), d);
+            }
+#pragma unroll
+            for (int u = LANES / 2; u > 0; u >>= 1) d += __shfl_xor_sync(0xffffffffu, d, u);
+            if (lane % LANES == 0) sDelta[warp * 16 + i * ROWS + lane / LANES] = d;
+        }
         asm volatile("bar.sync 1, 256;\n" ::: "memory");
-        delta = sDelta[row] + sDelta[TILE + row];
+        const float delta = sDelta[row];
         if (half == 0) p.delta[stat] = delta;
         bool ok = true;
         for (int n = 0; n < steps; ++n) {
