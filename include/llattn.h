@@ -403,14 +403,15 @@ int llattn_recurrence_bwd(const void* x, int x_is_f32, const void* g, int g_is_f
 int llattn_recurrence_step(float* h, const void* x, int x_is_f32, const void* g, int g_is_f32, void* o, int B, int D, void* stream);
 
 /* Softmax attention over a sliding window with sinks: query t sees the tokens s <= t with t - s < window or s < sinks.  q, o, do, dq (B,T,H,K),
- * k, v, dk, dv (B,T,G,K) bf16, K in {64,128}; head h uses k / v head h / (H/G).  window >= 1, sinks >= 0, scale > 0.  lse (llattn_window_lse_bytes)
- * receives the softmax statistics that the backward reads; NULL in a forward without one.  The workspace (256 bytes for the forward,
+ * k, v, dk, dv (B,T,G,K) bf16, K in {64,128}; head h uses k / v head h / (H/G).  window >= 1, sinks >= 0, scale > 0.  stats (llattn_window_stats_bytes)
+ * receives what the backward reads beside o: the softmax statistics, and what rounding took off the outputs of rows that see few tokens; NULL in a forward
+ * without one.  The workspace (256 bytes for the forward,
  * llattn_window_workspace_bytes for the backward) begins with a status word, see above.  o, dq, dk and dv start at 32-byte boundaries.  Values that a query does not see have to be finite. */
-size_t llattn_window_lse_bytes(int B, int T, int H);
+size_t llattn_window_stats_bytes(int B, int T, int H, int K, int window, int sinks);
 size_t llattn_window_workspace_bytes(int B, int T, int H, int G, int K, int window, int sinks);
-int llattn_window_fwd(const void* q, const void* k, const void* v, void* o, float* lse, void* workspace, size_t workspace_bytes, int B, int T, int H, int G,
+int llattn_window_fwd(const void* q, const void* k, const void* v, void* o, void* stats, void* workspace, size_t workspace_bytes, int B, int T, int H, int G,
                       int K, int window, int sinks, float scale, void* stream);
-int llattn_window_bwd(const void* q, const void* k, const void* v, const void* o, const float* lse, const void* d_o, void* dq, void* dk, void* dv,
+int llattn_window_bwd(const void* q, const void* k, const void* v, const void* o, const void* stats, const void* d_o, void* dq, void* dk, void* dv,
                       void* workspace, size_t workspace_bytes, int B, int T, int H, int G, int K, int window, int sinks, float scale, void* stream);
 /* The cache of a decoding sequence: sinks + window slots of (G,K), k_cache and v_cache (B,sinks + window,G,K) bf16.  Token t is in slot t if t < sinks, else in
  * slot sinks + (t - sinks) % window.  counts (B,G): tokens seen so far, the same number for every head of a sequence.

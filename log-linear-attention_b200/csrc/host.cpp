@@ -33,7 +33,7 @@ using torch::autograd::variable_list;
     F(llattn_gdn_prompt) F(llattn_gdn_prompt_scratch_bytes) F(llattn_gdn_bwd_workspace_bytes) F(llattn_gdn_bwd)                      \
     F(llattn_gdn_bwd_kept_workspace_bytes) F(llattn_gdn_bwd_kept_bf16dv) F(llattn_gdn_bwd_kept_normed) F(llattn_gdn_grad_out) F(llattn_workspace_status) F(llattn_clear) \
     F(llattn_recurrence_states_bytes) F(llattn_recurrence_fwd) F(llattn_recurrence_bwd) F(llattn_recurrence_step)                    \
-    F(llattn_window_lse_bytes) F(llattn_window_workspace_bytes) F(llattn_window_fwd) F(llattn_window_bwd) F(llattn_window_fill)      \
+    F(llattn_window_stats_bytes) F(llattn_window_workspace_bytes) F(llattn_window_fwd) F(llattn_window_bwd) F(llattn_window_fill)      \
     F(llattn_window_step) F(llattn_layer_norm_bwd_workspace_bytes) F(llattn_layer_norm_fwd) F(llattn_layer_norm_bwd)
 
 struct Library {
@@ -904,15 +904,15 @@ bool window_operands(const Tensor& q, const Tensor& k, const Tensor& v, int64_t 
            window <= WINDOW_MAX && sinks <= WINDOW_MAX && (float)scale > 0.f && std::isfinite((float)scale);
 }
 struct Windowed {
-    Tensor o, lse;
+    Tensor o, stats;
 };
 Windowed window_fwd(const Tensor& q, const Tensor& k, const Tensor& v, int64_t window, int64_t sinks, double scale, bool keep, bool status, void* stream) {
     const int B = q.size(0), T = q.size(1), H = q.size(2), G = k.size(2), K = q.size(3);
     Windowed r;
     r.o = contiguous_like(q);
-    if (keep) r.lse = empty({(int64_t)(lib.llattn_window_lse_bytes(B, T, H) / sizeof(float))}, at::kFloat, q);
+    if (keep) r.stats = empty({(int64_t)lib.llattn_window_stats_bytes(B, T, H, K, (int)window, (int)sinks)}, at::kByte, q);
     const Tensor ws = empty({256}, at::kByte, q);
-    check(lib.llattn_window_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), r.o.data_ptr(), fptr(r.lse), ws.data_ptr(), 256, B, T, H, G, K, (int)window, (int)sinks,
+    check(lib.llattn_window_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), r.o.data_ptr(), ptr(r.stats), ws.data_ptr(), 256, B, T, H, G, K, (int)window, (int)sinks,
                                 (float)scale, stream),
           "llattn_window_fwd");
     if (status) check_status(ws, stream, "llattn_window_fwd");
@@ -921,12 +921,12 @@ Windowed window_fwd(const Tensor& q, const Tensor& k, const Tensor& v, int64_t w
 struct WindowGrads {
     Tensor dq, dk, dv;
 };
-WindowGrads window_bwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o, const Tensor& lse, const Tensor& d_o, int64_t window, int64_t sinks,
+WindowGrads window_bwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o, const Tensor& stats, const Tensor& d_o, int64_t window, int64_t sinks,
                        double scale, bool status, void* stream) {
     const int B = q.size(0), T = q.size(1), H = q.size(2), G = k.size(2), K = q.size(3);
     const WindowGrads r = {contiguous_like(q), contiguous_like(k), contiguous_like(v)};
     const Tensor ws = empty({(int64_t)lib.llattn_window_workspace_bytes(B, T, H, G, K, (int)window, (int)sinks)}, at::kByte, q);
-    check(lib.llattn_window_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), fptr(lse), d_o.data_ptr(), r.dq.data_ptr(), r.dk.data_ptr(),
+    check(lib.llattn_window_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), stats.data_ptr(), d_o.data_ptr(), r.dq.data_ptr(), r.dk.data_ptr(),
                                 r.dv.data_ptr(), ws.data_ptr(), ws.numel(), B, T, H, G, K, (int)window, (int)sinks, (float)scale, stream),
           "llattn_window_bwd");
     if (status) check_status(ws, stream, "llattn_window_bwd");
@@ -938,7 +938,7 @@ struct WindowAttention : torch::autograd::Function<WindowAttention> {
         const Tensor q_ = contiguous(q), k_ = contiguous(k), v_ = contiguous(v);
         const Windowed r = window_fwd(q_, k_, v_, window, sinks, scale, ctx != nullptr, status, on.stream);
         if (ctx) {
-            ctx->save_for_backward({q_, k_, v_, r.o, r.lse});
+            ctx->save_for_backward({q_, k_, v_, r.o, r.stats});
             ctx->saved_data["window"] = window;
             ctx->saved_data["sinks"] = sinks;
             ctx->saved_data["scale"] = scale;
@@ -967,16 +967,16 @@ py::object window_forward(const Tensor& q, const Tensor& k, const Tensor& v, int
     if (!window_operands(q, k, v, window, sinks, scale)) return py::none();
     On on(q);
     const Windowed r = window_fwd(contiguous(q), contiguous(k), contiguous(v), window, sinks, scale, true, status, on.stream);
-    return py::make_tuple(r.o, r.lse);
+    return py::make_tuple(r.o, r.stats);
 }
-py::object window_backward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o, const Tensor& lse, const Tensor& d_o, int64_t window, int64_t sinks,
+py::object window_backward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o, const Tensor& stats, const Tensor& d_o, int64_t window, int64_t sinks,
                            double scale, bool status) {
-    if (!window_operands(q, k, v, window, sinks, scale) || !bf16(o) || o.sizes() != q.sizes() || d_o.sizes() != q.sizes() || !is(lse, at::kFloat) ||
-        !lse.is_contiguous() || !same_device({q, o, lse, d_o}) ||
-        lse.numel() * sizeof(float) != lib.llattn_window_lse_bytes(q.size(0), q.size(1), q.size(2)))
+    if (!window_operands(q, k, v, window, sinks, scale) || !bf16(o) || o.sizes() != q.sizes() || d_o.sizes() != q.sizes() || !is(stats, at::kByte) ||
+        !stats.is_contiguous() || !same_device({q, o, stats, d_o}) ||
+        (size_t)stats.numel() != lib.llattn_window_stats_bytes(q.size(0), q.size(1), q.size(2), q.size(3), (int)window, (int)sinks))
         return py::none();
     On on(q);
-    const WindowGrads r = window_bwd(contiguous(q), contiguous(k), contiguous(v), contiguous(o), contiguous(lse), contiguous(d_o.to(at::kBFloat16)), window, sinks,
+    const WindowGrads r = window_bwd(contiguous(q), contiguous(k), contiguous(v), contiguous(o), contiguous(stats), contiguous(d_o.to(at::kBFloat16)), window, sinks,
                                      scale, status, on.stream);
     return py::make_tuple(r.dq, r.dk, r.dv);
 }

@@ -42,6 +42,13 @@ int check(long B, long T, long H, long G, int K, long window, long sinks, float 
     return 0;
 }
 int padded(int T) { return (T + TILE - 1) / TILE * TILE; }
+size_t lse_bytes(int B, int T, int H) { return (size_t)B * H * padded(T) * sizeof(float); }
+void statistics(Params& p, void* stats) {
+    if (!stats) return;
+    p.lse = static_cast<float*>(stats);
+    p.low = reinterpret_cast<bf16*>(static_cast<char*>(stats) + lse_bytes(p.B, p.T, p.H));
+    p.low_rows = low_rows(p.T, p.window, p.sinks);
+}
 void shape(Params& p, void* workspace, int B, int T, int H, int G, int window, int sinks, float scale) {
     p.err = static_cast<int*>(workspace);
     p.B = B;
@@ -65,27 +72,27 @@ using namespace llattn;
 
 extern "C" {
 
-size_t llattn_window_lse_bytes(int B, int T, int H) {
-    if (win::check(B, T, H, 1, 64, 1, 0, 1.f) != 0) return 0;
-    return (size_t)B * H * win::padded(T) * sizeof(float);
+size_t llattn_window_stats_bytes(int B, int T, int H, int K, int window, int sinks) {
+    if (win::check(B, T, H, 1, K, window, sinks, 1.f) != 0) return 0;
+    return win::lse_bytes(B, T, H) + (size_t)B * win::low_rows(T, window, sinks) * H * K * sizeof(win::bf16);
 }
 size_t llattn_window_workspace_bytes(int B, int T, int H, int G, int K, int window, int sinks) {
     if (win::check(B, T, H, G, K, window, sinks, 1.f) != 0) return 0;
     const win::Shares sh(B, T, H, G, window, sinks);
-    return 256 + llattn_window_lse_bytes(B, T, H) + (sh.near_floats(B, G, K) + sh.far_floats(B, G, K, sinks)) * sizeof(float);
+    return 256 + win::lse_bytes(B, T, H) + (sh.near_floats(B, G, K) + sh.far_floats(B, G, K, sinks)) * sizeof(float);
 }
 
-int llattn_window_fwd(const void* q, const void* k, const void* v, void* o, float* lse, void* workspace, size_t workspace_bytes, int B, int T, int H, int G, int K,
+int llattn_window_fwd(const void* q, const void* k, const void* v, void* o, void* stats, void* workspace, size_t workspace_bytes, int B, int T, int H, int G, int K,
                       int window, int sinks, float scale, void* stream) {
     const int rc = win::check(B, T, H, G, K, window, sinks, scale);
     if (rc != 0) return rc;
     if (!q || !k || !v || !o) return LLATTN_ERR_NULL;
-    if (misaligned(16, {q, k, v, lse}) || misaligned(32, {o})) return LLATTN_ERR_ALIGNMENT;
+    if (misaligned(16, {q, k, v}) || misaligned(32, {o, stats})) return LLATTN_ERR_ALIGNMENT;
     if (!workspace || misaligned(256, {workspace}) || workspace_bytes < 256) return LLATTN_ERR_WORKSPACE;
     win::Params p = {};
     p.out = (win::bf16*)o;
-    p.lse = lse;
     win::shape(p, workspace, B, T, H, G, window, sinks, scale);
+    win::statistics(p, stats);
     cudaStream_t st = (cudaStream_t)stream;
     const cudaError_t e = cudaMemsetAsync(workspace, 0, 4, st);        // (before the maps: the first runtime call of a thread gives it the context that they need)
     if (e != cudaSuccess) return (int)e;
@@ -93,12 +100,12 @@ int llattn_window_fwd(const void* q, const void* k, const void* v, void* o, floa
     return (int)win::forward_tc(p, K, st);
 }
 
-int llattn_window_bwd(const void* q, const void* k, const void* v, const void* o, const float* lse, const void* d_o, void* dq, void* dk, void* dv, void* workspace,
+int llattn_window_bwd(const void* q, const void* k, const void* v, const void* o, const void* stats, const void* d_o, void* dq, void* dk, void* dv, void* workspace,
                       size_t workspace_bytes, int B, int T, int H, int G, int K, int window, int sinks, float scale, void* stream) {
     const int rc = win::check(B, T, H, G, K, window, sinks, scale);
     if (rc != 0) return rc;
-    if (!q || !k || !v || !o || !lse || !d_o || !dq || !dk || !dv) return LLATTN_ERR_NULL;
-    if (misaligned(16, {q, k, v, o, lse, d_o}) || misaligned(32, {dq, dk, dv})) return LLATTN_ERR_ALIGNMENT;
+    if (!q || !k || !v || !o || !stats || !d_o || !dq || !dk || !dv) return LLATTN_ERR_NULL;
+    if (misaligned(16, {q, k, v, o, d_o}) || misaligned(32, {stats, dq, dk, dv})) return LLATTN_ERR_ALIGNMENT;
     if (!workspace || misaligned(256, {workspace}) || workspace_bytes < llattn_window_workspace_bytes(B, T, H, G, K, window, sinks)) return LLATTN_ERR_WORKSPACE;
     win::Params p = {};
     p.o = (const win::bf16*)o;
@@ -106,11 +113,11 @@ int llattn_window_bwd(const void* q, const void* k, const void* v, const void* o
     p.dq = (win::bf16*)dq;
     p.dk = (win::bf16*)dk;
     p.dv = (win::bf16*)dv;
-    p.lse = const_cast<float*>(lse);
     p.delta = reinterpret_cast<float*>(static_cast<char*>(workspace) + 256);
     p.near_part = p.delta + (long)B * H * win::padded(T);
     p.far_part = p.near_part + win::Shares(B, T, H, G, window, sinks).near_floats(B, G, K);
     win::shape(p, workspace, B, T, H, G, window, sinks, scale);
+    win::statistics(p, const_cast<void*>(stats));
     cudaStream_t st = (cudaStream_t)stream;
     const cudaError_t e = cudaMemsetAsync(workspace, 0, 4, st);
     if (e != cudaSuccess) return (int)e;

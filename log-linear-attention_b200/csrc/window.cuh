@@ -19,6 +19,8 @@ struct Params {
     const bf16 *q, *k, *v, *o, *d_o;
     bf16 *out, *dq, *dk, *dv;
     float *lse, *delta;               // (B,H,TP), TP the length up to whole tiles; lse = log2 of the sum, infinity behind the sequence
+    bf16* low;                        // (B,low_rows,H,K): what rounding took off the first rows of o
+    int low_rows;
     int* err;                         // status word of the workspace
     int B, T, TP, H, G, window, sinks;
     float scale;
@@ -56,6 +58,12 @@ struct Shares {
     size_t near_floats(int B, int G, int K) const { return (size_t)B * G * splits * near_tiles() * TILE * 2 * K; }
     size_t far_floats(int B, int G, int K, int sinks) const { return (size_t)B * G * far_tiles * chunks * far_rows(sinks) * 2 * K; }
 };
+
+// delta = do . o is subtracted from do . v.  For a row that sees n tokens the rounding of o to bf16 leaves an error in dS of sqrt(e / n) of the rounding of dS itself (the output is a mean
+// of about n / e values); where n is small it is the larger of the two (n = 2: dq and dk 3.1e-3 off in the place of 2.4e-3).  So the forward keeps what the rounding took off for
+// such rows: all of them where the window is short, else those of the first tile.
+constexpr int FEW = 64;
+inline int low_rows(int T, int window, int sinks) { return window + sinks < FEW || T < TILE ? T : TILE; }
 
 // The tiles of keys that the queries [q0, q0 + 128) see are the first `sink` ones and [lo, hi].
 struct Span {

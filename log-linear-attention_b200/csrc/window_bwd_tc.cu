@@ -246,6 +246,23 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dq_tc_kernel(const __
             for (int u = LANES / 2; u > 0; u >>= 1) d += __shfl_xor_sync(0xffffffffu, d, u);
             if (lane % LANES == 0) sDelta[warp * 16 + i * ROWS + lane / LANES] = d;
         }
+        if (q0 < p.low_rows) {                             // with what the rounding of o took off
+#pragma unroll
+            for (int i = 0; i < 16 / ROWS; ++i) {
+                const int r = q0 + warp * 16 + i * ROWS + lane / LANES;
+                const uint4 xl = r < p.low_rows ? *reinterpret_cast<const uint4*>(p.low + (((long)b * p.low_rows + r) * p.H + h) * K + lane % LANES * 8) : make_uint4(0, 0, 0, 0);
+                const uint32_t xs[4] = {xl.x, xl.y, xl.z, xl.w}, ys[4] = {xd[i].x, xd[i].y, xd[i].z, xd[i].w};
+                float d = 0.f;
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    d = fmaf(__uint_as_float(xs[u] << 16), __uint_as_float(ys[u] << 16), d);
+                    d = fmaf(__uint_as_float(xs[u] & 0xffff0000u), __uint_as_float(ys[u] & 0xffff0000u), d);
+                }
+#pragma unroll
+                for (int u = LANES / 2; u > 0; u >>= 1) d += __shfl_xor_sync(0xffffffffu, d, u);
+                if (lane % LANES == 0) sDelta[warp * 16 + i * ROWS + lane / LANES] += d;
+            }
+        }
         asm volatile("bar.sync 1, 256;\n" ::: "memory");
         const float delta = sDelta[row];
         if (half == 0) p.delta[stat] = delta;

@@ -246,10 +246,15 @@ __global__ void __launch_bounds__(fwd::NTHREADS, 1) window_fwd_tc_kernel(const _
             for (int i = 0; i < K; i += 16) {
                 float o[16];
                 umma::tmem_ld16(tO + i, o);
-                uint32_t w8[8];
+                uint32_t w8[8], l8[8];
 #pragma unroll
-                for (int u = 0; u < 8; ++u) w8[u] = pack_bf16(o[2 * u] * f, o[2 * u + 1] * f);
+                for (int u = 0; u < 8; ++u) {
+                    const float a = o[2 * u] * f, b = o[2 * u + 1] * f;
+                    w8[u] = pack_bf16(a, b);
+                    l8[u] = pack_bf16(a - __uint_as_float(w8[u] << 16), b - __uint_as_float(w8[u] & 0xffff0000u));
+                }
                 if (t < p.T) store_32B(out + i, w8);
+                if (t < p.low_rows) store_32B(p.low + (((long)b * p.low_rows + t) * p.H + h) * K + i, l8);
             }
             if (p.lse) p.lse[((long)b * p.H + h) * p.TP + t] = t < p.T ? m + log2f(sum) : INFINITY;
         }

@@ -103,7 +103,7 @@ def lib():
         ("llattn_recurrence_fwd", _I, [_P, _I, _P, _I] + [_P] * 4 + [_I] * 3 + [_P]),
         ("llattn_recurrence_bwd", _I, [_P, _I, _P, _I] + [_P] * 6 + [_I] * 3 + [_P]),
         ("llattn_recurrence_step", _I, [_P, _P, _I, _P, _I, _P, _I, _I, _P]),
-        ("llattn_window_lse_bytes", _Z, [_I] * 3),
+        ("llattn_window_stats_bytes", _Z, [_I] * 6),
         ("llattn_window_workspace_bytes", _Z, [_I] * 7),
         ("llattn_window_fwd", _I, [_P] * 6 + [_Z] + [_I] * 7 + [_F, _P]),
         ("llattn_window_bwd", _I, [_P] * 10 + [_Z] + [_I] * 7 + [_F, _P]),

@@ -12,13 +12,13 @@ the interface that mirrors the reference (`hattention/chunkwise.py`, `hattention
     llattn::l2norm_scale_bwd(x, dy, scale)                   -> dx
     llattn::recurrence_fwd(x, g, h0)                         -> (o, h_last, states)
     llattn::recurrence_bwd(x, g, states, do, dh_last)        -> (dx, dg, dh0)
-    llattn::window_fwd(q, k, v, window, sinks, scale)        -> (o, lse)
-    llattn::window_bwd(q, k, v, o, lse, do, window, sinks, scale) -> (dq, dk, dv)
+    llattn::window_fwd(q, k, v, window, sinks, scale)        -> (o, stats)
+    llattn::window_bwd(q, k, v, o, stats, do, window, sinks, scale) -> (dq, dk, dv)
     llattn::layer_norm_fwd(x, weight, bias, eps)             -> (y, stats)
     llattn::layer_norm_bwd(x, weight, stats, dy)             -> (dx, dweight, dbias)
 
 `workspace` of mamba2_fwd is the call's scratch (uint8); handing it to mamba2_bwd lets the backward read the
-segment-level states instead of recomputing them (pass an empty tensor to recompute).  `states`, `lse` and `stats` are what the forward
+segment-level states instead of recomputing them (pass an empty tensor to recompute).  `states` and `stats` are what the forward
 passes of the hybrid-stack operators keep for their backward passes.
 """
 from typing import Optional, Tuple
@@ -147,18 +147,18 @@ def window_fwd(q: _T, k: _T, v: _T, window: int, sinks: int, scale: float) -> Tu
 
 @window_fwd.register_fake
 def _(q, k, v, window, sinks, scale):
-    B, T, H, _ = q.shape
-    n = _lib.lib().llattn_window_lse_bytes(B, T, H) // 4
-    return q.new_empty(q.shape), q.new_empty((int(n),), dtype=torch.float32)
+    B, T, H, K = q.shape
+    n = _lib.lib().llattn_window_stats_bytes(B, T, H, K, window, sinks)
+    return q.new_empty(q.shape), q.new_empty((int(n),), dtype=torch.uint8)
 
 
 @torch.library.custom_op("llattn::window_bwd", mutates_args=())
-def window_bwd(q: _T, k: _T, v: _T, o: _T, lse: _T, do: _T, window: int, sinks: int, scale: float) -> Tuple[_T, _T, _T]:
-    return _taken(_lib.host().window_backward(q, k, v, o, lse, do, window, sinks, scale, _lib.CHECK_STATUS), "window_bwd")
+def window_bwd(q: _T, k: _T, v: _T, o: _T, stats: _T, do: _T, window: int, sinks: int, scale: float) -> Tuple[_T, _T, _T]:
+    return _taken(_lib.host().window_backward(q, k, v, o, stats, do, window, sinks, scale, _lib.CHECK_STATUS), "window_bwd")
 
 
 @window_bwd.register_fake
-def _(q, k, v, o, lse, do, window, sinks, scale):
+def _(q, k, v, o, stats, do, window, sinks, scale):
     return q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
 
 

@@ -99,8 +99,8 @@ def test_c_entries_reject_bad_arguments(pkg):
     assert wfwd(H=3) == -4 and wfwd(q=null) == -6 and wfwd(q=odd) == -9
     assert wfwd(ws=null) == -5 and wfwd(n=255) == -5 and wfwd(ws=P(4096 + 16)) == -5
     need = lib.llattn_window_workspace_bytes(1, 8, 4, 2, 64, 4, 0)
-    assert need >= 256 + 4 * 8 * 4 and lib.llattn_window_lse_bytes(1, 8, 4) >= 4 * 8 * 4
-    wbwd = lambda lse, n: lib.llattn_window_bwd(*[ok] * 4, lse, *[ok] * 5, n, 1, 8, 4, 2, 64, 4, 0, 1.0, null)
+    assert need >= 256 + 4 * 8 * 4 and lib.llattn_window_stats_bytes(1, 8, 4, 64, 4, 0) >= 4 * 8 * 4
+    wbwd = lambda stats, n: lib.llattn_window_bwd(*[ok] * 4, stats, *[ok] * 5, n, 1, 8, 4, 2, 64, 4, 0, 1.0, null)
     assert wbwd(null, need) == -6 and wbwd(odd, need) == -9 and wbwd(ok, need - 1) == -5
     assert lib.llattn_window_fill(null, ok, null, ok, ok, ok, 1, 8, 2, 64, 4, 0, null) == -6
     assert lib.llattn_window_fill(ok, ok, null, ok, odd, ok, 1, 8, 2, 64, 4, 0, null) == -9
@@ -125,8 +125,8 @@ def test_operators_trace_with_fake_tensors(pkg):
         dx, dg, dh = op.recurrence_bwd(x, x.float(), states, o, None)
         assert dx.dtype == torch.bfloat16 and dg.dtype == torch.float32 and dh.shape == (2, 6)
         q, k = torch.empty(1, 5, 4, 64, dtype=torch.bfloat16), torch.empty(1, 5, 2, 64, dtype=torch.bfloat16)
-        o, lse = op.window_fwd(q, k, k, 3, 1, 0.125)
-        assert [t.shape for t in op.window_bwd(q, k, k, o, lse, o, 3, 1, 0.125)] == [q.shape, k.shape, k.shape]
+        o, stats = op.window_fwd(q, k, k, 3, 1, 0.125)
+        assert [t.shape for t in op.window_bwd(q, k, k, o, stats, o, 3, 1, 0.125)] == [q.shape, k.shape, k.shape]
         w = torch.empty(6)
         y, stats = op.layer_norm_fwd(x, w, None, 1e-5)
         assert [t.shape for t in op.layer_norm_bwd(x, w, stats, y)] == [x.shape, w.shape, w.shape]
