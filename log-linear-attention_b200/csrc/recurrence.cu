@@ -4,8 +4,9 @@
 //     dh_t = do_t + e_{t+1},   dx_t = dh_t,   dg_t = e_t h_{t-1},   dh_0 = e_1.
 //
 // A run of tokens acts on a state as h -> A h + H, with A the product of its decays and H its own final state, and on e in the same form
-// from its other end; runs compose.  A warp takes RUN tokens of 32 VEC neighbouring channels, a CTA the runs of a tile of TILE tokens, a cluster of CTAs
-// neighbouring tiles of a strip of channels, and the cluster walks the strip: one pass over the data, all sums in fp32, in an order that the sizes alone decide.
+// from its other end; runs compose.  LPR lanes of a warp take RUN tokens of LPR VEC neighbouring channels, the others the runs behind them; a CTA takes the runs of a
+// tile of TILE tokens, a cluster of CTAs neighbouring tiles of a strip of channels, and the cluster walks the strip: one pass over the data, all sums in fp32, in an
+// order that the sizes alone decide.
 //
 // It is bound by memory as long as little else is issued.  Tiles come to shared memory by asynchronous copies a round ahead, each warp its own rows, and are
 // read, and their decays formed, once.  A cluster's barrier costs its CTAs about a microsecond a round, hence runs as long as registers and shared memory
@@ -76,34 +77,37 @@ struct Row<float, 2> {
     static __device__ __forceinline__ void store(float* p, const float (&v)[2]) { *reinterpret_cast<float2*>(p) = make_float2(v[0], v[1]); }
 };
 
-// A warp's RUN rows of 32 VEC values of a tensor in shared memory, brought there by asynchronous copies of CP bytes (0: by loads and stores); what lies behind
-// the sequence or the channels is filled with zeros, which change nothing (a decay of 1, nothing added).
-template <int RUN, typename E, int VEC, int CP>
+// A warp's rows (tokens) of LPR VEC values of a tensor in shared memory, RUN of them for each of its 32 / LPR runs, brought there by asynchronous copies of CP bytes (0: by
+// loads and stores); what lies behind the sequence or the channels is filled with zeros, which change nothing (a decay of 1, nothing added).  Runs are a row further
+// apart than they are long, so that lanes of different runs read different banks.
+template <int RUN, int LPR, typename E, int VEC, int CP>
 struct Stage {
-    static constexpr int ROW = 32 * VEC * sizeof(E), BYTES = RUN * ROW;
+    static constexpr int SUB = 32 / LPR, ROWS = SUB * RUN, ROW = LPR * VEC * sizeof(E), PAD = SUB > 1 ? ROW : 0, BYTES = ROWS * ROW + SUB * PAD;
     // `src`: row 0, channel 0 of the strip (read where `left` > 0 alone); `cols` channels and `left` tokens are there
     static __device__ __forceinline__ void issue(unsigned char* dst, const E* src, long ld, int left, int cols, int lane) {
         if constexpr (CP == 0) {
             static_assert(VEC == 1, "a value a lane");
+            const int first = lane / LPR * RUN, c = lane % LPR;
             E v[RUN];
 #pragma unroll
-            for (int i = 0; i < RUN; ++i) v[i] = i < left && lane < cols ? src[i * ld + lane] : E(0.f);
+            for (int i = 0; i < RUN; ++i) v[i] = first + i < left && c < cols ? src[(first + i) * ld + c] : E(0.f);
 #pragma unroll
-            for (int i = 0; i < RUN; ++i) reinterpret_cast<E*>(dst + i * ROW)[lane] = v[i];
+            for (int i = 0; i < RUN; ++i) reinterpret_cast<E*>(dst + (first + i) * ROW + lane / LPR * PAD)[c] = v[i];
         } else {
-            constexpr int PER = CP / (int)sizeof(E), A_ROW = ROW / CP, N = RUN * A_ROW / 32;              // values a copy, copies a row, copies a lane
-            static_assert(32 % A_ROW == 0, "a copy of the warp takes whole rows");
+            constexpr int PER = CP / (int)sizeof(E), A_ROW = ROW / CP, N = ROWS * A_ROW / 32;              // values a copy, copies a row, copies a lane
+            constexpr int STEP = 32 / A_ROW;                                                              // rows that a copy of the warp takes
+            static_assert(32 % A_ROW == 0 && (RUN % STEP == 0 || STEP % RUN == 0), "whole rows, and whole runs of them or parts of one run");
             const int row = lane / A_ROW, at = lane % A_ROW * PER;
-            const uint32_t to = (uint32_t)__cvta_generic_to_shared(dst + lane * CP);
+            const uint32_t to = (uint32_t)__cvta_generic_to_shared(dst + lane * CP) + (STEP > RUN ? row / RUN * PAD : 0);
             const E* from = src + row * ld + at;
-            if (left >= RUN && cols == 32 * VEC) {                                                        // most tiles: nothing to test
+            if (left >= ROWS && cols == LPR * VEC) {                                                      // most tiles: nothing to test
 #pragma unroll
-                for (int i = 0; i < N; ++i, from += 32 / A_ROW * ld) copy(to + i * 32 * CP, from, CP);
+                for (int i = 0; i < N; ++i, from += STEP * ld) copy(to + i * 32 * CP + i * STEP / RUN * PAD, from, CP);
             } else {
 #pragma unroll
-                for (int i = 0; i < N; ++i, from += 32 / A_ROW * ld) {
-                    const bool in = row + i * (32 / A_ROW) < left && at < cols;                           // (cols is a multiple of PER)
-                    copy(to + i * 32 * CP, in ? from : src, in ? CP : 0);
+                for (int i = 0; i < N; ++i, from += STEP * ld) {
+                    const bool in = row + i * STEP < left && at < cols;                                   // (cols is a multiple of PER)
+                    copy(to + i * 32 * CP + i * STEP / RUN * PAD, in ? from : src, in ? CP : 0);
                 }
             }
         }
@@ -113,9 +117,11 @@ struct Stage {
         if constexpr (CP == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(to), "l"(from), "r"(bytes) : "memory");
         else if constexpr (CP > 0) asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;\n" ::"r"(to), "l"(from), "n"(CP), "r"(bytes) : "memory");
     }
+    // the lane's run
     static __device__ __forceinline__ void read(const unsigned char* at, int lane, float (&v)[RUN][VEC]) {
+        at += lane / LPR * (RUN * ROW + PAD);
 #pragma unroll
-        for (int i = 0; i < RUN; ++i) Row<E, VEC>::load(reinterpret_cast<const E*>(at + i * ROW) + lane * VEC, v[i]);
+        for (int i = 0; i < RUN; ++i) Row<E, VEC>::load(reinterpret_cast<const E*>(at + i * ROW) + lane % LPR * VEC, v[i]);
     }
 };
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
@@ -130,66 +136,92 @@ __device__ __forceinline__ void decays(float (&a)[RUN][VEC]) {
 }
 
 // Where a CTA is, and what forward and backward do alike.
-template <int VEC, int TILE>
+template <int LPR, int VEC, int TILE>
 struct Place {
+    static constexpr int SUB = 32 / LPR;
     cg::cluster_group cluster;
-    int ranks, rank, lane, warp, b, c0, c, cols, NT, rounds;
+    int ranks, rank, lane, sub, col, warp, b, c0, c, cols, NT, rounds;
     bool there;
-    float2 (*all)[32][VEC];       // [2][ranks]: the cluster's tiles' (A, H) of every other round
+    float2 (*all)[LPR][VEC];      // [2][ranks]: the cluster's tiles' (A, H) of every other round
     __device__ Place(const Params& p, unsigned char* behind_slots) : cluster(cg::this_cluster()) {
         ranks = cluster.num_blocks();
         rank = cluster.block_rank();
         lane = threadIdx.x & 31;
+        sub = lane / LPR;
+        col = lane % LPR;
         warp = threadIdx.x >> 5;
         const int unit = blockIdx.x / ranks;
         b = unit / p.strips;
-        c0 = unit % p.strips * 32 * VEC;
-        c = c0 + lane * VEC;
-        cols = min(32 * VEC, p.D - c0);
+        c0 = unit % p.strips * LPR * VEC;
+        c = c0 + col * VEC;
+        cols = min(LPR * VEC, p.D - c0);
         there = c < p.D;
         NT = (p.T + TILE - 1) / TILE;
         rounds = (NT + ranks - 1) / ranks;
-        all = reinterpret_cast<float2(*)[32][VEC]>(behind_slots);
+        all = reinterpret_cast<float2(*)[LPR][VEC]>(behind_slots);
     }
-    // a round's (A, H) of this CTA's tile to every CTA of the cluster: warp w writes those of ranks w and w + 8
-    __device__ __forceinline__ void publish(int round, const float (&A)[VEC], const float (&H)[VEC]) {
-        for (int x = warp; x < ranks; x += WARPS) {
-            float2* to = cluster.map_shared_rank(&all[(round & 1) * ranks + rank][lane][0], x);
+    // Takes `carry` over the round's tiles, in the order of the ranks, given (A, H) of this CTA's; `mine` is what reaches it.  Every run of a warp writes to other ranks.
+    __device__ __forceinline__ void exchange(int round, const float (&A)[VEC], const float (&H)[VEC], float (&carry)[VEC], float (&mine)[VEC]) {
+        for (int x = warp * SUB + sub; x < ranks; x += WARPS * SUB) {
+            float2* to = cluster.map_shared_rank(&all[(round & 1) * ranks + rank][col][0], x);
 #pragma unroll
             for (int u = 0; u < VEC; ++u) to[u] = make_float2(A[u], H[u]);
         }
-        asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
-    }
-    // takes `carry` over the round's tiles, in the order of the ranks; `mine` is what reaches this CTA's
-    __device__ __forceinline__ void collect(int round, float (&carry)[VEC], float (&mine)[VEC]) {
-        asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+        __syncwarp();
+        cluster.sync();
         for (int x = 0; x < ranks; ++x)
 #pragma unroll
             for (int u = 0; u < VEC; ++u) {
-                const float2 r = all[(round & 1) * ranks + x][lane][u];
+                const float2 r = all[(round & 1) * ranks + x][col][u];
                 if (x == rank) mine[u] = carry[u];
                 carry[u] = fmaf(r.x, carry[u], r.y);
             }
     }
 };
 
-template <typename X, typename G, int VEC, int CPX, int CPG>
+// (A, H) of a run -> of the warp's runs up to it and, in (Ae, He), of those before it.  UP: tokens in order, else from the last run on.
+template <bool UP, int LPR>
+__device__ __forceinline__ void warp_scan(int sub, float& A, float& H, float& Ae, float& He) {
+    constexpr int SUB = 32 / LPR;
+    const int place = UP ? sub : SUB - 1 - sub;
+#pragma unroll
+    for (int d = 1; d < SUB; d *= 2) {
+        const float a = UP ? __shfl_up_sync(0xffffffffu, A, d * LPR) : __shfl_down_sync(0xffffffffu, A, d * LPR);
+        const float h = UP ? __shfl_up_sync(0xffffffffu, H, d * LPR) : __shfl_down_sync(0xffffffffu, H, d * LPR);
+        if (place >= d) {
+            H = fmaf(A, h, H);
+            A *= a;
+        }
+    }
+    Ae = 1.f;
+    He = 0.f;
+    if constexpr (SUB > 1) {
+        const float a = UP ? __shfl_up_sync(0xffffffffu, A, LPR) : __shfl_down_sync(0xffffffffu, A, LPR);
+        const float h = UP ? __shfl_up_sync(0xffffffffu, H, LPR) : __shfl_down_sync(0xffffffffu, H, LPR);
+        if (place > 0) {
+            Ae = a;
+            He = h;
+        }
+    }
+}
+
+template <typename X, typename G, int LPR, int VEC, int CPX, int CPG>
 __global__ void __launch_bounds__(32 * WARPS, 2) recurrence_fwd_kernel(const __grid_constant__ Params p) {
     chain_wait();
-    constexpr int RUN = FWD_RUN, TILE = WARPS * RUN;
+    constexpr int RUN = FWD_RUN, SUB = 32 / LPR, TILE = WARPS * SUB * RUN;
     static_assert(STATES % RUN == 0, "states are kept at the starts of runs");
-    using SX = Stage<RUN, X, VEC, CPX>;
-    using SG = Stage<RUN, G, VEC, CPG>;
+    using SX = Stage<RUN, LPR, X, VEC, CPX>;
+    using SG = Stage<RUN, LPR, G, VEC, CPG>;
     constexpr int BYTES = SX::BYTES + SG::BYTES;
     extern __shared__ __align__(16) unsigned char staged[];           // [SLOTS][WARPS][BYTES], then Place::all
-    __shared__ float2 agg[2][WARPS][32][VEC];                         // (A, H) of the warps' runs, for every other round
-    Place<VEC, TILE> at(p, staged + SLOTS * WARPS * BYTES);
+    __shared__ float2 agg[2][WARPS][LPR][VEC];                        // (A, H) of the warps' runs, for every other round
+    Place<LPR, VEC, TILE> at(p, staged + SLOTS * WARPS * BYTES);
     const int lane = at.lane, warp = at.warp;
     const long ld = p.D, base = (long)at.b * p.T * ld + at.c0;
     const auto slot = [&](int round) { return staged + (round % SLOTS * WARPS + warp) * BYTES; };
     const auto bring = [&](int round) {
         if (round < at.rounds) {
-            const int t0 = (round * at.ranks + at.rank) * TILE + warp * RUN, left = p.T - t0;
+            const int t0 = (round * at.ranks + at.rank) * TILE + warp * SUB * RUN, left = p.T - t0;
             const long from = base + (left > 0 ? t0 * ld : 0);
             SX::issue(slot(round), static_cast<const X*>(p.x) + from, ld, left, at.cols, lane);
             SG::issue(slot(round) + SX::BYTES, static_cast<const G*>(p.g) + from, ld, left, at.cols, lane);
@@ -202,24 +234,24 @@ __global__ void __launch_bounds__(32 * WARPS, 2) recurrence_fwd_kernel(const __g
 #pragma unroll
     for (int u = 0; u < VEC; ++u) carry[u] = p.h0 && at.there ? p.h0[(long)at.b * p.D + at.c + u] : 0.f;
     for (int round = 0; round < at.rounds; ++round) {
-        const int t0 = (round * at.ranks + at.rank) * TILE + warp * RUN, left = p.T - t0;      // (a tile behind the last changes nothing)
+        const int t0 = (round * at.ranks + at.rank) * TILE + (warp * SUB + at.sub) * RUN, left = p.T - t0;      // (a tile behind the last changes nothing)
         bring(round + 1);                                             // (into the slot of the round before, which all lanes have read)
         copies_but<1>();
         __syncwarp();
-        float v[RUN][VEC], a[RUN][VEC], A[VEC], H[VEC], h[VEC];
+        float v[RUN][VEC], a[RUN][VEC], h[VEC], Ae[VEC], He[VEC];
         SX::read(slot(round), lane, v);
         SG::read(slot(round) + SX::BYTES, lane, a);
         decays<RUN, VEC>(a);
 #pragma unroll
         for (int u = 0; u < VEC; ++u) {
-            A[u] = 1.f;
-            H[u] = 0.f;
+            float A = 1.f, H = 0.f;
 #pragma unroll
             for (int i = 0; i < RUN; ++i) {
-                A[u] *= a[i][u];
-                H[u] = fmaf(a[i][u], H[u], v[i][u]);
+                A *= a[i][u];
+                H = fmaf(a[i][u], H, v[i][u]);
             }
-            agg[round & 1][warp][lane][u] = make_float2(A[u], H[u]);
+            warp_scan<true, LPR>(at.sub, A, H, Ae[u], He[u]);
+            if (at.sub == SUB - 1) agg[round & 1][warp][at.col][u] = make_float2(A, H);
         }
         __syncthreads();
         if (at.ranks == 1) {
@@ -227,12 +259,12 @@ __global__ void __launch_bounds__(32 * WARPS, 2) recurrence_fwd_kernel(const __g
             for (int w = 0; w < WARPS; ++w)
 #pragma unroll
                 for (int u = 0; u < VEC; ++u) {
-                    const float2 r = agg[round & 1][w][lane][u];
+                    const float2 r = agg[round & 1][w][at.col][u];
                     if (w == warp) h[u] = carry[u];
                     carry[u] = fmaf(r.x, carry[u], r.y);
                 }
         } else {
-            float Ab[VEC], Hb[VEC], mine[VEC];                        // of the runs before this warp's; A, H: of the tile
+            float A[VEC], H[VEC], Ab[VEC], Hb[VEC], mine[VEC];        // of the tile; of the warps before this one
 #pragma unroll
             for (int u = 0; u < VEC; ++u) {
                 A[u] = 1.f;
@@ -242,7 +274,7 @@ __global__ void __launch_bounds__(32 * WARPS, 2) recurrence_fwd_kernel(const __g
             for (int w = 0; w < WARPS; ++w)
 #pragma unroll
                 for (int u = 0; u < VEC; ++u) {
-                    const float2 r = agg[round & 1][w][lane][u];
+                    const float2 r = agg[round & 1][w][at.col][u];
                     if (w == warp) {
                         Ab[u] = A[u];
                         Hb[u] = H[u];
@@ -250,15 +282,18 @@ __global__ void __launch_bounds__(32 * WARPS, 2) recurrence_fwd_kernel(const __g
                     A[u] *= r.x;
                     H[u] = fmaf(r.x, H[u], r.y);
                 }
-            at.publish(round, A, H);
-            at.collect(round, carry, mine);
+            at.exchange(round, A, H, carry, mine);
 #pragma unroll
             for (int u = 0; u < VEC; ++u) h[u] = fmaf(Ab[u], mine[u], Hb[u]);
+        }
+        if constexpr (SUB > 1) {
+#pragma unroll
+            for (int u = 0; u < VEC; ++u) h[u] = fmaf(Ae[u], h[u], He[u]);
         }
         if (p.starts && t0 % STATES == 0 && at.there && left > 0)
             Row<float, VEC>::store(p.starts + ((long)at.b * ((p.T + STATES - 1) / STATES) + t0 / STATES) * p.D + at.c, h);
         if (at.there) {
-            X* o = static_cast<X*>(p.o) + base + t0 * ld + lane * VEC;
+            X* o = static_cast<X*>(p.o) + base + t0 * ld + at.col * VEC;
 #pragma unroll
             for (int i = 0; i < RUN; ++i, o += ld) {
                 if (i < left) {
@@ -270,29 +305,29 @@ __global__ void __launch_bounds__(32 * WARPS, 2) recurrence_fwd_kernel(const __g
         }
         __syncwarp();
     }
-    if (p.h_last && at.rank == 0 && warp == 0 && at.there) Row<float, VEC>::store(p.h_last + (long)at.b * p.D + at.c, carry);
+    if (p.h_last && at.rank == 0 && threadIdx.x < LPR && at.there) Row<float, VEC>::store(p.h_last + (long)at.b * p.D + at.c, carry);
 }
 
 // The same from the other end: e takes the place of the state, the cluster's tiles are counted from the last one.  The states before a tile's tokens are
 // made again from the one that the forward kept.
-template <typename X, typename G, int VEC, int CPX, int CPG>
+template <typename X, typename G, int LPR, int VEC, int CPX, int CPG>
 __global__ void __launch_bounds__(32 * WARPS, 2) recurrence_bwd_kernel(const __grid_constant__ Params p) {
     chain_wait();
-    constexpr int RUN = BWD_RUN, TILE = WARPS * RUN;
+    constexpr int RUN = BWD_RUN, SUB = 32 / LPR, TILE = WARPS * SUB * RUN;
     static_assert(TILE % STATES == 0, "a tile starts where a state is kept");
-    using SX = Stage<RUN, X, VEC, CPX>;
-    using SG = Stage<RUN, G, VEC, CPG>;
+    using SX = Stage<RUN, LPR, X, VEC, CPX>;
+    using SG = Stage<RUN, LPR, G, VEC, CPG>;
     constexpr int BYTES = 2 * SX::BYTES + SG::BYTES;
     extern __shared__ __align__(16) unsigned char staged[];
-    __shared__ float agg[2][3][WARPS][32][VEC];                       // A, H and E of the warps' runs
-    Place<VEC, TILE> at(p, staged + SLOTS * WARPS * BYTES);
+    __shared__ float agg[2][3][WARPS][LPR][VEC];                      // A, H and E of the warps' runs
+    Place<LPR, VEC, TILE> at(p, staged + SLOTS * WARPS * BYTES);
     const int lane = at.lane, warp = at.warp, NS = (p.T + STATES - 1) / STATES;
     const long ld = p.D, base = (long)at.b * p.T * ld + at.c0;
     const auto tile_of = [&](int round) { return at.NT - 1 - round * at.ranks - at.rank; };        // (below 0: nothing there)
     const auto slot = [&](int round) { return staged + (round % SLOTS * WARPS + warp) * BYTES; };
     const auto bring = [&](int round) {
         if (round < at.rounds) {
-            const int tile = tile_of(round), t0 = tile * TILE + warp * RUN, left = tile < 0 ? 0 : p.T - t0;
+            const int tile = tile_of(round), t0 = tile * TILE + warp * SUB * RUN, left = tile < 0 ? 0 : p.T - t0;
             const long from = base + (left > 0 ? t0 * ld : 0);
             SX::issue(slot(round), static_cast<const X*>(p.x) + from, ld, left, at.cols, lane);
             SX::issue(slot(round) + SX::BYTES, static_cast<const X*>(p.d_o) + from, ld, left, at.cols, lane);
@@ -306,9 +341,9 @@ __global__ void __launch_bounds__(32 * WARPS, 2) recurrence_bwd_kernel(const __g
 #pragma unroll
     for (int u = 0; u < VEC; ++u) carry[u] = p.h0 && at.there ? p.h0[(long)at.b * p.D + at.c + u] : 0.f;
     for (int round = 0; round < at.rounds; ++round) {
-        const int tile = tile_of(round), t0 = tile * TILE + warp * RUN, left = tile < 0 ? 0 : p.T - t0, par = round & 1;
+        const int tile = tile_of(round), t0 = tile * TILE + (warp * SUB + at.sub) * RUN, left = tile < 0 ? 0 : p.T - t0, par = round & 1;
         bring(round + 1);
-        float v[RUN][VEC], a[RUN][VEC], d[RUN][VEC], h[VEC], e[VEC];
+        float v[RUN][VEC], a[RUN][VEC], d[RUN][VEC], h[VEC], e[VEC], Au[VEC], Hu[VEC], Ad[VEC], Ed[VEC];
 #pragma unroll
         for (int u = 0; u < VEC; ++u) h[u] = at.there && tile >= 0 ? p.starts[((long)at.b * NS + tile * (TILE / STATES)) * p.D + at.c + u] : 0.f;
         copies_but<1>();
@@ -326,57 +361,66 @@ __global__ void __launch_bounds__(32 * WARPS, 2) recurrence_bwd_kernel(const __g
                 H = fmaf(a[i][u], H, v[i][u]);
                 E = a[RUN - 1 - i][u] * (d[RUN - 1 - i][u] + E);
             }
-            agg[par][0][warp][lane][u] = A;
-            agg[par][1][warp][lane][u] = H;
-            agg[par][2][warp][lane][u] = E;
+            float A2 = A;
+            warp_scan<true, LPR>(at.sub, A, H, Au[u], Hu[u]);
+            warp_scan<false, LPR>(at.sub, A2, E, Ad[u], Ed[u]);
+            if (at.sub == SUB - 1) {
+                agg[par][0][warp][at.col][u] = A;
+                agg[par][1][warp][at.col][u] = H;
+            }
+            if (at.sub == 0) agg[par][2][warp][at.col][u] = E;
         }
         __syncthreads();
 #pragma unroll
         for (int u = 0; u < VEC; ++u)
 #pragma unroll
             for (int w = 0; w < WARPS; ++w)
-                if (w < warp) h[u] = fmaf(agg[par][0][w][lane][u], h[u], agg[par][1][w][lane][u]);
+                if (w < warp) h[u] = fmaf(agg[par][0][w][at.col][u], h[u], agg[par][1][w][at.col][u]);
         if (at.ranks == 1) {
 #pragma unroll
             for (int u = 0; u < VEC; ++u)
 #pragma unroll
                 for (int w = WARPS - 1; w >= 0; --w) {
                     if (w == warp) e[u] = carry[u];
-                    carry[u] = fmaf(agg[par][0][w][lane][u], carry[u], agg[par][2][w][lane][u]);
+                    carry[u] = fmaf(agg[par][0][w][at.col][u], carry[u], agg[par][2][w][at.col][u]);
                 }
         } else {
-            float A[VEC], E[VEC], Ab[VEC], Eb[VEC], mine[VEC];        // of the tile; of the runs behind this warp's
+            float A[VEC], E[VEC], Ab[VEC], Eb[VEC], mine[VEC];        // of the tile; of the warps behind this one
 #pragma unroll
             for (int u = 0; u < VEC; ++u) {
                 A[u] = 1.f;
                 E[u] = 0.f;
 #pragma unroll
                 for (int w = WARPS - 1; w >= 0; --w) {
-                    const float aw = agg[par][0][w][lane][u];
+                    const float aw = agg[par][0][w][at.col][u];
                     if (w == warp) {
                         Ab[u] = A[u];
                         Eb[u] = E[u];
                     }
                     A[u] *= aw;
-                    E[u] = fmaf(aw, E[u], agg[par][2][w][lane][u]);
+                    E[u] = fmaf(aw, E[u], agg[par][2][w][at.col][u]);
                 }
             }
-            at.publish(round, A, E);
-            at.collect(round, carry, mine);
+            at.exchange(round, A, E, carry, mine);
 #pragma unroll
             for (int u = 0; u < VEC; ++u) e[u] = fmaf(Ab[u], mine[u], Eb[u]);
         }
         // the states before the run's tokens, in the place of x
 #pragma unroll
-        for (int u = 0; u < VEC; ++u)
+        for (int u = 0; u < VEC; ++u) {
+            if constexpr (SUB > 1) {
+                h[u] = fmaf(Au[u], h[u], Hu[u]);
+                e[u] = fmaf(Ad[u], e[u], Ed[u]);
+            }
 #pragma unroll
             for (int i = 0; i < RUN; ++i) {
                 const float next = fmaf(a[i][u], h[u], v[i][u]);
                 v[i][u] = h[u];
                 h[u] = next;
             }
+        }
         if (at.there && left > 0) {
-            const long to = base + t0 * ld + lane * VEC;
+            const long to = base + t0 * ld + at.col * VEC;
             X* dx = static_cast<X*>(p.dx) + to;
             G* dg = static_cast<G*>(p.dg) + to;
 #pragma unroll
@@ -396,7 +440,7 @@ __global__ void __launch_bounds__(32 * WARPS, 2) recurrence_bwd_kernel(const __g
         }
         __syncwarp();
     }
-    if (p.h_last && at.rank == 0 && warp == 0 && at.there) Row<float, VEC>::store(p.h_last + (long)at.b * p.D + at.c, carry);
+    if (p.h_last && at.rank == 0 && threadIdx.x < LPR && at.there) Row<float, VEC>::store(p.h_last + (long)at.b * p.D + at.c, carry);
 }
 
 template <typename X, typename G>
@@ -412,78 +456,113 @@ __global__ void __launch_bounds__(256) recurrence_step_kernel(float* h, const X*
     Row<X, 1>::store(o + i, v);
 }
 
-// Clusters of as many CTAs as there are tiles, and as run at once for all strips: a second wave costs what the first one does.
+// How many CTAs share a strip: as many as there are tiles, and as run at once for all strips, since a second wave costs what the first one does.
 template <typename KernT>
-cudaError_t launch(KernT kern, const Params& p, long units, int NT, size_t smem, size_t tile, cudaStream_t st) {
-    struct Room {
-        int dev;
-        const void* kern;
-        int clusters[MAX_RANKS + 1];          // of n CTAs that the device runs at once (0: not asked yet)
-    };
-    static thread_local Room room = {-1, nullptr, {}};        // (a template's own: one a kernel)
-    int dev;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return e;
-    if (room.dev != dev || room.kern != reinterpret_cast<const void*>(kern)) {
-        e = allow_smem(kern, smem + 2 * MAX_RANKS * tile);
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-        if (e != cudaSuccess) return e;
-        room = Room{dev, reinterpret_cast<const void*>(kern), {}};
+struct Launch {
+    KernT kern;
+    long units;                       // sequences x strips
+    int NT;
+    size_t smem, summary;             // of a CTA, and more for each CTA of the cluster
+    cudaLaunchAttribute attr[2];
+    cudaLaunchConfig_t cfg;
+    int ranks;
+    Launch(KernT kern, long units, int NT, size_t smem, size_t summary) : kern(kern), units(units), NT(NT), smem(smem), summary(summary), attr{}, cfg{}, ranks(1) {
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[1].val.programmaticStreamSerializationAllowed = 1;
+        cfg.blockDim = dim3(32 * WARPS);
     }
-    cudaLaunchAttribute attr[2] = {};
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.blockDim = dim3(32 * WARPS);
-    cfg.stream = st;
-    cfg.attrs = attr;
-    int n = NT < MAX_RANKS ? NT : MAX_RANKS;
-    for (;; --n) {
+    void clusters_of(int n) {
+        ranks = n;
         attr[0].val.clusterDim.x = n;
         cfg.gridDim = dim3((unsigned)(units * n));
-        cfg.dynamicSmemBytes = smem + 2 * n * tile;
-        if (n == 1) break;
-        if (units * n > 148 * 8) continue;    // (more than could be there)
-        if (room.clusters[n] == 0) {
-            cfg.numAttrs = 1;
-            e = cudaOccupancyMaxActiveClusters(&room.clusters[n], kern, &cfg);
-            if (e != cudaSuccess) return e;
-            if (room.clusters[n] == 0) room.clusters[n] = -1;
-        }
-        if (room.clusters[n] >= units) break;
+        cfg.dynamicSmemBytes = smem + 2 * n * summary;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
     }
-    cfg.numAttrs = 2;
-    e = cudaLaunchKernelEx(&cfg, kern, p);
-    if (e == cudaSuccess) LLATTN_LAUNCHED();
-    return e;
+    cudaError_t choose() {
+        struct Room {
+            int dev;
+            const void* kern;
+            int clusters[MAX_RANKS + 1];          // of n CTAs that the device runs at once (0: not asked yet)
+        };
+        static thread_local Room table[128] = {};
+        int dev;
+        cudaError_t e = cudaGetDevice(&dev);
+        if (e != cudaSuccess) return e;
+        Room& room = table[((reinterpret_cast<uintptr_t>(kern) >> 4) + dev) & 127];
+        if (room.dev != dev || room.kern != reinterpret_cast<const void*>(kern)) {
+            e = allow_smem(kern, smem + 2 * MAX_RANKS * summary);
+            if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+            if (e != cudaSuccess) return e;
+            room = Room{dev, reinterpret_cast<const void*>(kern), {}};
+        }
+        for (int n = NT < MAX_RANKS ? NT : MAX_RANKS; n > 1; --n) {
+            clusters_of(n);
+            if (units * n > 148 * 8) continue;    // (more than could be there)
+            if (room.clusters[n] == 0) {
+                e = cudaOccupancyMaxActiveClusters(&room.clusters[n], kern, &cfg);
+                if (e != cudaSuccess) return e;
+                if (room.clusters[n] == 0) room.clusters[n] = -1;
+            }
+            if (room.clusters[n] >= units) return cudaSuccess;
+        }
+        clusters_of(1);
+        return cudaSuccess;
+    }
+    // Rounds, weighted with what one takes (us, backward of bf16 with fp32 decays and 64 x 64 values a tile: one CTA a strip 2.4, four 3.5, fourteen 5.4; narrow strips, by
+    // themselves, 3.1), for waves of two CTAs an SM.
+    float cost(int LPR) const {
+        const int rounds = (NT + ranks - 1) / ranks;
+        const long waves = (units * ranks + 2 * 148 - 1) / (2 * 148);
+        return (float)(rounds * waves) * (LPR == 32 ? 1.f : LPR == 16 ? 1.15f : 1.25f) * (1.f + 0.1f * (float)(ranks - 1));
+    }
+    cudaError_t go(const Params& p, cudaStream_t st) {
+        cfg.stream = st;
+        cfg.attrs = attr;
+        cfg.numAttrs = 2;
+        const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
+        if (e == cudaSuccess) LLATTN_LAUNCHED();
+        return e;
+    }
+};
+// LPR lanes of VEC channels a run; copies of CPX and CPG bytes (0: straight loads)
+template <bool BACK, typename X, typename G, int LPR, int VEC, int CPX, int CPG>
+auto launch_of(const Params& p, int B) {
+    constexpr int RUN = BACK ? BWD_RUN : FWD_RUN, TILE = WARPS * (32 / LPR) * RUN;
+    constexpr size_t SMEM = (size_t)SLOTS * WARPS * ((BACK ? 2 : 1) * Stage<RUN, LPR, X, VEC, CPX>::BYTES + Stage<RUN, LPR, G, VEC, CPG>::BYTES);
+    const long units = (long)B * ((p.D + LPR * VEC - 1) / (LPR * VEC));
+    if constexpr (BACK) return Launch<void (*)(Params)>(recurrence_bwd_kernel<X, G, LPR, VEC, CPX, CPG>, units, (p.T + TILE - 1) / TILE, SMEM, LPR * VEC * sizeof(float2));
+    else return Launch<void (*)(Params)>(recurrence_fwd_kernel<X, G, LPR, VEC, CPX, CPG>, units, (p.T + TILE - 1) / TILE, SMEM, LPR * VEC * sizeof(float2));
 }
-// VEC channels a lane; copies of CPX and CPG bytes (0: straight loads)
-template <typename X, typename G, int VEC, int CPX, int CPG>
-cudaError_t scan_as(bool backward, Params p, int B, cudaStream_t st) {
-    p.strips = (p.D + 32 * VEC - 1) / (32 * VEC);
-    const int tile = WARPS * (backward ? BWD_RUN : FWD_RUN), NT = (p.T + tile - 1) / tile;
-    const size_t smem = (size_t)SLOTS * tile * 32 * VEC * ((backward ? 2 : 1) * sizeof(X) + sizeof(G));
-    const long units = (long)B * p.strips;
-    if (backward) return launch(recurrence_bwd_kernel<X, G, VEC, CPX, CPG>, p, units, NT, smem, 32 * VEC * sizeof(float2), st);
-    return launch(recurrence_fwd_kernel<X, G, VEC, CPX, CPG>, p, units, NT, smem, 32 * VEC * sizeof(float2), st);
+// Strips as wide as a warp, or a half or a quarter of that with longer tiles: clusters of many CTAs wait longer for each other than narrow strips cost.
+template <bool BACK, typename X, typename G, int VEC, int CPX, int CPG>
+cudaError_t scan_with(Params p, int B, cudaStream_t st) {
+    Launch<void (*)(Params)> l[3] = {launch_of<BACK, X, G, 32, VEC, CPX, CPG>(p, B), launch_of<BACK, X, G, 16, VEC, CPX, CPG>(p, B), launch_of<BACK, X, G, 8, VEC, CPX, CPG>(p, B)};
+    int best = 0;
+    for (int i = 0; i < 3; ++i) {
+        const cudaError_t e = l[i].choose();
+        if (e != cudaSuccess) return e;
+        if (l[i].cost(32 >> i) < l[best].cost(32 >> best)) best = i;
+        if (l[i].ranks == 1) break;               // (narrower ones would only be slower)
+    }
+    p.strips = (p.D + (32 >> best) * VEC - 1) / ((32 >> best) * VEC);
+    return l[best].go(p, st);
 }
 // Copies as wide as rows of D values start: 16 bytes where D fills whole words of them, else the pair or the value of a lane.
-template <typename X, typename G>
-cudaError_t scan(bool backward, const Params& p, int B, cudaStream_t st) {
-    if (p.D % (16 / (int)sizeof(X)) == 0) return scan_as<X, G, 2, 16, 16>(backward, p, B, st);
-    if (p.D % 2 == 0) return scan_as<X, G, 2, 2 * sizeof(X), 2 * sizeof(G)>(backward, p, B, st);
-    if (sizeof(X) == 4) return scan_as<X, G, 1, 4, 4>(backward, p, B, st);
-    return scan_as<X, G, 1, 0, 0>(backward, p, B, st);
+template <bool BACK, typename X, typename G>
+cudaError_t scan(const Params& p, int B, cudaStream_t st) {
+    if (p.D % (16 / (int)sizeof(X)) == 0) return scan_with<BACK, X, G, 2, 16, 16>(p, B, st);
+    if (p.D % 2 == 0) return scan_with<BACK, X, G, 2, 2 * sizeof(X), 2 * sizeof(G)>(p, B, st);
+    if constexpr (sizeof(X) == 4) return scan_with<BACK, X, G, 1, 4, 4>(p, B, st);
+    else return scan_with<BACK, X, G, 1, 0, 0>(p, B, st);
 }
-int scan_of(bool backward, int x_f32, int g_f32, const Params& p, int B, void* stream) {
+template <bool BACK>
+int scan_of(int x_f32, int g_f32, const Params& p, int B, void* stream) {
     cudaStream_t st = (cudaStream_t)stream;
-    cudaError_t e;
-    if (x_f32) e = scan<float, float>(backward, p, B, st);
-    else if (g_f32) e = scan<bf16, float>(backward, p, B, st);
-    else e = scan<bf16, bf16>(backward, p, B, st);
-    return (int)e;
+    if (x_f32) return (int)scan<BACK, float, float>(p, B, st);
+    return (int)(g_f32 ? scan<BACK, bf16, float>(p, B, st) : scan<BACK, bf16, bf16>(p, B, st));
 }
 int check(int x_f32, int g_f32, long B, long T, long D) {
     if (B < 1 || T < 1 || D < 1 || (x_f32 && !g_f32)) return LLATTN_ERR_UNSUPPORTED_SHAPE;
@@ -518,7 +597,7 @@ int llattn_recurrence_fwd(const void* x, int x_is_f32, const void* g, int g_is_f
     p.starts = states;
     p.T = T;
     p.D = D;
-    return rec::scan_of(false, x_is_f32, g_is_f32, p, B, stream);
+    return rec::scan_of<false>(x_is_f32, g_is_f32, p, B, stream);
 }
 
 int llattn_recurrence_bwd(const void* x, int x_is_f32, const void* g, int g_is_f32, const float* states, const void* d_o, const float* dh_last,
@@ -538,7 +617,7 @@ int llattn_recurrence_bwd(const void* x, int x_is_f32, const void* g, int g_is_f
     p.starts = const_cast<float*>(states);
     p.T = T;
     p.D = D;
-    return rec::scan_of(true, x_is_f32, g_is_f32, p, B, stream);
+    return rec::scan_of<true>(x_is_f32, g_is_f32, p, B, stream);
 }
 
 int llattn_recurrence_step(float* h, const void* x, int x_is_f32, const void* g, int g_is_f32, void* o, int B, int D, void* stream) {
