@@ -14,6 +14,7 @@
 
 #include "../../include/llattn.h"
 #include "launch_count.h"
+#include "pairs.cuh"
 
 namespace llattn {
 namespace norm {
@@ -34,50 +35,6 @@ __device__ __forceinline__ float get(const float* p) { return *p; }
 __device__ __forceinline__ float get(const bf16* p) { return __bfloat162float(*p); }
 __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 __device__ __forceinline__ void put(bf16* p, float v) { *p = __float2bfloat16(v); }
-
-// ---- one value, or two in one 64-bit register
-struct F2 {
-    unsigned long long v;
-};
-__device__ __forceinline__ F2 pair(float lo, float hi) {
-    F2 r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(lo), "f"(hi));
-    return r;
-}
-__device__ __forceinline__ float2 both(F2 a) {
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
-    return r;
-}
-__device__ __forceinline__ F2 add(F2 a, F2 b) {
-    F2 r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-    return r;
-}
-__device__ __forceinline__ F2 mul(F2 a, F2 b) {
-    F2 r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-    return r;
-}
-__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
-    F2 r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-    return r;
-}
-__device__ __forceinline__ float add(float a, float b) { return a + b; }
-__device__ __forceinline__ float mul(float a, float b) { return a * b; }
-__device__ __forceinline__ float fma2(float a, float b, float c) { return fmaf(a, b, c); }
-__device__ __forceinline__ float total(F2 a) {
-    const float2 f = both(a);
-    return f.x + f.y;
-}
-__device__ __forceinline__ float total(float a) { return a; }
-template <typename T>
-__device__ __forceinline__ T splat(float a);
-template <>
-__device__ __forceinline__ float splat<float>(float a) { return a; }
-template <>
-__device__ __forceinline__ F2 splat<F2>(float a) { return pair(a, a); }
 
 // VEC neighbouring values of a row as N numbers; VEC is 1 or a multiple of a 16-byte word
 template <int VEC>

@@ -17,6 +17,7 @@
 
 #include "../../include/llattn.h"
 #include "launch_count.h"
+#include "pairs.cuh"
 
 namespace llattn {
 namespace rec {
@@ -44,37 +45,44 @@ __device__ __forceinline__ float decay(float g) {
     return y;
 }
 
-template <typename E, int VEC>
-struct Row;
-template <>
-struct Row<bf16, 1> {
-    static __device__ __forceinline__ void load(const bf16* p, float (&v)[1]) { v[0] = __bfloat162float(*p); }
-    static __device__ __forceinline__ void store(bf16* p, const float (&v)[1]) { *p = __float2bfloat16(v[0]); }
+__device__ __forceinline__ F2 decay(F2 g) {
+    const float2 t = both(mul(g, splat<F2>(1.4426950408889634f)));
+    float2 y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y.x) : "f"(t.x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y.y) : "f"(t.y));
+    return pair(y.x, y.y);
+}
+
+// The VEC channels of a lane as a number: one value, or a pair.
+template <int VEC>
+struct Number {
+    typedef F2 T;
 };
 template <>
-struct Row<bf16, 2> {
-    static __device__ __forceinline__ void load(const bf16* p, float (&v)[2]) {
-        const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(p));
-        v[0] = f.x;
-        v[1] = f.y;
-    }
-    static __device__ __forceinline__ void store(bf16* p, const float (&v)[2]) {
-        *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(v[0], v[1]);
-    }
+struct Number<1> {
+    typedef float T;
 };
-template <>
-struct Row<float, 1> {
-    static __device__ __forceinline__ void load(const float* p, float (&v)[1]) { v[0] = *p; }
-    static __device__ __forceinline__ void store(float* p, const float (&v)[1]) { *p = v[0]; }
-};
-template <>
-struct Row<float, 2> {
-    static __device__ __forceinline__ void load(const float* p, float (&v)[2]) {
-        const float2 f = *reinterpret_cast<const float2*>(p);
-        v[0] = f.x;
-        v[1] = f.y;
-    }
-    static __device__ __forceinline__ void store(float* p, const float (&v)[2]) { *reinterpret_cast<float2*>(p) = make_float2(v[0], v[1]); }
+__device__ __forceinline__ void load(const bf16* p, float& v) { v = __bfloat162float(*p); }
+__device__ __forceinline__ void load(const float* p, float& v) { v = *p; }
+__device__ __forceinline__ void load(const bf16* p, F2& v) {
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(p);
+    v = pair(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+__device__ __forceinline__ void load(const float* p, F2& v) { v.v = *reinterpret_cast<const unsigned long long*>(p); }
+__device__ __forceinline__ void store(bf16* p, float v) { *p = __float2bfloat16(v); }
+__device__ __forceinline__ void store(float* p, float v) { *p = v; }
+__device__ __forceinline__ void store(bf16* p, F2 v) {
+    const float2 f = both(v);
+    uint32_t w;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(f.y), "f"(f.x));
+    *reinterpret_cast<uint32_t*>(p) = w;
+}
+__device__ __forceinline__ void store(float* p, F2 v) { *reinterpret_cast<unsigned long long*>(p) = v.v; }
+// (A, H): h -> A h + H
+template <typename T>
+struct Map {
+    T A, H;
+    __device__ __forceinline__ T operator()(T h) const { return fma2(A, h, H); }
 };
 
 // A warp's rows (tokens) of LPR VEC values of a tensor in shared memory, RUN of them for each of its 32 / LPR runs, brought there by asynchronous copies of CP bytes (0: by
@@ -118,23 +126,15 @@ struct Stage {
         else if constexpr (CP > 0) asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;\n" ::"r"(to), "l"(from), "n"(CP), "r"(bytes) : "memory");
     }
     // the lane's run
-    static __device__ __forceinline__ void read(const unsigned char* at, int lane, float (&v)[RUN][VEC]) {
+    static __device__ __forceinline__ void read(const unsigned char* at, int lane, typename Number<VEC>::T (&v)[RUN]) {
         at += lane / LPR * (RUN * ROW + PAD);
 #pragma unroll
-        for (int i = 0; i < RUN; ++i) Row<E, VEC>::load(reinterpret_cast<const E*>(at + i * ROW) + lane % LPR * VEC, v[i]);
+        for (int i = 0; i < RUN; ++i) load(reinterpret_cast<const E*>(at + i * ROW) + lane % LPR * VEC, v[i]);
     }
 };
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void copies_but() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory"); }
-template <int RUN, int VEC>
-__device__ __forceinline__ void decays(float (&a)[RUN][VEC]) {
-#pragma unroll
-    for (int i = 0; i < RUN; ++i)
-#pragma unroll
-        for (int u = 0; u < VEC; ++u) a[i][u] = decay(a[i][u]);
-}
-
 // Where a CTA is, and what forward and backward do alike.
 template <int LPR, int VEC, int TILE>
 struct Place {
@@ -142,7 +142,8 @@ struct Place {
     cg::cluster_group cluster;
     int ranks, rank, lane, sub, col, warp, b, c0, c, cols, NT, rounds;
     bool there;
-    float2 (*all)[LPR][VEC];      // [2][ranks]: the cluster's tiles' (A, H) of every other round
+    typedef typename Number<VEC>::T T;
+    Map<T> (*all)[LPR];           // [2][ranks]: the cluster's tiles', of every other round
     __device__ Place(const Params& p, unsigned char* behind_slots) : cluster(cg::this_cluster()) {
         ranks = cluster.num_blocks();
         rank = cluster.block_rank();
@@ -158,51 +159,41 @@ struct Place {
         there = c < p.D;
         NT = (p.T + TILE - 1) / TILE;
         rounds = (NT + ranks - 1) / ranks;
-        all = reinterpret_cast<float2(*)[LPR][VEC]>(behind_slots);
+        all = reinterpret_cast<Map<T>(*)[LPR]>(behind_slots);
     }
-    // Takes `carry` over the round's tiles, in the order of the ranks, given (A, H) of this CTA's; `mine` is what reaches it.  Every run of a warp writes to other ranks.
-    __device__ __forceinline__ void exchange(int round, const float (&A)[VEC], const float (&H)[VEC], float (&carry)[VEC], float (&mine)[VEC]) {
-        for (int x = warp * SUB + sub; x < ranks; x += WARPS * SUB) {
-            float2* to = cluster.map_shared_rank(&all[(round & 1) * ranks + rank][col][0], x);
-#pragma unroll
-            for (int u = 0; u < VEC; ++u) to[u] = make_float2(A[u], H[u]);
-        }
+    // Takes `carry` over the round's tiles, in the order of the ranks, given this CTA's; returns what reaches it.  Every run of a warp writes to other ranks.
+    __device__ __forceinline__ T exchange(int round, const Map<T>& m, T& carry) {
+        for (int x = warp * SUB + sub; x < ranks; x += WARPS * SUB) *cluster.map_shared_rank(&all[(round & 1) * ranks + rank][col], x) = m;
         __syncwarp();
         cluster.sync();
-        for (int x = 0; x < ranks; ++x)
-#pragma unroll
-            for (int u = 0; u < VEC; ++u) {
-                const float2 r = all[(round & 1) * ranks + x][col][u];
-                if (x == rank) mine[u] = carry[u];
-                carry[u] = fmaf(r.x, carry[u], r.y);
-            }
+        T mine = carry;
+        for (int x = 0; x < ranks; ++x) {
+            if (x == rank) mine = carry;
+            carry = all[(round & 1) * ranks + x][col](carry);
+        }
+        return mine;
     }
 };
 
-// (A, H) of a run -> of the warp's runs up to it and, in (Ae, He), of those before it.  UP: tokens in order, else from the last run on.
-template <bool UP, int LPR>
-__device__ __forceinline__ void warp_scan(int sub, float& A, float& H, float& Ae, float& He) {
+// A run's map -> that of the warp's runs up to it; returns that of those before it.  UP: tokens in order, else from the last run on.
+template <bool UP, int LPR, typename T>
+__device__ __forceinline__ Map<T> warp_scan(int sub, Map<T>& m) {
     constexpr int SUB = 32 / LPR;
     const int place = UP ? sub : SUB - 1 - sub;
+    Map<T> before = {splat<T>(1.f), splat<T>(0.f)};
 #pragma unroll
     for (int d = 1; d < SUB; d *= 2) {
-        const float a = UP ? __shfl_up_sync(0xffffffffu, A, d * LPR) : __shfl_down_sync(0xffffffffu, A, d * LPR);
-        const float h = UP ? __shfl_up_sync(0xffffffffu, H, d * LPR) : __shfl_down_sync(0xffffffffu, H, d * LPR);
+        const T a = UP ? shfl_up(m.A, d * LPR) : shfl_down(m.A, d * LPR), h = UP ? shfl_up(m.H, d * LPR) : shfl_down(m.H, d * LPR);
         if (place >= d) {
-            H = fmaf(A, h, H);
-            A *= a;
+            m.H = fma2(m.A, h, m.H);
+            m.A = mul(m.A, a);
         }
     }
-    Ae = 1.f;
-    He = 0.f;
     if constexpr (SUB > 1) {
-        const float a = UP ? __shfl_up_sync(0xffffffffu, A, LPR) : __shfl_down_sync(0xffffffffu, A, LPR);
-        const float h = UP ? __shfl_up_sync(0xffffffffu, H, LPR) : __shfl_down_sync(0xffffffffu, H, LPR);
-        if (place > 0) {
-            Ae = a;
-            He = h;
-        }
+        const T a = UP ? shfl_up(m.A, LPR) : shfl_down(m.A, LPR), h = UP ? shfl_up(m.H, LPR) : shfl_down(m.H, LPR);
+        if (place > 0) before = Map<T>{a, h};
     }
+    return before;
 }
 
 template <typename X, typename G, int LPR, int VEC, int CPX, int CPG>
@@ -214,7 +205,8 @@ __global__ void __launch_bounds__(32 * WARPS, 2) recurrence_fwd_kernel(const __g
     using SG = Stage<RUN, LPR, G, VEC, CPG>;
     constexpr int BYTES = SX::BYTES + SG::BYTES;
     extern __shared__ __align__(16) unsigned char staged[];           // [SLOTS][WARPS][BYTES], then Place::all
-    __shared__ float2 agg[2][WARPS][LPR][VEC];                        // (A, H) of the warps' runs, for every other round
+    typedef typename Number<VEC>::T T;
+    __shared__ Map<T> agg[2][WARPS][LPR];                             // of the warps' runs, for every other round
     Place<LPR, VEC, TILE> at(p, staged + SLOTS * WARPS * BYTES);
     const int lane = at.lane, warp = at.warp;
     const long ld = p.D, base = (long)at.b * p.T * ld + at.c0;
@@ -230,82 +222,58 @@ __global__ void __launch_bounds__(32 * WARPS, 2) recurrence_fwd_kernel(const __g
     };
     bring(0);
     if (at.ranks > 1) at.cluster.sync();                              // every CTA is there to be written to
-    float carry[VEC];
-#pragma unroll
-    for (int u = 0; u < VEC; ++u) carry[u] = p.h0 && at.there ? p.h0[(long)at.b * p.D + at.c + u] : 0.f;
+    T carry = splat<T>(0.f);
+    if (p.h0 && at.there) load(p.h0 + (long)at.b * p.D + at.c, carry);
     for (int round = 0; round < at.rounds; ++round) {
         const int t0 = (round * at.ranks + at.rank) * TILE + (warp * SUB + at.sub) * RUN, left = p.T - t0;      // (a tile behind the last changes nothing)
         bring(round + 1);                                             // (into the slot of the round before, which all lanes have read)
         copies_but<1>();
         __syncwarp();
-        float v[RUN][VEC], a[RUN][VEC], h[VEC], Ae[VEC], He[VEC];
+        T v[RUN], a[RUN], h;
         SX::read(slot(round), lane, v);
         SG::read(slot(round) + SX::BYTES, lane, a);
-        decays<RUN, VEC>(a);
+        Map<T> m = {splat<T>(1.f), splat<T>(0.f)};
 #pragma unroll
-        for (int u = 0; u < VEC; ++u) {
-            float A = 1.f, H = 0.f;
-#pragma unroll
-            for (int i = 0; i < RUN; ++i) {
-                A *= a[i][u];
-                H = fmaf(a[i][u], H, v[i][u]);
-            }
-            warp_scan<true, LPR>(at.sub, A, H, Ae[u], He[u]);
-            if (at.sub == SUB - 1) agg[round & 1][warp][at.col][u] = make_float2(A, H);
+        for (int i = 0; i < RUN; ++i) {
+            a[i] = decay(a[i]);
+            m.A = mul(m.A, a[i]);
+            m.H = fma2(a[i], m.H, v[i]);
         }
+        const Map<T> before = warp_scan<true, LPR>(at.sub, m);
+        if (at.sub == SUB - 1) agg[round & 1][warp][at.col] = m;
         __syncthreads();
         if (at.ranks == 1) {
 #pragma unroll
-            for (int w = 0; w < WARPS; ++w)
-#pragma unroll
-                for (int u = 0; u < VEC; ++u) {
-                    const float2 r = agg[round & 1][w][at.col][u];
-                    if (w == warp) h[u] = carry[u];
-                    carry[u] = fmaf(r.x, carry[u], r.y);
-                }
-        } else {
-            float A[VEC], H[VEC], Ab[VEC], Hb[VEC], mine[VEC];        // of the tile; of the warps before this one
-#pragma unroll
-            for (int u = 0; u < VEC; ++u) {
-                A[u] = 1.f;
-                H[u] = 0.f;
+            for (int w = 0; w < WARPS; ++w) {
+                if (w == warp) h = carry;
+                carry = agg[round & 1][w][at.col](carry);
             }
+        } else {
+            Map<T> all = {splat<T>(1.f), splat<T>(0.f)}, warps;       // of the tile; of the warps before this one
 #pragma unroll
-            for (int w = 0; w < WARPS; ++w)
-#pragma unroll
-                for (int u = 0; u < VEC; ++u) {
-                    const float2 r = agg[round & 1][w][at.col][u];
-                    if (w == warp) {
-                        Ab[u] = A[u];
-                        Hb[u] = H[u];
-                    }
-                    A[u] *= r.x;
-                    H[u] = fmaf(r.x, H[u], r.y);
-                }
-            at.exchange(round, A, H, carry, mine);
-#pragma unroll
-            for (int u = 0; u < VEC; ++u) h[u] = fmaf(Ab[u], mine[u], Hb[u]);
+            for (int w = 0; w < WARPS; ++w) {
+                const Map<T> r = agg[round & 1][w][at.col];
+                if (w == warp) warps = all;
+                all.A = mul(all.A, r.A);
+                all.H = r(all.H);
+            }
+            h = warps(at.exchange(round, all, carry));
         }
-        if constexpr (SUB > 1) {
-#pragma unroll
-            for (int u = 0; u < VEC; ++u) h[u] = fmaf(Ae[u], h[u], He[u]);
-        }
-        if (p.starts && t0 % STATES == 0 && at.there && left > 0)
-            Row<float, VEC>::store(p.starts + ((long)at.b * ((p.T + STATES - 1) / STATES) + t0 / STATES) * p.D + at.c, h);
+        if constexpr (SUB > 1) h = before(h);
+        if (p.starts && t0 % STATES == 0 && at.there && left > 0) store(p.starts + ((long)at.b * ((p.T + STATES - 1) / STATES) + t0 / STATES) * p.D + at.c, h);
         if (at.there) {
             X* o = static_cast<X*>(p.o) + base + t0 * ld + at.col * VEC;
 #pragma unroll
             for (int i = 0; i < RUN; ++i, o += ld) {
                 if (i < left) {
-#pragma unroll
-                    for (int u = 0; u < VEC; ++u) h[u] = fmaf(a[i][u], h[u], v[i][u]);
-                    Row<X, VEC>::store(o, h);
+                    h = fma2(a[i], h, v[i]);
+                    store(o, h);
                 }
             }
         }
         __syncwarp();
     }
-    if (p.h_last && at.rank == 0 && threadIdx.x < LPR && at.there) Row<float, VEC>::store(p.h_last + (long)at.b * p.D + at.c, carry);
+    if (p.h_last && at.rank == 0 && threadIdx.x < LPR && at.there) store(p.h_last + (long)at.b * p.D + at.c, carry);
 }
 
 // The same from the other end: e takes the place of the state, the cluster's tiles are counted from the last one.  The states before a tile's tokens are
@@ -319,7 +287,9 @@ __global__ void __launch_bounds__(32 * WARPS, 2) recurrence_bwd_kernel(const __g
     using SG = Stage<RUN, LPR, G, VEC, CPG>;
     constexpr int BYTES = 2 * SX::BYTES + SG::BYTES;
     extern __shared__ __align__(16) unsigned char staged[];
-    __shared__ float agg[2][3][WARPS][LPR][VEC];                      // A, H and E of the warps' runs
+    typedef typename Number<VEC>::T T;
+    __shared__ Map<T> agg[2][WARPS][LPR];                             // of the warps' runs: A and E
+    __shared__ T own[2][WARPS][LPR];                                  // H
     Place<LPR, VEC, TILE> at(p, staged + SLOTS * WARPS * BYTES);
     const int lane = at.lane, warp = at.warp, NS = (p.T + STATES - 1) / STATES;
     const long ld = p.D, base = (long)at.b * p.T * ld + at.c0;
@@ -337,87 +307,62 @@ __global__ void __launch_bounds__(32 * WARPS, 2) recurrence_bwd_kernel(const __g
     };
     bring(0);
     if (at.ranks > 1) at.cluster.sync();
-    float carry[VEC];
-#pragma unroll
-    for (int u = 0; u < VEC; ++u) carry[u] = p.h0 && at.there ? p.h0[(long)at.b * p.D + at.c + u] : 0.f;
+    T carry = splat<T>(0.f);
+    if (p.h0 && at.there) load(p.h0 + (long)at.b * p.D + at.c, carry);
     for (int round = 0; round < at.rounds; ++round) {
         const int tile = tile_of(round), t0 = tile * TILE + (warp * SUB + at.sub) * RUN, left = tile < 0 ? 0 : p.T - t0, par = round & 1;
         bring(round + 1);
-        float v[RUN][VEC], a[RUN][VEC], d[RUN][VEC], h[VEC], e[VEC], Au[VEC], Hu[VEC], Ad[VEC], Ed[VEC];
-#pragma unroll
-        for (int u = 0; u < VEC; ++u) h[u] = at.there && tile >= 0 ? p.starts[((long)at.b * NS + tile * (TILE / STATES)) * p.D + at.c + u] : 0.f;
+        T v[RUN], a[RUN], d[RUN], h = splat<T>(0.f), e;
+        if (at.there && tile >= 0) load(p.starts + ((long)at.b * NS + tile * (TILE / STATES)) * p.D + at.c, h);
         copies_but<1>();
         __syncwarp();
         SX::read(slot(round), lane, v);
         SX::read(slot(round) + SX::BYTES, lane, d);
         SG::read(slot(round) + 2 * SX::BYTES, lane, a);
-        decays<RUN, VEC>(a);
+        Map<T> up = {splat<T>(1.f), splat<T>(0.f)}, down = up;
 #pragma unroll
-        for (int u = 0; u < VEC; ++u) {
-            float A = 1.f, H = 0.f, E = 0.f;
-#pragma unroll
-            for (int i = 0; i < RUN; ++i) {
-                A *= a[i][u];
-                H = fmaf(a[i][u], H, v[i][u]);
-                E = a[RUN - 1 - i][u] * (d[RUN - 1 - i][u] + E);
-            }
-            float A2 = A;
-            warp_scan<true, LPR>(at.sub, A, H, Au[u], Hu[u]);
-            warp_scan<false, LPR>(at.sub, A2, E, Ad[u], Ed[u]);
-            if (at.sub == SUB - 1) {
-                agg[par][0][warp][at.col][u] = A;
-                agg[par][1][warp][at.col][u] = H;
-            }
-            if (at.sub == 0) agg[par][2][warp][at.col][u] = E;
+        for (int i = 0; i < RUN; ++i) {
+            a[i] = decay(a[i]);
+            up.A = mul(up.A, a[i]);
+            up.H = fma2(a[i], up.H, v[i]);
         }
+#pragma unroll
+        for (int i = RUN - 1; i >= 0; --i) down.H = mul(a[i], add(d[i], down.H));
+        down.A = up.A;
+        const Map<T> before = warp_scan<true, LPR>(at.sub, up), behind = warp_scan<false, LPR>(at.sub, down);
+        if (at.sub == SUB - 1) own[par][warp][at.col] = up.H;
+        if (at.sub == 0) agg[par][warp][at.col] = down;
         __syncthreads();
 #pragma unroll
-        for (int u = 0; u < VEC; ++u)
-#pragma unroll
-            for (int w = 0; w < WARPS; ++w)
-                if (w < warp) h[u] = fmaf(agg[par][0][w][at.col][u], h[u], agg[par][1][w][at.col][u]);
+        for (int w = 0; w < WARPS; ++w)
+            if (w < warp) h = fma2(agg[par][w][at.col].A, h, own[par][w][at.col]);
         if (at.ranks == 1) {
 #pragma unroll
-            for (int u = 0; u < VEC; ++u)
-#pragma unroll
-                for (int w = WARPS - 1; w >= 0; --w) {
-                    if (w == warp) e[u] = carry[u];
-                    carry[u] = fmaf(agg[par][0][w][at.col][u], carry[u], agg[par][2][w][at.col][u]);
-                }
-        } else {
-            float A[VEC], E[VEC], Ab[VEC], Eb[VEC], mine[VEC];        // of the tile; of the warps behind this one
-#pragma unroll
-            for (int u = 0; u < VEC; ++u) {
-                A[u] = 1.f;
-                E[u] = 0.f;
-#pragma unroll
-                for (int w = WARPS - 1; w >= 0; --w) {
-                    const float aw = agg[par][0][w][at.col][u];
-                    if (w == warp) {
-                        Ab[u] = A[u];
-                        Eb[u] = E[u];
-                    }
-                    A[u] *= aw;
-                    E[u] = fmaf(aw, E[u], agg[par][2][w][at.col][u]);
-                }
+            for (int w = WARPS - 1; w >= 0; --w) {
+                if (w == warp) e = carry;
+                carry = agg[par][w][at.col](carry);
             }
-            at.exchange(round, A, E, carry, mine);
+        } else {
+            Map<T> all = {splat<T>(1.f), splat<T>(0.f)}, warps;       // of the tile; of the warps behind this one
 #pragma unroll
-            for (int u = 0; u < VEC; ++u) e[u] = fmaf(Ab[u], mine[u], Eb[u]);
+            for (int w = WARPS - 1; w >= 0; --w) {
+                const Map<T> r = agg[par][w][at.col];
+                if (w == warp) warps = all;
+                all.A = mul(all.A, r.A);
+                all.H = r(all.H);
+            }
+            e = warps(at.exchange(round, all, carry));
+        }
+        if constexpr (SUB > 1) {
+            h = before(h);
+            e = behind(e);
         }
         // the states before the run's tokens, in the place of x
 #pragma unroll
-        for (int u = 0; u < VEC; ++u) {
-            if constexpr (SUB > 1) {
-                h[u] = fmaf(Au[u], h[u], Hu[u]);
-                e[u] = fmaf(Ad[u], e[u], Ed[u]);
-            }
-#pragma unroll
-            for (int i = 0; i < RUN; ++i) {
-                const float next = fmaf(a[i][u], h[u], v[i][u]);
-                v[i][u] = h[u];
-                h[u] = next;
-            }
+        for (int i = 0; i < RUN; ++i) {
+            const T next = fma2(a[i], h, v[i]);
+            v[i] = h;
+            h = next;
         }
         if (at.there && left > 0) {
             const long to = base + t0 * ld + at.col * VEC;
@@ -426,21 +371,16 @@ __global__ void __launch_bounds__(32 * WARPS, 2) recurrence_bwd_kernel(const __g
 #pragma unroll
             for (int i = RUN - 1; i >= 0; --i) {
                 if (i < left) {
-                    float dh[VEC], dgi[VEC];
-#pragma unroll
-                    for (int u = 0; u < VEC; ++u) {
-                        dh[u] = d[i][u] + e[u];
-                        e[u] = a[i][u] * dh[u];
-                        dgi[u] = e[u] * v[i][u];
-                    }
-                    Row<X, VEC>::store(dx + i * ld, dh);
-                    Row<G, VEC>::store(dg + i * ld, dgi);
+                    const T dh = add(d[i], e);
+                    e = mul(a[i], dh);
+                    store(dx + i * ld, dh);
+                    store(dg + i * ld, mul(e, v[i]));
                 }
             }
         }
         __syncwarp();
     }
-    if (p.h_last && at.rank == 0 && threadIdx.x < LPR && at.there) Row<float, VEC>::store(p.h_last + (long)at.b * p.D + at.c, carry);
+    if (p.h_last && at.rank == 0 && threadIdx.x < LPR && at.there) store(p.h_last + (long)at.b * p.D + at.c, carry);
 }
 
 template <typename X, typename G>
@@ -448,12 +388,12 @@ __global__ void __launch_bounds__(256) recurrence_step_kernel(float* h, const X*
     chain_wait();
     const long i = (long)blockIdx.x * 256 + threadIdx.x;
     if (i >= n) return;
-    float v[1], a[1];
-    Row<X, 1>::load(x + i, v);
-    Row<G, 1>::load(g + i, a);
-    v[0] = fmaf(decay(a[0]), h[i], v[0]);
-    h[i] = v[0];
-    Row<X, 1>::store(o + i, v);
+    float v, a;
+    load(x + i, v);
+    load(g + i, a);
+    v = fmaf(decay(a), h[i], v);
+    h[i] = v;
+    store(o + i, v);
 }
 
 // How many CTAs share a strip: as many as there are tiles, and as run at once for all strips, since a second wave costs what the first one does.

@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 
 #include "launch_count.h"
+#include "pairs.cuh"
 #include "tma.cuh"
 #include "umma.cuh"
 
@@ -94,48 +95,20 @@ __device__ __forceinline__ uint32_t seeing_bits(int t0, int s, int window, int s
     return ~below(s - t0) & (s < sinks ? 0xffffffffu : below(s + window - t0));
 }
 
-// ---- two fp32 values in a 64-bit register
-typedef unsigned long long f32x2;
-__device__ __forceinline__ f32x2 pack2(float lo, float hi) {
-    f32x2 r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-    return r;
-}
-__device__ __forceinline__ float2 unpack2(f32x2 a) {
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a));
-    return r;
-}
-__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
-    f32x2 r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
-    f32x2 r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
-    f32x2 r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-
 // 2^x of a pair on the FMA pipes, for a share of the exponentials where the special-function unit (four lanes a cycle and scheduler) is the bottleneck.  x = n + f with n the
 // nearest integer, which adding 1.5 2^23 leaves in the low bits; 2^f, f in [-1/2, 1/2], by the minimax polynomial of degree 4 in the relative error (Remez exchange:
 // 2.6e-6); n goes to the exponent by an integer addition.  Below -126 the result is 2^-126.
-__device__ __forceinline__ float2 exp2_poly(f32x2 x) {
-    const float2 v = unpack2(x);
-    x = pack2(fmaxf(v.x, -126.f), fmaxf(v.y, -126.f));
-    const f32x2 magic = pack2(12582912.f, 12582912.f), back = pack2(-12582912.f, -12582912.f);
-    const f32x2 r = add2(x, magic), n = add2(r, back), f = fma2(n, pack2(-1.f, -1.f), x);
-    f32x2 y = pack2(0.009570102207362652f, 0.009570102207362652f);
-    y = fma2(y, f, pack2(0.05591785907745361f, 0.05591785907745361f));
-    y = fma2(y, f, pack2(0.240247443318367f, 0.240247443318367f));
-    y = fma2(y, f, pack2(0.6931217908859253f, 0.6931217908859253f));
-    y = fma2(y, f, pack2(0.9999992847442627f, 0.9999992847442627f));
-    const float2 a = unpack2(y), k = unpack2(r);
+__device__ __forceinline__ float2 exp2_poly(F2 x) {
+    const float2 v = both(x);
+    x = pair(fmaxf(v.x, -126.f), fmaxf(v.y, -126.f));
+    const F2 magic = pair(12582912.f, 12582912.f), back = pair(-12582912.f, -12582912.f);
+    const F2 r = add(x, magic), n = add(r, back), f = fma2(n, pair(-1.f, -1.f), x);
+    F2 y = pair(0.009570102207362652f, 0.009570102207362652f);
+    y = fma2(y, f, pair(0.05591785907745361f, 0.05591785907745361f));
+    y = fma2(y, f, pair(0.240247443318367f, 0.240247443318367f));
+    y = fma2(y, f, pair(0.6931217908859253f, 0.6931217908859253f));
+    y = fma2(y, f, pair(0.9999992847442627f, 0.9999992847442627f));
+    const float2 a = both(y), k = both(r);
     return make_float2(__int_as_float(__float_as_int(a.x) + (__float_as_int(k.x) << 23)), __int_as_float(__float_as_int(a.y) + (__float_as_int(k.y) << 23)));
 }
 

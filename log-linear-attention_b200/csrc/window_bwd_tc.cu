@@ -54,12 +54,12 @@ __device__ __forceinline__ void regs_rows() { asm volatile("setmaxnreg.inc.sync.
 // exp2(c s - shift) of 64 scores, a quarter of them on the FMA pipes where no key is hidden (whose value has to be an exact zero); shift(u) gives the pair of values for keys u, u + 1
 template <typename ShiftT>
 __device__ __forceinline__ void exponentials(float (&e)[64], float c, bool whole, ShiftT shift) {
-    const f32x2 c2 = pack2(c, c);
+    const F2 c2 = pair(c, c);
     if (whole) {
 #pragma unroll
         for (int u = 0; u < 64; u += 2) {
-            const f32x2 y = fma2(pack2(e[u], e[u + 1]), c2, shift(u));
-            float2 v = unpack2(y);
+            const F2 y = fma2(pair(e[u], e[u + 1]), c2, shift(u));
+            float2 v = both(y);
             if (u % 8 == 6) v = exp2_poly(y);
             else v = make_float2(exp2_fast(v.x), exp2_fast(v.y));
             e[u] = v.x;
@@ -68,7 +68,7 @@ __device__ __forceinline__ void exponentials(float (&e)[64], float c, bool whole
     } else {
 #pragma unroll
         for (int u = 0; u < 64; u += 2) {
-            const float2 v = unpack2(fma2(pack2(e[u], e[u + 1]), c2, shift(u)));
+            const float2 v = both(fma2(pair(e[u], e[u + 1]), c2, shift(u)));
             e[u] = exp2_fast(v.x);
             e[u + 1] = exp2_fast(v.y);
         }
@@ -275,7 +275,7 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dq_tc_kernel(const __
             float e[64], d[64];
             tmem_ld64(tS + 128 * (n & 1), e);
             const bool whole = all_seen(q0, s0, p.window, p.sinks);
-            exponentials(e, c, whole, [&](int) { return pack2(-lse, -lse); });
+            exponentials(e, c, whole, [&](int) { return pair(-lse, -lse); });
             if (!whole) {
 #pragma unroll
                 for (int i = 0; i < 64; i += 32) {
@@ -291,7 +291,7 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dq_tc_kernel(const __
             tmem_ld64(tDP, d);
 #pragma unroll
             for (int i = 0; i < 64; i += 2) {
-                const float2 v = unpack2(mul2(pack2(e[i], e[i + 1]), add2(pack2(d[i], d[i + 1]), pack2(-delta, -delta))));
+                const float2 v = both(mul(pair(e[i], e[i + 1]), add(pair(d[i], d[i + 1]), pair(-delta, -delta))));
                 e[i] = v.x;
                 e[i + 1] = v.y;
             }
@@ -444,7 +444,7 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dkv_tc_kernel(const _
             const bool whole = all_seen(t0, s0, p.window, p.sinks);
             exponentials(e, c, whole, [&](int u) {
                 const float2 m = *reinterpret_cast<const float2*>(lse + u);
-                return pack2(-m.x, -m.y);
+                return pair(-m.x, -m.y);
             });
             if (!whole) {
                 // token s is seen by the queries from s on, as far as the window goes; a sink by all of them
@@ -465,7 +465,7 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dkv_tc_kernel(const _
 #pragma unroll
             for (int u = 0; u < 64; u += 2) {
                 const float2 m = *reinterpret_cast<const float2*>(delta + u);
-                const float2 v = unpack2(mul2(pack2(e[u], e[u + 1]), add2(pack2(d[u], d[u + 1]), pack2(-m.x, -m.y))));
+                const float2 v = both(mul(pair(e[u], e[u + 1]), add(pair(d[u], d[u + 1]), pair(-m.x, -m.y))));
                 e[u] = v.x;
                 e[u + 1] = v.y;
             }

@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(fwd::NTHREADS, 1) window_fwd_tc_kernel(const _
         const int x = warp >> 2, row = (warp & 3) * 32 + lane, t0 = q0 + x * TILE, t = t0 + row;
         const uint32_t tS = umma::tmem_addr(tmem, warp, TM_S + 128 * x), tO = umma::tmem_addr(tmem, warp, TM_O + 128 * x);
         const float c = p.scale * LOG2E;
-        const f32x2 c2 = pack2(c, c);
+        const F2 c2 = pair(c, c);
         const Span span(t0, p.T, p.window, p.sinks);
         const int n = span.count();
         float m = -INFINITY, sum = 0.f;
@@ -202,8 +202,8 @@ __global__ void __launch_bounds__(fwd::NTHREADS, 1) window_fwd_tc_kernel(const _
                 }
             }
             const float ref = m == -INFINITY ? 0.f : m;        // a row that has seen nothing yet
-            const f32x2 shift = pack2(-ref, -ref);
-            f32x2 part[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
+            const F2 shift = pair(-ref, -ref);
+            F2 part[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 const auto exponentials = [&](auto mixed) {
@@ -212,15 +212,15 @@ __global__ void __launch_bounds__(fwd::NTHREADS, 1) window_fwd_tc_kernel(const _
                         uint32_t w[16];
 #pragma unroll
                         for (int u = 0; u < 16; ++u) {
-                            const f32x2 y = fma2(pack2(s[half][k + 2 * u], s[half][k + 2 * u + 1]), c2, shift);
+                            const F2 y = fma2(pair(s[half][k + 2 * u], s[half][k + 2 * u + 1]), c2, shift);
                             float2 e;
                             if (decltype(mixed)::value && u % POLY == POLY - 1) {
                                 e = exp2_poly(y);
                             } else {
-                                const float2 v = unpack2(y);
+                                const float2 v = both(y);
                                 e = make_float2(exp2_fast(v.x), exp2_fast(v.y));
                             }
-                            part[u & 1] = add2(part[u & 1], pack2(e.x, e.y));
+                            part[u & 1] = add(part[u & 1], pair(e.x, e.y));
                             w[u] = pack_bf16(e.x, e.y);
                         }
                         umma::tmem_st16u(tS + 32 * half + k / 2, w);
@@ -234,7 +234,7 @@ __global__ void __launch_bounds__(fwd::NTHREADS, 1) window_fwd_tc_kernel(const _
                 __syncwarp();
                 if (lane == 0) arrive(barP + 2 * x + half);
             }
-            const float2 a = unpack2(add2(part[0], part[1]));
+            const float2 a = both(add(part[0], part[1]));
             sum += a.x + a.y;
         }
         if (ok && n > 0) ok = umma::mbar_wait_warp(barO + x, (n - 1) & 1, abort_flag);
