@@ -111,26 +111,26 @@ __device__ __forceinline__ void row_sum(float (&s)[V], float (*sh)[THREADS / 32]
     }
 }
 
-// The rows to come, in shared memory.  Words of 16 bytes, or of one fp32 value: [STAGES][ROWS][ITER][TENSORS][THREADS], each lane's own.  bf16 rows that do not start
-// at 16-byte boundaries: [STAGES][ROWS][TENSORS][GROUPS] rows as they are in memory, from the 4-byte boundary at or before their start on (there are no copies
+// The rows to come, in shared memory.  Words of 16 bytes, or of one fp32 value: [STAGES][ITER][TENSORS][THREADS], each lane's own.  bf16 rows that do not start
+// at 16-byte boundaries: [STAGES][TENSORS][GROUPS] rows as they are in memory, from the 4-byte boundary at or before their start on (there are no copies
 // of two bytes), so that a lane's values come with another lane's copies.
-template <typename X, int VEC, int ITER, int ROWS, int LANES, int THREADS, int TENSORS>
+template <typename X, int VEC, int ITER, int LANES, int THREADS, int TENSORS>
 struct Ring {
     static constexpr bool SHARED = VEC * sizeof(X) == 2;
     static constexpr int GROUPS = THREADS / LANES, CAP = LANES * ITER * VEC + (SHARED ? 8 : 0);         // values of a row
-    static constexpr int BYTES = VEC * ITER * (int)sizeof(X), STAGES = BYTES * TENSORS * ROWS > 64 ? 3 : 4;
-    static constexpr size_t SIZE = (size_t)STAGES * ROWS * TENSORS * GROUPS * CAP * sizeof(X);
-    static __device__ __forceinline__ X* word(X* ring, int stage, int j, int i, int t) {
-        return ring + ((((stage * ROWS + j) * ITER + i) * TENSORS + t) * THREADS + (int)threadIdx.x) * VEC;
+    static constexpr int BYTES = VEC * ITER * (int)sizeof(X), STAGES = BYTES * TENSORS > 64 ? 3 : 4;
+    static constexpr size_t SIZE = (size_t)STAGES * TENSORS * GROUPS * CAP * sizeof(X);
+    static __device__ __forceinline__ X* word(X* ring, int stage, int i, int t) {
+        return ring + (((stage * ITER + i) * TENSORS + t) * THREADS + (int)threadIdx.x) * VEC;
     }
-    static __device__ __forceinline__ X* whole(X* ring, int stage, int j, int t) {
-        return ring + (((stage * ROWS + j) * TENSORS + t) * GROUPS + (int)threadIdx.x / LANES) * CAP;
+    static __device__ __forceinline__ X* whole(X* ring, int stage, int t) {
+        return ring + ((stage * TENSORS + t) * GROUPS + (int)threadIdx.x / LANES) * CAP;
     }
-    static __device__ __forceinline__ void bring(X* ring, int stage, int j, int t, const X* x, long row, long rows, int N, int lane) {
+    static __device__ __forceinline__ void bring(X* ring, int stage, int t, const X* x, long row, long rows, int N, int lane) {
         if constexpr (SHARED) {
             const int odd = (int)(row * N & 1), words = (N + odd + 1) / 2;
             const X* from = x + row * N - odd;
-            const uint32_t to = (uint32_t)__cvta_generic_to_shared(whole(ring, stage, j, t));
+            const uint32_t to = (uint32_t)__cvta_generic_to_shared(whole(ring, stage, t));
             const bool last = row + 1 == rows && (N + odd) % 2 != 0;                 // the tensor ends in the middle of the last word
 #pragma unroll
             for (int i = 0; i < ITER / 2 + 1; ++i) {
@@ -142,7 +142,7 @@ struct Ring {
 #pragma unroll
             for (int i = 0; i < ITER; ++i) {
                 const int c = (i * LANES + lane) * VEC;
-                const uint32_t to = (uint32_t)__cvta_generic_to_shared(word(ring, stage, j, i, t));
+                const uint32_t to = (uint32_t)__cvta_generic_to_shared(word(ring, stage, i, t));
                 if (c < N) {
                     if constexpr (VEC * sizeof(X) == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(to), "l"(x + row * N + c) : "memory");
                     else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"(to), "l"(x + row * N + c) : "memory");
@@ -151,9 +151,9 @@ struct Ring {
         }
     }
     template <typename T, int N_>
-    static __device__ __forceinline__ void read(X* ring, int stage, int j, int i, int t, long row, int N, int lane, T (&v)[N_]) {
-        if constexpr (SHARED) Lane<VEC>::load(whole(ring, stage, j, t) + (int)(row * N & 1) + i * LANES + lane, v);
-        else Lane<VEC>::load(word(ring, stage, j, i, t), v);
+    static __device__ __forceinline__ void read(X* ring, int stage, int i, int t, long row, int N, int lane, T (&v)[N_]) {
+        if constexpr (SHARED) Lane<VEC>::load(whole(ring, stage, t) + (int)(row * N & 1) + i * LANES + lane, v);
+        else Lane<VEC>::load(word(ring, stage, i, t), v);
     }
 };
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
@@ -165,7 +165,7 @@ template <typename X, typename W, int VEC, int ITER, int LANES, int THREADS>
 __global__ void __launch_bounds__(THREADS, 2) layer_norm_fwd_kernel(const __grid_constant__ Params p) {
     chain_wait();
     constexpr int GROUPS = THREADS / LANES;
-    using R = Ring<X, VEC, ITER, 1, LANES, THREADS, 1>;
+    using R = Ring<X, VEC, ITER, LANES, THREADS, 1>;
     using L = Lane<VEC>;
     typedef typename L::T T;
     __shared__ float sh[2][1][THREADS / 32];
@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(THREADS, 2) layer_norm_fwd_kernel(const __grid
     const W *w = static_cast<const W*>(p.w), *b = static_cast<const W*>(p.b);
     const long stride = (long)gridDim.x * GROUPS, first = (long)blockIdx.x * GROUPS + group;
     const auto fetch = [&](long row, int stage) {
-        if (row < p.rows) R::bring(ring, stage, 0, 0, x, row, p.rows, N, lane);
+        if (row < p.rows) R::bring(ring, stage, 0, x, row, p.rows, N, lane);
         copies_commit();
     };
 #pragma unroll
@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(THREADS, 2) layer_norm_fwd_kernel(const __grid
 #pragma unroll
         for (int i = 0; i < ITER; ++i) {
             if (row < p.rows && (i * LANES + lane) * VEC < N) {
-                R::read(ring, stage, 0, i, 0, row, N, lane, v[i]);
+                R::read(ring, stage, i, 0, row, N, lane, v[i]);
             } else {
 #pragma unroll
                 for (int u = 0; u < L::N; ++u) v[i][u] = splat<T>(0.f);
@@ -245,15 +245,14 @@ __global__ void __launch_bounds__(THREADS, 2) layer_norm_fwd_kernel(const __grid
     }
 }
 
-// The same with ROWS rows a lane at once, which share the latency of the sums over the lanes (most of what a round of one row consists of).
-template <typename X, typename W, int VEC, int ITER, int ROWS, int LANES, int THREADS>
+template <typename X, typename W, int VEC, int ITER, int LANES, int THREADS>
 __global__ void __launch_bounds__(THREADS, 1) layer_norm_bwd_kernel(const __grid_constant__ Params p) {
     chain_wait();
     constexpr int GROUPS = THREADS / LANES;
-    using R = Ring<X, VEC, ITER, ROWS, LANES, THREADS, 2>;
+    using R = Ring<X, VEC, ITER, LANES, THREADS, 2>;
     using L = Lane<VEC>;
     typedef typename L::T T;
-    __shared__ float sh[2][2 * ROWS][THREADS / 32];
+    __shared__ float sh[2][2][THREADS / 32];
     extern __shared__ __align__(16) unsigned char ring_raw[];
     X* ring = reinterpret_cast<X*>(ring_raw);
     float* cols = reinterpret_cast<float*>(ring_raw);     // [2][N], after the last row
@@ -262,15 +261,11 @@ __global__ void __launch_bounds__(THREADS, 1) layer_norm_bwd_kernel(const __grid
     const X *x = static_cast<const X*>(p.x), *dy = static_cast<const X*>(p.dy);
     X* dx = static_cast<X*>(p.dx);
     const W* w = static_cast<const W*>(p.w);
-    const long stride = (long)gridDim.x * GROUPS * ROWS, first = (long)blockIdx.x * GROUPS * ROWS;
-    const auto fetch = [&](long base, int stage) {
-#pragma unroll
-        for (int j = 0; j < ROWS; ++j) {
-            const long row = base + j * GROUPS + group;
-            if (row < p.rows) {
-                R::bring(ring, stage, j, 0, x, row, p.rows, N, lane);
-                R::bring(ring, stage, j, 1, dy, row, p.rows, N, lane);
-            }
+    const long stride = (long)gridDim.x * GROUPS, first = (long)blockIdx.x * GROUPS + group;
+    const auto fetch = [&](long row, int stage) {
+        if (row < p.rows) {
+            R::bring(ring, stage, 0, x, row, p.rows, N, lane);
+            R::bring(ring, stage, 1, dy, row, p.rows, N, lane);
         }
         copies_commit();
     };
@@ -287,71 +282,52 @@ __global__ void __launch_bounds__(THREADS, 1) layer_norm_bwd_kernel(const __grid
         }
         if (w && c < N) L::load(w + c, wv[i]);
     }
-    float mean[ROWS], rstd[ROWS];
-    const auto stats = [&](long base) {
-#pragma unroll
-        for (int j = 0; j < ROWS; ++j) {
-            const long row = base + j * GROUPS + group;
-            mean[j] = row < p.rows ? p.mean[row] : 0.f;
-            rstd[j] = row < p.rows ? p.rstd[row] : 0.f;
-        }
-    };
-    stats(first);
+    float mean = first < p.rows ? p.mean[first] : 0.f, rstd = first < p.rows ? p.rstd[first] : 0.f;
     int stage = 0, par = 0;
-    for (long base = first; base < p.rows; base += stride, par ^= 1, stage = stage + 1 == R::STAGES ? 0 : stage + 1) {
+    for (long row = first; row - group < p.rows; row += stride, par ^= 1, stage = stage + 1 == R::STAGES ? 0 : stage + 1) {
         copies_but<R::STAGES - 2>();
         if constexpr (R::SHARED) __syncthreads();
-        T xh[ROWS][ITER][L::N], d[ROWS][ITER][L::N];
+        T xh[ITER][L::N], d[ITER][L::N];
 #pragma unroll
-        for (int j = 0; j < ROWS; ++j)
+        for (int i = 0; i < ITER; ++i) {
+            if (row < p.rows && (i * LANES + lane) * VEC < N) {
+                R::read(ring, stage, i, 0, row, N, lane, xh[i]);
+                R::read(ring, stage, i, 1, row, N, lane, d[i]);
+            } else {
 #pragma unroll
-            for (int i = 0; i < ITER; ++i) {
-                const long row = base + j * GROUPS + group;
-                if (row < p.rows && (i * LANES + lane) * VEC < N) {
-                    R::read(ring, stage, j, i, 0, row, N, lane, xh[j][i]);
-                    R::read(ring, stage, j, i, 1, row, N, lane, d[j][i]);
-                } else {
-#pragma unroll
-                    for (int u = 0; u < L::N; ++u) xh[j][i][u] = d[j][i][u] = splat<T>(0.f);      // (d of zero adds nothing)
-                }
+                for (int u = 0; u < L::N; ++u) xh[i][u] = d[i][u] = splat<T>(0.f);      // (d of zero adds nothing)
             }
-        fetch(base + (R::STAGES - 1) * stride, stage == 0 ? R::STAGES - 1 : stage - 1);
-        float s[2 * ROWS], r[ROWS];
-#pragma unroll
-        for (int j = 0; j < ROWS; ++j) {
-            const T neg = splat<T>(-mean[j]), r2 = splat<T>(rstd[j]);
-            T s0 = splat<T>(0.f), s1 = s0;
-            r[j] = rstd[j];
-#pragma unroll
-            for (int i = 0; i < ITER; ++i)
-#pragma unroll
-                for (int u = 0; u < L::N; ++u) {
-                    xh[j][i][u] = mul(add(xh[j][i][u], neg), r2);
-                    dw[i][u] = fma2(d[j][i][u], xh[j][i][u], dw[i][u]);
-                    db[i][u] = add(db[i][u], d[j][i][u]);
-                    d[j][i][u] = mul(d[j][i][u], wv[i][u]);
-                    s0 = add(s0, d[j][i][u]);
-                    s1 = fma2(d[j][i][u], xh[j][i][u], s1);
-                }
-            s[2 * j] = total(s0);
-            s[2 * j + 1] = total(s1);
         }
-        stats(base + stride);
+        fetch(row + (R::STAGES - 1) * stride, stage == 0 ? R::STAGES - 1 : stage - 1);
+        const T neg = splat<T>(-mean), r = splat<T>(rstd);
+        if (row + stride < p.rows) {
+            mean = p.mean[row + stride];
+            rstd = p.rstd[row + stride];
+        }
+        T s0 = splat<T>(0.f), s1 = s0;
+#pragma unroll
+        for (int i = 0; i < ITER; ++i)
+#pragma unroll
+            for (int u = 0; u < L::N; ++u) {
+                xh[i][u] = mul(add(xh[i][u], neg), r);
+                dw[i][u] = fma2(d[i][u], xh[i][u], dw[i][u]);
+                db[i][u] = add(db[i][u], d[i][u]);
+                d[i][u] = mul(d[i][u], wv[i][u]);
+                s0 = add(s0, d[i][u]);
+                s1 = fma2(d[i][u], xh[i][u], s1);
+            }
+        float s[2] = {total(s0), total(s1)};
         row_sum<LANES, THREADS>(s, sh[par]);
         // rstd (z - mean(z) - xhat mean(z xhat))
+        const T m1 = splat<T>(-s[0] * inv), m2 = splat<T>(-s[1] * inv);
+        if (row < p.rows) {
 #pragma unroll
-        for (int j = 0; j < ROWS; ++j) {
-            const long row = base + j * GROUPS + group;
-            const T m1 = splat<T>(-s[2 * j] * inv), m2 = splat<T>(-s[2 * j + 1] * inv), rr = splat<T>(r[j]);
-            if (row < p.rows) {
+            for (int i = 0; i < ITER; ++i) {
+                const int c = (i * LANES + lane) * VEC;
+                if (c < N) {
 #pragma unroll
-                for (int i = 0; i < ITER; ++i) {
-                    const int c = (i * LANES + lane) * VEC;
-                    if (c < N) {
-#pragma unroll
-                        for (int u = 0; u < L::N; ++u) d[j][i][u] = mul(fma2(xh[j][i][u], m2, add(d[j][i][u], m1)), rr);
-                        L::store(dx + row * N + c, d[j][i]);
-                    }
+                    for (int u = 0; u < L::N; ++u) d[i][u] = mul(fma2(xh[i][u], m2, add(d[i][u], m1)), r);
+                    L::store(dx + row * N + c, d[i]);
                 }
             }
         }
@@ -516,43 +492,65 @@ cudaError_t run(KernT kern, dim3 grid, int threads, size_t smem, const Params& p
     if (e == cudaSuccess) LLATTN_LAUNCHED();
     return e;
 }
-// 512 threads, as many lanes a row as give each 8 values of it (16 in rows above 4096).  Two CTAs an SM in the forward, one in the backward, and no more than there are rows
-// for; several rows a lane at once as soon as every CTA has more than one.
-constexpr int THREADS = 512, MAX_N = THREADS * 16, SMS = 148;
-int lanes_of(int N) {
+// Lanes a row, so that each has `values` of it; a power of two of at least a warp and at most the CTA.
+constexpr int SMS = 148, MAX_N = 8192;
+int lanes_of(int N, int values, int threads) {
     int lanes = 32;
-    while (lanes * 8 < N && lanes < THREADS) lanes *= 2;
+    while (lanes * values < N && lanes < threads) lanes *= 2;
     return lanes;
 }
-int ctas_of(long rows, int N, int per_sm) {
-    const long g = THREADS / lanes_of(N), n = (rows + g - 1) / g;
+int ctas_of(long rows, int groups, int per_sm) {
+    const long n = (rows + groups - 1) / groups;
     return (int)(n < per_sm * SMS ? n : per_sm * SMS);
 }
-int parts_of(long rows, int N) { return N > MAX_N ? (int)(rows < 64 ? rows : 64) : ctas_of(rows, N, 1); }
-// Rows of x at once that a lane of the backward takes: two where it has 16 bytes of each (32768 x 2048 bf16, us: one 111, two 92, four 102).  The forward is better off
-// with a second CTA on the SM (one row a lane 59, two 70, four 104; one CTA with two or four 64).
+// Forward: 16 values a lane, two CTAs of 256 threads an SM (32768 x 2048 bf16, us: 51; 8 values in two CTAs of 512 59, 16 in one of 512 59, 16 in three of 256 51, 32 in two
+// of 256 49, but there 16384 x 4096 fp32 and short rows lose).  Backward: 32 bytes of a row a lane, one CTA of 512 (82; 16 bytes of one row 111, of two rows at once
+// 92..100, 32 bytes in two CTAs of 256 80, in three 133).  The longest rows have twice that a lane.
+constexpr int FWD_THREADS = 256, FWD_VALUES = 16, BWD_THREADS = 512;
+constexpr int bwd_values(size_t bytes) { return 32 / (int)bytes; }
+int parts_of(long rows, int N, int bytes) {
+    if (N > MAX_N) return (int)(rows < 64 ? rows : 64);
+    return ctas_of(rows, BWD_THREADS / lanes_of(N, bwd_values(bytes), BWD_THREADS), 1);
+}
 template <typename X, typename W, int VEC, int ITER, int LANES>
-cudaError_t pass(bool back, const Params& p, cudaStream_t st) {
-    if (!back) return run(layer_norm_fwd_kernel<X, W, VEC, ITER, LANES, THREADS>, ctas_of(p.rows, p.N, 2), THREADS, Ring<X, VEC, ITER, 1, LANES, THREADS, 1>::SIZE, p, st);
-    constexpr int ROWS = VEC * ITER * sizeof(X) > 16 ? 1 : 2;
-    if (ROWS == 1 || p.rows <= (long)p.parts * (THREADS / LANES))
-        return run(layer_norm_bwd_kernel<X, W, VEC, ITER, 1, LANES, THREADS>, p.parts, THREADS, Ring<X, VEC, ITER, 1, LANES, THREADS, 2>::SIZE, p, st);
-    return run(layer_norm_bwd_kernel<X, W, VEC, ITER, ROWS, LANES, THREADS>, p.parts, THREADS, Ring<X, VEC, ITER, ROWS, LANES, THREADS, 2>::SIZE, p, st);
+cudaError_t fwd_pass(const Params& p, cudaStream_t st) {
+    return run(layer_norm_fwd_kernel<X, W, VEC, ITER, LANES, FWD_THREADS>, ctas_of(p.rows, FWD_THREADS / LANES, 2), FWD_THREADS,
+               Ring<X, VEC, ITER, LANES, FWD_THREADS, 1>::SIZE, p, st);
+}
+template <typename X, typename W, int VEC, int ITER, int LANES>
+cudaError_t bwd_pass(const Params& p, cudaStream_t st) {
+    return run(layer_norm_bwd_kernel<X, W, VEC, ITER, LANES, BWD_THREADS>, p.parts, BWD_THREADS, Ring<X, VEC, ITER, LANES, BWD_THREADS, 2>::SIZE, p, st);
 }
 template <typename X, typename W, int VEC>
-cudaError_t pass_vec(bool back, const Params& p, cudaStream_t st) {
-    switch (lanes_of(p.N)) {
-        case 32: return pass<X, W, VEC, 8 / VEC, 32>(back, p, st);
-        case 64: return pass<X, W, VEC, 8 / VEC, 64>(back, p, st);
-        case 128: return pass<X, W, VEC, 8 / VEC, 128>(back, p, st);
-        case 256: return pass<X, W, VEC, 8 / VEC, 256>(back, p, st);
-        default: return p.N <= 8 * THREADS ? pass<X, W, VEC, 8 / VEC, THREADS>(back, p, st) : pass<X, W, VEC, 16 / VEC, THREADS>(back, p, st);
+cudaError_t fwd_vec(const Params& p, cudaStream_t st) {
+    constexpr int I = FWD_VALUES / VEC, MOST = MAX_N / FWD_THREADS / VEC;
+    switch (lanes_of(p.N, FWD_VALUES, FWD_THREADS)) {
+        case 32:                                            // short rows: no more than they have
+            if (VEC <= 4 && p.N <= 4 * 32) return fwd_pass<X, W, VEC, (VEC <= 4 ? 4 / VEC : 1), 32>(p, st);
+            return p.N <= 8 * 32 ? fwd_pass<X, W, VEC, 8 / VEC, 32>(p, st) : fwd_pass<X, W, VEC, I, 32>(p, st);
+        case 64: return fwd_pass<X, W, VEC, I, 64>(p, st);
+        case 128: return fwd_pass<X, W, VEC, I, 128>(p, st);
+        default: return p.N <= FWD_VALUES * FWD_THREADS ? fwd_pass<X, W, VEC, I, FWD_THREADS>(p, st) : fwd_pass<X, W, VEC, MOST, FWD_THREADS>(p, st);
+    }
+}
+template <typename X, typename W, int VEC>
+cudaError_t bwd_vec(const Params& p, cudaStream_t st) {
+    constexpr int V = bwd_values(sizeof(X)), I = V / VEC, MOST = MAX_N / BWD_THREADS / VEC;
+    switch (lanes_of(p.N, V, BWD_THREADS)) {
+        case 32:
+            if (VEC <= 4 && p.N <= 4 * 32) return bwd_pass<X, W, VEC, (VEC <= 4 ? 4 / VEC : 1), 32>(p, st);
+            return p.N <= 8 * 32 ? bwd_pass<X, W, VEC, 8 / VEC, 32>(p, st) : bwd_pass<X, W, VEC, I, 32>(p, st);
+        case 64: return bwd_pass<X, W, VEC, I, 64>(p, st);
+        case 128: return bwd_pass<X, W, VEC, I, 128>(p, st);
+        case 256: return bwd_pass<X, W, VEC, I, 256>(p, st);
+        default: return p.N <= V * BWD_THREADS ? bwd_pass<X, W, VEC, I, BWD_THREADS>(p, st) : bwd_pass<X, W, VEC, MOST, BWD_THREADS>(p, st);
     }
 }
 template <typename X, typename W>
 cudaError_t rows_in_registers(bool back, const Params& p, cudaStream_t st) {
     constexpr int VEC = 16 / (int)sizeof(X);
-    return p.N % VEC == 0 ? pass_vec<X, W, VEC>(back, p, st) : pass_vec<X, W, 1>(back, p, st);
+    if (back) return p.N % VEC == 0 ? bwd_vec<X, W, VEC>(p, st) : bwd_vec<X, W, 1>(p, st);
+    return p.N % VEC == 0 ? fwd_vec<X, W, VEC>(p, st) : fwd_vec<X, W, 1>(p, st);
 }
 template <typename X, typename W>
 cudaError_t forward(const Params& p, cudaStream_t st) {
@@ -587,7 +585,7 @@ extern "C" {
 
 size_t llattn_layer_norm_bwd_workspace_bytes(long rows, int N) {
     if (norm::check(0, 0, rows, N) != 0) return 0;
-    return (size_t)norm::parts_of(rows, N) * 2 * N * sizeof(float);
+    return (size_t)norm::parts_of(rows, N, 2) * 2 * N * sizeof(float);
 }
 
 int llattn_layer_norm_fwd(const void* x, int x_is_f32, const void* w, const void* b, int w_is_f32, void* y, float* mean, float* rstd, float eps, long rows,
@@ -630,7 +628,7 @@ int llattn_layer_norm_bwd(const void* x, int x_is_f32, const void* w, int w_is_f
     p.part = static_cast<float*>(workspace);
     p.rows = rows;
     p.N = N;
-    p.parts = norm::parts_of(rows, N);
+    p.parts = norm::parts_of(rows, N, x_is_f32 ? 4 : 2);
     cudaStream_t st = (cudaStream_t)stream;
     if (x_is_f32) return (int)norm::backward<float, float>(p, st);
     return (int)(w_is_f32 ? norm::backward<norm::bf16, float>(p, st) : norm::backward<norm::bf16, norm::bf16>(p, st));
