@@ -38,7 +38,7 @@ __global__ void __launch_bounds__(256) window_fill_kernel(const bf16* k, const b
 int check(long B, long T, long H, long G, int K, long window, long sinks, float scale) {
     if (B < 1 || T < 1 || G < 1 || H < 1 || (K != 64 && K != 128) || window < 1 || sinks < 0 || !(scale > 0.f) || !(scale < INFINITY)) return LLATTN_ERR_UNSUPPORTED_SHAPE;
     if (H % G != 0) return LLATTN_ERR_BAD_GROUPS;
-    if (T > (1 << 24) || window > (1 << 29) || sinks > (1 << 29) || B > 65535 || H > 65535) return LLATTN_ERR_UNSUPPORTED_SHAPE;
+    if (T > (1 << 24) || window > (1 << 29) || sinks > (1 << 29) || B > 65535 || H > 65535 || (T + 127) / 128 * H > 0x7fffffffl) return LLATTN_ERR_UNSUPPORTED_SHAPE;
     return 0;
 }
 int padded(int T) { return (T + TILE - 1) / TILE * TILE; }

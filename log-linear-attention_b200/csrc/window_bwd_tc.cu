@@ -141,7 +141,8 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dq_tc_kernel(const __
     float* sDelta = reinterpret_cast<float*>(smem + SM::stat_off);           // [128]
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int q0 = blockIdx.x * TILE, h = blockIdx.y, b = blockIdx.z, grp = h / (p.H / p.G);
+    // heads first, later queries first: those see more tiles, and the last CTAs of a launch are its short ones
+    const int h = blockIdx.x % p.H, q0 = (gridDim.x / p.H - 1 - blockIdx.x / p.H) * TILE, b = blockIdx.y, grp = h / (p.H / p.G);
     const Span span(q0, p.T, p.window, p.sinks);
     const int steps = span.count();
     const auto tile = [&](int n) { return span.tile(n); };
@@ -547,7 +548,7 @@ static cudaError_t launch(const Params& p, cudaStream_t st) {
     cudaError_t e = allow_smem(dq, smem);
     if (e == cudaSuccess) e = allow_smem(dkv, smem);
     if (e != cudaSuccess) return e;
-    e = launch_chained(dq, dim3(sh.tiles, p.H, p.B), bwd::NTHREADS, smem, st, p);
+    e = launch_chained(dq, dim3((unsigned)(sh.tiles * p.H), p.B), bwd::NTHREADS, smem, st, p);
     if (e != cudaSuccess) return e;
     LLATTN_LAUNCHED();
     e = launch_chained(dkv, dim3(sh.far_tiles * sh.chunks + sh.tiles * sh.splits, p.G, p.B), bwd::NTHREADS, smem, st, p, sh);

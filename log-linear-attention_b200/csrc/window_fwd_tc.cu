@@ -62,7 +62,8 @@ __global__ void __launch_bounds__(fwd::NTHREADS, 1) window_fwd_tc_kernel(const _
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int q0 = blockIdx.x * 2 * TILE, h = blockIdx.y, b = blockIdx.z, grp = h / (p.H / p.G);
+    // heads first, later queries first: those see more tiles, and the last CTAs of a launch are its short ones
+    const int h = blockIdx.x % p.H, q0 = (gridDim.x / p.H - 1 - blockIdx.x / p.H) * 2 * TILE, b = blockIdx.y, grp = h / (p.H / p.G);
     if (tid == 0) {
         for (int i = 0; i < NST; ++i) {
             umma::mbar_init(full + i, 1);
@@ -279,7 +280,7 @@ static cudaError_t launch(const Params& p, cudaStream_t st) {
     const auto kern = window_fwd_tc_kernel<K>;
     cudaError_t e = allow_smem(kern, fwd::Smem<K>::total);
     if (e != cudaSuccess) return e;
-    const dim3 grid((unsigned)((p.T + 2 * TILE - 1) / (2 * TILE)), p.H, p.B);
+    const dim3 grid((unsigned)((p.T + 2 * TILE - 1) / (2 * TILE) * p.H), p.B);
     e = launch_chained(kern, grid, fwd::NTHREADS, fwd::Smem<K>::total, st, p);
     if (e == cudaSuccess) LLATTN_LAUNCHED();
     return e;
