@@ -585,7 +585,7 @@ extern "C" {
 
 size_t llattn_layer_norm_bwd_workspace_bytes(long rows, int N) {
     if (norm::check(0, 0, rows, N) != 0) return 0;
-    return (size_t)norm::parts_of(rows, N, 2) * 2 * N * sizeof(float);
+    return (size_t)norm::parts_of(rows, N, 4) * 2 * N * sizeof(float);       // (of either type: fp32 rows have the more parts)
 }
 
 int llattn_layer_norm_fwd(const void* x, int x_is_f32, const void* w, const void* b, int w_is_f32, void* y, float* mean, float* rstd, float eps, long rows,
