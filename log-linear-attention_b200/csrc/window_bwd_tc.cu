@@ -51,27 +51,16 @@ struct Ring {
 __device__ __forceinline__ void regs_issue() { asm volatile("setmaxnreg.dec.sync.aligned.u32 72;\n"); }
 __device__ __forceinline__ void regs_rows() { asm volatile("setmaxnreg.inc.sync.aligned.u32 216;\n"); }
 
-// exp2(c s - shift) of 64 scores, a quarter of them on the FMA pipes where no key is hidden (whose value has to be an exact zero); shift(u) gives the pair of values for keys u, u + 1
+// exp2(c s - shift) of 64 scores; shift(u) gives the pair of values for keys u, u + 1.  (A share of them on the FMA pipes, as in the forward, changes nothing here: 1.63 to
+// 1.65 ms for none to a half of them at T = 16384.)
 template <typename ShiftT>
-__device__ __forceinline__ void exponentials(float (&e)[64], float c, bool whole, ShiftT shift) {
+__device__ __forceinline__ void exponentials(float (&e)[64], float c, ShiftT minus_shift) {
     const F2 c2 = pair(c, c);
-    if (whole) {
 #pragma unroll
-        for (int u = 0; u < 64; u += 2) {
-            const F2 y = fma2(pair(e[u], e[u + 1]), c2, shift(u));
-            float2 v = both(y);
-            if (u % 8 == 6) v = exp2_poly(y);
-            else v = make_float2(exp2_fast(v.x), exp2_fast(v.y));
-            e[u] = v.x;
-            e[u + 1] = v.y;
-        }
-    } else {
-#pragma unroll
-        for (int u = 0; u < 64; u += 2) {
-            const float2 v = both(fma2(pair(e[u], e[u + 1]), c2, shift(u)));
-            e[u] = exp2_fast(v.x);
-            e[u + 1] = exp2_fast(v.y);
-        }
+    for (int u = 0; u < 64; u += 2) {
+        const float2 v = both(fma2(pair(e[u], e[u + 1]), c2, minus_shift(u)));
+        e[u] = exp2_fast(v.x);
+        e[u + 1] = exp2_fast(v.y);
     }
 }
 // 64 values of a row as bf16 into the first half of the columns they came from
@@ -275,9 +264,8 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dq_tc_kernel(const __
             umma::fence_after_sync();
             float e[64], d[64];
             tmem_ld64(tS + 128 * (n & 1), e);
-            const bool whole = all_seen(q0, s0, p.window, p.sinks);
-            exponentials(e, c, whole, [&](int) { return pair(-lse, -lse); });
-            if (!whole) {
+            exponentials(e, c, [&](int) { return pair(-lse, -lse); });
+            if (!all_seen(q0, s0, p.window, p.sinks)) {
 #pragma unroll
                 for (int i = 0; i < 64; i += 32) {
                     const uint32_t bits = seen_bits(t, s0 + half * 64 + i, p.window, p.sinks);
@@ -442,12 +430,11 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dkv_tc_kernel(const _
             umma::fence_after_sync();
             float e[64], d[64];
             tmem_ld64(tS, e);
-            const bool whole = all_seen(t0, s0, p.window, p.sinks);
-            exponentials(e, c, whole, [&](int u) {
+            exponentials(e, c, [&](int u) {
                 const float2 m = *reinterpret_cast<const float2*>(lse + u);
                 return pair(-m.x, -m.y);
             });
-            if (!whole) {
+            if (!all_seen(t0, s0, p.window, p.sinks)) {
                 // token s is seen by the queries from s on, as far as the window goes; a sink by all of them
 #pragma unroll
                 for (int k = 0; k < 64; k += 32) {
