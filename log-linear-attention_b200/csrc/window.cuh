@@ -97,10 +97,15 @@ __device__ __forceinline__ uint32_t seeing_bits(int t0, int s, int window, int s
 
 // 2^x of a pair on the FMA pipes, for a share of the exponentials where the special-function unit (four lanes a cycle and scheduler) is the bottleneck.  x = n + f with n the
 // nearest integer, which adding 1.5 2^23 leaves in the low bits; 2^f, f in [-1/2, 1/2], by the minimax polynomial of degree 4 in the relative error (Remez exchange:
-// 2.6e-6); n goes to the exponent by an integer addition.  Below -126 the result is 2^-126.
+// 2.6e-6), times 2^n (a product, not an addition to the exponent, so that NaN stays NaN).  Below -126 the result is 2^-126.
+__device__ __forceinline__ float at_least(float x, float low) {                // NaN if x is
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(x), "f"(low));
+    return y;
+}
 __device__ __forceinline__ float2 exp2_poly(F2 x) {
     const float2 v = both(x);
-    x = pair(fmaxf(v.x, -126.f), fmaxf(v.y, -126.f));
+    x = pair(at_least(v.x, -126.f), at_least(v.y, -126.f));
     const F2 magic = pair(12582912.f, 12582912.f), back = pair(-12582912.f, -12582912.f);
     const F2 r = add(x, magic), n = add(r, back), f = fma2(n, pair(-1.f, -1.f), x);
     F2 y = pair(0.009570102207362652f, 0.009570102207362652f);
@@ -108,8 +113,8 @@ __device__ __forceinline__ float2 exp2_poly(F2 x) {
     y = fma2(y, f, pair(0.240247443318367f, 0.240247443318367f));
     y = fma2(y, f, pair(0.6931217908859253f, 0.6931217908859253f));
     y = fma2(y, f, pair(0.9999992847442627f, 0.9999992847442627f));
-    const float2 a = both(y), k = both(r);
-    return make_float2(__int_as_float(__float_as_int(a.x) + (__float_as_int(k.x) << 23)), __int_as_float(__float_as_int(a.y) + (__float_as_int(k.y) << 23)));
+    const float2 k = both(r);
+    return both(mul(y, pair(__int_as_float(0x3f800000 + (__float_as_int(k.x) << 23)), __int_as_float(0x3f800000 + (__float_as_int(k.y) << 23)))));
 }
 
 __device__ __forceinline__ float exp2_fast(float x) {

@@ -8,6 +8,8 @@
 // In both, eight warps do the exponentials (two threads a row, 64 columns each), one issues products, one brings tiles through a ring; the products of one
 // half of a step run under the other half's exponentials.  (Summing dQ beside dK and dV would save two of the seven products a pair of tiles, for
 // atomics on 64 KB of fp32 a pair.)
+// T = 16384, 32 query heads on 8, K = 128, window 2048: 1.61 ms, 0.80 PFLOP/s counting five products (1.12 of the seven made).  The exponentials' side of a step is longer
+// than its products: about 2160 cycles for 1536 of dQ, 2850 for 2048 of dK and dV.
 #include "window.cuh"
 
 namespace llattn {

@@ -8,6 +8,7 @@
 //
 // The slots of a (sequence, group) are spread over the warps of a cluster of CTAs, which join their maxima, sums and outputs through each other's shared memory:
 // one launch, no workspace, the order of every sum given by the sizes.
+// 64 sequences, 32 heads on 8, K = 128, 2052 slots: 92 us, 5.9 TB/s.  One sequence: 9.8 us, latency (two loads, a cluster's barriers and two joins one after another).
 #include <cooperative_groups.h>
 
 #include "../../include/llattn.h"

@@ -300,3 +300,31 @@ def test_empty_operands():
     assert o.shape == q.shape and torch.autograd.grad(o.sum(), [q, k])[1].shape == k.shape
     _, state = sliding_window_prefill(q, k, k, 4, 1)
     assert state.k.shape == (2, 5, 2, 64) and (state.lengths == 0).all()
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("K", [64, 128])
+def test_non_finite_keys(K, bad):
+    """A key that is not finite spoils the rows that see it, whatever its place in a tile, and none of the others."""
+    from hattention_b200 import sliding_window_attention
+    T, window = 500, 200
+    q, k, v = make(1, T, 2, 1, K)[:3]
+    q[..., 0] = 1.0                                    # (a product with inf is +-inf, never NaN: of one sign in every row)
+    clean = sliding_window_attention(q, k, v, window)
+    for s in list(range(128, 144)) + [0, 255, 256, 499]:
+        spoiled = k.clone()
+        spoiled[0, s, 0, 0] = bad
+        o = sliding_window_attention(q, spoiled, v, window)
+        rows = orc.seen(T, window, 0, "cuda")[:, s]
+        assert torch.equal(o[0, ~rows], clean[0, ~rows]), s
+        if bad != -math.inf:
+            assert o[0, rows].isnan().all(), s
+            continue
+        # weight 0: the row without that key; nothing is left of a row that sees it alone
+        alone = rows & (torch.arange(T, device="cuda") == 0)
+        assert o[0, alone].isnan().all()
+        left = orc.seen(T, window, 0, "cuda")
+        left[:, s] = False
+        P = torch.einsum("thk,sk->ths", q[0].double(), k[0, :, 0].double()).mul(K ** -0.5).masked_fill(~left[:, None], -math.inf).softmax(-1)
+        mean = lambda x: torch.einsum("ths,sk->thk", P, x[0, :, 0].double())[rows & ~alone]
+        within(o[0, rows & ~alone], mean(v), (HALF + 2 * D) * mean(v.abs()), f"without {s}")
