@@ -38,7 +38,7 @@ __global__ void __launch_bounds__(256) window_fill_kernel(const bf16* k, const b
 int check(long B, long T, long H, long G, int K, long window, long sinks, float scale) {
     if (B < 1 || T < 1 || G < 1 || H < 1 || (K != 64 && K != 128) || window < 1 || sinks < 0 || !(scale > 0.f) || !(scale < INFINITY)) return LLATTN_ERR_UNSUPPORTED_SHAPE;
     if (H % G != 0) return LLATTN_ERR_BAD_GROUPS;
-    if (T > (1 << 24) || window > (1 << 29) || sinks > (1 << 29) || B > 65535 || H > 65535 || (T + 127) / 128 * H > 0x7fffffffl) return LLATTN_ERR_UNSUPPORTED_SHAPE;
+    if (T > (1 << 24) || window > (1 << 29) || sinks > (1 << 29) || B > 65535 || H > 65535 || (T + 127) / 128 * H * B > 0x3fffffffl) return LLATTN_ERR_UNSUPPORTED_SHAPE;
     return 0;
 }
 int padded(int T) { return (T + TILE - 1) / TILE * TILE; }
@@ -59,6 +59,12 @@ void shape(Params& p, void* workspace, int B, int T, int H, int G, int window, i
     p.window = window;
     p.sinks = sinks;
     p.scale = scale;
+}
+// Tensor maps are made by the driver, for the calling thread's context: a thread that has made no runtime call yet gets it here.
+cudaError_t current_context() {
+    int device;
+    const cudaError_t e = cudaGetDevice(&device);
+    return e == cudaSuccess ? cudaSetDevice(device) : e;
 }
 bool maps(Params& p, const void* q, const void* k, const void* v, int K) {
     return tma::make_seq_map(&p.tq, q, p.B, p.T, p.H, K, TILE, 2) == 0 && tma::make_seq_map(&p.tk, k, p.B, p.T, p.G, K, TILE, 2) == 0 &&
@@ -94,7 +100,7 @@ int llattn_window_fwd(const void* q, const void* k, const void* v, void* o, void
     win::shape(p, workspace, B, T, H, G, window, sinks, scale);
     win::statistics(p, stats);
     cudaStream_t st = (cudaStream_t)stream;
-    const cudaError_t e = cudaMemsetAsync(workspace, 0, 4, st);        // (before the maps: the first runtime call of a thread gives it the context that they need)
+    const cudaError_t e = win::current_context();
     if (e != cudaSuccess) return (int)e;
     if (!win::maps(p, q, k, v, K)) return LLATTN_ERR_TENSOR_MAP;
     return (int)win::forward_tc(p, K, st);
@@ -119,7 +125,7 @@ int llattn_window_bwd(const void* q, const void* k, const void* v, const void* o
     win::shape(p, workspace, B, T, H, G, window, sinks, scale);
     win::statistics(p, const_cast<void*>(stats));
     cudaStream_t st = (cudaStream_t)stream;
-    const cudaError_t e = cudaMemsetAsync(workspace, 0, 4, st);
+    const cudaError_t e = win::current_context();
     if (e != cudaSuccess) return (int)e;
     if (!win::maps(p, q, k, v, K) || tma::make_seq_map(&p.tdo, d_o, B, T, H, K, win::TILE, 2) != 0) return LLATTN_ERR_TENSOR_MAP;
     return (int)win::backward_tc(p, K, st);

@@ -84,30 +84,33 @@ __device__ __forceinline__ void gemm_halves(uint32_t lead, uint32_t d, uint32_t 
     umma::gemm_tm_lead<TILE, 64>(lead, d, a, b_saddr, idesc, accumulate);
     umma::gemm_tm_lead<TILE, 64>(lead, d, a + 64, b_saddr + 64 * umma::ROW_BYTES, idesc, true);
 }
-// row of K / 2 fp32 columns times f, as bf16
+// 32 rows of K / 2 fp32 columns times f, as bf16, rows [first, last) of them to `out`, `stride` bytes apart; buf: K * 64 bytes of shared memory a warp
 template <int K>
-__device__ __forceinline__ void put_row(uint32_t taddr, bf16* out, float f, bool there) {
+__device__ __forceinline__ void put_rows(uint32_t taddr, unsigned char* buf, int lane, bf16* out, long stride, float f, int first, int last) {
+    const Rows<K / 16> rows = {reinterpret_cast<uint4*>(buf), lane};
 #pragma unroll
-    for (int i = 0; i < K / 2; i += 16) {
-        float o[16];
-        umma::tmem_ld16(taddr + i, o);
-        uint32_t w[8];
+    for (int i = 0; i < K / 2; i += 32) {
+        float o[32];
+        umma::tmem_ld32(taddr + i, o);
 #pragma unroll
-        for (int u = 0; u < 8; ++u) w[u] = pack_bf16(o[2 * u] * f, o[2 * u + 1] * f);
-        if (there) store_32B(out + i, w);
+        for (int u = 0; u < 32; u += 8)
+            rows.put((i + u) / 8, pack_bf16(o[u] * f, o[u + 1] * f), pack_bf16(o[u + 2] * f, o[u + 3] * f), pack_bf16(o[u + 4] * f, o[u + 5] * f), pack_bf16(o[u + 6] * f, o[u + 7] * f));
     }
+    rows.store(out, stride, first, last);
 }
 // the same unrounded
 template <int K>
-__device__ __forceinline__ void put_part(uint32_t taddr, float* out, bool there) {
+__device__ __forceinline__ void put_parts(uint32_t taddr, unsigned char* buf, int lane, float* out, int first, int last) {
+    const Rows<K / 8> rows = {reinterpret_cast<uint4*>(buf), lane};
 #pragma unroll
-    for (int i = 0; i < K / 2; i += 16) {
-        float o[16];
-        umma::tmem_ld16(taddr + i, o);
-        if (there)
+    for (int i = 0; i < K / 2; i += 32) {
+        float o[32];
+        umma::tmem_ld32(taddr + i, o);
 #pragma unroll
-            for (int u = 0; u < 16; u += 4) *reinterpret_cast<float4*>(out + i + u) = make_float4(o[u], o[u + 1], o[u + 2], o[u + 3]);
+        for (int u = 0; u < 32; u += 4)
+            rows.put((i + u) / 4, __float_as_uint(o[u]), __float_as_uint(o[u + 1]), __float_as_uint(o[u + 2]), __float_as_uint(o[u + 3]));
     }
+    rows.store(out, 2 * K * sizeof(float), first, last);
 }
 __device__ __forceinline__ void load_stat(float* dst, const float* src, uint64_t* bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n"
@@ -118,6 +121,7 @@ __device__ __forceinline__ void load_stat(float* dst, const float* src, uint64_t
 template <int K>
 __global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dq_tc_kernel(const __grid_constant__ Params p) {
     chain_wait();
+    clear_status(p);
     using namespace bwd;
     using SM = Smem<K>;
     constexpr int NA = SM::NA, NB = SM::NB, TM_S = 0, TM_DP = 256, TM_DQ = 384;         // S twice
@@ -132,12 +136,13 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dq_tc_kernel(const __
     float* sDelta = reinterpret_cast<float*>(smem + SM::stat_off);           // [128]
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    // heads first, later queries first: those see more tiles, and the last CTAs of a launch are its short ones
+    // heads first, later queries first: those see more tiles, and the last CTAs of a launch are its short ones.  (Sequences before tiles too, as in the other kernels: 92.3 us for
+    // 89.0, both kernels, 4 x 1000 tokens.)
     const int h = blockIdx.x % p.H, q0 = (gridDim.x / p.H - 1 - blockIdx.x / p.H) * TILE, b = blockIdx.y, grp = h / (p.H / p.G);
     const Span span(q0, p.T, p.window, p.sinks);
     const int steps = span.count();
     const auto tile = [&](int n) { return span.tile(n); };
-    if (tid == 0) {
+    if (tid == TMA_WARP * 32) {              // (the thread that brings the tiles need not wait for the others)
         ringK.init();
         ringV.init();
         umma::mbar_init(barQ, 1);
@@ -148,6 +153,9 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dq_tc_kernel(const __
         umma::mbar_init(barDone, 1);
         umma::fence_mbar_init();
         *abort_flag = 0;
+        tma::expect_tx(barQ, 2 * SM::TILE_BYTES);
+        load_tile<K>(smem + SM::stay_off, &p.tq, h, q0, b, barQ);
+        load_tile<K>(smem + SM::stay_off + SM::TILE_BYTES, &p.tdo, h, q0, b, barQ);
     }
     if (warp == MMA_WARP) umma::tmem_alloc(tmem_slot, 512);
     umma::fence_before_sync();
@@ -158,9 +166,6 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dq_tc_kernel(const __
     if (warp >= 8) {
         regs_issue();
         if (warp == TMA_WARP && lane == 0) {
-            tma::expect_tx(barQ, 2 * SM::TILE_BYTES);
-            load_tile<K>(smem + SM::stay_off, &p.tq, h, q0, b, barQ);
-            load_tile<K>(smem + SM::stay_off + SM::TILE_BYTES, &p.tdo, h, q0, b, barQ);
             int nk = 0, nv = 0;
             while (nv < steps) {
                 if (!ringK.wait_free(nk, abort_flag)) break;
@@ -211,8 +216,7 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dq_tc_kernel(const __
     } else {
         regs_rows();
         const int half = warp >> 2, row = (warp & 3) * 32 + lane, t = q0 + row;
-        const bool there = t < p.T;
-        const long at = (((long)b * p.T + t) * p.H + h) * K + half * (K / 2), stat = ((long)b * p.H + h) * p.TP + t;
+        const long stat = ((long)b * p.H + h) * p.TP + t;
         const uint32_t tS = umma::tmem_addr(tmem, warp, TM_S + 64 * half), tDP = umma::tmem_addr(tmem, warp, TM_DP + 64 * half);
         const float c = p.scale * LOG2E, lse = p.lse[stat];
         // delta of the tile's rows: a warp takes 16 of them, K / 8 lanes a row (a thread a row: 10 k cycles, for loads that touch a line a lane)
@@ -292,7 +296,10 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dq_tc_kernel(const __
         if (ok) ok = umma::mbar_wait_warp(barDone, 0, abort_flag);
         if (ok) {
             umma::fence_after_sync();
-            put_row<K>(umma::tmem_addr(tmem, warp, TM_DQ + half * (K / 2)), p.dq + at, p.scale, there);
+            // (all products are done: the place of Q and dO is free)
+            const int first = q0 + (warp & 3) * 32;
+            put_rows<K>(umma::tmem_addr(tmem, warp, TM_DQ + half * (K / 2)), smem + SM::stay_off + warp * K * 64, lane,
+                        p.dq + (((long)b * p.T + first) * p.H + h) * K + half * (K / 2), (long)p.H * K * 2, p.scale, 0, min(p.T - first, 32));
         }
         umma::fence_before_sync();
     }
@@ -325,15 +332,17 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dkv_tc_kernel(const _
     float* sStat = reinterpret_cast<float*>(smem + SM::stat_off);
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int grp = blockIdx.y, b = blockIdx.z, R = p.H / p.G, last = sh.tiles - 1;
+    // groups and sequences first; tiles of sinks first, the last tiles, which few queries see, last  (sequences, then groups, outermost: 414 us for 394, both kernels, T = 4096, 32 heads
+    // on 8, window 2048)
+    const int units = p.B * p.G, x0 = blockIdx.x / units, grp = blockIdx.x % units % p.G, b = blockIdx.x % units / p.G, R = p.H / p.G, last = sh.tiles - 1;
     // far shares first, then the near ones; tile j of k and v, tiles [lo, hi] of queries, heads h0 on
-    const bool far = (int)blockIdx.x < sh.far_tiles * sh.chunks;
-    const int x = far ? blockIdx.x : blockIdx.x - sh.far_tiles * sh.chunks, j = far ? x / sh.chunks : x / sh.splits, share = far ? x % sh.chunks : x % sh.splits;
+    const bool far = x0 < sh.far_tiles * sh.chunks;
+    const int x = far ? x0 : x0 - sh.far_tiles * sh.chunks, j = far ? x / sh.chunks : x / sh.splits, share = far ? x % sh.chunks : x % sh.splits;
     const int lo = far ? j + sh.near + share * sh.chunk : j, end = far ? lo + sh.chunk - 1 : j + sh.near - 1, hi = end < last ? end : last;
     const int each = far ? R : (R + sh.splits - 1) / sh.splits, h0 = grp * R + (far ? 0 : share * each), heads = min(each, grp * R + R - h0);
     if (lo > last || heads <= 0) return;                    // (a share that the last tiles do not reach; fewer heads than shares)
     const int s0 = j * TILE, per = hi - lo + 1, steps = heads * per;
-    if (tid == 0) {
+    if (tid == TMA_WARP * 32) {              // (the thread that brings the tiles need not wait for the others)
         ringQ.init();
         ringDO.init();
         umma::mbar_init(barKV, 1);
@@ -344,6 +353,9 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dkv_tc_kernel(const _
         umma::mbar_init(barDone, 1);
         umma::fence_mbar_init();
         *abort_flag = 0;
+        tma::expect_tx(barKV, 2 * SM::TILE_BYTES);
+        load_tile<K>(smem + SM::stay_off, &p.tk, grp, s0, b, barKV);
+        load_tile<K>(smem + SM::stay_off + SM::TILE_BYTES, &p.tv, grp, s0, b, barKV);
     }
     if (warp == MMA_WARP) umma::tmem_alloc(tmem_slot, 512);
     umma::fence_before_sync();
@@ -354,9 +366,6 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dkv_tc_kernel(const _
     if (warp >= 8) {
         regs_issue();
         if (warp == TMA_WARP && lane == 0) {
-            tma::expect_tx(barKV, 2 * SM::TILE_BYTES);
-            load_tile<K>(smem + SM::stay_off, &p.tk, grp, s0, b, barKV);
-            load_tile<K>(smem + SM::stay_off + SM::TILE_BYTES, &p.tv, grp, s0, b, barKV);
             int nq = 0, nd = 0, h = h0, i = lo;
             while (nd < steps) {
                 const long stat = ((long)b * p.H + h) * p.TP + i * TILE;
@@ -465,20 +474,21 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dkv_tc_kernel(const _
         if (ok) ok = umma::mbar_wait_warp(barDone, 0, abort_flag);
         if (ok) {
             umma::fence_after_sync();
-            const long at = (((long)b * p.T + s) * p.G + grp) * K + half * (K / 2), unit = (long)b * p.G + grp;
+            const int row0 = (warp & 3) * 32, first = s0 + row0, last = min(p.T - first, 32);
+            const long at = (((long)b * p.T + first) * p.G + grp) * K + half * (K / 2), unit = (long)b * p.G + grp;
             const uint32_t tDV = umma::tmem_addr(tmem, warp, TM_DV + half * (K / 2)), tDK = umma::tmem_addr(tmem, warp, TM_DK + half * (K / 2));
-            const bool sink = j < sh.far_tiles && s < p.sinks;                     // a token with parts from far
+            unsigned char* buf = smem + SM::stay_off + warp * K * 64;              // (all products are done: the place of K and V is free)
+            const int sink = j < sh.far_tiles ? max(min(p.sinks - first, 32), 0) : 0;        // tokens with parts from far
             if (far || sh.splits > 1 || j < sh.far_tiles) {
-                const int row = s - s0;
-                float* part = far ? p.far_part + (((unit * sh.far_tiles + j) * sh.chunks + share) * sh.far_rows(p.sinks) + row) * 2 * K
-                                  : p.near_part + (((unit * sh.splits + share) * sh.near_tiles() + j) * TILE + row) * 2 * K;
-                const bool there = s < p.T && (sink || (!far && sh.splits > 1));
-                put_part<K>(tDK, part + half * (K / 2), there);
-                put_part<K>(tDV, part + K + half * (K / 2), there);
+                float* part = far ? p.far_part + (((unit * sh.far_tiles + j) * sh.chunks + share) * sh.far_rows(p.sinks) + row0) * 2 * K
+                                  : p.near_part + (((unit * sh.splits + share) * sh.near_tiles() + j) * TILE + row0) * 2 * K;
+                const int parts = !far && sh.splits > 1 ? last : min(sink, last);
+                put_parts<K>(tDK, buf, lane, part + half * (K / 2), 0, parts);
+                put_parts<K>(tDV, buf, lane, part + K + half * (K / 2), 0, parts);
             }
             if (!far && sh.splits == 1) {
-                put_row<K>(tDV, p.dv + at, 1.f, s < p.T && !sink);
-                put_row<K>(tDK, p.dk + at, p.scale, s < p.T && !sink);
+                put_rows<K>(tDV, buf, lane, p.dv + at, (long)p.G * K * 2, 1.f, sink, last);
+                put_rows<K>(tDK, buf, lane, p.dk + at, (long)p.G * K * 2, p.scale, sink, last);
             }
         }
         umma::fence_before_sync();
@@ -537,10 +547,10 @@ static cudaError_t launch(const Params& p, cudaStream_t st) {
     cudaError_t e = allow_smem(dq, smem);
     if (e == cudaSuccess) e = allow_smem(dkv, smem);
     if (e != cudaSuccess) return e;
-    e = launch_chained(dq, dim3((unsigned)(sh.tiles * p.H), p.B), bwd::NTHREADS, smem, st, p);
+    e = launch_chained(dq, dim3((unsigned)sh.tiles * p.H, p.B), bwd::NTHREADS, smem, st, p);
     if (e != cudaSuccess) return e;
     LLATTN_LAUNCHED();
-    e = launch_chained(dkv, dim3(sh.far_tiles * sh.chunks + sh.tiles * sh.splits, p.G, p.B), bwd::NTHREADS, smem, st, p, sh);
+    e = launch_chained(dkv, (unsigned)(sh.far_tiles * sh.chunks + sh.tiles * sh.splits) * p.G * p.B, bwd::NTHREADS, smem, st, p, sh);
     if (e != cudaSuccess) return e;
     LLATTN_LAUNCHED();
     const int some = sh.far_tiles * TILE < p.sinks ? sh.far_tiles * TILE : p.sinks, tokens = sh.splits > 1 ? p.T : some;
