@@ -20,6 +20,7 @@ namespace win {
 namespace step {
 namespace cg = cooperative_groups;
 constexpr int BLOCK = 16;                      // slots a warp takes at once
+constexpr int MAX_RANKS = 16;
 template <int NT>
 struct Cta {
     static constexpr int WARPS = NT == 1 ? 8 : 4;      // (16 heads: twice the registers, twice the shared memory a warp)
@@ -45,6 +46,23 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {       // of an 8 x 
 __device__ __forceinline__ uint4 slot_words(const bf16* p, bool there) {
     return there ? *reinterpret_cast<const uint4*>(p) : make_uint4(0, 0, 0, 0);
 }
+// NT tiles of eight heads from h0 on, q at the first of them
+template <int K, int NT>
+__device__ __forceinline__ void load_queries(uint32_t (&qf)[NT][K / 8], const Params& p, const bf16* q, int h0, int r, int c) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < K / 32; ++i) {
+            const uint4 w = slot_words(q + (long)(8 * n + r) * K + (c + 4 * i) * 8, h0 + 8 * n + r < p.R);
+            qf[n][4 * i] = w.x;
+            qf[n][4 * i + 1] = w.y;
+            qf[n][4 * i + 2] = w.z;
+            qf[n][4 * i + 3] = w.w;
+        }
+}
+// the cluster's barrier in two halves; what is written before one is there behind the other
+__device__ __forceinline__ void arrive(const cg::cluster_group&) { cg::cluster_group::barrier_arrive(); }
+__device__ __forceinline__ void wait(const cg::cluster_group&) { cg::cluster_group::barrier_wait(); }
 }  // namespace step
 
 // NT tiles of eight heads together
@@ -54,37 +72,40 @@ __global__ void __launch_bounds__(32 * step::Cta<NT>::WARPS, 2) window_step_kern
     using namespace step;
     constexpr int HEADS = 8 * NT, WARPS = Cta<NT>::WARPS;
     __shared__ float sO[WARPS][HEADS][K + 4];            // (the warps' outputs; the CTA's in the first)
-    __shared__ float sM[WARPS + 1][HEADS], sL[WARPS + 1][HEADS];
+    __shared__ float sM[WARPS][HEADS], sL[WARPS][HEADS];
+    // what the cluster's CTAs send this one: their outputs, maxima and sums of the elements (head, column) that it joins
+    __shared__ float rO[HEADS * K], rM[MAX_RANKS][HEADS], rL[MAX_RANKS][HEADS];
     cg::cluster_group cluster = cg::this_cluster();
     const int ranks = cluster.num_blocks(), rank = cluster.block_rank();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, c = lane & 3;
     const int unit = blockIdx.x / ranks, grp = unit % p.G;
     const long b = unit / p.G;
-    const long long count = p.counts[unit], seen = count > 0 ? count : 0;
-    const int slots = p.sinks + p.window, slot = (int)(seen < p.sinks ? seen : p.sinks + (seen - p.sinks) % p.window);
-    const int held = (int)min((long long)slots, seen + 1), stride = ranks * WARPS * BLOCK, first = (rank * WARPS + warp) * BLOCK;
+    const int slots = p.sinks + p.window, stride = ranks * WARPS * BLOCK, first = (rank * WARPS + warp) * BLOCK;
     const long ld = (long)p.G * K;
     bf16 *kb = p.kc + (b * slots * p.G + grp) * K, *vb = p.vc + (b * slots * p.G + grp) * K;
+    // what does not depend on the count is on its way before the count is there
+    arrive(cluster);
+    const long long count = p.counts[unit];
+    const uint4 none = make_uint4(0, 0, 0, 0);
+    const uint4 new_k = lane < K / 8 ? reinterpret_cast<const uint4*>(p.k + (long)unit * K)[lane] : none;
+    const uint4 new_v = lane < K / 8 ? reinterpret_cast<const uint4*>(p.v + (long)unit * K)[lane] : none;
+    uint32_t qf[NT][K / 8];
+    load_queries<K, NT>(qf, p, p.q + (b * p.H + grp * p.R) * K, 0, r, c);
+    const long long seen = count > 0 ? count : 0;
+    const int slot = (int)(seen < p.sinks ? seen : p.sinks + (seen - p.sinks) % p.window), held = (int)min((long long)slots, seen + 1);
     // the warp whose block of slots the new token falls into stores it, and reads it back with the others
     if (slot / BLOCK % (ranks * WARPS) == rank * WARPS + warp) {
-        if (lane < K / 8) reinterpret_cast<uint4*>(kb + slot * ld)[lane] = reinterpret_cast<const uint4*>(p.k + (long)unit * K)[lane];
-        if (lane < K / 8) reinterpret_cast<uint4*>(vb + slot * ld)[lane] = reinterpret_cast<const uint4*>(p.v + (long)unit * K)[lane];
+        if (lane < K / 8) {
+            reinterpret_cast<uint4*>(kb + slot * ld)[lane] = new_k;
+            reinterpret_cast<uint4*>(vb + slot * ld)[lane] = new_v;
+        }
         __syncwarp();
     }
     const float scale = p.scale * LOG2E;
     for (int h0 = 0; h0 < p.R; h0 += HEADS) {
-        const bf16* q = p.q + (b * p.H + grp * p.R + h0) * K;
-        uint32_t qf[NT][K / 8];
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int i = 0; i < K / 32; ++i) {
-                const uint4 w = slot_words(q + (long)(8 * n + r) * K + (c + 4 * i) * 8, h0 + 8 * n + r < p.R);
-                qf[n][4 * i] = w.x;
-                qf[n][4 * i + 1] = w.y;
-                qf[n][4 * i + 2] = w.z;
-                qf[n][4 * i + 3] = w.w;
-            }
+        if (h0 > 0) {
+            load_queries<K, NT>(qf, p, p.q + (b * p.H + grp * p.R + h0) * K, h0, r, c);
+        }
         float acc[NT][K / 16][4], m[NT][2], l[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -123,11 +144,12 @@ __global__ void __launch_bounds__(32 * step::Cta<NT>::WARPS, 2) window_step_kern
                     float top = fmaxf(y0, y1);
 #pragma unroll
                     for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-                    top = fmaxf(top, m[n][u]);                  // finite: slot s0 is held
-                    const float f = exp2_fast(m[n][u] - top);
+                    top = fmaxf(top, m[n][u]);
+                    const float ref = top == -INFINITY ? 0.f : top;
+                    const float f = exp2_fast(m[n][u] - ref);
                     m[n][u] = top;
-                    d[u] = exp2_fast(y0 - top);
-                    d[2 + u] = exp2_fast(y1 - top);
+                    d[u] = exp2_fast(y0 - ref);
+                    d[2 + u] = exp2_fast(y1 - ref);
                     l[n][u] = fmaf(l[n][u], f, d[u] + d[2 + u]);
 #pragma unroll
                     for (int i = 0; i < K / 16; ++i) {
@@ -171,8 +193,11 @@ __global__ void __launch_bounds__(32 * step::Cta<NT>::WARPS, 2) window_step_kern
                 }
             }
         __syncthreads();
+        // the cluster's CTAs have begun, and read what they were sent before
+        wait(cluster);
+        const int each = HEADS * K / ranks;
         for (int e = threadIdx.x; e < HEADS * K; e += 32 * WARPS) {
-            const int h = e / K, col = e % K;
+            const int h = e / K, col = e % K, to = e / each;
             float top = -INFINITY, sum = 0.f, o = 0.f;
 #pragma unroll
             for (int w = 0; w < WARPS; ++w) top = fmaxf(top, sM[w][h]);
@@ -183,25 +208,27 @@ __global__ void __launch_bounds__(32 * step::Cta<NT>::WARPS, 2) window_step_kern
                 sum = fmaf(f, sL[w][h], sum);
                 o = fmaf(f, sO[w][h][col], o);
             }
-            sO[0][h][col] = o;             // (its own element of the first warp's)
-            if (col == 0) {
-                sM[WARPS][h] = top;
-                sL[WARPS][h] = sum;
+            *cluster.map_shared_rank(&rO[rank * each + e - to * each], to) = o;
+            if (e == to * each || col == 0) {
+                *cluster.map_shared_rank(&rM[rank][h], to) = top;
+                *cluster.map_shared_rank(&rL[rank][h], to) = sum;
             }
         }
-        cluster.sync();
-        for (int e = rank * 32 * WARPS + threadIdx.x; e < HEADS * K; e += ranks * 32 * WARPS) {
-            const int h = e / K, col = e % K;
+        arrive(cluster);
+        wait(cluster);
+        for (int i = threadIdx.x; i < each; i += 32 * WARPS) {
+            const int e = rank * each + i, h = e / K, col = e % K;
             float top = -INFINITY, sum = 0.f, o = 0.f;
-            for (int x = 0; x < ranks; ++x) top = fmaxf(top, *cluster.map_shared_rank(&sM[WARPS][h], x));
+            for (int x = 0; x < ranks; ++x) top = fmaxf(top, rM[x][h]);
+#pragma unroll 4
             for (int x = 0; x < ranks; ++x) {
-                const float f = exp2_fast(*cluster.map_shared_rank(&sM[WARPS][h], x) - top);
-                sum = fmaf(f, *cluster.map_shared_rank(&sL[WARPS][h], x), sum);
-                o = fmaf(f, *cluster.map_shared_rank(&sO[0][h][col], x), o);
+                const float f = exp2_fast(rM[x][h] - top);
+                sum = fmaf(f, rL[x][h], sum);
+                o = fmaf(f, rO[x * each + i], o);
             }
             if (h0 + h < p.R) p.o[(b * p.H + grp * p.R + h0 + h) * K + col] = __float2bfloat16(o / sum);
         }
-        cluster.sync();                    // nobody's memory goes, or is written again, before it has been read
+        if (h0 + HEADS < p.R) arrive(cluster);
     }
     // every CTA of the cluster has read the count
     if (rank == 0 && threadIdx.x == 0) p.counts[unit] = seen + 1;
@@ -210,7 +237,7 @@ __global__ void __launch_bounds__(32 * step::Cta<NT>::WARPS, 2) window_step_kern
 // Clusters of 1 to 16 CTAs: as many as leave every warp two blocks of slots, up to two CTAs an SM.
 static int ranks_of(long units, int slots, int warps) {
     int n = 1;
-    while (n < 16 && slots > n * warps * step::BLOCK * 2 && units * n < 148) n *= 2;
+    while (n < step::MAX_RANKS && slots > n * warps * step::BLOCK * 2 && units * n < 148) n *= 2;
     return n;
 }
 template <int K, int NT>
