@@ -391,7 +391,7 @@ int llattn_gdn_grad_out(const void* q, const void* k, const float* dq, const flo
 /* ---- operators of the layers that stand between the log-linear ones in a hybrid stack.  (No counterparts in the reference.)
  *
  * Gated linear recurrence of independent channels: o_t = h_t = exp(g_t) h_{t-1} + x_t.  x, o, dx (B,T,D) bf16 or fp32; g, dg (B,T,D) fp32 (g_is_f32)
- * or, with bf16 x, bf16; g is a log decay, <= 0 (-inf starts a channel anew; above 0 the products over 128 tokens have to stay finite).  States are
+ * or, with bf16 x, bf16; g is a log decay, <= 0 (-inf starts a channel anew; above 0 the products over 512 tokens have to stay finite).  States are
  * (B,D) fp32: h0 may be NULL (zeros), h_last and the gradients dh_last, dh0 may be NULL.  `states` (llattn_recurrence_states_bytes) receives the states
  * that the backward starts from; NULL in a forward without one.  Any T >= 1 and D >= 1. */
 size_t llattn_recurrence_states_bytes(int B, int T, int D);

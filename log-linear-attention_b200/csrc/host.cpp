@@ -12,6 +12,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <dlfcn.h>
 #include <torch/extension.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 
 #include <ATen/cuda/EmptyTensor.h>
 #include <cmath>
@@ -80,6 +81,14 @@ inline variable_list saved(AutogradContext* ctx) {
     for (Tensor& t : s)
         if (t.defined() && !(t.is_contiguous() && aligned(t))) t = contiguous(t);
     return s;
+}
+// Gradients that come out of a kernel have no graph: where one is asked for (create_graph), differentiating them again raises, in the place of leaving their part out.
+inline variable_list once(variable_list r, const char* what) {
+    if (!at::GradMode::is_enabled()) return r;
+    for (Tensor& t : r)
+        if (t.defined()) t = t.detach().requires_grad_(true);
+    const int n = r.size();
+    return (*std::make_shared<torch::autograd::DelayedError>(std::string(what) + " is differentiable once", n))(std::move(r));
 }
 using Maybe = std::optional<Tensor>;     // a tensor that may be absent: autograd functions take no undefined tensors
 inline Tensor of(const Maybe& t) { return t.has_value() ? *t : Tensor(); }
@@ -852,7 +861,7 @@ struct Recurrence : torch::autograd::Function<Recurrence> {
         const Tensor d_o = d[0].defined() ? contiguous(d[0].to(x.scalar_type())) : at::zeros_like(x);
         const Tensor dlast = d.size() > 1 && d[1].defined() ? contiguous(d[1].to(at::kFloat)) : Tensor();
         const ScannedGrads r = recurrence_bwd(x, g, s[2], d_o, dlast, ctx->saved_data["h0"].toBool(), on.stream);
-        return {r.dx, r.dg, r.dh0, Tensor()};
+        return once({r.dx, r.dg, r.dh0, Tensor()}, "gated_recurrence");
     }
 };
 // (o, last state or None), or None
@@ -951,7 +960,7 @@ struct WindowAttention : torch::autograd::Function<WindowAttention> {
         On on(s[0]);
         const WindowGrads r = window_bwd(s[0], s[1], s[2], s[3], s[4], contiguous(d[0].to(at::kBFloat16)), ctx->saved_data["window"].toInt(),
                                          ctx->saved_data["sinks"].toInt(), ctx->saved_data["scale"].toDouble(), ctx->saved_data["status"].toBool(), on.stream);
-        return {r.dq, r.dk, r.dv, Tensor(), Tensor(), Tensor(), Tensor()};
+        return once({r.dq, r.dk, r.dv, Tensor(), Tensor(), Tensor(), Tensor()}, "sliding_window_attention");
     }
 };
 py::object sliding_window_attention(const Tensor& q, const Tensor& k, const Tensor& v, int64_t window, int64_t sinks, double scale, bool status) {
@@ -1012,7 +1021,7 @@ py::object sliding_window_step(const Tensor& q, const Tensor& k, const Tensor& v
     const int64_t B = q.size(0), H = q.size(1), K = q.size(2), G = k.size(1);
     if (k.size(0) != B || k.size(2) != K || (K != 64 && K != 128) || H % G != 0 || window < 1 || sinks < 0 || window > WINDOW_MAX || sinks > WINDOW_MAX ||
         !((float)scale > 0.f) || !std::isfinite((float)scale) || kc.sizes() != at::IntArrayRef({B, sinks + window, G, K}) || vc.sizes() != kc.sizes() ||
-        counts.sizes() != at::IntArrayRef({B, G}) || !kc.is_contiguous() || !vc.is_contiguous() || !counts.is_contiguous() || !aligned(kc) || !aligned(vc) ||
+        counts.sizes() != at::IntArrayRef({B, G}) || kc.data_ptr() == vc.data_ptr() || !kc.is_contiguous() || !vc.is_contiguous() || !counts.is_contiguous() || !aligned(kc) || !aligned(vc) ||
         !aligned(counts))
         return py::none();
     On on(q);
@@ -1080,7 +1089,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
         On on(s[0]);
         const NormGrads r = norm_bwd(s[0], s[1], s[2], contiguous(d[0].to(s[0].scalar_type())), (at::ScalarType)ctx->saved_data["param"].toInt(),
                                      ctx->saved_data["dw"].toBool(), ctx->saved_data["db"].toBool(), on.stream);
-        return {r.dx, r.dw, r.db, Tensor()};
+        return once({r.dx, r.dw, r.db, Tensor()}, "layer_norm");
     }
 };
 py::object layer_norm(const Tensor& x, const Maybe& w, const Maybe& b, double eps) {

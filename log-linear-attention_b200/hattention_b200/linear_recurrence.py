@@ -29,7 +29,7 @@ def gated_recurrence(x: torch.Tensor, g: torch.Tensor, initial_state: Optional[t
 
     x is bf16 or fp32 and o has its type; g has x's type or is fp32; states are (B,D) fp32, an absent one is zeros.  All sums are fp32.
     g <= 0, as log decays are; -inf starts a channel anew at that token, so that packed sequences stay apart.  (Above 0 the products of
-    exp(g) over 128 tokens have to stay finite.)  T and D are any sizes; even D moves two channels a load."""
+    exp(g) over 512 tokens have to stay finite.)  T and D are any sizes; even D moves two channels a load."""
     r = _lib.host().gated_recurrence(x, g, initial_state, output_final_state)
     if r is not None:
         return r

@@ -98,6 +98,8 @@ def sliding_window_step(state: WindowState, q: torch.Tensor, k: torch.Tensor, v:
             raise ValueError(f"the state holds bfloat16 {(B, state.sinks + state.window, G, K)} on q's device; got {c.dtype} {tuple(c.shape)}")
         if not c.is_contiguous() or c.data_ptr() % 16 != 0:
             raise ValueError("the state is advanced in place: it has to be contiguous and to start at 16-byte boundaries")
+    if q.numel() > 0 and state.k.data_ptr() == state.v.data_ptr():
+        raise ValueError("the state's k and v are one tensor")
     if state.lengths.shape != (B, G) or state.lengths.dtype != torch.int64 or state.lengths.device != q.device or not state.lengths.is_contiguous():
         raise ValueError("the state's lengths are a contiguous int64 tensor (B,G) on q's device")
     if q.numel() > 0:
