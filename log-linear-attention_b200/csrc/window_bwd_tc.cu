@@ -9,7 +9,8 @@
 // half of a step run under the other half's exponentials.  (Summing dQ beside dK and dV would save two of the seven products a pair of tiles, for
 // atomics on 64 KB of fp32 a pair.)
 // T = 16384, 32 query heads on 8, K = 128, window 2048: 1.61 ms, 0.80 PFLOP/s counting five products (1.12 of the seven made).  The exponentials' side of a step is longer
-// than its products: about 2160 cycles for 1536 of dQ, 2850 for 2048 of dK and dV.
+// than its products: about 2100 cycles for 1536 of dQ, 2750 for 2048 of dK and dV; call after call the clocks give way to the power limit.  (Q and dO as operands in tensor memory, which
+// halves what their products read from shared memory: 1.4 % less there, 2 to 3 % more for short sequences.)
 #include "window.cuh"
 
 namespace llattn {
@@ -53,16 +54,19 @@ struct Ring {
 __device__ __forceinline__ void regs_issue() { asm volatile("setmaxnreg.dec.sync.aligned.u32 72;\n"); }
 __device__ __forceinline__ void regs_rows() { asm volatile("setmaxnreg.inc.sync.aligned.u32 216;\n"); }
 
-// exp2(c s - shift) of 64 scores; shift(u) gives the pair of values for keys u, u + 1.  (A share of them on the FMA pipes, as in the forward, changes nothing here: 1.63 to
-// 1.65 ms for none to a half of them at T = 16384.)
+// exp2(c s - shift) of 64 scores; shift(u) gives the pair of values for keys u, u + 1.  Every fourth pair goes to the FMA pipes, as in the forward (2 x 1999 tokens, 16 heads of 64, window
+// 512, us: none 73.1, every fourth 71.1; 8 x 2000 tokens, 8 heads on 2 of 64, window 300: 118.4, 113.8; T = 8192, 32 heads on 8 of 128, window 2048: none 761, every fourth 755,
+// third 759, second 767).  Where long calls run on end power decides, and it makes no difference.
+constexpr int POLY = 4;
 template <typename ShiftT>
 __device__ __forceinline__ void exponentials(float (&e)[64], float c, ShiftT minus_shift) {
     const F2 c2 = pair(c, c);
 #pragma unroll
     for (int u = 0; u < 64; u += 2) {
-        const float2 v = both(fma2(pair(e[u], e[u + 1]), c2, minus_shift(u)));
-        e[u] = exp2_fast(v.x);
-        e[u + 1] = exp2_fast(v.y);
+        const F2 y = fma2(pair(e[u], e[u + 1]), c2, minus_shift(u));
+        const float2 x = both(y), v = u / 2 % POLY == POLY - 1 ? exp2_poly(y) : make_float2(exp2_fast(x.x), exp2_fast(x.y));
+        e[u] = v.x;
+        e[u + 1] = v.y;
     }
 }
 // 64 values of a row as bf16 into the first half of the columns they came from
