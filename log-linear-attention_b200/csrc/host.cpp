@@ -90,6 +90,10 @@ inline variable_list once(variable_list r, const char* what) {
     const int n = r.size();
     return (*std::make_shared<torch::autograd::DelayedError>(std::string(what) + " is differentiable once", n))(std::move(r));
 }
+// A kernel has written to t: a graph that kept t for its backward pass has to notice.
+inline void written(const Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
 using Maybe = std::optional<Tensor>;     // a tensor that may be absent: autograd functions take no undefined tensors
 inline Tensor of(const Maybe& t) { return t.has_value() ? *t : Tensor(); }
 inline Tensor empty(at::IntArrayRef size, at::ScalarType dt, const Tensor& like) {
@@ -894,12 +898,14 @@ py::object recurrence_backward(const Tensor& x, const Tensor& g, const Tensor& s
 // o (B,D); the state is advanced in place
 py::object gated_recurrence_step(const Tensor& h, const Tensor& x, const Tensor& g) {
     if (!row_types(x, g) || x.dim() != 2 || g.sizes() != x.sizes() || x.numel() == 0 || !is(h, at::kFloat) || h.sizes() != x.sizes() || !h.is_contiguous() ||
-        !aligned(h) || !native_set({h, x, g}) || wants_grad({h, x, g}))
+        !aligned(h) || !native_set({h, x, g}))
         return py::none();
+    at::NoGradGuard no_grad;                     // (a state goes on without a graph)
     On on(x);
     const Tensor x_ = contiguous(x), g_ = contiguous(g), o = contiguous_like(x_);
     check(lib.llattn_recurrence_step(fptr(h), x_.data_ptr(), f32(x_), g_.data_ptr(), f32(g_), o.data_ptr(), x.size(0), x.size(1), on.stream),
           "llattn_recurrence_step");
+    written(h);
     return py::cast(o);
 }
 
@@ -1016,7 +1022,7 @@ py::object sliding_window_prefill(const Tensor& q, const Tensor& k, const Tensor
 py::object sliding_window_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& kc, const Tensor& vc, const Tensor& counts, int64_t window,
                                int64_t sinks, double scale) {
     if (!bf16(q) || !bf16(k) || !bf16(v) || !bf16(kc) || !bf16(vc) || !is(counts, at::kLong) || q.dim() != 3 || k.dim() != 3 || v.sizes() != k.sizes() ||
-        q.numel() == 0 || k.numel() == 0 || !native_set({q, k, v, kc, vc, counts}) || wants_grad({q, k, v, kc, vc}))
+        q.numel() == 0 || k.numel() == 0 || !native_set({q, k, v, kc, vc, counts}))
         return py::none();
     const int64_t B = q.size(0), H = q.size(1), K = q.size(2), G = k.size(1);
     if (k.size(0) != B || k.size(2) != K || (K != 64 && K != 128) || H % G != 0 || window < 1 || sinks < 0 || window > WINDOW_MAX || sinks > WINDOW_MAX ||
@@ -1024,11 +1030,13 @@ py::object sliding_window_step(const Tensor& q, const Tensor& k, const Tensor& v
         counts.sizes() != at::IntArrayRef({B, G}) || kc.data_ptr() == vc.data_ptr() || !kc.is_contiguous() || !vc.is_contiguous() || !counts.is_contiguous() || !aligned(kc) || !aligned(vc) ||
         !aligned(counts))
         return py::none();
+    at::NoGradGuard no_grad;
     On on(q);
     const Tensor q_ = contiguous(q), k_ = contiguous(k), v_ = contiguous(v), o = contiguous_like(q_);
     check(lib.llattn_window_step(q_.data_ptr(), k_.data_ptr(), v_.data_ptr(), kc.data_ptr(), vc.data_ptr(), reinterpret_cast<long long*>(counts.data_ptr()),
                                  o.data_ptr(), B, H, G, K, (int)window, (int)sinks, (float)scale, on.stream),
           "llattn_window_step");
+    for (const Tensor& t : {kc, vc, counts}) written(t);
     return py::cast(o);
 }
 

@@ -40,7 +40,6 @@ def gated_recurrence(x: torch.Tensor, g: torch.Tensor, initial_state: Optional[t
     return x + g.to(x.dtype), h.clone() if output_final_state else None
 
 
-@torch.no_grad()
 def gated_recurrence_step(state: torch.Tensor, x: torch.Tensor, g: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """One token: x, g (B,D) -> (o (B,D), state).  `state` (B,D) fp32, contiguous, is advanced in place.  One launch that reads no host
     values, so it can be captured into a CUDA graph and replayed."""

@@ -65,7 +65,6 @@ def sliding_window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, 
     return q + 0 * (k.sum() + v.sum())
 
 
-@torch.no_grad()
 def sliding_window_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int, sinks: int = 0, scale: Optional[float] = None,
                            lengths: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, WindowState]:
     """Outputs for prompts and the state to continue from.  With `lengths` (B,) int64 on the device, sequence b has lengths[b] tokens (0 to T)
@@ -79,10 +78,9 @@ def sliding_window_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, wi
         raise TypeError("lengths is an int64 tensor (B,) on q's device")
     if q.numel() > 0:
         raise NotImplementedError("sliding_window_prefill takes at most 2^24 tokens of at most 65535 sequences")
-    return q.clone(), WindowState.empty(q.shape[0], k.shape[2], q.shape[3], window, sinks, q.device)
+    return q.detach().clone(), WindowState.empty(q.shape[0], k.shape[2], q.shape[3], window, sinks, q.device)
 
 
-@torch.no_grad()
 def sliding_window_step(state: WindowState, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                         scale: Optional[float] = None) -> Tuple[torch.Tensor, WindowState]:
     """One token of every sequence: q (B,H,K), k, v (B,G,K) -> (o (B,H,K), state).  The token's k and v take the place of the one that leaves

@@ -208,3 +208,28 @@ def test_cache_of_one_tensor_is_refused():
     q = torch.zeros(1, 2, 64, dtype=BF, device="cuda")
     with pytest.raises(ValueError, match="one tensor"):
         sliding_window_step(s._replace(v=s.k), q, q, q)
+
+
+def test_steps_and_graphs():
+    """A step has no graph, whatever its operands; a graph that kept a state notices that a step has advanced it; inference tensors are advanced too."""
+    from hattention_b200 import WindowState, gated_recurrence, gated_recurrence_step, sliding_window_step
+    x = torch.randn(2, 30, 64, device="cuda", requires_grad=True)
+    _, h = gated_recurrence(x, -x.detach().abs(), output_final_state=True)
+    loss = h.square().sum()                              # (keeps h)
+    want = (-x[:, 0].detach().abs()).exp() * h.detach() + x[:, 0].detach()
+    o, h2 = gated_recurrence_step(h, x[:, 0], -x[:, 0].abs())
+    assert h2 is h and not o.requires_grad and torch.allclose(h.detach(), want, rtol=1e-5, atol=1e-6)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    q = torch.randn(1, 2, 64, device="cuda").to(BF).requires_grad_(True)
+    s = WindowState.empty(1, 2, 64, 8)
+    kept = s.k.float().requires_grad_(False)
+    o, s = sliding_window_step(s, q, q, q)
+    assert not o.requires_grad and torch.equal(o, q) and (kept == 0).all() and s.k._version == 1 and s.lengths._version == 1
+    with torch.inference_mode():
+        s = WindowState.empty(1, 2, 64, 8)
+        h = torch.zeros(2, 64, device="cuda")
+        for _ in range(2):
+            o, s = sliding_window_step(s, q, q, q)
+            gated_recurrence_step(h, x[:, 0], -x[:, 0].abs())
+        assert (s.lengths == 2).all()
