@@ -1,15 +1,15 @@
 // Sliding-window attention forward on the 5th-generation tensor cores.
 //
-// A CTA takes two tiles of 128 queries of a head, A and B, and walks the tiles of keys that either sees.  For each of them and each tile of queries
+// A CTA takes one or two tiles of 128 queries of a head and walks the tiles of keys that they see.  For each of them and each tile of queries
 //     S = Q K^T            128 x 128 x K     into tensor memory
 //     P = exp2(c S - m)    a warpgroup, a thread a row: running maximum m and sum, P as bf16 in the place of S
 //     O += P V             128 x K x 128     P from tensor memory
-// with the products of one tile of queries under the softmax of the other.  The maximum that the exponents refer to moves only when a row's has grown by more than
-// 2^8: O, in tensor memory, is rescaled then alone, and P never exceeds 2^8.
-//     warps 0..3, 4..7   softmax, rescaling and output of A, of B
-//     warp 8             issues the products
-//     warp 9             brings Q, then K and V tiles through a ring
-// It is bound by the chain S, softmax, P V of a tile of queries, of which two are in flight: about 3500 cycles a pair of tiles for 2048 of products (T = 16384, 32 query heads
+// with the products of one tile of queries under the softmax of another: of the same CTA, or of the SM's other one.  The maximum that the exponents refer to moves only when
+// a row's has grown by more than 2^8: O, in tensor memory, is rescaled then alone, and P never exceeds 2^8.
+//     four warps a tile  softmax, rescaling and output
+//     the next one       issues the products
+//     the one after it   brings Q, then K and V tiles through a ring
+// It is bound by the chain S, softmax, P V of a tile of queries, of which an SM has two in flight: about 3500 cycles a pair of tiles for 2048 of products (T = 16384, 32 query heads
 // on 8, K = 128, window 2048: 563 us, 0.92 PFLOP/s of products that are not masked).  Two threads a row in the softmax were slower, 618 us for 572: the rows' maxima then
 // go through shared memory.
 // A wait that gives up sets the CTA's abort flag, after which every other wait ends at once, and the workspace's status word.
@@ -21,40 +21,52 @@ namespace llattn {
 namespace win {
 
 namespace fwd {
-constexpr int NST = 4, NTHREADS = 384, MMA_WARP = 8, TMA_WARP = 9;
-constexpr int TM_S = 0, TM_O = 256;            // S of A and B, 128 columns each; O of A and B, 128 columns apart
 constexpr float GROWTH = 8.f;
 
-template <int K>
-struct Smem {
+// X tiles of queries a CTA
+template <int K, int X>
+struct Cta {
+    static constexpr int THREADS = 128 * X + 128, MMA_WARP = 4 * X, TMA_WARP = 4 * X + 1, PER_SM = X == 2 ? 1 : 2;
+    static constexpr int TM_S = 0, TM_O = 128 * X, TM = 256 * X;              // S, then O, 128 columns a tile
+    static constexpr int NST = K == 128 && X == 1 ? 2 : 4;                     // tiles in the ring (two CTAs an SM leave room for two of K = 128)
     static constexpr uint32_t TILE_BYTES = TILE * K * 2;
-    static constexpr uint32_t q_off = 0, st_off = 2 * TILE_BYTES, bar_off = st_off + NST * TILE_BYTES, total = bar_off + 256 + 1024;
+    static constexpr uint32_t q_off = 0, st_off = X * TILE_BYTES, bar_off = st_off + NST * TILE_BYTES, total = bar_off + 256 + 1024;
+    // registers: 384 threads are launched with 168 each, 256 (two CTAs an SM) with 128; 4 warps give theirs to the softmax
+    static __device__ __forceinline__ void regs_issue() {
+        if constexpr (X == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;\n");
+        else asm volatile("setmaxnreg.dec.sync.aligned.u32 56;\n");
+    }
+    static __device__ __forceinline__ void regs_rows() {
+        if constexpr (X == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;\n");
+        else asm volatile("setmaxnreg.inc.sync.aligned.u32 200;\n");
+    }
 };
-// 128 x (168 - 72) registers go to the 256 threads of the softmax
-__device__ __forceinline__ void regs_issue() { asm volatile("setmaxnreg.dec.sync.aligned.u32 72;\n"); }
-__device__ __forceinline__ void regs_rows() { asm volatile("setmaxnreg.inc.sync.aligned.u32 216;\n"); }
 
 // Of the pairs of exponentials of a tile every POLY-th goes to the FMA pipes, which are idle while the special-function units work (T = 16384, 32 heads, window 2048, us: none
 // 590, every eighth 582, fourth 572, third 576, second 604).
 constexpr int POLY = 4;
 
-// The tiles of keys that A or B sees: A's list up to the end of the longer one.  (B's band starts no earlier, and where more of the sinks' tiles are in front of it than in
+// The tiles of keys that A, or one of A and B, sees: A's list up to the end of the longer one.  (B's band starts no earlier, and where more of the sinks' tiles are in front of it than in
 // front of A's, those are tiles of A's band.)
-struct Both {
+template <int X>
+struct Seen {
     Span a, b;
     int count;
-    __device__ Both(const Params& p, int q0) : a(q0, p.T, p.window, p.sinks), b(q0 + TILE, p.T, p.window, p.sinks) { count = a.count() + (b.hi > a.hi ? b.hi - a.hi : 0); }
+    __device__ Seen(const Params& p, int q0) : a(q0, p.T, p.window, p.sinks), b(X == 2 ? q0 + TILE : q0, p.T, p.window, p.sinks) {
+        count = a.count() + (b.hi > a.hi ? b.hi - a.hi : 0);
+    }
     __device__ int tile(int n) const { return a.tile(n); }
     __device__ bool in(int x, int j) const { return x == 0 ? a.has(j) : b.has(j); }
 };
 }  // namespace fwd
 
-template <int K>
-__global__ void __launch_bounds__(fwd::NTHREADS, 1) window_fwd_tc_kernel(const __grid_constant__ Params p) {
+template <int K, int X>
+__global__ void __launch_bounds__(fwd::Cta<K, X>::THREADS, fwd::Cta<K, X>::PER_SM) window_fwd_tc_kernel(const __grid_constant__ Params p) {
     chain_wait();
     clear_status(p);
     using namespace fwd;
-    using SM = Smem<K>;
+    using SM = Cta<K, X>;
+    constexpr int NST = SM::NST, MMA_WARP = SM::MMA_WARP, TMA_WARP = SM::TMA_WARP, TM_S = SM::TM_S, TM_O = SM::TM_O;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = umma::align_1024(smem_raw);
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + SM::bar_off);
@@ -66,8 +78,8 @@ __global__ void __launch_bounds__(fwd::NTHREADS, 1) window_fwd_tc_kernel(const _
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     // heads and sequences first, later queries first: those see more tiles, and the last CTAs of a launch are its short ones  (sequences outermost: 41.2 us for 37.4, 4 x 1000 tokens)
     const unsigned units = p.B * p.H, unit = blockIdx.x % units;
-    const int h = unit % p.H, q0 = (gridDim.x / units - 1 - blockIdx.x / units) * 2 * TILE, b = unit / p.H, grp = h / (p.H / p.G);
-    const Both w(p, q0);
+    const int h = unit % p.H, q0 = (gridDim.x / units - 1 - blockIdx.x / units) * X * TILE, b = unit / p.H, grp = h / (p.H / p.G);
+    const Seen<X> w(p, q0);
     // position n of the ring's sequence: K, V of the first tile, K, V of the second, ...
     const auto bring = [&](int n) {
         tma::expect_tx(full + n % NST, SM::TILE_BYTES);
@@ -78,7 +90,7 @@ __global__ void __launch_bounds__(fwd::NTHREADS, 1) window_fwd_tc_kernel(const _
             umma::mbar_init(full + i, 1);
             umma::mbar_init(empty + i, 1);
         }
-        for (int x = 0; x < 2; ++x) {
+        for (int x = 0; x < X; ++x) {
             umma::mbar_init(barQ + x, 1);
             umma::mbar_init(barS + x, 1);
             umma::mbar_init(barP + 2 * x, 4);
@@ -91,19 +103,19 @@ __global__ void __launch_bounds__(fwd::NTHREADS, 1) window_fwd_tc_kernel(const _
         tma::expect_tx(barQ, SM::TILE_BYTES);
         load_tile<K>(smem + SM::q_off, &p.tq, h, q0, b, barQ);
         bring(0);
-        if (q0 + TILE < p.T) {
+        if (X == 2 && q0 + TILE < p.T) {
             tma::expect_tx(barQ + 1, SM::TILE_BYTES);
             load_tile<K>(smem + SM::q_off + SM::TILE_BYTES, &p.tq, h, q0 + TILE, b, barQ + 1);
         }
     }
-    if (warp == MMA_WARP) umma::tmem_alloc(tmem_slot, 512);
+    if (warp == MMA_WARP) umma::tmem_alloc(tmem_slot, SM::TM);
     umma::fence_before_sync();
     __syncthreads();
     umma::fence_after_sync();
     const uint32_t tmem = *tmem_slot;
 
-    if (warp >= 8) {
-        regs_issue();
+    if (warp >= MMA_WARP) {
+        SM::regs_issue();
         if (warp == TMA_WARP && lane == 0) {
             int n = 1;
             for (; n < 2 * w.count; ++n) {
@@ -113,7 +125,7 @@ __global__ void __launch_bounds__(fwd::NTHREADS, 1) window_fwd_tc_kernel(const _
             // nobody may be left to wait for the last copies after a wait that gave up: they end before the CTA does
             if (*abort_flag) {
                 umma::mbar_wait(barQ, 0);
-                if (q0 + TILE < p.T) umma::mbar_wait(barQ + 1, 0);
+                if (X == 2 && q0 + TILE < p.T) umma::mbar_wait(barQ + 1, 0);
                 for (int i = n > NST ? n - NST : 0; i < n; ++i) umma::mbar_wait(full + i % NST, (i / NST) & 1);
             }
         } else if (warp == MMA_WARP) {
@@ -126,7 +138,7 @@ __global__ void __launch_bounds__(fwd::NTHREADS, 1) window_fwd_tc_kernel(const _
             for (int i = 0; i <= w.count && ok; ++i) {
                 bool haveK = false, haveV = false;
                 const int nk = 2 * i, nv = 2 * i - 1;   // positions of K of this step and V of the one before in the ring's sequence
-                for (int x = 0; x < 2 && ok; ++x) {
+                for (int x = 0; x < X && ok; ++x) {
                     if (before[x]) {
                         if (!haveV) ok = umma::mbar_wait_warp(full + nv % NST, (nv / NST) & 1, abort_flag);
                         haveV = true;
@@ -159,7 +171,7 @@ __global__ void __launch_bounds__(fwd::NTHREADS, 1) window_fwd_tc_kernel(const _
             }
         }
     } else {
-        regs_rows();
+        SM::regs_rows();
         const int x = warp >> 2, row = (warp & 3) * 32 + lane, t0 = q0 + x * TILE, t = t0 + row;
         const uint32_t tS = umma::tmem_addr(tmem, warp, TM_S + 128 * x), tO = umma::tmem_addr(tmem, warp, TM_O + 128 * x);
         const float c = p.scale * LOG2E;
@@ -295,21 +307,28 @@ __global__ void __launch_bounds__(fwd::NTHREADS, 1) window_fwd_tc_kernel(const _
             umma::mbar_wait(barQ, 1);
             if (lane == 0) atomicExch(p.err, 1);
         }
-        umma::tmem_dealloc(tmem, 512);
+        umma::tmem_dealloc(tmem, SM::TM);
     }
 }
 
-template <int K>
+template <int K, int X>
 static cudaError_t launch(const Params& p, cudaStream_t st) {
-    const auto kern = window_fwd_tc_kernel<K>;
-    cudaError_t e = allow_smem(kern, fwd::Smem<K>::total);
+    using C = fwd::Cta<K, X>;
+    const auto kern = window_fwd_tc_kernel<K, X>;
+    cudaError_t e = allow_smem(kern, C::total);
     if (e != cudaSuccess) return e;
-    const unsigned grid = (unsigned)(p.T + 2 * TILE - 1) / (2 * TILE) * p.H * p.B;
-    e = launch_chained(kern, grid, fwd::NTHREADS, fwd::Smem<K>::total, st, p);
+    const unsigned grid = (unsigned)(p.T + X * TILE - 1) / (X * TILE) * p.H * p.B;
+    e = launch_chained(kern, grid, C::THREADS, C::total, st, p);
     if (e == cudaSuccess) LLATTN_LAUNCHED();
     return e;
 }
-cudaError_t forward_tc(const Params& p, int K, cudaStream_t st) { return K == 64 ? launch<64>(p, st) : launch<128>(p, st); }
+// One tile a CTA, two CTAs an SM, whose starts and ends run under each other's steps; or, where K = 128 and a query sees thousands of keys, two tiles that share what comes from memory (us,
+// one tile / two: K = 128, 32 heads on 8, window 512, 8192 tokens 119 / 128; window 1024 164 / 169; window 2048, 4096 tokens 110 / 109, 8192 tokens 249 / 239; 8192 tokens, all that are
+// before 482 / 439; K = 64, 16 heads, 2 x 1999 tokens, window 512 25.4 / 31.2; 8 heads on 2, 32768 tokens, window 4096 417 / 440; 32 heads on 8, 8192 tokens, all before 469 / 455).
+cudaError_t forward_tc(const Params& p, int K, cudaStream_t st) {
+    if (K == 64) return launch<64, 1>(p, st);
+    return p.T >= 2048 && p.window >= 2048 ? launch<128, 2>(p, st) : launch<128, 1>(p, st);
+}
 
 }  // namespace win
 }  // namespace llattn

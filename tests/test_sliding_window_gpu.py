@@ -75,6 +75,12 @@ def test_forward_and_gradients(B, T, H, G, K, window, sinks):
     run(B, T, H, G, K, window, sinks)
 
 
+@pytest.mark.parametrize("B,T,H,G,window,sinks", [(1, 2048, 2, 1, 2048, 0), (2, 2305, 4, 2, 2048, 130), (1, 2500, 2, 2, 2100, 3), (1, 2177, 3, 1, 5000, 9), (1, 4200, 1, 1, 2050, 600)])
+def test_long_windows(B, T, H, G, window, sinks):
+    """Windows of thousands: two tiles of queries a CTA where heads are 128 wide."""
+    run(B, T, H, G, 128, window, sinks)
+
+
 @pytest.mark.parametrize("scale", [0.01, 0.3])
 def test_scale(scale):
     run(1, 200, 2, 1, 64, 90, 2, scale)
@@ -303,15 +309,14 @@ def test_empty_operands():
 
 
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
-@pytest.mark.parametrize("K", [64, 128])
-def test_non_finite_keys(K, bad):
+@pytest.mark.parametrize("K,T,window", [(64, 500, 200), (128, 500, 200), (128, 2200, 2048)])
+def test_non_finite_keys(K, T, window, bad):
     """A key that is not finite spoils the rows that see it, whatever its place in a tile, and none of the others."""
     from hattention_b200 import sliding_window_attention
-    T, window = 500, 200
     q, k, v = make(1, T, 2, 1, K)[:3]
     q[..., 0] = 1.0                                    # (a product with inf is +-inf, never NaN: of one sign in every row)
     clean = sliding_window_attention(q, k, v, window)
-    for s in list(range(128, 144)) + [0, 255, 256, 499]:
+    for s in list(range(128, 144)) + [0, 255, 256, T - 1]:
         spoiled = k.clone()
         spoiled[0, s, 0, 0] = bad
         o = sliding_window_attention(q, spoiled, v, window)
