@@ -5,7 +5,7 @@
 //     S = Q K^T, dP = dO V^T,   dS = exp2(c S - lse) (dP - delta) as bf16 in the place of S,   dQ += dS K.
 // dK, dV: a CTA takes a tile of 128 tokens of k and v and walks the tiles of queries that see it, of all heads that share it,
 //     S^T = K Q^T, dP^T = V dO^T,   P^T = exp2(c S^T - lse), dV += P^T dO,   dS^T = P^T (dP^T - delta), dK += dS^T Q.
-// In both, eight warps do the exponentials (two threads a row, 64 columns each), one issues products, one brings tiles through a ring; the products of one
+// In both, four or eight warps do the exponentials (64 columns a thread), one issues products, one brings tiles through two rings; the products of one
 // half of a step run under the other half's exponentials.  (Summing dQ beside dK and dV would save two of the seven products a pair of tiles, for
 // atomics on 64 KB of fp32 a pair.)
 // T = 16384, 32 query heads on 8, K = 128, window 2048: 1.61 ms, 0.80 PFLOP/s counting five products (1.12 of the seven made).  The exponentials' side of a step is longer
@@ -17,18 +17,33 @@ namespace llattn {
 namespace win {
 
 namespace bwd {
-constexpr int NTHREADS = 384, MMA_WARP = 8, TMA_WARP = 9;
 // Two rings of tiles: those that two products of a step need, far apart (NA of them), and those of one (NB).  With K = 128 five tiles fit beside the two that stay, three
-// and two: the next but one of either kind is on its way while a step runs.  (One ring of four for both kinds: the dQ kernel waited for its keys, 527 us at T = 8192,
+// and two: the next but one of either kind is on its way while a step runs; with K = 64 two and two, in each of two CTAs.  (One ring of four for both kinds: the dQ kernel waited for its keys, 527 us at T = 8192,
 // 32 heads, window 2048.)
+//
+// A step is K columns of scores (keys in the dQ kernel, queries in the other) by 128 rows, 64 columns a thread: with K = 128 a whole tile, two threads a row, a CTA an SM; with
+// K = 64 half a tile, a thread a row, and two CTAs an SM, whose waits and products run under each other's exponentials (whole tiles in one CTA there: 71 us for 62, 2 x 1999 tokens, 16 heads,
+// window 512; 114 for 101, 8 x 2000 tokens, 8 heads on 2, window 300).  (With K = 128 the sums dV and dK alone fill half of tensor memory.)
 template <int K>
-struct Smem {
-    static constexpr int NA = K == 64 ? 4 : 3, NB = K == 64 ? 4 : 2;
+struct Cta {
+    static constexpr int HALVES = K / 64, STEPS = TILE / K;                          // threads a row; steps a tile
+    static constexpr int WARPS = 4 * HALVES, MMA_WARP = WARPS, TMA_WARP = WARPS + 1, THREADS = 32 * WARPS + 128, PER_SM = K == 64 ? 2 : 1;
+    static constexpr int TM = 4 * K;                                                 // columns of tensor memory: four blocks of K
+    static constexpr int NA = K == 64 ? 2 : 3, NB = 2;
     static constexpr uint32_t TILE_BYTES = TILE * K * 2;
     static constexpr uint32_t stay_off = 0, a_off = 2 * TILE_BYTES, b_off = a_off + NA * TILE_BYTES;
     static constexpr uint32_t stat_off = b_off + NB * TILE_BYTES;                    // float [NA + NB][128]: lse beside A tiles of queries, delta beside B tiles
     static constexpr uint32_t bar_off = stat_off + (NA + NB) * TILE * 4, total = bar_off + 256;
-    static_assert(total <= 227 * 1024, "one CTA");
+    static_assert((total + 1024) * PER_SM <= 228 * 1024, "CTAs an SM");
+    // registers: 384 threads are launched with 168 each, 256 (two CTAs an SM) with 128; 4 warps give theirs to the exponentials
+    static __device__ __forceinline__ void regs_issue() {
+        if constexpr (K == 128) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;\n");
+        else asm volatile("setmaxnreg.dec.sync.aligned.u32 56;\n");
+    }
+    static __device__ __forceinline__ void regs_rows() {
+        if constexpr (K == 128) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;\n");
+        else asm volatile("setmaxnreg.inc.sync.aligned.u32 200;\n");
+    }
 };
 // The steps of a ring of N tiles: slot and phase of step n.
 template <int N>
@@ -50,9 +65,6 @@ struct Ring {
         for (int i = issued > N ? issued - N : 0; i < issued; ++i) umma::mbar_wait(filled(i), phase(i));
     }
 };
-// 128 x (168 - 72) registers go to the 256 threads of the exponentials
-__device__ __forceinline__ void regs_issue() { asm volatile("setmaxnreg.dec.sync.aligned.u32 72;\n"); }
-__device__ __forceinline__ void regs_rows() { asm volatile("setmaxnreg.inc.sync.aligned.u32 216;\n"); }
 
 // exp2(c s - shift) of 64 scores; shift(u) gives the pair of values for keys u, u + 1.  Every fourth pair goes to the FMA pipes, as in the forward (2 x 1999 tokens, 16 heads of 64, window
 // 512, us: none 73.1, every fourth 71.1; 8 x 2000 tokens, 8 heads on 2 of 64, window 300: 118.4, 113.8; T = 8192, 32 heads on 8 of 128, window 2048: none 761, every fourth 755,
@@ -82,18 +94,17 @@ __device__ __forceinline__ void put_half(uint32_t taddr, const float (&v)[64]) {
     umma::fence_before_sync();
     __syncwarp();
 }
-// D += A B, A (128 x 128) as put_half leaves it, B a tile stored [128][K]
+// D += A B, A (128 x K) as put_half leaves it, B rows [0, K) of a tile stored [128][K]
 template <int K>
-__device__ __forceinline__ void gemm_halves(uint32_t lead, uint32_t d, uint32_t a, uint32_t b_saddr, uint32_t idesc, bool accumulate) {
+__device__ __forceinline__ void gemm_step(uint32_t lead, uint32_t d, uint32_t a, uint32_t b_saddr, uint32_t idesc, bool accumulate) {
     umma::gemm_tm_lead<TILE, 64>(lead, d, a, b_saddr, idesc, accumulate);
-    umma::gemm_tm_lead<TILE, 64>(lead, d, a + 64, b_saddr + 64 * umma::ROW_BYTES, idesc, true);
+    if constexpr (K == 128) umma::gemm_tm_lead<TILE, 64>(lead, d, a + 64, b_saddr + 64 * umma::ROW_BYTES, idesc, true);
 }
-// 32 rows of K / 2 fp32 columns times f, as bf16, rows [first, last) of them to `out`, `stride` bytes apart; buf: K * 64 bytes of shared memory a warp
-template <int K>
+// 32 rows of 64 fp32 columns times f, as bf16, rows [first, last) of them to `out`, `stride` bytes apart; buf: 4 KB of shared memory a warp
 __device__ __forceinline__ void put_rows(uint32_t taddr, unsigned char* buf, int lane, bf16* out, long stride, float f, int first, int last) {
-    const Rows<K / 16> rows = {reinterpret_cast<uint4*>(buf), lane};
+    const Rows<8> rows = {reinterpret_cast<uint4*>(buf), lane};
 #pragma unroll
-    for (int i = 0; i < K / 2; i += 32) {
+    for (int i = 0; i < 64; i += 32) {
         float o[32];
         umma::tmem_ld32(taddr + i, o);
 #pragma unroll
@@ -102,19 +113,18 @@ __device__ __forceinline__ void put_rows(uint32_t taddr, unsigned char* buf, int
     }
     rows.store(out, stride, first, last);
 }
-// the same unrounded
-template <int K>
-__device__ __forceinline__ void put_parts(uint32_t taddr, unsigned char* buf, int lane, float* out, int first, int last) {
-    const Rows<K / 8> rows = {reinterpret_cast<uint4*>(buf), lane};
+// the same unrounded; 8 KB
+__device__ __forceinline__ void put_parts(uint32_t taddr, unsigned char* buf, int lane, float* out, long stride, int first, int last) {
+    const Rows<16> rows = {reinterpret_cast<uint4*>(buf), lane};
 #pragma unroll
-    for (int i = 0; i < K / 2; i += 32) {
+    for (int i = 0; i < 64; i += 32) {
         float o[32];
         umma::tmem_ld32(taddr + i, o);
 #pragma unroll
         for (int u = 0; u < 32; u += 4)
             rows.put((i + u) / 4, __float_as_uint(o[u]), __float_as_uint(o[u + 1]), __float_as_uint(o[u + 2]), __float_as_uint(o[u + 3]));
     }
-    rows.store(out, 2 * K * sizeof(float), first, last);
+    rows.store(out, stride, first, last);
 }
 __device__ __forceinline__ void load_stat(float* dst, const float* src, uint64_t* bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n"
@@ -123,12 +133,13 @@ __device__ __forceinline__ void load_stat(float* dst, const float* src, uint64_t
 }  // namespace bwd
 
 template <int K>
-__global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dq_tc_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(bwd::Cta<K>::THREADS, bwd::Cta<K>::PER_SM) window_dq_tc_kernel(const __grid_constant__ Params p) {
     chain_wait();
     clear_status(p);
     using namespace bwd;
-    using SM = Smem<K>;
-    constexpr int NA = SM::NA, NB = SM::NB, TM_S = 0, TM_DP = 256, TM_DQ = 384;         // S twice
+    using SM = Cta<K>;
+    constexpr int STEPS = SM::STEPS, WARPS = SM::WARPS, MMA_WARP = SM::MMA_WARP, TMA_WARP = SM::TMA_WARP;
+    constexpr int NA = SM::NA, NB = SM::NB, TM_S = 0, TM_DP = 2 * K, TM_DQ = 3 * K;         // S twice
     extern __shared__ __align__(1024) unsigned char smem[];
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + SM::bar_off);
     const Ring<NA> ringK = {bars, bars + NA};
@@ -153,7 +164,7 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dq_tc_kernel(const __
         umma::mbar_init(barS, 1);
         umma::mbar_init(barS + 1, 1);
         umma::mbar_init(barDP, 1);
-        umma::mbar_init(barE, 8);
+        umma::mbar_init(barE, WARPS);
         umma::mbar_init(barDone, 1);
         umma::fence_mbar_init();
         *abort_flag = 0;
@@ -161,14 +172,14 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dq_tc_kernel(const __
         load_tile<K>(smem + SM::stay_off, &p.tq, h, q0, b, barQ);
         load_tile<K>(smem + SM::stay_off + SM::TILE_BYTES, &p.tdo, h, q0, b, barQ);
     }
-    if (warp == MMA_WARP) umma::tmem_alloc(tmem_slot, 512);
+    if (warp == MMA_WARP) umma::tmem_alloc(tmem_slot, SM::TM);
     umma::fence_before_sync();
     __syncthreads();
     umma::fence_after_sync();
     const uint32_t tmem = *tmem_slot;
 
-    if (warp >= 8) {
-        regs_issue();
+    if (warp >= WARPS) {
+        SM::regs_issue();
         if (warp == TMA_WARP && lane == 0) {
             int nk = 0, nv = 0;
             while (nv < steps) {
@@ -189,52 +200,56 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dq_tc_kernel(const __
         } else if (warp == MMA_WARP) {
             const uint32_t lead = umma::elect_one(), sQ = umma::smem_addr(smem + SM::stay_off), sDO = sQ + SM::TILE_BYTES;
             const uint32_t sK = umma::smem_addr(smem + SM::a_off), sV = umma::smem_addr(smem + SM::b_off);
-            constexpr uint32_t idS = umma::idesc_bf16(128, 128, false, false), idQ = umma::idesc_bf16(128, K, false, true);
+            constexpr uint32_t idS = umma::idesc_bf16(128, K, false, false), idQ = umma::idesc_bf16(128, K, false, true);
             bool ok = umma::mbar_wait_warp(barQ, 0, abort_flag);
-            const auto scores = [&](int n) {
-                ok = ok && umma::mbar_wait_warp(ringK.filled(n), ringK.phase(n), abort_flag);
+            // step m: part m % STEPS of tile m / STEPS
+            const auto scores = [&](int m) {
+                const int n = m / STEPS, u = m % STEPS;
+                ok = ok && (u > 0 || umma::mbar_wait_warp(ringK.filled(n), ringK.phase(n), abort_flag));
                 if (!ok) return;
-                umma::gemm_kk_lead<TILE, TILE, K>(lead, tmem + TM_S + 128 * (n & 1), sQ, sK + n % NA * SM::TILE_BYTES, idS, false);
-                umma::commit_lead(lead, barS + (n & 1));
+                umma::gemm_kk_lead<TILE, TILE, K>(lead, tmem + TM_S + K * (m & 1), sQ, sK + n % NA * SM::TILE_BYTES + u * K * umma::ROW_BYTES, idS, false);
+                umma::commit_lead(lead, barS + (m & 1));
             };
-            const auto products = [&](int n) {
-                ok = ok && umma::mbar_wait_warp(ringV.filled(n), ringV.phase(n), abort_flag);
+            const auto products = [&](int m) {
+                const int n = m / STEPS, u = m % STEPS;
+                ok = ok && (u > 0 || umma::mbar_wait_warp(ringV.filled(n), ringV.phase(n), abort_flag));
                 if (!ok) return;
-                umma::gemm_kk_lead<TILE, TILE, K>(lead, tmem + TM_DP, sDO, sV + n % NB * SM::TILE_BYTES, idS, false);
+                umma::gemm_kk_lead<TILE, TILE, K>(lead, tmem + TM_DP, sDO, sV + n % NB * SM::TILE_BYTES + u * K * umma::ROW_BYTES, idS, false);
                 umma::commit_lead(lead, barDP);
-                umma::commit_lead(lead, ringV.freed(n));
+                if (u == STEPS - 1) umma::commit_lead(lead, ringV.freed(n));
             };
             scores(0);
             products(0);
-            for (int n = 0; n < steps && ok; ++n) {
-                if (n + 1 < steps) scores(n + 1);
-                ok = ok && umma::mbar_wait_warp(barE, n & 1, abort_flag);
+            for (int m = 0; m < steps * STEPS && ok; ++m) {
+                const int n = m / STEPS, u = m % STEPS;
+                if (m + 1 < steps * STEPS) scores(m + 1);
+                ok = ok && umma::mbar_wait_warp(barE, m & 1, abort_flag);
                 umma::fence_after_sync();
-                if (n + 1 < steps) products(n + 1);
+                if (m + 1 < steps * STEPS) products(m + 1);
                 if (!ok) break;
-                gemm_halves<K>(lead, tmem + TM_DQ, tmem + TM_S + 128 * (n & 1), sK + n % NA * SM::TILE_BYTES, idQ, n > 0);
-                umma::commit_lead(lead, ringK.freed(n));
+                gemm_step<K>(lead, tmem + TM_DQ, tmem + TM_S + K * (m & 1), sK + n % NA * SM::TILE_BYTES + u * K * umma::ROW_BYTES, idQ, m > 0);
+                if (u == STEPS - 1) umma::commit_lead(lead, ringK.freed(n));
             }
             if (ok) umma::commit_lead(lead, barDone);
         }
     } else {
-        regs_rows();
+        SM::regs_rows();
         const int half = warp >> 2, row = (warp & 3) * 32 + lane, t = q0 + row;
         const long stat = ((long)b * p.H + h) * p.TP + t;
         const uint32_t tS = umma::tmem_addr(tmem, warp, TM_S + 64 * half), tDP = umma::tmem_addr(tmem, warp, TM_DP + 64 * half);
         const float c = p.scale * LOG2E, lse = p.lse[stat];
-        // delta of the tile's rows: a warp takes 16 of them, K / 8 lanes a row (a thread a row: 10 k cycles, for loads that touch a line a lane)
-        constexpr int LANES = K / 8, ROWS = 32 / LANES;
-        uint4 xo[16 / ROWS], xd[16 / ROWS];
+        // delta of the tile's rows, each warp its share of them, K / 8 lanes a row (a thread a row: 10 k cycles, for loads that touch a line a lane)
+        constexpr int LANES = K / 8, ROWS = 32 / LANES, EACH = TILE / WARPS;
+        uint4 xo[EACH / ROWS], xd[EACH / ROWS];
 #pragma unroll
-        for (int i = 0; i < 16 / ROWS; ++i) {
-            const int r = q0 + warp * 16 + i * ROWS + lane / LANES;
+        for (int i = 0; i < EACH / ROWS; ++i) {
+            const int r = q0 + warp * EACH + i * ROWS + lane / LANES;
             const long from = (((long)b * p.T + r) * p.H + h) * K + lane % LANES * 8;
             xo[i] = r < p.T ? *reinterpret_cast<const uint4*>(p.o + from) : make_uint4(0, 0, 0, 0);
             xd[i] = r < p.T ? *reinterpret_cast<const uint4*>(p.d_o + from) : make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
-        for (int i = 0; i < 16 / ROWS; ++i) {
+        for (int i = 0; i < EACH / ROWS; ++i) {
             const uint32_t xs[4] = {xo[i].x, xo[i].y, xo[i].z, xo[i].w}, ys[4] = {xd[i].x, xd[i].y, xd[i].z, xd[i].w};
             float d = 0.f;
 #pragma unroll
@@ -244,12 +259,12 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dq_tc_kernel(const __
             }
 #pragma unroll
             for (int u = LANES / 2; u > 0; u >>= 1) d += __shfl_xor_sync(0xffffffffu, d, u);
-            if (lane % LANES == 0) sDelta[warp * 16 + i * ROWS + lane / LANES] = d;
+            if (lane % LANES == 0) sDelta[warp * EACH + i * ROWS + lane / LANES] = d;
         }
         if (q0 < p.low_rows) {                             // with what the rounding of o took off
 #pragma unroll
-            for (int i = 0; i < 16 / ROWS; ++i) {
-                const int r = q0 + warp * 16 + i * ROWS + lane / LANES;
+            for (int i = 0; i < EACH / ROWS; ++i) {
+                const int r = q0 + warp * EACH + i * ROWS + lane / LANES;
                 const uint4 xl = r < p.low_rows ? *reinterpret_cast<const uint4*>(p.low + (((long)b * p.low_rows + r) * p.H + h) * K + lane % LANES * 8) : make_uint4(0, 0, 0, 0);
                 const uint32_t xs[4] = {xl.x, xl.y, xl.z, xl.w}, ys[4] = {xd[i].x, xd[i].y, xd[i].z, xd[i].w};
                 float d = 0.f;
@@ -260,31 +275,31 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dq_tc_kernel(const __
                 }
 #pragma unroll
                 for (int u = LANES / 2; u > 0; u >>= 1) d += __shfl_xor_sync(0xffffffffu, d, u);
-                if (lane % LANES == 0) sDelta[warp * 16 + i * ROWS + lane / LANES] += d;
+                if (lane % LANES == 0) sDelta[warp * EACH + i * ROWS + lane / LANES] += d;
             }
         }
-        asm volatile("bar.sync 1, 256;\n" ::: "memory");
+        asm volatile("bar.sync 1, %0;\n" ::"n"(32 * WARPS) : "memory");
         const float delta = sDelta[row];
         if (half == 0) p.delta[stat] = delta;
         bool ok = true;
-        for (int n = 0; n < steps; ++n) {
-            const int s0 = tile(n) * TILE;
-            ok = umma::mbar_wait_warp(barS + (n & 1), (n >> 1) & 1, abort_flag);
+        for (int m = 0; m < steps * STEPS; ++m) {
+            const int s0 = tile(m / STEPS) * TILE, from = s0 + m % STEPS * K + half * 64;
+            ok = umma::mbar_wait_warp(barS + (m & 1), (m >> 1) & 1, abort_flag);
             if (!ok) break;
             umma::fence_after_sync();
             float e[64], d[64];
-            tmem_ld64(tS + 128 * (n & 1), e);
+            tmem_ld64(tS + K * (m & 1), e);
             exponentials(e, c, [&](int) { return pair(-lse, -lse); });
             if (!all_seen(q0, s0, p.window, p.sinks)) {
 #pragma unroll
                 for (int i = 0; i < 64; i += 32) {
-                    const uint32_t bits = seen_bits(t, s0 + half * 64 + i, p.window, p.sinks);
+                    const uint32_t bits = seen_bits(t, from + i, p.window, p.sinks);
 #pragma unroll
                     for (int u = 0; u < 32; ++u)
                         if (!(bits & (1u << u))) e[i + u] = 0.f;
                 }
             }
-            ok = umma::mbar_wait_warp(barDP, n & 1, abort_flag);
+            ok = umma::mbar_wait_warp(barDP, m & 1, abort_flag);
             if (!ok) break;
             umma::fence_after_sync();
             tmem_ld64(tDP, d);
@@ -294,7 +309,7 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dq_tc_kernel(const __
                 e[i] = v.x;
                 e[i + 1] = v.y;
             }
-            put_half(tS + 128 * (n & 1), e);
+            put_half(tS + K * (m & 1), e);
             if (lane == 0) arrive(barE);
         }
         if (ok) ok = umma::mbar_wait_warp(barDone, 0, abort_flag);
@@ -302,8 +317,8 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dq_tc_kernel(const __
             umma::fence_after_sync();
             // (all products are done: the place of Q and dO is free)
             const int first = q0 + (warp & 3) * 32;
-            put_rows<K>(umma::tmem_addr(tmem, warp, TM_DQ + half * (K / 2)), smem + SM::stay_off + warp * K * 64, lane,
-                        p.dq + (((long)b * p.T + first) * p.H + h) * K + half * (K / 2), (long)p.H * K * 2, p.scale, 0, min(p.T - first, 32));
+            put_rows(umma::tmem_addr(tmem, warp, TM_DQ + half * 64), smem + SM::stay_off + warp * 8192, lane, p.dq + (((long)b * p.T + first) * p.H + h) * K + half * 64,
+                     (long)p.H * K * 2, p.scale, 0, min(p.T - first, 32));
         }
         umma::fence_before_sync();
     }
@@ -316,16 +331,17 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dq_tc_kernel(const __
             umma::mbar_wait(barQ, 1);
             if (lane == 0) atomicExch(p.err, 1);
         }
-        umma::tmem_dealloc(tmem, 512);
+        umma::tmem_dealloc(tmem, SM::TM);
     }
 }
 
 template <int K>
-__global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dkv_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Shares sh) {
+__global__ void __launch_bounds__(bwd::Cta<K>::THREADS, bwd::Cta<K>::PER_SM) window_dkv_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Shares sh) {
     chain_wait();
     using namespace bwd;
-    using SM = Smem<K>;
-    constexpr int NA = SM::NA, NB = SM::NB, TM_S = 0, TM_DP = 128, TM_DV = 256, TM_DK = 384;
+    using SM = Cta<K>;
+    constexpr int STEPS = SM::STEPS, WARPS = SM::WARPS, MMA_WARP = SM::MMA_WARP, TMA_WARP = SM::TMA_WARP;
+    constexpr int NA = SM::NA, NB = SM::NB, TM_S = 0, TM_DP = K, TM_DV = 2 * K, TM_DK = 3 * K;
     extern __shared__ __align__(1024) unsigned char smem[];
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + SM::bar_off);
     const Ring<NA> ringQ = {bars, bars + NA};
@@ -352,8 +368,8 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dkv_tc_kernel(const _
         umma::mbar_init(barKV, 1);
         umma::mbar_init(barS, 1);
         umma::mbar_init(barDP, 1);
-        umma::mbar_init(barP, 8);
-        umma::mbar_init(barDS, 8);
+        umma::mbar_init(barP, WARPS);
+        umma::mbar_init(barDS, WARPS);
         umma::mbar_init(barDone, 1);
         umma::fence_mbar_init();
         *abort_flag = 0;
@@ -361,14 +377,14 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dkv_tc_kernel(const _
         load_tile<K>(smem + SM::stay_off, &p.tk, grp, s0, b, barKV);
         load_tile<K>(smem + SM::stay_off + SM::TILE_BYTES, &p.tv, grp, s0, b, barKV);
     }
-    if (warp == MMA_WARP) umma::tmem_alloc(tmem_slot, 512);
+    if (warp == MMA_WARP) umma::tmem_alloc(tmem_slot, SM::TM);
     umma::fence_before_sync();
     __syncthreads();
     umma::fence_after_sync();
     const uint32_t tmem = *tmem_slot;
 
-    if (warp >= 8) {
-        regs_issue();
+    if (warp >= WARPS) {
+        SM::regs_issue();
         if (warp == TMA_WARP && lane == 0) {
             int nq = 0, nd = 0, h = h0, i = lo;
             while (nd < steps) {
@@ -396,51 +412,56 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dkv_tc_kernel(const _
         } else if (warp == MMA_WARP) {
             const uint32_t lead = umma::elect_one(), sK = umma::smem_addr(smem + SM::stay_off), sV = sK + SM::TILE_BYTES;
             const uint32_t sQ = umma::smem_addr(smem + SM::a_off), sDO = umma::smem_addr(smem + SM::b_off);
-            constexpr uint32_t idS = umma::idesc_bf16(128, 128, false, false), idG = umma::idesc_bf16(128, K, false, true);
+            constexpr uint32_t idS = umma::idesc_bf16(128, K, false, false), idG = umma::idesc_bf16(128, K, false, true);
             bool ok = umma::mbar_wait_warp(barKV, 0, abort_flag);
-            const auto scores = [&](int n) {
-                ok = ok && umma::mbar_wait_warp(ringQ.filled(n), ringQ.phase(n), abort_flag);
+            const auto scores = [&](int m) {
+                const int n = m / STEPS, u = m % STEPS;
+                ok = ok && (u > 0 || umma::mbar_wait_warp(ringQ.filled(n), ringQ.phase(n), abort_flag));
                 if (!ok) return;
-                umma::gemm_kk_lead<TILE, TILE, K>(lead, tmem + TM_S, sK, sQ + n % NA * SM::TILE_BYTES, idS, false);
+                umma::gemm_kk_lead<TILE, TILE, K>(lead, tmem + TM_S, sK, sQ + n % NA * SM::TILE_BYTES + u * K * umma::ROW_BYTES, idS, false);
                 umma::commit_lead(lead, barS);
             };
-            const auto products = [&](int n) {
-                ok = ok && umma::mbar_wait_warp(ringDO.filled(n), ringDO.phase(n), abort_flag);
+            const auto products = [&](int m) {
+                const int n = m / STEPS, u = m % STEPS;
+                ok = ok && (u > 0 || umma::mbar_wait_warp(ringDO.filled(n), ringDO.phase(n), abort_flag));
                 if (!ok) return;
-                umma::gemm_kk_lead<TILE, TILE, K>(lead, tmem + TM_DP, sV, sDO + n % NB * SM::TILE_BYTES, idS, false);
+                umma::gemm_kk_lead<TILE, TILE, K>(lead, tmem + TM_DP, sV, sDO + n % NB * SM::TILE_BYTES + u * K * umma::ROW_BYTES, idS, false);
                 umma::commit_lead(lead, barDP);
             };
             scores(0);
             products(0);
-            for (int n = 0; n < steps && ok; ++n) {
-                ok = umma::mbar_wait_warp(barP, n & 1, abort_flag);
+            for (int m = 0; m < steps * STEPS && ok; ++m) {
+                const int n = m / STEPS, u = m % STEPS;
+                ok = umma::mbar_wait_warp(barP, m & 1, abort_flag);
                 if (!ok) break;
                 umma::fence_after_sync();
-                gemm_halves<K>(lead, tmem + TM_DV, tmem + TM_S, sDO + n % NB * SM::TILE_BYTES, idG, n > 0);
-                if (n + 1 < steps) scores(n + 1);
-                ok = ok && umma::mbar_wait_warp(barDS, n & 1, abort_flag);
+                gemm_step<K>(lead, tmem + TM_DV, tmem + TM_S, sDO + n % NB * SM::TILE_BYTES + u * K * umma::ROW_BYTES, idG, m > 0);
+                if (m + 1 < steps * STEPS) scores(m + 1);
+                ok = ok && umma::mbar_wait_warp(barDS, m & 1, abort_flag);
                 if (!ok) break;
                 umma::fence_after_sync();
-                gemm_halves<K>(lead, tmem + TM_DK, tmem + TM_DP, sQ + n % NA * SM::TILE_BYTES, idG, n > 0);
+                gemm_step<K>(lead, tmem + TM_DK, tmem + TM_DP, sQ + n % NA * SM::TILE_BYTES + u * K * umma::ROW_BYTES, idG, m > 0);
                 // (delta, beside dO, is read until dS is there)
-                umma::commit_lead(lead, ringDO.freed(n));
-                umma::commit_lead(lead, ringQ.freed(n));
-                if (n + 1 < steps) products(n + 1);
+                if (u == STEPS - 1) {
+                    umma::commit_lead(lead, ringDO.freed(n));
+                    umma::commit_lead(lead, ringQ.freed(n));
+                }
+                if (m + 1 < steps * STEPS) products(m + 1);
             }
             if (ok) umma::commit_lead(lead, barDone);
         }
     } else {
-        regs_rows();
+        SM::regs_rows();
         const int half = warp >> 2, s = s0 + (warp & 3) * 32 + lane;
         const uint32_t tS = umma::tmem_addr(tmem, warp, TM_S + 64 * half), tDP = umma::tmem_addr(tmem, warp, TM_DP + 64 * half);
         const float c = p.scale * LOG2E;
         bool ok = true;
         int i = lo;
-        for (int n = 0; n < steps; ++n) {
-            const int t0 = i * TILE;
-            if (++i > hi) i = lo;
-            const float *lse = sStat + n % NA * TILE + half * 64, *delta = sStat + (NA + n % NB) * TILE + half * 64;
-            ok = umma::mbar_wait_warp(ringQ.filled(n), ringQ.phase(n), abort_flag) && umma::mbar_wait_warp(barS, n & 1, abort_flag);
+        for (int m = 0; m < steps * STEPS; ++m) {
+            const int n = m / STEPS, u0 = m % STEPS * K + half * 64, t0 = i * TILE;
+            if (m % STEPS == STEPS - 1 && ++i > hi) i = lo;
+            const float *lse = sStat + n % NA * TILE + u0, *delta = sStat + (NA + n % NB) * TILE + u0;
+            ok = umma::mbar_wait_warp(ringQ.filled(n), ringQ.phase(n), abort_flag) && umma::mbar_wait_warp(barS, m & 1, abort_flag);
             if (!ok) break;
             umma::fence_after_sync();
             float e[64], d[64];
@@ -453,7 +474,7 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dkv_tc_kernel(const _
                 // token s is seen by the queries from s on, as far as the window goes; a sink by all of them
 #pragma unroll
                 for (int k = 0; k < 64; k += 32) {
-                    const uint32_t bits = seeing_bits(t0 + half * 64 + k, s, p.window, p.sinks);
+                    const uint32_t bits = seeing_bits(t0 + u0 + k, s, p.window, p.sinks);
 #pragma unroll
                     for (int u = 0; u < 32; ++u)
                         if (!(bits & (1u << u))) e[k + u] = 0.f;
@@ -461,7 +482,7 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dkv_tc_kernel(const _
             }
             put_half(tS, e);
             if (lane == 0) arrive(barP);
-            ok = umma::mbar_wait_warp(ringDO.filled(n), ringDO.phase(n), abort_flag) && umma::mbar_wait_warp(barDP, n & 1, abort_flag);
+            ok = umma::mbar_wait_warp(ringDO.filled(n), ringDO.phase(n), abort_flag) && umma::mbar_wait_warp(barDP, m & 1, abort_flag);
             if (!ok) break;
             umma::fence_after_sync();
             tmem_ld64(tDP, d);
@@ -479,20 +500,20 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dkv_tc_kernel(const _
         if (ok) {
             umma::fence_after_sync();
             const int row0 = (warp & 3) * 32, first = s0 + row0, last = min(p.T - first, 32);
-            const long at = (((long)b * p.T + first) * p.G + grp) * K + half * (K / 2), unit = (long)b * p.G + grp;
-            const uint32_t tDV = umma::tmem_addr(tmem, warp, TM_DV + half * (K / 2)), tDK = umma::tmem_addr(tmem, warp, TM_DK + half * (K / 2));
-            unsigned char* buf = smem + SM::stay_off + warp * K * 64;              // (all products are done: the place of K and V is free)
+            const long at = (((long)b * p.T + first) * p.G + grp) * K + half * 64, unit = (long)b * p.G + grp;
+            const uint32_t tDV = umma::tmem_addr(tmem, warp, TM_DV + half * 64), tDK = umma::tmem_addr(tmem, warp, TM_DK + half * 64);
+            unsigned char* buf = smem + SM::stay_off + warp * 8192;              // (all products are done: the place of K and V is free)
             const int sink = j < sh.far_tiles ? max(min(p.sinks - first, 32), 0) : 0;        // tokens with parts from far
             if (far || sh.splits > 1 || j < sh.far_tiles) {
                 float* part = far ? p.far_part + (((unit * sh.far_tiles + j) * sh.chunks + share) * sh.far_rows(p.sinks) + row0) * 2 * K
                                   : p.near_part + (((unit * sh.splits + share) * sh.near_tiles() + j) * TILE + row0) * 2 * K;
                 const int parts = !far && sh.splits > 1 ? last : min(sink, last);
-                put_parts<K>(tDK, buf, lane, part + half * (K / 2), 0, parts);
-                put_parts<K>(tDV, buf, lane, part + K + half * (K / 2), 0, parts);
+                put_parts(tDK, buf, lane, part + half * 64, 2 * K * sizeof(float), 0, parts);
+                put_parts(tDV, buf, lane, part + K + half * 64, 2 * K * sizeof(float), 0, parts);
             }
             if (!far && sh.splits == 1) {
-                put_rows<K>(tDV, buf, lane, p.dv + at, (long)p.G * K * 2, 1.f, sink, last);
-                put_rows<K>(tDK, buf, lane, p.dk + at, (long)p.G * K * 2, p.scale, sink, last);
+                put_rows(tDV, buf, lane, p.dv + at, (long)p.G * K * 2, 1.f, sink, last);
+                put_rows(tDK, buf, lane, p.dk + at, (long)p.G * K * 2, p.scale, sink, last);
             }
         }
         umma::fence_before_sync();
@@ -505,7 +526,7 @@ __global__ void __launch_bounds__(bwd::NTHREADS, 1) window_dkv_tc_kernel(const _
             umma::mbar_wait(barKV, 1);
             if (lane == 0) atomicExch(p.err, 1);
         }
-        umma::tmem_dealloc(tmem, 512);
+        umma::tmem_dealloc(tmem, SM::TM);
     }
 }
 
@@ -544,17 +565,18 @@ __global__ void __launch_bounds__(256) window_join_kernel(const __grid_constant_
 
 template <int K>
 static cudaError_t launch(const Params& p, cudaStream_t st) {
-    const size_t smem = bwd::Smem<K>::total;
+    const size_t smem = bwd::Cta<K>::total;
+    constexpr int THREADS = bwd::Cta<K>::THREADS;
     const Shares sh(p.B, p.T, p.H, p.G, p.window, p.sinks);
     const auto dq = window_dq_tc_kernel<K>;
     const auto dkv = window_dkv_tc_kernel<K>;
     cudaError_t e = allow_smem(dq, smem);
     if (e == cudaSuccess) e = allow_smem(dkv, smem);
     if (e != cudaSuccess) return e;
-    e = launch_chained(dq, dim3((unsigned)sh.tiles * p.H, p.B), bwd::NTHREADS, smem, st, p);
+    e = launch_chained(dq, dim3((unsigned)sh.tiles * p.H, p.B), THREADS, smem, st, p);
     if (e != cudaSuccess) return e;
     LLATTN_LAUNCHED();
-    e = launch_chained(dkv, (unsigned)(sh.far_tiles * sh.chunks + sh.tiles * sh.splits) * p.G * p.B, bwd::NTHREADS, smem, st, p, sh);
+    e = launch_chained(dkv, (unsigned)(sh.far_tiles * sh.chunks + sh.tiles * sh.splits) * p.G * p.B, THREADS, smem, st, p, sh);
     if (e != cudaSuccess) return e;
     LLATTN_LAUNCHED();
     const int some = sh.far_tiles * TILE < p.sinks ? sh.far_tiles * TILE : p.sinks, tokens = sh.splits > 1 ? p.T : some;
