@@ -84,7 +84,7 @@ size_t llattn_window_stats_bytes(int B, int T, int H, int K, int window, int sin
 }
 size_t llattn_window_workspace_bytes(int B, int T, int H, int G, int K, int window, int sinks) {
     if (win::check(B, T, H, G, K, window, sinks, 1.f) != 0) return 0;
-    const win::Shares sh(B, T, H, G, window, sinks);
+    const win::Shares sh(B, T, H, G, K, window, sinks);
     return 256 + win::lse_bytes(B, T, H) + (sh.near_floats(B, G, K) + sh.far_floats(B, G, K, sinks)) * sizeof(float);
 }
 
@@ -121,7 +121,7 @@ int llattn_window_bwd(const void* q, const void* k, const void* v, const void* o
     p.dv = (win::bf16*)dv;
     p.delta = reinterpret_cast<float*>(static_cast<char*>(workspace) + 256);
     p.near_part = p.delta + (long)B * H * win::padded(T);
-    p.far_part = p.near_part + win::Shares(B, T, H, G, window, sinks).near_floats(B, G, K);
+    p.far_part = p.near_part + win::Shares(B, T, H, G, K, window, sinks).near_floats(B, G, K);
     win::shape(p, workspace, B, T, H, G, window, sinks, scale);
     win::statistics(p, const_cast<void*>(stats));
     cudaStream_t st = (cudaStream_t)stream;

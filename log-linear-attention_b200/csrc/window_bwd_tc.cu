@@ -567,7 +567,7 @@ template <int K>
 static cudaError_t launch(const Params& p, cudaStream_t st) {
     const size_t smem = bwd::Cta<K>::total;
     constexpr int THREADS = bwd::Cta<K>::THREADS;
-    const Shares sh(p.B, p.T, p.H, p.G, p.window, p.sinks);
+    const Shares sh(p.B, p.T, p.H, p.G, K, p.window, p.sinks);
     const auto dq = window_dq_tc_kernel<K>;
     const auto dkv = window_dkv_tc_kernel<K>;
     cudaError_t e = allow_smem(dq, smem);
