@@ -30,8 +30,9 @@ struct Params {
 };
 
 // How the sums of dK and dV are shared out.  A tile of 128 tokens is seen by the queries of its own tile and of the `near - 1` behind it; its CTA takes their heads, or
-// one of `splits` shares of them where there are too few tiles to fill the chip (a second CTA an SM only for shares of 16 steps and more: 16 heads on 2 of 64, 2048 tokens, all that are
-// before 100 us for 73, but 8 on 2, 4096 tokens, window 512 72 for 76).  The first `far_tiles` tiles, of sinks, are seen by all later queries too: those come in
+// one of `splits` shares of them where there are too few tiles to fill the chip; twice as many as SMs where two fit on one (K = 64), or
+// where the window reaches back to the start, so that the first tiles have several times the steps of the last, if 16 steps and more are left to a share (us, fewer / more: 2048 tokens, all
+// before, 16 heads on 2 of 64 100 / 73, of 128 91 / 74, 32 on 4 169 / 128; but 4096 tokens, 8 heads on 2 of 64, window 512 72 / 76, 16 on 2 of 128, window 1024 129 / 137).  The first `far_tiles` tiles, of sinks, are seen by all later queries too: those come in
 // `chunks` shares of `chunk` tiles, about as long as the others (one CTA for all of them would run on alone: T = 16384, window 2048, 4 sinks, 8 groups 2.7 ms
 // in the place of 1.9 for the whole backward).  What is shared is left as fp32 parts, and added up in a fixed order.
 struct Shares {
@@ -43,8 +44,8 @@ struct Shares {
         near = (TILE - 1 + window - 1) / TILE + 1;
         const auto shares = [&](int ctas) { return (int)(ctas / (units * tiles) < R ? ctas / (units * tiles) : R); };
         splits = shares(148);
-        // (K = 64: two CTAs an SM)
-        if (K == 64 && shares(2 * 148) > splits && (R + shares(2 * 148) - 1) / shares(2 * 148) * near >= 16) splits = shares(2 * 148);
+        const int more = shares(2 * 148), reach = near < tiles ? near : tiles;
+        if ((K == 64 || near >= tiles) && more > splits && (long)((R + more - 1) / more) * reach >= 16) splits = more;
         if (splits < 1) splits = 1;
         const int sink_tiles = ((sinks < T ? sinks : T) + TILE - 1) / TILE;
         far_tiles = sink_tiles < tiles - near ? sink_tiles : tiles - near > 0 ? tiles - near : 0;
