@@ -132,6 +132,15 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
+// A sequence of at most FEW tokens visits each tile twice, the second time with what the rounding of P and dS to bf16 took off: a gradient that is a sum of two or three products has
+// no other roundings for theirs to average with (2 to 5 tokens, one head: dq and dk 2.2e-3 to 3.3e-3 off in the place of 1.7e-3), and such calls are the host's time in any case.
+// (Kernels of their own: the tests cost the others 1 to 3 %.)  Steps are shifted by `twice`, and those of the second visits have the bit.
+inline bool visits_twice(int T) { return T <= FEW; }
+template <int N>
+__device__ __forceinline__ void leave_rest(float (&e)[N]) {
+#pragma unroll
+    for (int u = 0; u < N; ++u) e[u] -= __bfloat162float(__float2bfloat16(e[u]));
+}
 // 64 consecutive fp32 columns of this thread's lane, both loads in flight before the wait
 __device__ __forceinline__ void tmem_ld64(uint32_t taddr, float (&v)[64]) {
     uint32_t r[64];

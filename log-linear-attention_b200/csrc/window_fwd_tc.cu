@@ -60,7 +60,7 @@ struct Seen {
 };
 }  // namespace fwd
 
-template <int K, int X>
+template <int K, int X, bool TWICE>
 __global__ void __launch_bounds__(fwd::Cta<K, X>::THREADS, fwd::Cta<K, X>::PER_SM) window_fwd_tc_kernel(const __grid_constant__ Params p) {
     chain_wait();
     clear_status(p);
@@ -80,10 +80,12 @@ __global__ void __launch_bounds__(fwd::Cta<K, X>::THREADS, fwd::Cta<K, X>::PER_S
     const unsigned units = p.B * p.H, unit = blockIdx.x % units;
     const int h = unit % p.H, q0 = (gridDim.x / units - 1 - blockIdx.x / units) * X * TILE, b = unit / p.H, grp = h / (p.H / p.G);
     const Seen<X> w(p, q0);
+    constexpr int twice = TWICE;
+    const int count = w.count << twice;
     // position n of the ring's sequence: K, V of the first tile, K, V of the second, ...
     const auto bring = [&](int n) {
         tma::expect_tx(full + n % NST, SM::TILE_BYTES);
-        load_tile<K>(smem + SM::st_off + n % NST * SM::TILE_BYTES, n & 1 ? &p.tv : &p.tk, grp, w.tile(n >> 1) * TILE, b, full + n % NST);
+        load_tile<K>(smem + SM::st_off + n % NST * SM::TILE_BYTES, n & 1 ? &p.tv : &p.tk, grp, w.tile(n >> 1 >> twice) * TILE, b, full + n % NST);
     };
     if (tid == TMA_WARP * 32) {              // (the thread that brings the tiles need not wait for the others)
         for (int i = 0; i < NST; ++i) {
@@ -118,7 +120,7 @@ __global__ void __launch_bounds__(fwd::Cta<K, X>::THREADS, fwd::Cta<K, X>::PER_S
         SM::regs_issue();
         if (warp == TMA_WARP && lane == 0) {
             int n = 1;
-            for (; n < 2 * w.count; ++n) {
+            for (; n < 2 * count; ++n) {
                 if (n >= NST && !umma::mbar_wait(empty + n % NST, (n / NST - 1) & 1, abort_flag)) break;
                 bring(n);
             }
@@ -135,7 +137,7 @@ __global__ void __launch_bounds__(fwd::Cta<K, X>::THREADS, fwd::Cta<K, X>::PER_S
             int done[2] = {0, 0};                       // products P V of A, B issued
             // step i: the products P V with tile i - 1, and S with tile i
             bool before[2] = {false, false};
-            for (int i = 0; i <= w.count && ok; ++i) {
+            for (int i = 0; i <= count && ok; ++i) {
                 bool haveK = false, haveV = false;
                 const int nk = 2 * i, nv = 2 * i - 1;   // positions of K of this step and V of the one before in the ring's sequence
                 for (int x = 0; x < X && ok; ++x) {
@@ -154,7 +156,7 @@ __global__ void __launch_bounds__(fwd::Cta<K, X>::THREADS, fwd::Cta<K, X>::PER_S
                         umma::commit_lead(lead, barO + x);
                         ++done[x];
                     }
-                    before[x] = i < w.count && w.in(x, w.tile(i));
+                    before[x] = i < count && w.in(x, w.tile(i >> twice));
                     if (before[x]) {
                         ok = umma::mbar_wait_warp(barQ + x, 0, abort_flag);
                         if (!ok) break;
@@ -167,7 +169,7 @@ __global__ void __launch_bounds__(fwd::Cta<K, X>::THREADS, fwd::Cta<K, X>::PER_S
                 }
                 if (!ok) break;
                 if (i > 0) umma::commit_lead(lead, empty + nv % NST);
-                if (i < w.count) umma::commit_lead(lead, empty + nk % NST);
+                if (i < count) umma::commit_lead(lead, empty + nk % NST);
             }
         }
     } else {
@@ -177,11 +179,11 @@ __global__ void __launch_bounds__(fwd::Cta<K, X>::THREADS, fwd::Cta<K, X>::PER_S
         const float c = p.scale * LOG2E;
         const F2 c2 = pair(c, c);
         const Span span(t0, p.T, p.window, p.sinks);
-        const int n = span.count();
+        const int n = span.count() << twice;
         float m = -INFINITY, sum = 0.f;
         bool ok = true;
         for (int i = 0; i < n; ++i) {
-            const int s0 = span.tile(i) * TILE;
+            const int s0 = span.tile(i >> twice) * TILE;
             const bool whole = all_seen(t0, s0, p.window, p.sinks);
             ok = umma::mbar_wait_warp(barS + x, i & 1, abort_flag);
             if (!ok) break;
@@ -231,7 +233,7 @@ __global__ void __launch_bounds__(fwd::Cta<K, X>::THREADS, fwd::Cta<K, X>::PER_S
             F2 part[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-                const auto exponentials = [&](auto mixed) {
+                const auto exponentials = [&](auto mixed, auto rest) {
 #pragma unroll
                     for (int k = 0; k < 64; k += 32) {
                         uint32_t w[16];
@@ -245,15 +247,17 @@ __global__ void __launch_bounds__(fwd::Cta<K, X>::THREADS, fwd::Cta<K, X>::PER_S
                                 const float2 v = both(y);
                                 e = make_float2(exp2_fast(v.x), exp2_fast(v.y));
                             }
-                            part[u & 1] = add(part[u & 1], pair(e.x, e.y));
                             w[u] = pack_bf16(e.x, e.y);
+                            if (decltype(rest)::value) w[u] = pack_bf16(e.x - __uint_as_float(w[u] << 16), e.y - __uint_as_float(w[u] & 0xffff0000u));
+                            else part[u & 1] = add(part[u & 1], pair(e.x, e.y));
                         }
                         umma::tmem_st16u(tS + 32 * half + k / 2, w);
                     }
                 };
                 // (hidden keys are exact zeros: the special-function unit's)
-                if (whole) exponentials(std::true_type{});
-                else exponentials(std::false_type{});
+                if (whole) exponentials(std::true_type{}, std::false_type{});
+                else if (i & twice) exponentials(std::false_type{}, std::true_type{});
+                else exponentials(std::false_type{}, std::false_type{});
                 umma::tmem_wait_st();
                 umma::fence_before_sync();
                 __syncwarp();
@@ -311,10 +315,10 @@ __global__ void __launch_bounds__(fwd::Cta<K, X>::THREADS, fwd::Cta<K, X>::PER_S
     }
 }
 
-template <int K, int X>
+template <int K, int X, bool TWICE>
 static cudaError_t launch(const Params& p, cudaStream_t st) {
     using C = fwd::Cta<K, X>;
-    const auto kern = window_fwd_tc_kernel<K, X>;
+    const auto kern = window_fwd_tc_kernel<K, X, TWICE>;
     cudaError_t e = allow_smem(kern, C::total);
     if (e != cudaSuccess) return e;
     const unsigned grid = (unsigned)(p.T + X * TILE - 1) / (X * TILE) * p.H * p.B;
@@ -326,8 +330,9 @@ static cudaError_t launch(const Params& p, cudaStream_t st) {
 // one tile / two: K = 128, 32 heads on 8, window 512, 8192 tokens 119 / 128; window 1024 164 / 169; window 2048, 4096 tokens 110 / 109, 8192 tokens 249 / 239; 8192 tokens, all that are
 // before 482 / 439; K = 64, 16 heads, 2 x 1999 tokens, window 512 25.4 / 31.2; 8 heads on 2, 32768 tokens, window 4096 417 / 440; 32 heads on 8, 8192 tokens, all before 469 / 455).
 cudaError_t forward_tc(const Params& p, int K, cudaStream_t st) {
-    if (K == 64) return launch<64, 1>(p, st);
-    return p.T >= 2048 && p.window >= 2048 ? launch<128, 2>(p, st) : launch<128, 1>(p, st);
+    if (visits_twice(p.T)) return K == 64 ? launch<64, 1, true>(p, st) : launch<128, 1, true>(p, st);
+    if (K == 64) return launch<64, 1, false>(p, st);
+    return p.T >= 2048 && p.window >= 2048 ? launch<128, 2, false>(p, st) : launch<128, 1, false>(p, st);
 }
 
 }  // namespace win
