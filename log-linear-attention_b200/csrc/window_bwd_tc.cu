@@ -563,10 +563,15 @@ __global__ void __launch_bounds__(256) window_join_kernel(const __grid_constant_
             sum[i].y += v.y;
         }
     };
-    const int each = (R + sh.splits - 1) / sh.splits;
-    for (int x = 0; x * each < R; ++x) add(p.near_part + (((unit * sh.splits + x) * sh.near_tiles() + j) * TILE + s % TILE) * 2 * K);
-    if (j < sh.far_tiles && s < p.sinks)
-        for (int x = 0; j + sh.near + x * sh.chunk < sh.tiles; ++x) add(p.far_part + (((unit * sh.far_tiles + j) * sh.chunks + x) * sh.far_rows(p.sinks) + s % TILE) * 2 * K);
+    // (four parts' loads in flight)
+    const int each = (R + sh.splits - 1) / sh.splits, shares = (R + each - 1) / each;
+#pragma unroll 4
+    for (int x = 0; x < shares; ++x) add(p.near_part + (((unit * sh.splits + x) * sh.near_tiles() + j) * TILE + s % TILE) * 2 * K);
+    if (j < sh.far_tiles && s < p.sinks) {
+        const int chunks = (sh.tiles - j - sh.near + sh.chunk - 1) / sh.chunk;
+#pragma unroll 4
+        for (int x = 0; x < chunks; ++x) add(p.far_part + (((unit * sh.far_tiles + j) * sh.chunks + x) * sh.far_rows(p.sinks) + s % TILE) * 2 * K);
+    }
     const long at = ((b * p.T + s) * p.G + grp) * K;
 #pragma unroll
     for (int i = 0; i < N; ++i) {

@@ -6,9 +6,10 @@
 // Operands go from memory to the registers that the instructions read, 16 bytes a load: the order of a product's reduction index is free, so a lane takes 8
 // neighbouring columns of k as the indices of two instructions, and 8 neighbouring columns of v as the rows of eight.  No shared memory, no barrier in the loop.
 //
-// The slots of a (sequence, group) are spread over the warps of a cluster of CTAs, which join their maxima, sums and outputs through each other's shared memory:
+// The slots of a (sequence, group) are spread over the warps of a cluster of CTAs, which write their maxima, sums and outputs to the shared memory of the one that joins them:
 // one launch, no workspace, the order of every sum given by the sizes.
-// 64 sequences, 32 heads on 8, K = 128, 2052 slots: 92 us, 5.9 TB/s.  One sequence: 9.8 us, latency (two loads, a cluster's barriers and two joins one after another).
+// 64 sequences, 32 heads on 8, K = 128, 2052 slots: 92 us, 5.9 TB/s.  One sequence, 4100 slots: 8.6 us, latency (count, slots,
+// a cluster's barrier and two joins one after another).
 #include <cooperative_groups.h>
 
 #include "../../include/llattn.h"
