@@ -33,8 +33,8 @@ struct Params {
 // one of `splits` shares of them where there are too few tiles to fill the chip; twice as many as SMs where two fit on one (K = 64), or
 // where the window reaches back to the start, so that the first tiles have several times the steps of the last, if 16 steps and more are left to a share (us, fewer / more: 2048 tokens, all
 // before, 16 heads on 2 of 64 100 / 73, of 128 91 / 74, 32 on 4 169 / 128; but 4096 tokens, 8 heads on 2 of 64, window 512 72 / 76, 16 on 2 of 128, window 1024 129 / 137).  The first `far_tiles` tiles, of sinks, are seen by all later queries too: those come in
-// `chunks` shares of `chunk` tiles, about as long as the others (one CTA for all of them would run on alone: T = 16384, window 2048, 4 sinks, 8 groups 2.7 ms
-// in the place of 1.9 for the whole backward).  What is shared is left as fp32 parts, and added up in a fixed order.
+// `chunks` shares of `chunk` tiles, about as many steps as a share of the others (one CTA for all of them would run on alone: T = 16384, window 2048, 4 sinks, 8 groups 2.7 ms
+// in the place of 1.9 for the whole backward; chunks of `near` tiles where the others are split by heads: 1024 tokens, 4 heads on one, window 256 37 us for 24).  What is shared is left as fp32 parts, and added up in a fixed order.
 struct Shares {
     int tiles, near, splits, far_tiles, chunks, chunk;
     Shares(int B, int T, int H, int G, int K, int window, int sinks) {
@@ -54,7 +54,8 @@ struct Shares {
             const int length = tiles - near;
             long n = 2 * 148 / (units * far_tiles);
             if (n > 32) n = 32;
-            if (n > (length + near - 1) / near) n = (length + near - 1) / near;
+            const long most = ((long)length * splits + near - 1) / near;       // (all heads of chunk tiles: as many steps as a share of near ones)
+            if (n > most) n = most;
             chunk = (int)((length + (n < 1 ? 1 : n) - 1) / (n < 1 ? 1 : n));
             chunks = (length + chunk - 1) / chunk;
         }
