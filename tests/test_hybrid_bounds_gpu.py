@@ -83,7 +83,8 @@ def test_recurrence(B, T, D, xt, gt):
 
 
 @pytest.mark.parametrize("K", [64, 128])
-@pytest.mark.parametrize("B,T,H,G,window,sinks", [(1, 1, 1, 1, 1, 0), (2, 3, 2, 1, 2, 1), (1, 129, 4, 2, 40, 0), (2, 300, 2, 2, 20, 3), (1, 700, 8, 1, 100, 5), (1, 900, 2, 1, 130, 300)])
+@pytest.mark.parametrize("B,T,H,G,window,sinks", [(1, 1, 1, 1, 1, 0), (2, 3, 2, 1, 2, 1), (1, 129, 4, 2, 40, 0), (2, 300, 2, 2, 20, 3), (1, 700, 8, 1, 100, 5), (1, 900, 2, 1, 130, 300),
+                                                  (1, 1024, 4, 1, 256, 4), (1, 2000, 8, 1, 200, 16), (1, 2048, 16, 2, 2048, 0), (2, 1000, 16, 4, 1000, 0)])
 def test_window(B, T, H, G, window, sinks, K):
     b = Buffers()
     r = lambda n: b.of(torch.randn(B, T, n, K, device="cuda").to(torch.bfloat16))

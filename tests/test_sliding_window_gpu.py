@@ -92,6 +92,13 @@ def test_long_windows(B, T, H, G, window, sinks):
     run(B, T, H, G, 128, window, sinks)
 
 
+@pytest.mark.parametrize("K", [64, 128])
+@pytest.mark.parametrize("B,T,H,G,window,sinks", [(1, 1024, 4, 1, 256, 4), (1, 2000, 8, 1, 200, 16), (1, 1500, 16, 2, 1500, 0), (2, 1000, 6, 2, 1000, 0), (1, 1800, 5, 1, 130, 200)])
+def test_shared_out_sums(B, T, H, G, K, window, sinks):
+    """Sums of dK and dV that several CTAs share: heads of a group, sinks, windows that reach back to the start."""
+    run(B, T, H, G, K, window, sinks)
+
+
 @pytest.mark.parametrize("scale", [0.01, 0.3])
 def test_scale(scale):
     run(1, 200, 2, 1, 64, 90, 2, scale)
