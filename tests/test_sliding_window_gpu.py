@@ -86,6 +86,13 @@ def test_short_sequences(B, T, H, G, K, window, sinks):
     check(q, k, v, window, sinks, o.detach(), None, do, torch.autograd.grad(o, leaves, do), half=2.0 ** -16)
 
 
+@pytest.mark.parametrize("K", [64, 128])
+@pytest.mark.parametrize("B,T,H,G,window,sinks", [(1, 500, 4, 2, 60, 3), (1, 1500, 5, 1, 130, 150), (2, 200, 8, 8, 200, 0), (1, 8192, 1, 1, 100, 0), (1, 8193, 1, 1, 100, 0), (1, 1025, 1, 1, 1025, 0)])
+def test_few_rows(B, T, H, G, K, window, sinks):
+    """Longer sequences whose backward visits each tile twice, and the first ones that do not."""
+    run(B, T, H, G, K, window, sinks)
+
+
 @pytest.mark.parametrize("B,T,H,G,window,sinks", [(1, 2048, 2, 1, 2048, 0), (2, 2305, 4, 2, 2048, 130), (1, 2500, 2, 2, 2100, 3), (1, 2177, 3, 1, 5000, 9), (1, 4200, 1, 1, 2050, 600)])
 def test_long_windows(B, T, H, G, window, sinks):
     """Windows of thousands: two tiles of queries a CTA where heads are 128 wide."""
