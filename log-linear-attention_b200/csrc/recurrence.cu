@@ -11,7 +11,7 @@
 // It is bound by memory as long as little else is issued.  Tiles come to shared memory by asynchronous copies a round ahead, each warp its own rows, and are
 // read, and their decays formed, once.  A cluster's barrier costs its CTAs about a microsecond a round, hence runs as long as registers and shared memory
 // leave room for with two CTAs an SM, and clusters no larger than fill the chip.
-// 2 x 16384 tokens of 2048 channels, bf16 with fp32 decays: forward 108 us, backward 195 us, 5.0 and 4.8 TB/s of what they cannot do without.
+// 2 x 16384 tokens of 2048 channels, bf16 with fp32 decays: forward 98 us, backward 188 us behind other calls (107 and 195 with cold caches), 5.5 and 5.0 TB/s of what they cannot do without.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -409,17 +409,20 @@ __global__ void __launch_bounds__(256) recurrence_step_kernel(float* h, const X*
     store(o + i, v);
 }
 
-// How many CTAs share a strip: as many as there are tiles, and as run at once for all strips, since a second wave costs what the first one does.
+// How wide a strip is and how many CTAs share it: what costs the fewest rounds, among clusters that run at once for all strips.
 template <typename KernT>
 struct Launch {
     KernT kern;
     long units;                       // sequences x strips
     int NT;
     size_t smem, summary;             // of a CTA, and more for each CTA of the cluster
+    int LPR;
+    float best;                       // cost
     cudaLaunchAttribute attr[2];
     cudaLaunchConfig_t cfg;
     int ranks;
-    Launch(KernT kern, long units, int NT, size_t smem, size_t summary) : kern(kern), units(units), NT(NT), smem(smem), summary(summary), attr{}, cfg{}, ranks(1) {
+    Launch(KernT kern, long units, int NT, size_t smem, size_t summary, int LPR)
+        : kern(kern), units(units), NT(NT), smem(smem), summary(summary), LPR(LPR), best(INFINITY), attr{}, cfg{}, ranks(1) {
         attr[0].id = cudaLaunchAttributeClusterDimension;
         attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
         attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -451,25 +454,33 @@ struct Launch {
             if (e != cudaSuccess) return e;
             room = Room{dev, reinterpret_cast<const void*>(kern), {}};
         }
-        for (int n = NT < MAX_RANKS ? NT : MAX_RANKS; n > 1; --n) {
+        if (units > 0x7fffffffl) return cudaSuccess;                   // (too narrow)
+        int fastest = 1;
+        best = cost(1);
+        for (int n = 2; n <= NT && n <= MAX_RANKS && units * n <= AT_ONCE; ++n) {
+            if (cost(n) >= best) continue;
             clusters_of(n);
-            if (units * n > 148 * 8) continue;    // (more than could be there)
             if (room.clusters[n] == 0) {
                 e = cudaOccupancyMaxActiveClusters(&room.clusters[n], kern, &cfg);
                 if (e != cudaSuccess) return e;
                 if (room.clusters[n] == 0) room.clusters[n] = -1;
             }
-            if (room.clusters[n] >= units) return cudaSuccess;
+            if (room.clusters[n] < units) continue;
+            best = cost(n);
+            fastest = n;
         }
-        clusters_of(1);
+        clusters_of(fastest);
         return cudaSuccess;
     }
-    // Rounds, weighted with what one takes (us, backward of bf16 with fp32 decays and 64 x 64 values a tile: one CTA a strip 2.4, four 3.5, fourteen 5.4; narrow strips, by
-    // themselves, 3.1), for waves of two CTAs an SM.
-    float cost(int LPR) const {
-        const int rounds = (NT + ranks - 1) / ranks;
-        const long waves = (units * ranks + 2 * 148 - 1) / (2 * 148);
-        return (float)(rounds * waves) * (LPR == 32 ? 1.f : LPR == 16 ? 1.15f : 1.25f) * (1.f + 0.1f * (float)(ranks - 1));
+    // Rounds, and two for the start, weighted with what one takes in this width and with what a cluster's CTAs wait for each other, for waves of two CTAs an SM, or one.  (Fitted to 18 shapes,
+    // 1 to 32 sequences of 100 to 32768 tokens, 64 to 4096 channels, with 1 to 16 CTAs a strip of each width.  Forward and backward in us where few CTAs a strip, or many, are faster: 3 x
+    // 1999 tokens of 1001 channels, fp32, strips of 16 alone 24 / 40, of 32 in clusters of two 26 / 50; 32768 tokens of 2048, bf16, strips of 32 in clusters of four 94 / 206, of 16
+    // alone 103 / 231.  Known to be off: 8192 tokens of 4096, fp32, backward, strips of 16 alone 158, of 32 alone 125.)
+    static constexpr int AT_ONCE = 2 * 148;
+    float cost(int n) const {
+        const long ctas = units * n, rest = ctas % AT_ONCE;
+        const float waves = (float)(ctas / AT_ONCE) + (rest == 0 ? 0.f : rest <= 148 ? 0.95f : 1.f);
+        return (float)((NT + n - 1) / n + 2) * waves * (LPR == 32 ? 1.f : LPR == 16 ? 1.04f : 1.3f) * (n > 1 ? 1.5f + 0.15f * (float)(n - 2) : 1.f);
     }
     cudaError_t go(const Params& p, cudaStream_t st) {
         cfg.stream = st;
@@ -486,8 +497,8 @@ auto launch_of(const Params& p, int B) {
     constexpr int RUN = BACK ? BWD_RUN : FWD_RUN, TILE = WARPS * (32 / LPR) * RUN;
     constexpr size_t SMEM = (size_t)SLOTS * WARPS * ((BACK ? 2 : 1) * Stage<RUN, LPR, X, VEC, CPX>::BYTES + Stage<RUN, LPR, G, VEC, CPG>::BYTES);
     const long units = (long)B * ((p.D + LPR * VEC - 1) / (LPR * VEC));
-    if constexpr (BACK) return Launch<void (*)(Params)>(recurrence_bwd_kernel<X, G, LPR, VEC, CPX, CPG>, units, (p.T + TILE - 1) / TILE, SMEM, LPR * VEC * sizeof(float2));
-    else return Launch<void (*)(Params)>(recurrence_fwd_kernel<X, G, LPR, VEC, CPX, CPG>, units, (p.T + TILE - 1) / TILE, SMEM, LPR * VEC * sizeof(float2));
+    if constexpr (BACK) return Launch<void (*)(Params)>(recurrence_bwd_kernel<X, G, LPR, VEC, CPX, CPG>, units, (p.T + TILE - 1) / TILE, SMEM, LPR * VEC * sizeof(float2), LPR);
+    else return Launch<void (*)(Params)>(recurrence_fwd_kernel<X, G, LPR, VEC, CPX, CPG>, units, (p.T + TILE - 1) / TILE, SMEM, LPR * VEC * sizeof(float2), LPR);
 }
 // Strips as wide as a warp, or a half or a quarter of that with longer tiles: clusters of many CTAs wait longer for each other than narrow strips cost.
 template <bool BACK, typename X, typename G, int VEC, int CPX, int CPG>
@@ -497,8 +508,7 @@ cudaError_t scan_with(Params p, int B, cudaStream_t st) {
     for (int i = 0; i < 3; ++i) {
         const cudaError_t e = l[i].choose();
         if (e != cudaSuccess) return e;
-        if (l[i].cost(32 >> i) < l[best].cost(32 >> best)) best = i;
-        if (l[i].ranks == 1) break;               // (narrower ones would only be slower)
+        if (l[i].best < l[best].best) best = i;
     }
     p.strips = (p.D + (32 >> best) * VEC - 1) / ((32 >> best) * VEC);
     return l[best].go(p, st);
