@@ -409,7 +409,7 @@ __global__ void __launch_bounds__(256) recurrence_step_kernel(float* h, const X*
     store(o + i, v);
 }
 
-// How wide a strip is and how many CTAs share it: what costs the fewest rounds, among clusters that run at once for all strips.
+// How wide a strip is and how many CTAs share it: what costs least, among clusters that run at once for all strips.
 template <typename KernT>
 struct Launch {
     KernT kern;
