@@ -133,6 +133,13 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
+// A value >= 0 as two bf16 terms: its upper half, and what that cuts off, which is rounded.  The lowest bit of the latter is set: it is never 0 where the value is not, so that infinity times
+// the value is infinity in both terms (and rounds to 0 where it is).
+__device__ __forceinline__ uint32_t cut_bf16(float lo, float hi) { return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632); }
+__device__ __forceinline__ float cut_off(float x) {
+    const uint32_t w = __float_as_uint(x);
+    return __uint_as_float(w | 1u) - __uint_as_float(w & 0xffff0000u);
+}
 // A sequence of at most FEW tokens visits each tile twice, the second time with what the rounding of P and dS to bf16 took off: a gradient that is a sum of two or three products has
 // no other roundings for theirs to average with (2 to 5 tokens, one head: dq and dk 2.2e-3 to 3.3e-3 off in the place of 1.7e-3), and such calls are the host's time in any case.
 // (Kernels of their own: the tests cost the others 1 to 3 %.)  Steps are shifted by `twice`, and those of the second visits have the bit.

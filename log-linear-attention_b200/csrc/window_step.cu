@@ -5,10 +5,12 @@
 //     S^T (16 slots x 8 heads) = K Q^T,   O^T (K columns x 8 heads) += V^T P^T.
 // Operands go from memory to the registers that the instructions read, 16 bytes a load: the order of a product's reduction index is free, so a lane takes 8
 // neighbouring columns of k as the indices of two instructions, and 8 neighbouring columns of v as the rows of eight.  No shared memory, no barrier in the loop.
+// P is multiplied in two bf16 terms, exact to 2^-16: one term, 2^-8, left outputs 2.3e-3 off 64 bits, of which 1.7e-3 are their own rounding.  The second instruction costs
+// 2 % of the figures below, 1 to 4 % of other calls.
 //
 // The slots of a (sequence, group) are spread over the warps of a cluster of CTAs, which write their maxima, sums and outputs to the shared memory of the one that joins them:
 // one launch, no workspace, the order of every sum given by the sizes.
-// 64 sequences, 32 heads on 8, K = 128, 2052 slots: 92 us, 5.9 TB/s.  One sequence, 4100 slots: 8.6 us, latency (count, slots,
+// 64 sequences, 32 heads on 8, K = 128, 2052 slots: 93 us, 5.8 TB/s.  One sequence, 4100 slots: 8.8 us, latency (count, slots,
 // a cluster's barrier and two joins one after another).
 #include <cooperative_groups.h>
 
@@ -128,7 +130,7 @@ __global__ void __launch_bounds__(32 * step::Cta<NT>::WARPS, 2) window_step_kern
                     const int s = s0 + 2 * c + (u & 1) + 8 * (u >> 1);
                     vw[i][u] = slot_words(vb + s * ld + 64 * i + 8 * r, s < held);
                 }
-            uint32_t pf[NT][2];
+            uint32_t pf[NT][2], pl[NT][2];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 float d[4] = {0.f, 0.f, 0.f, 0.f};
@@ -158,8 +160,11 @@ __global__ void __launch_bounds__(32 * step::Cta<NT>::WARPS, 2) window_step_kern
                         acc[n][i][2 + u] *= f;
                     }
                 }
-                pf[n][0] = transposed(pack_bf16(d[0], d[1]));
-                pf[n][1] = transposed(pack_bf16(d[2], d[3]));
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    pf[n][u] = transposed(cut_bf16(d[2 * u], d[2 * u + 1]));
+                    pl[n][u] = transposed(pack_bf16(cut_off(d[2 * u]), cut_off(d[2 * u + 1])));
+                }
             }
             // rows of a tile: columns 64 i + 8 r + 2 t (d0, d1) and the one behind it (d2, d3)
 #pragma unroll
@@ -172,7 +177,10 @@ __global__ void __launch_bounds__(32 * step::Cta<NT>::WARPS, 2) window_step_kern
                     const uint32_t w3 = t == 0 ? vw[i][3].x : t == 1 ? vw[i][3].y : t == 2 ? vw[i][3].z : vw[i][3].w;
                     const uint32_t a0 = __byte_perm(w0, w1, 0x5410), a1 = __byte_perm(w0, w1, 0x7632), a2 = __byte_perm(w2, w3, 0x5410), a3 = __byte_perm(w2, w3, 0x7632);
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) mma(acc[n][4 * i + t], a0, a1, a2, a3, pf[n][0], pf[n][1]);
+                    for (int n = 0; n < NT; ++n) {
+                        mma(acc[n][4 * i + t], a0, a1, a2, a3, pf[n][0], pf[n][1]);
+                        mma(acc[n][4 * i + t], a0, a1, a2, a3, pl[n][0], pl[n][1]);
+                    }
                 }
         }
         // the warps' parts, joined in the CTA, then in the cluster

@@ -1,0 +1,54 @@
+"""What rounding leaves of the hybrid-stack operators' outputs, in norm: elementwise bounds that add up worst cases over long sums cannot tell a rounding too many from none."""
+import math
+
+import pytest
+import torch
+
+from oracle import hybrid_oracle as orc
+
+pytestmark = pytest.mark.gpu
+BF = torch.bfloat16
+
+
+def rel(got, ref):
+    return ((got.double() - ref).norm() / ref.norm()).item()
+
+
+# ------------------------------------------------------------------------------------------ steps of the windowed attention
+def step_case(K, B, H, G, slots, seed=0):
+    from hattention_b200 import WindowState
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    r = lambda *s: torch.randn(s, device="cuda", generator=gen).to(BF)
+    state = WindowState(r(B, slots, G, K), r(B, slots, G, K), torch.full((B, G), slots - 1, dtype=torch.int64, device="cuda"), slots, 0)
+    return state, r(B, H, K), r(B, G, K), r(B, G, K)
+
+
+@pytest.mark.parametrize("K", [64, 128])
+@pytest.mark.parametrize("H,G,slots", [(8, 2, 1), (8, 2, 5), (12, 1, 20), (8, 8, 40), (34, 2, 33)])
+def test_steps_lose_no_more_than_their_outputs_rounding(K, H, G, slots):
+    """Outputs are sum P v (1 + e) rounded to bf16.  e: P in two bf16 terms, 2^-16; scores of 128 products that sum to at most 45 in magnitude, each addition within 2^-23 of that, times the
+    scale: 128 * 45 * 2^-23 * 2^-3.5 < 2^-14, in P and once more in its sum.  In norm they are off by at most the rounding of the exact values and e of the magnitudes."""
+    from hattention_b200 import sliding_window_step
+    state, q, k, v = step_case(K, 64, H, G, slots)
+    o, state = sliding_window_step(state, q, k, v)
+    rep = lambda x: x.double().repeat_interleave(H // G, 2)
+    P = (torch.einsum("bhk,bshk->bhs", q.double(), rep(state.k)) / math.sqrt(K)).softmax(-1)
+    ref, mag = torch.einsum("bhs,bshk->bhk", P, rep(state.v)), torch.einsum("bhs,bshk->bhk", P, rep(state.v).abs())
+    assert (o.double() - ref).norm() <= (ref.to(BF).double() - ref).norm() + (2.0 ** -16 + 2 * 2.0 ** -14) * mag.norm()
+
+
+@pytest.mark.parametrize("K", [64, 128])
+@pytest.mark.parametrize("at", [0, 17, 39])
+def test_values_of_infinity_stay_infinite_in_a_step(K, at):
+    """Weights are positive: a row that sees an infinite value is infinite in that column, and as it was in the others."""
+    from hattention_b200 import sliding_window_step
+    (a, q, k, v), (b, *_) = step_case(K, 3, 8, 2, 40), step_case(K, 3, 8, 2, 40)
+    b.v[:, at, :, 5], b.v[:, at, :, 6] = math.inf, -math.inf
+    v2 = v.clone()
+    if at == 39:
+        v2[..., 5], v2[..., 6] = math.inf, -math.inf
+    clean, _ = sliding_window_step(a, q, k, v)
+    o, _ = sliding_window_step(b, q, k, v2)
+    assert (o[..., 5] == math.inf).all() and (o[..., 6] == -math.inf).all()
+    keep = [c for c in range(K) if c not in (5, 6)]
+    assert torch.equal(o[..., keep], clean[..., keep])
