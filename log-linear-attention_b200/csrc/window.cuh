@@ -140,10 +140,11 @@ __device__ __forceinline__ float cut_off(float x) {
     const uint32_t w = __float_as_uint(x);
     return __uint_as_float(w | 1u) - __uint_as_float(w & 0xffff0000u);
 }
-// A sequence of at most FEW tokens visits each tile twice, the second time with what the rounding of P and dS to bf16 took off: a gradient that is a sum of two or three products has
-// no other roundings for theirs to average with (2 to 5 tokens, one head: dq and dk 2.2e-3 to 3.3e-3 off in the place of 1.7e-3), and such calls are the host's time in any case.
-// (Kernels of their own: the tests cost the others 1 to 3 %.)  Steps are shifted by `twice`, and those of the second visits have the bit.
-inline bool visits_twice(int T) { return T <= FEW; }
+// A sequence of at most FEW tokens is computed without the rounding of P and dS: an output or a gradient that is a sum of two or three products has no other roundings for theirs to average with
+// (2 to 5 tokens, one head: dq and dk 2.2e-3 to 3.3e-3 off in the place of 1.7e-3), and such calls are the host's time in any case.  The forward multiplies P in two terms; the backward
+// visits each tile twice, the second time with what rounding took off.  (Kernels of their own: the tests cost the others 1 to 3 %.)  Steps are shifted by `twice`, and those of the second visits
+// have the bit.
+inline bool few_tokens(int T) { return T <= FEW; }
 template <int N>
 __device__ __forceinline__ void leave_rest(float (&e)[N]) {
 #pragma unroll

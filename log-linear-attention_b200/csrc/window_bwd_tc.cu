@@ -606,7 +606,7 @@ cudaError_t backward_tc(const Params& p, int K, cudaStream_t st) {
     // (And few rows in all, for the same reason: 65 to 500 tokens of two heads were 1.45 to 1.6 times as far off as rounding the results alone makes them, and are 1.03 to 1.2.  Up to
     // 2^20 pairs of tokens, where both visits take 20 to 40 us in the place of 15 to 25, the call is the host's 71 us in any case.)
     const long rows = (long)p.B * p.H * p.T;
-    if (visits_twice(p.T) || (rows <= 8192 && rows * (p.window < p.T ? p.window : p.T) <= 1 << 20)) return K == 64 ? launch<64, true>(p, st) : launch<128, true>(p, st);
+    if (few_tokens(p.T) || (rows <= 8192 && rows * (p.window < p.T ? p.window : p.T) <= 1 << 20)) return K == 64 ? launch<64, true>(p, st) : launch<128, true>(p, st);
     return K == 64 ? launch<64, false>(p, st) : launch<128, false>(p, st);
 }
 

@@ -12,6 +12,9 @@
 // It is bound by the chain S, softmax, P V of a tile of queries, of which an SM has two in flight: about 3500 cycles a pair of tiles for 2048 of products (T = 16384, 32 query heads
 // on 8, K = 128, window 2048: 563 us, 0.92 PFLOP/s of products that are not masked).  Two threads a row in the softmax were slower, 618 us for 572: the rows' maxima then
 // go through shared memory.
+// P is rounded to bf16, half a step 2^-8: outputs end 2.3e-3 off 64 bits, of which 1.7e-3 are their own rounding.  Two bf16 terms, the second in the other half of S's place, end at
+// 1.7e-3, for a second product and eight more instructions a pair of scores (us, one term / two: T = 16384, window 2048, K = 128 507 / 691; 2 x 1999, window 512, K = 64 34 / 47; 4 x 1000,
+// window 512, K = 128 39 / 51): TERMS, for sequences of at most FEW tokens alone.
 // A wait that gives up sets the CTA's abort flag, after which every other wait ends at once, and the workspace's status word.
 #include <type_traits>
 
@@ -60,7 +63,7 @@ struct Seen {
 };
 }  // namespace fwd
 
-template <int K, int X, bool TWICE>
+template <int K, int X, bool TERMS>
 __global__ void __launch_bounds__(fwd::Cta<K, X>::THREADS, fwd::Cta<K, X>::PER_SM) window_fwd_tc_kernel(const __grid_constant__ Params p) {
     chain_wait();
     clear_status(p);
@@ -80,12 +83,11 @@ __global__ void __launch_bounds__(fwd::Cta<K, X>::THREADS, fwd::Cta<K, X>::PER_S
     const unsigned units = p.B * p.H, unit = blockIdx.x % units;
     const int h = unit % p.H, q0 = (gridDim.x / units - 1 - blockIdx.x / units) * X * TILE, b = unit / p.H, grp = h / (p.H / p.G);
     const Seen<X> w(p, q0);
-    constexpr int twice = TWICE;
-    const int count = w.count << twice;
+    const int count = w.count;
     // position n of the ring's sequence: K, V of the first tile, K, V of the second, ...
     const auto bring = [&](int n) {
         tma::expect_tx(full + n % NST, SM::TILE_BYTES);
-        load_tile<K>(smem + SM::st_off + n % NST * SM::TILE_BYTES, n & 1 ? &p.tv : &p.tk, grp, w.tile(n >> 1 >> twice) * TILE, b, full + n % NST);
+        load_tile<K>(smem + SM::st_off + n % NST * SM::TILE_BYTES, n & 1 ? &p.tv : &p.tk, grp, w.tile(n >> 1) * TILE, b, full + n % NST);
     };
     if (tid == TMA_WARP * 32) {              // (the thread that brings the tiles need not wait for the others)
         for (int i = 0; i < NST; ++i) {
@@ -149,14 +151,15 @@ __global__ void __launch_bounds__(fwd::Cta<K, X>::THREADS, fwd::Cta<K, X>::PER_S
                             ok = ok && umma::mbar_wait_warp(barP + 2 * x + half, done[x] & 1, abort_flag);
                             if (!ok) break;
                             umma::fence_after_sync();
-                            umma::gemm_tm_lead<TILE, 64>(lead, tmem + TM_O + 128 * x, tmem + TM_S + 128 * x + 32 * half,
-                                                         sS + (nv % NST) * SM::TILE_BYTES + half * 64 * umma::ROW_BYTES, idO, done[x] > 0 || half > 0);
+                            const uint32_t sV = sS + (nv % NST) * SM::TILE_BYTES + half * 64 * umma::ROW_BYTES;
+                            umma::gemm_tm_lead<TILE, 64>(lead, tmem + TM_O + 128 * x, tmem + TM_S + 128 * x + 32 * half, sV, idO, done[x] > 0 || half > 0);
+                            if (TERMS) umma::gemm_tm_lead<TILE, 64>(lead, tmem + TM_O + 128 * x, tmem + TM_S + 128 * x + 64 + 32 * half, sV, idO, true);
                         }
                         if (!ok) break;
                         umma::commit_lead(lead, barO + x);
                         ++done[x];
                     }
-                    before[x] = i < count && w.in(x, w.tile(i >> twice));
+                    before[x] = i < count && w.in(x, w.tile(i));
                     if (before[x]) {
                         ok = umma::mbar_wait_warp(barQ + x, 0, abort_flag);
                         if (!ok) break;
@@ -179,11 +182,11 @@ __global__ void __launch_bounds__(fwd::Cta<K, X>::THREADS, fwd::Cta<K, X>::PER_S
         const float c = p.scale * LOG2E;
         const F2 c2 = pair(c, c);
         const Span span(t0, p.T, p.window, p.sinks);
-        const int n = span.count() << twice;
+        const int n = span.count();
         float m = -INFINITY, sum = 0.f;
         bool ok = true;
         for (int i = 0; i < n; ++i) {
-            const int s0 = span.tile(i >> twice) * TILE;
+            const int s0 = span.tile(i) * TILE;
             const bool whole = all_seen(t0, s0, p.window, p.sinks);
             ok = umma::mbar_wait_warp(barS + x, i & 1, abort_flag);
             if (!ok) break;
@@ -233,10 +236,10 @@ __global__ void __launch_bounds__(fwd::Cta<K, X>::THREADS, fwd::Cta<K, X>::PER_S
             F2 part[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-                const auto exponentials = [&](auto mixed, auto rest) {
+                const auto exponentials = [&](auto mixed) {
 #pragma unroll
                     for (int k = 0; k < 64; k += 32) {
-                        uint32_t w[16];
+                        uint32_t w[16], rest[16];
 #pragma unroll
                         for (int u = 0; u < 16; ++u) {
                             const F2 y = fma2(pair(s[half][k + 2 * u], s[half][k + 2 * u + 1]), c2, shift);
@@ -247,17 +250,17 @@ __global__ void __launch_bounds__(fwd::Cta<K, X>::THREADS, fwd::Cta<K, X>::PER_S
                                 const float2 v = both(y);
                                 e = make_float2(exp2_fast(v.x), exp2_fast(v.y));
                             }
-                            w[u] = pack_bf16(e.x, e.y);
-                            if (decltype(rest)::value) w[u] = pack_bf16(e.x - __uint_as_float(w[u] << 16), e.y - __uint_as_float(w[u] & 0xffff0000u));
-                            else part[u & 1] = add(part[u & 1], pair(e.x, e.y));
+                            w[u] = TERMS ? cut_bf16(e.x, e.y) : pack_bf16(e.x, e.y);
+                            if (TERMS) rest[u] = pack_bf16(cut_off(e.x), cut_off(e.y));
+                            part[u & 1] = add(part[u & 1], pair(e.x, e.y));
                         }
                         umma::tmem_st16u(tS + 32 * half + k / 2, w);
+                        if (TERMS) umma::tmem_st16u(tS + 64 + 32 * half + k / 2, rest);
                     }
                 };
                 // (hidden keys are exact zeros: the special-function unit's)
-                if (whole) exponentials(std::true_type{}, std::false_type{});
-                else if (i & twice) exponentials(std::false_type{}, std::true_type{});
-                else exponentials(std::false_type{}, std::false_type{});
+                if (whole) exponentials(std::true_type{});
+                else exponentials(std::false_type{});
                 umma::tmem_wait_st();
                 umma::fence_before_sync();
                 __syncwarp();
@@ -315,10 +318,10 @@ __global__ void __launch_bounds__(fwd::Cta<K, X>::THREADS, fwd::Cta<K, X>::PER_S
     }
 }
 
-template <int K, int X, bool TWICE>
+template <int K, int X, bool TERMS>
 static cudaError_t launch(const Params& p, cudaStream_t st) {
     using C = fwd::Cta<K, X>;
-    const auto kern = window_fwd_tc_kernel<K, X, TWICE>;
+    const auto kern = window_fwd_tc_kernel<K, X, TERMS>;
     cudaError_t e = allow_smem(kern, C::total);
     if (e != cudaSuccess) return e;
     const unsigned grid = (unsigned)(p.T + X * TILE - 1) / (X * TILE) * p.H * p.B;
@@ -330,7 +333,7 @@ static cudaError_t launch(const Params& p, cudaStream_t st) {
 // one tile / two: K = 128, 32 heads on 8, window 512, 8192 tokens 119 / 128; window 1024 164 / 169; window 2048, 4096 tokens 110 / 109, 8192 tokens 249 / 239; 8192 tokens, all that are
 // before 482 / 439; K = 64, 16 heads, 2 x 1999 tokens, window 512 25.4 / 31.2; 8 heads on 2, 32768 tokens, window 4096 417 / 440; 32 heads on 8, 8192 tokens, all before 469 / 455).
 cudaError_t forward_tc(const Params& p, int K, cudaStream_t st) {
-    if (visits_twice(p.T)) return K == 64 ? launch<64, 1, true>(p, st) : launch<128, 1, true>(p, st);
+    if (few_tokens(p.T)) return K == 64 ? launch<64, 1, true>(p, st) : launch<128, 1, true>(p, st);
     if (K == 64) return launch<64, 1, false>(p, st);
     return p.T >= 2048 && p.window >= 2048 ? launch<128, 2, false>(p, st) : launch<128, 1, false>(p, st);
 }

@@ -52,3 +52,22 @@ def test_values_of_infinity_stay_infinite_in_a_step(K, at):
     assert (o[..., 5] == math.inf).all() and (o[..., 6] == -math.inf).all()
     keep = [c for c in range(K) if c not in (5, 6)]
     assert torch.equal(o[..., keep], clean[..., keep])
+
+
+# ------------------------------------------------------------------------------------------ the windowed attention
+@pytest.mark.parametrize("K", [64, 128])
+@pytest.mark.parametrize("T,window", [(2, 2), (30, 12), (64, 64), (65, 40), (300, 64), (2100, 2048)])
+def test_values_of_infinity_stay_infinite(T, window, K):
+    """A row that sees an infinite value is infinite in that column (its weight there is at least 2^-25: scores within +-6 of each other, of at most 2048), and as it was in the others."""
+    from hattention_b200 import sliding_window_attention
+    gen = torch.Generator(device="cuda").manual_seed(T)
+    q, k, v = (torch.randn(1, T, n, K, device="cuda", generator=gen).to(BF).clamp(-1, 1) for n in (2, 1, 1))
+    clean = sliding_window_attention(q, k, v, window)
+    for s in {0, T // 2, T - 1}:
+        w = v.clone()
+        w[0, s, 0, 5], w[0, s, 0, 6] = math.inf, -math.inf
+        o = sliding_window_attention(q, k, w, window)
+        rows = orc.seen(T, window, 0, "cuda")[:, s]
+        assert (o[0, rows][..., 5] == math.inf).all() and (o[0, rows][..., 6] == -math.inf).all(), s
+        keep = [c for c in range(K) if c not in (5, 6)]
+        assert torch.equal(o[..., keep], clean[..., keep])
