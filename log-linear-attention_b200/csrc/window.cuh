@@ -184,6 +184,15 @@ __device__ __forceinline__ void arrive(uint64_t* bar) {
 __device__ __forceinline__ void clear_status(const Params& p) {
     if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *p.err = 0;
 }
+// The issuing warp, after a wait that gave up: the first tiles' copy, whose barrier `bar` is, and all products have ended; the status word says so.
+__device__ __forceinline__ void end_products(uint64_t* bar, int* err, int lane) {
+    umma::mbar_wait(bar, 0);
+    __syncwarp();
+    umma::commit_lead(umma::elect_one(), bar);
+    umma::mbar_wait(bar, 1);
+    if (lane == 0) atomicExch(err, 1);
+    __syncwarp();
+}
 // The way of a warp's 32 rows, a thread a row, to global memory: through 32 WORDS 16-byte words of shared memory, so that neighbouring lanes store neighbouring words of a row.  (Straight
 // from the threads, 32 bytes of a row each: 159 us for 156 in the forward of 4 x 4096 tokens, 36.9 for 35.7 in the backward of 8 x 256.)
 template <int WORDS>

@@ -60,7 +60,7 @@ struct Ring {
             umma::mbar_init(empty + i, 1);
         }
     }
-    // after a wait that gave up: the copies in flight end before the CTA does
+    // the copies in flight of `issued` tiles have ended
     __device__ __forceinline__ void drain(int issued) const {
         for (int i = issued > N ? issued - N : 0; i < issued; ++i) umma::mbar_wait(filled(i), phase(i));
     }
@@ -178,11 +178,11 @@ __global__ void __launch_bounds__(bwd::Cta<K>::THREADS, bwd::Cta<K>::PER_SM) win
     __syncthreads();
     umma::fence_after_sync();
     const uint32_t tmem = *tmem_slot;
+    int nk = 0, nv = 0;                      // tiles brought (by the thread that does)
 
     if (warp >= WARPS) {
         SM::regs_issue();
         if (warp == TMA_WARP && lane == 0) {
-            int nk = 0, nv = 0;
             while (nv < steps) {
                 if (!ringK.wait_free(nk, abort_flag)) break;
                 tma::expect_tx(ringK.filled(nk), SM::TILE_BYTES);
@@ -192,11 +192,6 @@ __global__ void __launch_bounds__(bwd::Cta<K>::THREADS, bwd::Cta<K>::PER_SM) win
                 tma::expect_tx(ringV.filled(nv), SM::TILE_BYTES);
                 load_tile<K>(smem + SM::b_off + nv % NB * SM::TILE_BYTES, &p.tv, grp, tile(nv) * TILE, b, ringV.filled(nv));
                 ++nv;
-            }
-            if (*abort_flag) {
-                umma::mbar_wait(barQ, 0);
-                ringK.drain(nk);
-                ringV.drain(nv);
             }
         } else if (warp == MMA_WARP) {
             const uint32_t lead = umma::elect_one(), sQ = umma::smem_addr(smem + SM::stay_off), sDO = sQ + SM::TILE_BYTES;
@@ -326,15 +321,15 @@ __global__ void __launch_bounds__(bwd::Cta<K>::THREADS, bwd::Cta<K>::PER_SM) win
     }
     __syncthreads();
     umma::fence_after_sync();
-    if (warp == MMA_WARP) {
-        // products that nobody waited for, after a wait that gave up, end before their memory is handed back
-        if (*abort_flag) {
-            umma::commit_lead(umma::elect_one(), barQ);
-            umma::mbar_wait(barQ, 1);
-            if (lane == 0) atomicExch(p.err, 1);
+    // after a wait that gave up (none can from here on): copies and products that nobody waited for end before the CTA does
+    if (*abort_flag) {
+        if (tid == TMA_WARP * 32) {
+            ringK.drain(nk);
+            ringV.drain(nv);
         }
-        umma::tmem_dealloc(tmem, SM::TM);
+        if (warp == MMA_WARP) end_products(barQ, p.err, lane);
     }
+    if (warp == MMA_WARP) umma::tmem_dealloc(tmem, SM::TM);
 }
 
 template <int K, bool TWICE>
@@ -385,11 +380,12 @@ __global__ void __launch_bounds__(bwd::Cta<K>::THREADS, bwd::Cta<K>::PER_SM) win
     __syncthreads();
     umma::fence_after_sync();
     const uint32_t tmem = *tmem_slot;
+    int nq = 0, nd = 0;                      // tiles brought (by the thread that does)
 
     if (warp >= WARPS) {
         SM::regs_issue();
         if (warp == TMA_WARP && lane == 0) {
-            int nq = 0, nd = 0, h = h0, i = lo;
+            int h = h0, i = lo;
             while (nd < steps) {
                 const long stat = ((long)b * p.H + h) * p.TP + i * TILE;
                 if (!ringQ.wait_free(nq, abort_flag)) break;
@@ -406,11 +402,6 @@ __global__ void __launch_bounds__(bwd::Cta<K>::THREADS, bwd::Cta<K>::PER_SM) win
                     i = lo;
                     ++h;
                 }
-            }
-            if (*abort_flag) {
-                umma::mbar_wait(barKV, 0);
-                ringQ.drain(nq);
-                ringDO.drain(nd);
             }
         } else if (warp == MMA_WARP) {
             const uint32_t lead = umma::elect_one(), sK = umma::smem_addr(smem + SM::stay_off), sV = sK + SM::TILE_BYTES;
@@ -532,14 +523,14 @@ __global__ void __launch_bounds__(bwd::Cta<K>::THREADS, bwd::Cta<K>::PER_SM) win
     }
     __syncthreads();
     umma::fence_after_sync();
-    if (warp == MMA_WARP) {
-        if (*abort_flag) {
-            umma::commit_lead(umma::elect_one(), barKV);
-            umma::mbar_wait(barKV, 1);
-            if (lane == 0) atomicExch(p.err, 1);
+    if (*abort_flag) {
+        if (tid == TMA_WARP * 32) {
+            ringQ.drain(nq);
+            ringDO.drain(nd);
         }
-        umma::tmem_dealloc(tmem, SM::TM);
+        if (warp == MMA_WARP) end_products(barKV, p.err, lane);
     }
+    if (warp == MMA_WARP) umma::tmem_dealloc(tmem, SM::TM);
 }
 
 // Adds up the parts: a warp a token and group.  The tokens with parts are all of them, or the sinks among the first tiles.

@@ -117,20 +117,14 @@ __global__ void __launch_bounds__(fwd::Cta<K, X>::THREADS, fwd::Cta<K, X>::PER_S
     __syncthreads();
     umma::fence_after_sync();
     const uint32_t tmem = *tmem_slot;
+    int brought = 1;                         // (by the thread that brings the tiles)
 
     if (warp >= MMA_WARP) {
         SM::regs_issue();
         if (warp == TMA_WARP && lane == 0) {
-            int n = 1;
-            for (; n < 2 * count; ++n) {
-                if (n >= NST && !umma::mbar_wait(empty + n % NST, (n / NST - 1) & 1, abort_flag)) break;
-                bring(n);
-            }
-            // nobody may be left to wait for the last copies after a wait that gave up: they end before the CTA does
-            if (*abort_flag) {
-                umma::mbar_wait(barQ, 0);
-                if (X == 2 && q0 + TILE < p.T) umma::mbar_wait(barQ + 1, 0);
-                for (int i = n > NST ? n - NST : 0; i < n; ++i) umma::mbar_wait(full + i % NST, (i / NST) & 1);
+            for (; brought < 2 * count; ++brought) {
+                if (brought >= NST && !umma::mbar_wait(empty + brought % NST, (brought / NST - 1) & 1, abort_flag)) break;
+                bring(brought);
             }
         } else if (warp == MMA_WARP) {
             const uint32_t lead = umma::elect_one(), sQ = umma::smem_addr(smem + SM::q_off), sS = umma::smem_addr(smem + SM::st_off);
@@ -171,8 +165,9 @@ __global__ void __launch_bounds__(fwd::Cta<K, X>::THREADS, fwd::Cta<K, X>::PER_S
                     }
                 }
                 if (!ok) break;
+                if (i == count) break;                  // (the last commit is one that the rows wait for: none arrives at a CTA that is gone)
                 if (i > 0) umma::commit_lead(lead, empty + nv % NST);
-                if (i < count) umma::commit_lead(lead, empty + nk % NST);
+                umma::commit_lead(lead, empty + nk % NST);
             }
         }
     } else {
@@ -306,16 +301,15 @@ __global__ void __launch_bounds__(fwd::Cta<K, X>::THREADS, fwd::Cta<K, X>::PER_S
     }
     __syncthreads();
     umma::fence_after_sync();
-    if (warp == MMA_WARP) {
-        // products that nobody waited for, after a wait that gave up, end before their memory is handed back
-        if (*abort_flag) {
-            const uint32_t lead = umma::elect_one();
-            umma::commit_lead(lead, barQ);
-            umma::mbar_wait(barQ, 1);
-            if (lane == 0) atomicExch(p.err, 1);
+    // after a wait that gave up (none can from here on): copies and products that nobody waited for end before the CTA does
+    if (*abort_flag) {
+        if (tid == TMA_WARP * 32) {
+            if (X == 2 && q0 + TILE < p.T) umma::mbar_wait(barQ + 1, 0);
+            for (int i = brought > NST ? brought - NST : 0; i < brought; ++i) umma::mbar_wait(full + i % NST, (i / NST) & 1);
         }
-        umma::tmem_dealloc(tmem, SM::TM);
+        if (warp == MMA_WARP) end_products(barQ, p.err, lane);
     }
+    if (warp == MMA_WARP) umma::tmem_dealloc(tmem, SM::TM);
 }
 
 template <int K, int X, bool TERMS>

@@ -1,0 +1,50 @@
+"""Properties of the hybrid-stack kernels that no run on a sound GPU shows, held by reading their sources."""
+import os
+import re
+
+import pytest
+
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "log-linear-attention_b200", "csrc")
+
+
+def kernels(name):
+    """{kernel: its body without comments} of a source file."""
+    with open(os.path.join(CSRC, name)) as f:
+        text = re.sub(r"//[^\n]*", "", f.read())
+    found = {}
+    for m in re.finditer(r"__global__[^;{]*?\b(\w+_kernel)\(", text):
+        at = text.index("{", m.end())
+        depth, end = 0, at
+        while True:
+            depth += {"{": 1, "}": -1}.get(text[end], 0)
+            end += 1
+            if depth == 0:
+                break
+        found[m.group(1)] = text[at:end]
+    return found
+
+
+WINDOW = [("window_fwd_tc.cu", "window_fwd_tc_kernel"), ("window_bwd_tc.cu", "window_dq_tc_kernel"), ("window_bwd_tc.cu", "window_dkv_tc_kernel")]
+
+
+@pytest.mark.parametrize("file,kernel", WINDOW)
+def test_copies_and_products_end_before_the_cta_after_a_wait_that_gave_up(file, kernel):
+    """Any thread may give up until the CTA's last barrier.  Only behind it is the abort flag final: there, and not in front of it, the copies that were issued and the products are waited for.  (In front of it
+    the thread that issues them may look before another gives up, and the next CTA's shared memory would be written to.)"""
+    body = kernels(file)[kernel]
+    last = body.rindex("__syncthreads();")
+    before, behind = body[:last], body[last:]
+    assert not re.search(r"if \(\*abort_flag\)", before), "a decision on a flag that may still be set"
+    assert re.search(r"if \(\*abort_flag\)", behind) and "end_products(" in behind
+    assert len(re.findall(r"\.drain\(|mbar_wait\(full", behind)) >= (1 if "fwd" in kernel else 2)
+
+
+@pytest.mark.parametrize("file,kernel", WINDOW)
+def test_the_last_arrival_of_products_is_waited_for(file, kernel):
+    """An arrival that nobody waits for may come when the CTA's shared memory is another's: the issuing warp's last commit is one that the rows wait for."""
+    body = kernels(file)[kernel]
+    issue = body[body.index("warp == MMA_WARP) {\n            const uint32_t lead"):body.index("SM::regs_rows()")]
+    if "fwd" in kernel:                                  # (commits in a loop, whose last round ends with those for the rows)
+        assert "if (i == count) break;" in issue[issue.index("commit_lead(lead, barS"):issue.index("commit_lead(lead, empty")]
+    else:
+        assert re.findall(r"commit_lead\(lead, (\w+)", issue)[-1] == "barDone"
