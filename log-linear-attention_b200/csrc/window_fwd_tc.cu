@@ -117,15 +117,16 @@ __global__ void __launch_bounds__(fwd::Cta<K, X>::THREADS, fwd::Cta<K, X>::PER_S
     __syncthreads();
     umma::fence_after_sync();
     const uint32_t tmem = *tmem_slot;
-    int brought = 1;                         // (by the thread that brings the tiles)
 
     if (warp >= MMA_WARP) {
         SM::regs_issue();
         if (warp == TMA_WARP && lane == 0) {
-            for (; brought < 2 * count; ++brought) {
-                if (brought >= NST && !umma::mbar_wait(empty + brought % NST, (brought / NST - 1) & 1, abort_flag)) break;
-                bring(brought);
+            int n = 1;
+            for (; n < 2 * count; ++n) {
+                if (n >= NST && !umma::mbar_wait(empty + n % NST, (n / NST - 1) & 1, abort_flag)) break;
+                bring(n);
             }
+            abort_flag[1] = n;                          // (tiles brought; a register would cost the others 1 %)
         } else if (warp == MMA_WARP) {
             const uint32_t lead = umma::elect_one(), sQ = umma::smem_addr(smem + SM::q_off), sS = umma::smem_addr(smem + SM::st_off);
             constexpr uint32_t idS = umma::idesc_bf16(128, 128, false, false), idO = umma::idesc_bf16(128, K, false, true);
@@ -165,9 +166,9 @@ __global__ void __launch_bounds__(fwd::Cta<K, X>::THREADS, fwd::Cta<K, X>::PER_S
                     }
                 }
                 if (!ok) break;
-                if (i == count) break;                  // (the last commit is one that the rows wait for: none arrives at a CTA that is gone)
-                if (i > 0) umma::commit_lead(lead, empty + nv % NST);
-                umma::commit_lead(lead, empty + nk % NST);
+                // (not in the last round: the last commit is one that the rows wait for, so that none arrives at a CTA that is gone)
+                if (i > 0 && i < count) umma::commit_lead(lead, empty + nv % NST);
+                if (i < count) umma::commit_lead(lead, empty + nk % NST);
             }
         }
     } else {
@@ -305,6 +306,7 @@ __global__ void __launch_bounds__(fwd::Cta<K, X>::THREADS, fwd::Cta<K, X>::PER_S
     if (*abort_flag) {
         if (tid == TMA_WARP * 32) {
             if (X == 2 && q0 + TILE < p.T) umma::mbar_wait(barQ + 1, 0);
+            const int brought = abort_flag[1];
             for (int i = brought > NST ? brought - NST : 0; i < brought; ++i) umma::mbar_wait(full + i % NST, (i / NST) & 1);
         }
         if (warp == MMA_WARP) end_products(barQ, p.err, lane);

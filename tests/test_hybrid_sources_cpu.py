@@ -44,7 +44,7 @@ def test_the_last_arrival_of_products_is_waited_for(file, kernel):
     """An arrival that nobody waits for may come when the CTA's shared memory is another's: the issuing warp's last commit is one that the rows wait for."""
     body = kernels(file)[kernel]
     issue = body[body.index("warp == MMA_WARP) {\n            const uint32_t lead"):body.index("SM::regs_rows()")]
-    if "fwd" in kernel:                                  # (commits in a loop, whose last round ends with those for the rows)
-        assert "if (i == count) break;" in issue[issue.index("commit_lead(lead, barS"):issue.index("commit_lead(lead, empty")]
+    if "fwd" in kernel:                                  # (commits in a loop, whose last round has those for the rows alone)
+        assert re.findall(r"(.*)commit_lead\(lead, empty", issue) == ["                if (i > 0 && i < count) umma::", "                if (i < count) umma::"]
     else:
         assert re.findall(r"commit_lead\(lead, (\w+)", issue)[-1] == "barDone"
