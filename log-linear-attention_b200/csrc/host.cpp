@@ -814,8 +814,14 @@ py::object gdn_step(const Tensor& states, const py::list& counts, const Tensor& 
 // ------------------------------------------------------------------------------------------ gated linear recurrence
 // x and g of one of the type pairs that the kernels take: g in fp32, or in x's type
 inline bool row_types(const Tensor& x, const Tensor& g) { return (bf16(x) && (bf16(g) || is(g, at::kFloat))) || (is(x, at::kFloat) && is(g, at::kFloat)); }
+// every size fits the C ABI's int
+inline bool int_sizes(const Tensor& x) {
+    for (const int64_t n : x.sizes())
+        if (n > 0x7fffffffl) return false;
+    return true;
+}
 bool recurrence_operands(const Tensor& x, const Tensor& g, const Tensor& h0) {
-    return row_types(x, g) && x.dim() == 3 && g.sizes() == x.sizes() && x.numel() > 0 && native_set({x, g, h0}) &&
+    return row_types(x, g) && x.dim() == 3 && g.sizes() == x.sizes() && x.numel() > 0 && int_sizes(x) && native_set({x, g, h0}) &&
            (!h0.defined() || (is(h0, at::kFloat) && h0.sizes() == at::IntArrayRef({x.size(0), x.size(2)})));
 }
 struct Scanned {
@@ -897,7 +903,7 @@ py::object recurrence_backward(const Tensor& x, const Tensor& g, const Tensor& s
 }
 // o (B,D); the state is advanced in place
 py::object gated_recurrence_step(const Tensor& h, const Tensor& x, const Tensor& g) {
-    if (!row_types(x, g) || x.dim() != 2 || g.sizes() != x.sizes() || x.numel() == 0 || !is(h, at::kFloat) || h.sizes() != x.sizes() || !h.is_contiguous() ||
+    if (!row_types(x, g) || x.dim() != 2 || g.sizes() != x.sizes() || x.numel() == 0 || !int_sizes(x) || !is(h, at::kFloat) || h.sizes() != x.sizes() || !h.is_contiguous() ||
         !aligned(h) || !native_set({h, x, g}))
         return py::none();
     at::NoGradGuard no_grad;                     // (a state goes on without a graph)

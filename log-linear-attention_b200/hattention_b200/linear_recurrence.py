@@ -11,6 +11,8 @@ def _check(x: torch.Tensor, g: torch.Tensor, state: Optional[torch.Tensor], ndim
     """Raises for what the kernels do not take."""
     if x.ndim != ndim or g.shape != x.shape:
         raise ValueError(f"x and g have {ndim} dimensions and one shape; got {tuple(x.shape)} and {tuple(g.shape)}")
+    if x.numel() > 0 and max(x.shape) >= 2 ** 31:
+        raise ValueError(f"sizes are below 2^31; got {tuple(x.shape)}")
     if x.dtype not in (torch.bfloat16, torch.float32) or g.dtype not in (x.dtype, torch.float32):
         raise TypeError(f"x is bfloat16 or float32, g of x's type or float32; got {x.dtype} and {g.dtype}")
     if state is not None:
@@ -29,7 +31,7 @@ def gated_recurrence(x: torch.Tensor, g: torch.Tensor, initial_state: Optional[t
 
     x is bf16 or fp32 and o has its type; g has x's type or is fp32; states are (B,D) fp32, an absent one is zeros.  All sums are fp32.
     g <= 0, as log decays are; -inf starts a channel anew at that token, so that packed sequences stay apart.  (Above 0 the products of
-    exp(g) over 512 tokens have to stay finite.)  T and D are any sizes; even D moves two channels a load."""
+    exp(g) over 512 tokens have to stay finite.)  T is any size up to 2^30, D any, B ceil(D / 32) below 2^31; even D moves two channels a load."""
     r = _lib.host().gated_recurrence(x, g, initial_state, output_final_state)
     if r is not None:
         return r

@@ -71,3 +71,12 @@ def test_values_of_infinity_stay_infinite(T, window, K):
         assert (o[0, rows][..., 5] == math.inf).all() and (o[0, rows][..., 6] == -math.inf).all(), s
         keep = [c for c in range(K) if c not in (5, 6)]
         assert torch.equal(o[..., keep], clean[..., keep])
+
+
+# ------------------------------------------------------------------------------------------ sizes
+@pytest.mark.parametrize("shape", [(1, 2 ** 32 + 5, 1), (2 ** 31, 1, 1), (1, 1, 2 ** 32 + 64)])
+def test_recurrence_sizes_that_an_int_does_not_hold(shape):
+    from hattention_b200 import gated_recurrence
+    x = torch.zeros(1, 1, 1, dtype=BF, device="cuda").expand(shape)
+    with pytest.raises(ValueError, match="2\\^31"):
+        gated_recurrence(x, x)

@@ -1,8 +1,9 @@
-"""Properties of the hybrid-stack kernels that no run on a sound GPU shows, held by reading their sources."""
+"""What no run on a GPU shows: properties of the hybrid-stack kernels held by reading their sources, and refusals of sizes that no GPU holds."""
 import os
 import re
 
 import pytest
+import torch
 
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "log-linear-attention_b200", "csrc")
 
@@ -48,3 +49,23 @@ def test_the_last_arrival_of_products_is_waited_for(file, kernel):
         assert re.findall(r"(.*)commit_lead\(lead, empty", issue) == ["                if (i > 0 && i < count) umma::", "                if (i < count) umma::"]
     else:
         assert re.findall(r"commit_lead\(lead, (\w+)", issue)[-1] == "barDone"
+
+
+@pytest.fixture(scope="module")
+def pkg():
+    import __graft_entry__ as ge
+    ge.build()
+    import hattention_b200
+    return hattention_b200
+
+
+@pytest.mark.parametrize("shape", [(1, 2 ** 32 + 5, 1), (2 ** 31, 1, 1), (1, 1, 2 ** 32 + 64)])
+def test_recurrence_sizes_that_an_int_does_not_hold_are_refused(pkg, shape):
+    """(Such a size reached the kernels modulo 2^32, which then left most of the output as it was.)"""
+    x = torch.zeros(1, 1, 1, dtype=torch.bfloat16).expand(shape)
+    with pytest.raises(ValueError, match="2\\^31"):
+        pkg.gated_recurrence(x, x)
+    if shape[1] == 1:
+        x = x[:, 0]
+        with pytest.raises(ValueError, match="2\\^31"):
+            pkg.gated_recurrence_step(torch.zeros(1, 1).expand(x.shape), x, x)
