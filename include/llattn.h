@@ -422,7 +422,7 @@ int llattn_window_fill(const void* k, const void* v, const long long* lengths, v
 int llattn_window_step(const void* q, const void* k, const void* v, void* k_cache, void* v_cache, long long* counts, void* o, int B, int H, int G, int K,
                        int window, int sinks, float scale, void* stream);
 
-/* Layer norm of rows of N values: y = (x - mean) rstd w + b.  x, y, dy, dx (rows,N) bf16 or fp32; w, b, dw, db (N) fp32 (w_is_f32) or, with bf16 x, bf16;
+/* Layer norm of rows of N <= 2^30 values: y = (x - mean) rstd w + b.  x, y, dy, dx (rows,N) bf16 or fp32; w, b, dw, db (N) fp32 (w_is_f32) or, with bf16 x, bf16;
  * w and b may be NULL (ones, zeros).  mean and rstd (rows) fp32 are what the backward reads; NULL in a forward without one.  dw and db may be NULL; with one
  * of them the backward needs a workspace (llattn_layer_norm_bwd_workspace_bytes).  The sums over rows are in an order that the sizes alone decide. */
 size_t llattn_layer_norm_bwd_workspace_bytes(long rows, int N);

@@ -1047,8 +1047,9 @@ py::object sliding_window_step(const Tensor& q, const Tensor& k, const Tensor& v
 }
 
 // ------------------------------------------------------------------------------------------ layer norm
+constexpr int64_t NORM_MAX = int64_t(1) << 30;      // values of a row
 bool norm_operands(const Tensor& x, const Tensor& w, const Tensor& b) {
-    if (!(bf16(x) || is(x, at::kFloat)) || x.dim() < 1 || x.numel() == 0 || x.numel() / x.size(-1) > 0x7fffffffl || x.size(-1) > 0x7fffffffl || !native_set({x, w, b}))
+    if (!(bf16(x) || is(x, at::kFloat)) || x.dim() < 1 || x.numel() == 0 || x.numel() / x.size(-1) > 0x7fffffffl || x.size(-1) > NORM_MAX || !native_set({x, w, b}))
         return false;
     for (const Tensor* p : {&w, &b})
         if (p->defined() && (!row_types(x, *p) || p->sizes() != at::IntArrayRef({x.size(-1)}))) return false;

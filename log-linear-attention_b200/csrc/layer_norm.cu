@@ -573,7 +573,8 @@ cudaError_t backward(Params p, cudaStream_t st) {
     return e;
 }
 int check(int x_f32, int w_f32, long rows, int N) {
-    if (rows < 1 || N < 1 || rows > 0x7fffffffl || (x_f32 && !w_f32)) return LLATTN_ERR_UNSUPPORTED_SHAPE;
+    // (columns are counted in ints, a stride behind the row's end)
+    if (rows < 1 || N < 1 || rows > 0x7fffffffl || N > 1 << 30 || (x_f32 && !w_f32)) return LLATTN_ERR_UNSUPPORTED_SHAPE;
     return 0;
 }
 

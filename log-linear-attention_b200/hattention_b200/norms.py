@@ -8,15 +8,15 @@ from . import _lib
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, eps: float = 1e-5) -> torch.Tensor:
-    """y = (x - mean) / sqrt(var + eps) * weight + bias over the last dimension of x, with gradients for all three.
+    """y = (x - mean) / sqrt(var + eps) * weight + bias over the last dimension of x, with gradients for all three.  Rows have up to 2^30 values.
 
     x is bf16 or fp32 and y has its type; weight and bias (N,) have one type, x's or fp32.  Statistics and the sums over rows of the
     parameters' gradients are fp32, and those sums are taken in an order that the sizes alone decide: the same call gives the same bits."""
     y = _lib.host().layer_norm(x, weight, bias, eps)
     if y is not None:
         return y
-    if x.ndim < 1 or x.shape[-1] < 1:
-        raise ValueError("rows of at least one value")
+    if x.ndim < 1 or x.shape[-1] < 1 or (x.numel() > 0 and x.shape[-1] > 2 ** 30):
+        raise ValueError("rows of at least one value, and at most 2^30")
     if x.dtype not in (torch.bfloat16, torch.float32):
         raise TypeError(f"x is bfloat16 or float32; got {x.dtype}")
     for p in (weight, bias):

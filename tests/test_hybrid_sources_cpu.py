@@ -1,4 +1,5 @@
 """What no run on a GPU shows: properties of the hybrid-stack kernels held by reading their sources, and refusals of sizes that no GPU holds."""
+import ctypes
 import os
 import re
 
@@ -69,3 +70,16 @@ def test_recurrence_sizes_that_an_int_does_not_hold_are_refused(pkg, shape):
         x = x[:, 0]
         with pytest.raises(ValueError, match="2\\^31"):
             pkg.gated_recurrence_step(torch.zeros(1, 1).expand(x.shape), x, x)
+
+
+def test_rows_whose_columns_an_int_does_not_count_are_refused(pkg):
+    """The kernels for long rows count columns in ints, a stride of up to 256 past the end: rows of nearly 2^31 values would be read in front of their start."""
+    from hattention_b200 import _lib
+    lib, ok, null = _lib.lib(), ctypes.c_void_p(4096), ctypes.c_void_p(0)
+    for N in (2 ** 30 + 1, 2 ** 31 - 1):
+        assert lib.llattn_layer_norm_bwd_workspace_bytes(1, N) == 0
+        assert lib.llattn_layer_norm_bwd(ok, 0, null, 1, ok, ok, ok, ok, null, null, null, 0, 1, N, null) == -1
+        assert lib.llattn_layer_norm_fwd(null, 0, null, null, 1, ok, null, null, 1e-5, 1, N, null) == -1
+        with pytest.raises(ValueError, match="2\\^30"):
+            pkg.layer_norm(torch.zeros(1, dtype=torch.bfloat16).expand(N))
+    assert lib.llattn_layer_norm_bwd_workspace_bytes(1, 2 ** 30) == 2 ** 33
