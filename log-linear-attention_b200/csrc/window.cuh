@@ -143,7 +143,8 @@ __device__ __forceinline__ float cut_off(float x) {
 // A sequence of at most FEW tokens is computed without the rounding of P and dS: an output or a gradient that is a sum of two or three products has no other roundings for theirs to average with
 // (2 to 5 tokens, one head: dq and dk 2.2e-3 to 3.3e-3 off in the place of 1.7e-3), and such calls are the host's time in any case.  The forward multiplies P in two terms; the backward
 // visits each tile twice, the second time with what rounding took off.  (Kernels of their own: the tests cost the others 1 to 3 %.)  Steps are shifted by `twice`, and those of the second visits
-// have the bit.
+// have the bit.  (By the tokens alone: a sequence has the same gradients in any batch.  All others, from 65 tokens of two heads to 3000, are 1.40 to 1.47 times as far off 64 bits as rounding
+// dq and dk makes them, the square root of two roundings.)
 inline bool few_tokens(int T) { return T <= FEW; }
 template <int N>
 __device__ __forceinline__ void leave_rest(float (&e)[N]) {

@@ -53,6 +53,9 @@ def sliding_window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, 
     itself among them, and the first `sinks`; with gradients.  bf16, K = 64 or 128, any T up to 2^24, B and H up to 65535; scale K^-0.5 unless it is given.
     A window of T or more is plain causal attention.
 
+    Scores, statistics and sums are fp32; weights, and the scores' gradients, are rounded to bf16 for the matrix products, so that outputs and gradients are
+    off by about the square root of two of what their own rounding makes, 2.4e-3 in norm.  Sequences of up to 64 tokens, where sums are of few products, keep 16 bits of both.
+
     Values of tokens that a query does not see reach it as 0 times themselves where they share a tile with ones that it sees: a batch
     padded behind its sequences is fine, as long as the padding is finite."""
     scale = _scale(scale, q.shape[-1])

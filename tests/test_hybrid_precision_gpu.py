@@ -73,6 +73,22 @@ def test_values_of_infinity_stay_infinite(T, window, K):
         assert torch.equal(o[..., keep], clean[..., keep])
 
 
+@pytest.mark.parametrize("K", [64, 128])
+@pytest.mark.parametrize("T,window,B", [(50, 20, 200), (100, 30, 80), (500, 500, 9)])
+def test_gradients_of_a_sequence_are_those_of_any_batch(T, window, B, K):
+    """Heads that share nothing, no sinks: every sum is one CTA's, so the same sequence has the same bits alone and among others."""
+    from hattention_b200 import sliding_window_attention
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    q, k, v, do = (torch.randn(B, T, 2, K, device="cuda", generator=gen).to(BF) for _ in range(4))
+
+    def step(n):
+        leaves = [t[:n].clone().requires_grad_(True) for t in (q, k, v)]
+        o = sliding_window_attention(*leaves, window)
+        return (o.detach(),) + torch.autograd.grad(o, leaves, do[:n])
+    for a, b in zip(step(1), step(B)):
+        assert torch.equal(a, b[:1])
+
+
 # ------------------------------------------------------------------------------------------ sizes
 @pytest.mark.parametrize("shape", [(1, 2 ** 32 + 5, 1), (2 ** 31, 1, 1), (1, 1, 2 ** 32 + 64)])
 def test_recurrence_sizes_that_an_int_does_not_hold(shape):
