@@ -89,6 +89,35 @@ def test_gradients_of_a_sequence_are_those_of_any_batch(T, window, B, K):
         assert torch.equal(a, b[:1])
 
 
+# ------------------------------------------------------------------------------------------ decays of the recurrence
+@pytest.mark.parametrize("D", [100001, 100002, 100008])
+@pytest.mark.parametrize("xt", [torch.float32, BF])
+def test_decays(xt, D):
+    """A state of ones after one token of zeros is exp(g): from a multiplication and ex2.approx, 2^-22 of the value, with one or two roundings more, 2^-24 each.  bf16 callers have the rounding of
+    the argument too, |g| 2^-24, and that of log2 e, |g| 2^-26.  Down to -87, where the value is about to leave fp32's normal range."""
+    from hattention_b200 import gated_recurrence, gated_recurrence_step
+    g = torch.linspace(-87, 0, D, device="cuda")[None]
+    ref = g.double().exp()
+    tol = 2.0 ** -22 + 2 * 2.0 ** -24 + (g.double().abs() * (2.0 ** -24 + 2.0 ** -26) if xt is BF else 0.0)
+    x = torch.zeros_like(g, dtype=xt)
+    _, h = gated_recurrence_step(torch.ones_like(g), x, g)
+    assert ((h.double() - ref).abs() <= tol * ref).all()
+    _, h = gated_recurrence(x[:, None], g[:, None], torch.ones_like(g), output_final_state=True)
+    assert ((h.double() - ref).abs() <= tol * ref).all()
+
+
+@pytest.mark.parametrize("xt", [torch.float32, BF])
+def test_decays_that_are_not_finite(xt):
+    from hattention_b200 import gated_recurrence, gated_recurrence_step
+    g = torch.tensor([[-math.inf, math.nan, -100.0, -1e30, 0.0, -0.0]], device="cuda")
+    want = torch.tensor([[0.0, math.nan, 0.0, 0.0, 1.0, 1.0]], device="cuda")
+    x = torch.zeros_like(g, dtype=xt)
+    _, h = gated_recurrence_step(torch.ones_like(g), x, g)
+    assert torch.allclose(h, want, rtol=0, atol=1e-42, equal_nan=True)
+    _, h = gated_recurrence(x[:, None], g[:, None], torch.ones_like(g), output_final_state=True)
+    assert torch.allclose(h, want, rtol=0, atol=1e-42, equal_nan=True)
+
+
 # ------------------------------------------------------------------------------------------ sizes
 @pytest.mark.parametrize("shape", [(1, 2 ** 32 + 5, 1), (2 ** 31, 1, 1), (1, 1, 2 ** 32 + 64)])
 def test_recurrence_sizes_that_an_int_does_not_hold(shape):
