@@ -406,7 +406,7 @@ int llattn_recurrence_step(float* h, const void* x, int x_is_f32, const void* g,
  * k, v, dk, dv (B,T,G,K) bf16, K in {64,128}; head h uses k / v head h / (H/G).  window >= 1, sinks >= 0, scale > 0.  stats (llattn_window_stats_bytes)
  * receives what the backward reads beside o: the softmax statistics, and what rounding took off the outputs of rows that see few tokens; NULL in a forward
  * without one.  The workspace (256 bytes for the forward,
- * llattn_window_workspace_bytes for the backward) begins with a status word, see above.  o, dq, dk and dv start at 32-byte boundaries.  Values that a query does not see have to be finite.
+ * llattn_window_workspace_bytes for the backward) begins with a status word, see above.  Values that a query does not see have to be finite.
  * Weights and the scores' gradients are rounded to bf16 for the matrix products; where T <= 64 they keep 16 bits. */
 size_t llattn_window_stats_bytes(int B, int T, int H, int K, int window, int sinks);
 size_t llattn_window_workspace_bytes(int B, int T, int H, int G, int K, int window, int sinks);

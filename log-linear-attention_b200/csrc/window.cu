@@ -93,7 +93,7 @@ int llattn_window_fwd(const void* q, const void* k, const void* v, void* o, void
     const int rc = win::check(B, T, H, G, K, window, sinks, scale);
     if (rc != 0) return rc;
     if (!q || !k || !v || !o) return LLATTN_ERR_NULL;
-    if (misaligned(16, {q, k, v}) || misaligned(32, {o, stats})) return LLATTN_ERR_ALIGNMENT;
+    if (misaligned(16, {q, k, v, o, stats})) return LLATTN_ERR_ALIGNMENT;
     if (!workspace || misaligned(256, {workspace}) || workspace_bytes < 256) return LLATTN_ERR_WORKSPACE;
     win::Params p = {};
     p.out = (win::bf16*)o;
@@ -111,7 +111,7 @@ int llattn_window_bwd(const void* q, const void* k, const void* v, const void* o
     const int rc = win::check(B, T, H, G, K, window, sinks, scale);
     if (rc != 0) return rc;
     if (!q || !k || !v || !o || !stats || !d_o || !dq || !dk || !dv) return LLATTN_ERR_NULL;
-    if (misaligned(16, {q, k, v, o, d_o}) || misaligned(32, {stats, dq, dk, dv})) return LLATTN_ERR_ALIGNMENT;
+    if (misaligned(16, {q, k, v, o, stats, d_o, dq, dk, dv})) return LLATTN_ERR_ALIGNMENT;
     if (!workspace || misaligned(256, {workspace}) || workspace_bytes < llattn_window_workspace_bytes(B, T, H, G, K, window, sinks)) return LLATTN_ERR_WORKSPACE;
     win::Params p = {};
     p.o = (const win::bf16*)o;

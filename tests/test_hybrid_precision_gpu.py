@@ -125,3 +125,14 @@ def test_recurrence_sizes_that_an_int_does_not_hold(shape):
     x = torch.zeros(1, 1, 1, dtype=BF, device="cuda").expand(shape)
     with pytest.raises(ValueError, match="2\\^31"):
         gated_recurrence(x, x)
+
+
+def test_window_buffers_at_16_byte_boundaries():
+    """Statistics that came back from elsewhere (a hook on saved tensors, a program of its own) start at any boundary of 16 bytes."""
+    from hattention_b200 import ops  # noqa: F401
+    q, k, v, do = (torch.randn(1, 200, 2, 64, device="cuda").to(BF) for _ in range(4))
+    o, stats = torch.ops.llattn.window_fwd(q, k, v, 70, 2, 0.125)
+    moved = torch.empty(stats.numel() + 16, dtype=torch.uint8, device="cuda")[16:].copy_(stats)
+    assert moved.data_ptr() % 32 == 16
+    for a, b in zip(torch.ops.llattn.window_bwd(q, k, v, o, moved, do, 70, 2, 0.125), torch.ops.llattn.window_bwd(q, k, v, o, stats, do, 70, 2, 0.125)):
+        assert torch.equal(a, b)

@@ -83,3 +83,16 @@ def test_rows_whose_columns_an_int_does_not_count_are_refused(pkg):
         with pytest.raises(ValueError, match="2\\^30"):
             pkg.layer_norm(torch.zeros(1, dtype=torch.bfloat16).expand(N))
     assert lib.llattn_layer_norm_bwd_workspace_bytes(1, 2 ** 30) == 2 ** 33
+
+
+def test_window_entries_take_16_byte_boundaries(pkg):
+    """As those of the other operators: all loads and stores are of 16 bytes at most.  (A workspace that is too small is found behind the alignment, before a device is touched.)"""
+    from hattention_b200 import _lib
+    lib, P = _lib.lib(), ctypes.c_void_p
+    ok, at16, odd, sizes = P(4096), P(4096 + 16), P(4096 + 8), (1, 8, 4, 2, 64, 4, 0, 1.0, P(0))
+    fwd = lambda o, stats: lib.llattn_window_fwd(ok, ok, ok, o, stats, ok, 0, *sizes)
+    assert fwd(at16, at16) == -5 and fwd(odd, ok) == -9 and fwd(ok, odd) == -9
+    bwd = lambda stats, dq, dk, dv: lib.llattn_window_bwd(ok, ok, ok, ok, stats, ok, dq, dk, dv, ok, 0, *sizes)
+    assert bwd(at16, at16, at16, at16) == -5
+    for i in range(4):
+        assert bwd(*[odd if j == i else ok for j in range(4)]) == -9
