@@ -12,9 +12,8 @@ namespace llattn {
 namespace win {
 
 // Slot c of a sequence of n tokens holds token c if c < sinks, else the last token that is c modulo the window, counted from the end of the sinks; zeros where there is none.
-template <int K>
 __global__ void __launch_bounds__(256) window_fill_kernel(const bf16* k, const bf16* v, const long long* lengths, bf16* kc, bf16* vc, long long* counts, int T,
-                                                          int G, int window, int sinks) {
+                                                          int G, int K, int window, int sinks) {
     chain_wait();
     const int slots = sinks + window, b = blockIdx.y;
     const long words = (long)G * K / 8;                                    // of 16 bytes, a token
@@ -142,8 +141,7 @@ int llattn_window_fill(const void* k, const void* v, const long long* lengths, v
     cudaStream_t st = (cudaStream_t)stream;
     const dim3 grid((unsigned)blocks, B);
     const auto *kk = (const win::bf16*)k, *vv = (const win::bf16*)v;
-    const auto kern = K == 64 ? win::window_fill_kernel<64> : win::window_fill_kernel<128>;
-    const cudaError_t e = launch_chained(kern, grid, 256, 0, st, kk, vv, lengths, (win::bf16*)k_cache, (win::bf16*)v_cache, counts, T, G, window, sinks);
+    const cudaError_t e = launch_chained(win::window_fill_kernel, grid, 256, 0, st, kk, vv, lengths, (win::bf16*)k_cache, (win::bf16*)v_cache, counts, T, G, K, window, sinks);
     if (e == cudaSuccess) LLATTN_LAUNCHED();
     return (int)e;
 }

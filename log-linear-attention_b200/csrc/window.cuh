@@ -17,7 +17,7 @@ constexpr float LOG2E = 1.4426950408889634f;
 
 struct Params {
     CUtensorMap tq, tk, tv, tdo;      // (B,T,heads,K), boxes of 128 tokens x 64 columns of one head
-    const bf16 *q, *k, *v, *o, *d_o;
+    const bf16 *o, *d_o;
     bf16 *out, *dq, *dk, *dv;
     float *lse, *delta;               // (B,H,TP), TP the length up to whole tiles; lse = log2 of the sum, infinity behind the sequence
     bf16* low;                        // (B,low_rows,H,K): what rounding took off the first rows of o
@@ -179,7 +179,6 @@ __device__ __forceinline__ void tmem_ld64(uint32_t taddr, float (&v)[64]) {
 __device__ __forceinline__ void arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(umma::smem_addr(bar)) : "memory");
 }
-// one 32-byte global store: a full sector of a lane's own row
 // The first CTA of a call's first kernel clears the status word: a wait of another sets it when it gives up, 2^20 polls later.  (A memset in front of the
 // kernel costs every call 4 us.)
 __device__ __forceinline__ void clear_status(const Params& p) {
@@ -200,9 +199,9 @@ template <int WORDS>
 struct Rows {
     uint4* buf;
     int lane;
-    static_assert(WORDS == 4 || WORDS == 8 || WORDS == 16, "rows of 64 to 256 bytes");
-    // eight lanes that store together, and eight that load together, meet eight different quarters of a line
-    __device__ __forceinline__ uint4* word(int row, int w) const { return buf + row * WORDS + (w ^ (WORDS == 4 ? row >> 1 & 3 : row & 7)); }
+    static_assert(WORDS == 8 || WORDS == 16, "rows of 128 or 256 bytes");
+    // eight lanes that store together, and eight that load together, meet eight different words of a line
+    __device__ __forceinline__ uint4* word(int row, int w) const { return buf + row * WORDS + (w ^ (row & 7)); }
     __device__ __forceinline__ void put(int w, uint32_t a, uint32_t b, uint32_t c, uint32_t d) const { *word(lane, w) = make_uint4(a, b, c, d); }
     // rows [first, last) to `out` + row * stride bytes
     __device__ __forceinline__ void store(void* out, long stride, int first, int last) const {
