@@ -17,6 +17,10 @@ void llattn_testing_use_tensor_core_path(int enabled);
  * Negative: an error code. */
 int llattn_testing_mamba2_heads_per_cta(int B, int T, int H, int G, int K, int V, int L);
 
+/* CTAs of a cluster that a step of the windowed attention takes for `units` = sequences x groups, `slots` of a cache and `heads` a group, where the device places clusters of at most
+ * `most`. */
+int llattn_testing_window_step_ranks(long units, int slots, int heads, int most);
+
 /* One CTA waits on an mbarrier that nothing ever completes, with `spin_limit` polls as the bound, and then
  * reports through the same path as the production kernels: *status_dev (device memory) is set to 1 and the
  * kernel returns.  Lets a test see the give-up path without a hung GPU.  spin_limit is clamped to [1, 2^20]. */

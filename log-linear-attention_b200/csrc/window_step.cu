@@ -15,6 +15,7 @@
 #include <cooperative_groups.h>
 
 #include "../../include/llattn.h"
+#include "llattn_testing.h"
 #include "window.cuh"
 
 namespace llattn {
@@ -243,39 +244,50 @@ __global__ void __launch_bounds__(32 * step::Cta<NT>::WARPS, 2) window_step_kern
     if (rank == 0 && threadIdx.x == 0) p.counts[unit] = seen + 1;
 }
 
-// Clusters of 1 to 16 CTAs: as many as leave every warp two blocks of slots, up to two CTAs an SM.
-static int ranks_of(long units, int slots, int warps) {
+constexpr int PORTABLE_RANKS = 8;                // what every device places
+// Clusters of 1 to 16 CTAs, of at most `most`: as many as leave every warp two blocks of slots, up to two CTAs an SM.
+static int ranks_of(long units, int slots, int warps, int most) {
     int n = 1;
-    while (n < step::MAX_RANKS && slots > n * warps * step::BLOCK * 2 && units * n < 148) n *= 2;
+    while (2 * n <= most && slots > n * warps * step::BLOCK * 2 && units * n < 148) n *= 2;
     return n;
 }
 template <int K, int NT>
 static cudaError_t launch_step(const step::Params& p, long units, cudaStream_t st) {
     const auto kern = window_step_kernel<K, NT>;
-    const int n = ranks_of(units, p.sinks + p.window, step::Cta<NT>::WARPS);
-    cudaError_t e;
-    if (n > 8) {
-        static thread_local int allowed = -1;             // the device that this kernel may run clusters of 16 on
-        int dev;
-        e = cudaGetDevice(&dev);
-        if (e != cudaSuccess) return e;
-        if (allowed != dev) {
-            e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-            if (e != cudaSuccess) return e;
-            allowed = dev;
-        }
-    }
     cudaLaunchAttribute attr[2] = {};
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = n;
-    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(units * n));
     cfg.blockDim = dim3(32 * step::Cta<NT>::WARPS);
     cfg.stream = st;
     cfg.attrs = attr;
+    const auto clusters_of = [&](int n) {
+        attr[0].val.clusterDim.x = n;
+        cfg.gridDim = dim3((unsigned)(units * n));
+    };
+    int n = ranks_of(units, p.sinks + p.window, step::Cta<NT>::WARPS, step::MAX_RANKS);
+    cudaError_t e;
+    if (n > PORTABLE_RANKS) {
+        static thread_local int asked = -1, most = 0;     // the device that was asked for clusters of 16, and the largest that it places
+        int dev;
+        e = cudaGetDevice(&dev);
+        if (e != cudaSuccess) return e;
+        if (asked != dev) {
+            e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+            if (e != cudaSuccess) return e;
+            clusters_of(n);
+            cfg.numAttrs = 1;
+            int places = 0;
+            e = cudaOccupancyMaxActiveClusters(&places, kern, &cfg);
+            if (e != cudaSuccess) return e;
+            most = places > 0 ? step::MAX_RANKS : PORTABLE_RANKS;
+            asked = dev;
+        }
+        n = ranks_of(units, p.sinks + p.window, step::Cta<NT>::WARPS, most);
+    }
+    clusters_of(n);
     cfg.numAttrs = 2;
     e = cudaLaunchKernelEx(&cfg, kern, p);
     if (e == cudaSuccess) LLATTN_LAUNCHED();
@@ -292,3 +304,8 @@ cudaError_t decode_step(const bf16* q, const bf16* k, const bf16* v, bf16* kc, b
 
 }  // namespace win
 }  // namespace llattn
+
+extern "C" int llattn_testing_window_step_ranks(long units, int slots, int heads, int most) {
+    using namespace llattn::win;
+    return ranks_of(units, slots, heads <= 8 ? step::Cta<1>::WARPS : step::Cta<2>::WARPS, most);
+}

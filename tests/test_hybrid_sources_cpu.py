@@ -96,3 +96,19 @@ def test_window_entries_take_16_byte_boundaries(pkg):
     assert bwd(at16, at16, at16, at16) == -5
     for i in range(4):
         assert bwd(*[odd if j == i else ok for j in range(4)]) == -9
+
+
+def test_step_clusters_are_no_larger_than_the_device_places(pkg):
+    """Clusters of 16 CTAs are not placed by every device: the launch asks, and takes 8 where they are not."""
+    from hattention_b200 import _lib
+    f = _lib.lib().llattn_testing_window_step_ranks
+    f.argtypes = [ctypes.c_long] + [ctypes.c_int] * 3
+    assert f(8, 4100, 4, 16) == 16 and f(8, 4100, 4, 8) == 8 and f(8, 4100, 12, 8) == 8
+    for units in (1, 9, 40, 147, 148, 10 ** 9):
+        for slots in (1, 256, 257, 5000, 2 ** 30):
+            for heads in (1, 8, 9):
+                n = f(units, slots, heads, 16)
+                assert 1 <= n <= 16 and f(units, slots, heads, 8) == min(n, 8) and (n == 1 or units * n < 2 * 148)
+    body = open(os.path.join(CSRC, "window_step.cu")).read()
+    body = body[body.index("launch_step("):]
+    assert "cudaOccupancyMaxActiveClusters" in body[:body.index("cudaLaunchKernelEx")]
