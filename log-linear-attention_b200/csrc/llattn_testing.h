@@ -21,6 +21,9 @@ int llattn_testing_mamba2_heads_per_cta(int B, int T, int H, int G, int K, int V
  * `most`. */
 int llattn_testing_window_step_ranks(long units, int slots, int heads, int most);
 
+/* y = 2^x of n (even) values by the polynomial that the windowed attention's kernels use for a share of their exponentials. */
+int llattn_selftest_exp2_poly(const float* x, float* y, int n, void* stream);
+
 /* One CTA waits on an mbarrier that nothing ever completes, with `spin_limit` polls as the bound, and then
  * reports through the same path as the production kernels: *status_dev (device memory) is set to 1 and the
  * kernel returns.  Lets a test see the give-up path without a hung GPU.  spin_limit is clamped to [1, 2^20]. */

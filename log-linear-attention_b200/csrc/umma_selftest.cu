@@ -5,6 +5,7 @@
 #include "umma.cuh"
 #include "../../include/llattn.h"
 #include "llattn_testing.h"
+#include "window.cuh"
 
 namespace llattn {
 
@@ -408,4 +409,20 @@ extern "C" int llattn_selftest_ew_cycles(int reps, int spin_warps, int copies, i
     LLATTN_EW_CASE(64)
 #undef LLATTN_EW_CASE
     return LLATTN_ERR_UNSUPPORTED_SHAPE;
+}
+
+namespace llattn {
+__global__ void __launch_bounds__(256) exp2_poly_kernel(const float2* x, float2* y, int pairs) {
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    if (i < pairs) y[i] = win::exp2_poly(pair(x[i].x, x[i].y));
+}
+}  // namespace llattn
+
+extern "C" int llattn_selftest_exp2_poly(const float* x, float* y, int n, void* stream) {
+    if (!x || !y) return LLATTN_ERR_NULL;
+    if (n < 2 || n % 2 != 0) return LLATTN_ERR_UNSUPPORTED_SHAPE;
+    if (llattn::misaligned(8, {x, y})) return LLATTN_ERR_ALIGNMENT;
+    llattn::exp2_poly_kernel<<<(n / 2 + 255) / 256, 256, 0, (cudaStream_t)stream>>>((const float2*)x, (float2*)y, n / 2);
+    LLATTN_LAUNCHED();
+    return (int)cudaGetLastError();
 }
