@@ -136,3 +136,30 @@ def test_window_buffers_at_16_byte_boundaries():
     assert moved.data_ptr() % 32 == 16
     for a, b in zip(torch.ops.llattn.window_bwd(q, k, v, o, moved, do, 70, 2, 0.125), torch.ops.llattn.window_bwd(q, k, v, o, stats, do, 70, 2, 0.125)):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("xt,D", [(torch.float32, 40), (BF, 64), (BF, 33)])
+def test_prompts_of_different_lengths(xt, D):
+    """Padded with x = 0 and g = 0, a sequence has the state, outputs and gradients that it has alone.  (Other tiles and clusters, other orders of fp32 sums: states of at most 32, decays of a
+    tenth a token at least, 2^-21 of what passes a token: 2^-21 * 32 * 10, twice.)"""
+    from hattention_b200 import gated_recurrence
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    lengths, T = [700, 1, 0, 333, 128], 700
+    r = lambda: torch.randn(len(lengths), T, D, device="cuda", generator=gen)
+    real = torch.arange(T, device="cuda")[None, :, None] < torch.tensor(lengths, device="cuda")[:, None, None]
+    x, g, do = (r() * real).to(xt), (-(r().abs() + 0.1) * real), (r() * real).to(xt)
+    h0, dlast = r()[:, 0].contiguous(), r()[:, 0].contiguous()
+    leaves = [t.requires_grad_(True) for t in (x, g, h0)]
+    o, last = gated_recurrence(*leaves, output_final_state=True)
+    grads = torch.autograd.grad([o, last], leaves, [do, dlast])
+    tol = 2 * 2.0 ** -21 * 32 * 10
+    near = lambda a, b: ((a.float() - b.float()).abs() <= tol + 2.0 ** -7 * b.float().abs() * (a.dtype is BF)).all()
+    for b, n in enumerate(lengths):
+        if n == 0:
+            assert torch.equal(last[b], h0[b]) and torch.equal(grads[2][b], dlast[b])
+            continue
+        part = [t.detach()[b:b + 1, :n].clone().requires_grad_(True) for t in (x, g)] + [h0.detach()[b:b + 1].clone().requires_grad_(True)]
+        po, plast = gated_recurrence(*part, output_final_state=True)
+        pg = torch.autograd.grad([po, plast], part, [do[b:b + 1, :n].contiguous(), dlast[b:b + 1]])
+        assert near(o[b, :n], po[0]) and near(last[b], plast[0])
+        assert near(grads[0][b, :n], pg[0][0]) and near(grads[1][b, :n], pg[1][0]) and near(grads[2][b], pg[2][0])
