@@ -10,8 +10,8 @@
 //
 // It is bound by memory as long as little else is issued.  Tiles come to shared memory by asynchronous copies a round ahead, each warp its own rows, and are
 // read, and their decays formed, once.  A cluster's barrier costs its CTAs about a microsecond a round, hence runs as long as registers and shared memory
-// leave room for with two CTAs an SM, and clusters no larger than fill the chip.
-// 2 x 16384 tokens of 2048 channels, bf16 with fp32 decays: forward 98 us, backward 188 us behind other calls (107 and 195 with cold caches), 5.5 and 5.0 TB/s of what they cannot do without.
+// leave room for with two CTAs an SM (one in the forward of fp32 pairs of channels, whose two rounds take 131 KB), and clusters no larger than fill the chip.
+// 2 x 16384 tokens of 2048 channels, bf16 with fp32 decays: forward 99 us, backward 189 us behind other calls (108 and 197 with cold caches), 5.4 and 5.0 TB/s of what they cannot do without.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -481,10 +481,11 @@ struct Launch {
         clusters_of(fastest);
         return cudaSuccess;
     }
-    // Rounds, and two for the start, weighted with what one takes in this width and with what a cluster's CTAs wait for each other, for waves of two CTAs an SM, or one.  (Fitted to 18 shapes,
-    // 1 to 32 sequences of 100 to 32768 tokens, 64 to 4096 channels, with 1 to 16 CTAs a strip of each width.  Forward and backward in us where few CTAs a strip, or many, are faster: 3 x
-    // 1999 tokens of 1001 channels, fp32, strips of 16 alone 24 / 40, of 32 in clusters of two 26 / 50; 32768 tokens of 2048, bf16, strips of 32 in clusters of four 94 / 206, of 16
-    // alone 103 / 231.  Known to be off: 8192 tokens of 4096, fp32, backward, strips of 16 alone 158, of 32 alone 125.)
+    // Rounds, and two for the start, weighted with what one takes in this width and with what a cluster's CTAs wait for each other, for waves of two CTAs an SM, or one: a
+    // bound on what runs at once that the forward of fp32 pairs, one CTA an SM, does not reach.  (Fitted to 18 shapes, 1 to 32 sequences of 100 to 32768 tokens, 64 to 4096 channels, with 1 to
+    // 16 CTAs a strip of each width.  Forward and backward in us where few CTAs a strip, or many, are faster: 3 x 1999 tokens of 1001 channels, fp32, strips of 16 alone 24 / 40, of 32 in
+    // clusters of two 26 / 51; 32768 tokens of 2048, bf16, strips of 32 in clusters of four 94 / 206, of 16 alone 103 / 290; 8192 tokens of 4096, fp32, strips of 16 alone 69 / 112, of 32 alone
+    // 62 / 183: the forward is known to be off there.)
     static constexpr int AT_ONCE = 2 * 148;
     float cost(int n) const {
         const long ctas = units * n, rest = ctas % AT_ONCE;

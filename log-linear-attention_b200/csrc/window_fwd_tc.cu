@@ -10,7 +10,7 @@
 //     the next one       issues the products
 //     the one after it   brings Q, then K and V tiles through a ring
 // It is bound by the chain S, softmax, P V of a tile of queries, of which an SM has two in flight: about 3500 cycles a pair of tiles for 2048 of products (T = 16384, 32 query heads
-// on 8, K = 128, window 2048: 563 us, 0.92 PFLOP/s of products that are not masked).  Two threads a row in the softmax were slower, 618 us for 572: the rows' maxima then
+// on 8, K = 128, window 2048: 514 us, 1.0 PFLOP/s of products that are not masked).  Two threads a row in the softmax were slower, 618 us for 572: the rows' maxima then
 // go through shared memory.
 // P is rounded to bf16, half a step 2^-8: outputs end 2.3e-3 off 64 bits, of which 1.7e-3 are their own rounding.  Two bf16 terms, the second in the other half of S's place, end at
 // 1.7e-3, for a second product and eight more instructions a pair of scores (us, one term / two: T = 16384, window 2048, K = 128 507 / 691; 2 x 1999, window 512, K = 64 34 / 47; 4 x 1000,

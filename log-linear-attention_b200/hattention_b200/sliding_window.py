@@ -71,7 +71,7 @@ def sliding_window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, 
 def sliding_window_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int, sinks: int = 0, scale: Optional[float] = None,
                            lengths: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, WindowState]:
     """Outputs for prompts and the state to continue from.  With `lengths` (B,) int64 on the device, sequence b has lengths[b] tokens (0 to T)
-    and finite padding behind them, whose outputs say nothing."""
+    and finite padding behind them, whose outputs say nothing.  Rounded as sliding_window_attention is."""
     scale = _scale(scale, q.shape[-1])
     r = _lib.host().sliding_window_prefill(q, k, v, window, sinks, scale, lengths, _lib.CHECK_STATUS)
     if r is not None:
@@ -87,7 +87,8 @@ def sliding_window_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, wi
 def sliding_window_step(state: WindowState, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                         scale: Optional[float] = None) -> Tuple[torch.Tensor, WindowState]:
     """One token of every sequence: q (B,H,K), k, v (B,G,K) -> (o (B,H,K), state).  The token's k and v take the place of the one that leaves
-    the window.  One launch that reads no host values, so it can be captured into a CUDA graph and replayed."""
+    the window.  One launch that reads no host values, so it can be captured into a CUDA graph and replayed.  Weights keep 16 bits in its product with v: outputs are off by
+    their own rounding alone."""
     scale = _scale(scale, q.shape[-1])
     o = _lib.host().sliding_window_step(q, k, v, state.k, state.v, state.lengths, state.window, state.sinks, scale)
     if o is not None:
