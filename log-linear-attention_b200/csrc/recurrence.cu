@@ -38,29 +38,28 @@ struct Params {
     int T, D, strips;         // strips of channels a sequence
 };
 
-// exp(g) = 2^(g log2 e).  ex2.approx is off by 2^-22 of the value at most and flushes what is below 2^-126; the rounding of its argument adds |g| 2^-24, and that of log2 e |g| 2^-26.
-// bf16 callers round outputs to 2^-8 and have no use for more (expf has four times the instructions, which tiles that come from memory at full rate leave no room for); fp32 ones get what
-// the argument's two roundings took off, as a factor 1 + c, and 2^-22 for all g (in the time of the others: 2 x 4096 tokens of 2048 channels 45 / 66 us, without 45 / 68).  c is NaN for g = -inf, where the value is 0: fminf takes the bound, which c never reaches, there.
-constexpr float L2E = 1.4426950408889634f, L2E_LOW = 1.9259629911e-8f, LN2 = 0.6931471805599453f;
-__device__ __forceinline__ float ex2(float x) {
+// exp(g).  For bf16 callers 2^(g log2 e): ex2.approx is off by 2^-22 of the value at most and flushes what is below 2^-126; the rounding of its argument adds |g| 2^-24, and that of log2 e
+// |g| 2^-26.  They round outputs to 2^-8, and expf has four times the instructions, which tiles that come from memory at full rate leave no room for.  fp32 callers get expf, 2^-22 of the
+// value for all g and without the bias of ex2.approx (-1.9e-8 of the value on average where g is in (-1, 0)), which the states of tens of tokens add up: 3 x 1999
+// tokens of 1001 channels, gates as logsigmoid(N(3, 1)), o 2.2e-7 off 64 bits with ex2.approx, 1.2e-7 with expf, 24 / 40 us with either.
+template <bool EXACT>
+__device__ __forceinline__ float decay(float g) {
+    if constexpr (EXACT) return expf(g);
     float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(g * 1.4426950408889634f));
     return y;
 }
 template <bool EXACT>
-__device__ __forceinline__ float decay(float g) {
-    const float t = g * L2E, y = ex2(t);
-    if constexpr (!EXACT) return y;
-    return fmaf(y, fminf(fmaf(g, L2E_LOW * LN2, fmaf(g, L2E, -t) * LN2), 1e-3f), y);
-}
-template <bool EXACT>
 __device__ __forceinline__ F2 decay(F2 g) {
-    const F2 t = mul(g, splat<F2>(-L2E));
-    const float2 x = both(t);
-    const F2 y = pair(ex2(-x.x), ex2(-x.y));
-    if constexpr (!EXACT) return y;
-    const float2 c = both(fma2(g, splat<F2>(L2E_LOW * LN2), mul(fma2(g, splat<F2>(L2E), t), splat<F2>(LN2))));
-    return fma2(y, pair(fminf(c.x, 1e-3f), fminf(c.y, 1e-3f)), y);
+    if constexpr (EXACT) {
+        const float2 x = both(g);
+        return pair(expf(x.x), expf(x.y));
+    }
+    const float2 t = both(mul(g, splat<F2>(1.4426950408889634f)));
+    float2 y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y.x) : "f"(t.x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y.y) : "f"(t.y));
+    return pair(y.x, y.y);
 }
 
 // The VEC channels of a lane as a number: one value, or a pair.

@@ -30,7 +30,7 @@ def gated_recurrence(x: torch.Tensor, g: torch.Tensor, initial_state: Optional[t
     x, g and the initial state.
 
     x is bf16 or fp32 and o has its type; g has x's type or is fp32; states are (B,D) fp32, an absent one is zeros.  All sums are fp32.
-    exp(g) is exact to 2^-22 of itself for fp32 x, and for bf16 x to |g| 2^-24 more; below 2^-126 it is 0.
+    exp(g) is exact to 2^-22 of itself for fp32 x; for bf16 x to |g| 2^-24 more, and 0 below 2^-126.
     g <= 0, as log decays are; -inf starts a channel anew at that token, so that packed sequences stay apart.  (Above 0 the products of
     exp(g) over 512 tokens have to stay finite.)  Sequences of different lengths are padded with x = 0 and g = 0: the state behind the padding is the one at the
     sequence's end, and where the padding's outputs have no gradient, the sequence's own tokens have those that they have without it.  T is any size up to 2^30, D any, B ceil(D / 32) below 2^31; even D moves two channels a load."""

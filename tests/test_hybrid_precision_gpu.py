@@ -93,7 +93,7 @@ def test_gradients_of_a_sequence_are_those_of_any_batch(T, window, B, K):
 @pytest.mark.parametrize("D", [100001, 100002, 100008])
 @pytest.mark.parametrize("xt", [torch.float32, BF])
 def test_decays(xt, D):
-    """A state of ones after one token of zeros is exp(g): from a multiplication and ex2.approx, 2^-22 of the value, with one or two roundings more, 2^-24 each.  bf16 callers have the rounding of
+    """A state of ones after one token of zeros is exp(g): from a multiplication and ex2.approx, 2^-22 of the value, with one or two roundings more, 2^-24 each; expf is within two units, 2^-22 too.  bf16 callers have the rounding of
     the argument too, |g| 2^-24, and that of log2 e, |g| 2^-26.  Down to -87, where the value is about to leave fp32's normal range."""
     from hattention_b200 import gated_recurrence, gated_recurrence_step
     g = torch.linspace(-87, 0, D, device="cuda")[None]
@@ -104,6 +104,31 @@ def test_decays(xt, D):
     assert ((h.double() - ref).abs() <= tol * ref).all()
     _, h = gated_recurrence(x[:, None], g[:, None], torch.ones_like(g), output_final_state=True)
     assert ((h.double() - ref).abs() <= tol * ref).all()
+
+
+@pytest.mark.parametrize("D", [101, 128])
+def test_fp32_states_are_as_exact_as_a_loop_in_fp32(D):
+    """Long memories add up what decays are off on average: exponentials of a bias, however small, show here.  The same number of roundings a token in the kernel and in a loop of fp32 operations:
+    errors of one size, a fourth for the order of sums."""
+    from hattention_b200 import gated_recurrence
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    x, g = torch.randn(2, 1500, D, device="cuda", generator=gen), torch.nn.functional.logsigmoid(torch.randn(2, 1500, D, device="cuda", generator=gen) + 3)
+    do = torch.randn(2, 1500, D, device="cuda", generator=gen)
+
+    def gradients(f, dtype):
+        leaves = [t.to(dtype).requires_grad_(True) for t in (x, g)]
+        o = f(*leaves)
+        return (o.detach(),) + torch.autograd.grad(o, leaves, do.to(dtype))
+
+    def loop(x, g):
+        a, h, o = g.exp(), torch.zeros_like(x[:, 0]), []
+        for t in range(x.shape[1]):
+            h = a[:, t] * h + x[:, t]
+            o.append(h)
+        return torch.stack(o, 1)
+    exact = gradients(loop, torch.float64)
+    for ours, plain, ref in zip(gradients(lambda x, g: gated_recurrence(x, g)[0], torch.float32), gradients(loop, torch.float32), exact):
+        assert rel(ours, ref) <= 1.25 * rel(plain, ref)
 
 
 @pytest.mark.parametrize("xt", [torch.float32, BF])
